@@ -678,6 +678,53 @@ int ubv_dcn_col2im(const void* grad_columns, const void* x, const void* offset, 
                    float* grad_offset, float* grad_mask, int N, int H, int W, int C, int Ho, int Wo, int kh, int kw,
                    int sh, int sw, int ph, int pw, int dh, int dw, int deform_groups, int dtype, void* stream);
 
+/* ---- dense-attention decoder blocks: dropout, layer norm, differential attention -----------------------------------------
+ * The object-query decoder's element operators by themselves (the fused forms of the encoder layers are
+ * ubv_add_dropout_layernorm_* and ubv_relu_dropout_*), and a dense attention whose map is a difference of two softmax maps.
+ *
+ * ubv_dropout   y = identity + D o x (identity NULL: y = D o x), n elements.  D = keep / (1 - t / 2^16), t = p 2^16 rounded;
+ *               element i is kept where bits 16 (i % 4) .. + 15 of mix64(seed, i / 4) are >= t (seed_dev as in
+ *               ubv_relu_dropout_forward); nothing is stored: the backward pass is ubv_dropout(grad_y, NULL, grad_x, ...) with
+ *               the same seed.  y (and identity) of y_dtype; x_dtype equals it, or one of the two is f32.  Any n, any
+ *               element-aligned buffers; y may be x or identity. */
+int ubv_dropout(const void* x, const void* identity, void* y, int64_t n, float p, uint64_t seed, const uint64_t* seed_dev,
+                int x_dtype, int y_dtype, void* stream);
+/* Layer norm over the last axis of x [R, C], any C: y = (x - mean) rstd gamma + beta (gamma / beta f32 [C] or NULL); mean / rstd
+ * f32 [R] are written for the backward pass (or both NULL).  Backward: grad_x, grad_gamma and grad_beta written, each or NULL;
+ * the column sums go through the workspace (needed with grad_gamma or grad_beta) in fixed order: the same bits on every run. */
+int ubv_layer_norm_forward(const void* x, const float* gamma, const float* beta, void* y, float* mean, float* rstd, int64_t R,
+                           int C, float eps, int dtype, void* stream);
+int64_t ubv_layer_norm_backward_workspace(int64_t R, int C);
+int ubv_layer_norm_backward(const void* grad_y, const void* x, const float* gamma, const float* mean, const float* rstd,
+                            void* grad_x, float* grad_gamma, float* grad_beta, int64_t R, int C, int dtype, void* workspace,
+                            int64_t workspace_bytes, void* stream);
+/* Differential attention: A_m = softmax_j(scale q_m . k_m + mask), m = 1, 2; out = (D o (A_1 - lam_h A_2)) v; a query that sees no
+ * key gives a zero row (and zero gradients).
+ *   q [B, Nq, H, 2, Dh], k [B, Nk, Hk, 2, Dh], v [B, Nk, Hk, Dv] of dtype, lam [H] f32.  Query head h reads key / value head
+ *   h / (H / Hk).  Dh <= 128, Dv <= 256, the last axis contiguous and readable up to the next multiple of 16 bytes (zeros there);
+ *   16-byte aligned, other strides multiples of 16 bytes.
+ *   strides (HOST, elements): q batch, token, head, map | k the same | v batch, token, head | grad_out batch, token, head
+ *   (forward: 0) | mask batch, head, query, key.
+ *   key_padding_mask [B, Nk] bytes or NULL: nonzero hides the key from every query; what k and v hold there is never used.
+ *   mask_kind 0: mask NULL; 1: bytes, nonzero hides; 2: f32, added to the scaled scores (-inf hides).
+ *   causal: query i sees keys j <= i + Nk - Nq.
+ *   D as in ubv_dropout over the map: key j of row r = (b H + h) Nq + i is field j % 4 of group r ceil(Nk / 4) + j / 4.
+ *   out [B, Nq, H, Dv] contiguous; lse f32 [2, B, H, Nq] and maps f32 [2, B, H, Nq, Dv] (the two maps' products) are written for
+ *   the backward pass, or both NULL.
+ * Backward: grad_q / grad_k / grad_v contiguous in the shapes of q, k, v, grad_lam f32 [H]; grad_q and grad_lam each or NULL,
+ * grad_k and grad_v both or neither.  No atomics: the same bits on every run. */
+int ubv_diff_attention_forward(const void* q, const void* k, const void* v, const float* lam, const uint8_t* key_padding_mask,
+                               const void* mask, int mask_kind, void* out, float* lse, float* maps, const int64_t* strides, int B,
+                               int H, int Hk, int Nq, int Nk, int Dh, int Dv, float scale, int causal, float p, uint64_t seed,
+                               const uint64_t* seed_dev, int dtype, void* stream);
+int64_t ubv_diff_attention_backward_workspace(int B, int H, int Nq);
+int ubv_diff_attention_backward(const void* grad_out, const void* q, const void* k, const void* v, const float* lam,
+                                const uint8_t* key_padding_mask, const void* mask, int mask_kind, const float* lse,
+                                const float* maps, void* grad_q, void* grad_k, void* grad_v, float* grad_lam,
+                                const int64_t* strides, int B, int H, int Hk, int Nq, int Nk, int Dh, int Dv, float scale, int causal,
+                                float p, uint64_t seed, const uint64_t* seed_dev, int dtype, void* workspace,
+                                int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,100 @@
+"""Dropout, layer norm and differential attention where no GPU is needed: the C entries refuse bad arguments before any launch,
+the Python entries refuse CPU tensors, the module builds from the registry."""
+import ctypes
+
+import pytest
+import torch
+
+from unibev_amd import _lib
+
+P = ctypes.c_void_p(1 << 20)          # a 16-byte aligned address that no refused call may touch
+
+
+def refused(status, word):
+    assert status == -1, status
+    assert word in _lib.lib().ubv_last_error().decode()
+
+
+def test_dropout_entry_refuses():
+    f = _lib.lib().ubv_dropout
+    refused(f(None, None, P, 8, 0.1, 0, None, 0, 0, None), 'bad arguments')
+    refused(f(P, None, P, -1, 0.1, 0, None, 0, 0, None), 'bad arguments')
+    refused(f(P, None, P, 8, 0.1, 0, None, 3, 0, None), 'dtype')
+    refused(f(P, None, P, 8, 0.1, 0, None, 1, 2, None), '16-bit')
+    refused(f(P, None, P, 8, 1.5, 0, None, 0, 0, None), 'p = 1.5')
+    refused(f(P, None, P, 8, float('nan'), 0, None, 0, 0, None), 'p = ')
+    assert f(None, None, None, 0, 0.1, 0, None, 0, 0, None) == 0
+
+
+def test_layer_norm_entries_refuse():
+    f, b = _lib.lib().ubv_layer_norm_forward, _lib.lib().ubv_layer_norm_backward
+    refused(f(P, None, None, P, None, None, 4, 0, 1e-5, 0, None), 'out of range')
+    refused(f(P, None, None, P, None, None, 1 << 31, 4, 1e-5, 0, None), 'out of range')
+    refused(f(P, None, None, P, None, None, 4, 4, 1e-5, 7, None), 'dtype')
+    refused(f(None, None, None, P, None, None, 4, 4, 1e-5, 0, None), 'null')
+    refused(f(P, None, None, P, P, None, 4, 4, 1e-5, 0, None), 'null')
+    assert f(None, None, None, None, None, None, 0, 4, 1e-5, 0, None) == 0
+    refused(b(P, P, None, P, P, P, None, None, 0, 4, 0, None, 0, None), 'no rows')
+    refused(b(P, P, None, P, P, None, None, None, 4, 4, 0, None, 0, None), 'null')
+    refused(b(P, P, None, P, P, P, P, None, 4, 4, 0, None, 0, None), 'workspace')
+    need = _lib.lib().ubv_layer_norm_backward_workspace(4, 4)
+    assert need > 0
+    refused(b(P, P, None, P, P, P, P, P, 4, 4, 0, P, need - 1, None), 'workspace')
+
+
+def attn_call(q=P, k=P, v=P, lam=P, mask=None, kind=0, out=P, lse=None, maps=None, strides=None, B=1, H=4, Hk=2, Nq=8, Nk=8, Dh=32,
+              Dv=64, p=0.0, dtype=0):
+    s = strides if strides is not None else [0] * 18
+    return _lib.lib().ubv_diff_attention_forward(q, k, v, lam, None, mask, kind, out, lse, maps, (ctypes.c_int64 * 18)(*s), B, H, Hk, Nq,
+                                                 Nk, Dh, Dv, 0.1, 0, p, 0, None, dtype, None)
+
+
+@pytest.mark.parametrize('kw,word', [(dict(q=None), 'null'), (dict(lam=None), 'null'), (dict(dtype=3), 'dtype'), (dict(Nq=0), 'empty'),
+                                     (dict(Hk=3), 'share'), (dict(Dh=129), 'widths'), (dict(Dv=257), 'widths'), (dict(p=-0.1), 'p = '),
+                                     (dict(kind=1), 'mask kind'), (dict(mask=P, kind=3), 'mask kind'), (dict(out=None), 'out'),
+                                     (dict(lse=P), 'maps'), (dict(q=ctypes.c_void_p((1 << 20) + 2)), 'aligned'),
+                                     (dict(strides=[0] * 5 + [6] + [0] * 12), '16 bytes'), (dict(Nq=1 << 30, H=8, Hk=2), 'out of range')])
+def test_attention_forward_entry_refuses(kw, word):
+    refused(attn_call(**kw), word)
+
+
+def test_attention_backward_entry_refuses():
+    f = _lib.lib().ubv_diff_attention_backward
+    need = _lib.lib().ubv_diff_attention_backward_workspace(1, 4, 8)
+    s = (ctypes.c_int64 * 18)()
+
+    def call(go=P, lse=P, gq=P, gk=P, gv=P, ws=P, n=need):
+        return f(go, P, P, P, P, None, None, 0, lse, P, gq, gk, gv, P, s, 1, 4, 2, 8, 8, 32, 64, 0.1, 0, 0.0, 0, None, 0, ws, n, None)
+
+    assert need > 0 and _lib.lib().ubv_diff_attention_backward_workspace(0, 4, 8) == 0
+    refused(call(go=None), 'grad_out')
+    refused(call(lse=None), 'lse')
+    refused(call(gv=None), 'come together')
+    refused(call(gq=ctypes.c_void_p((1 << 20) + 4)), 'aligned')
+    refused(call(n=need - 1), 'workspace')
+    refused(call(ws=None), 'workspace')
+
+
+def test_cpu_tensors_are_refused():
+    from unibev_amd import functional as UF
+    x = torch.zeros(4, 8)
+    with pytest.raises(RuntimeError, match='GPU only'):
+        UF.dropout(x, 0.1, True)
+    with pytest.raises(RuntimeError, match='GPU only'):
+        UF.layer_norm(x)
+    with pytest.raises(RuntimeError, match='GPU only'):
+        UF.diff_attention(torch.zeros(1, 3, 2, 2, 8), torch.zeros(1, 3, 2, 2, 8), torch.zeros(1, 3, 2, 16), torch.ones(2))
+
+
+def test_module_builds_from_the_registry():
+    from unibev_amd import build_attention
+    m = build_attention(dict(type='DifferentialAttention', embed_dims=64, num_heads=4, num_kv_heads=2, dropout=0.1))
+    assert m.attn_drop == m.residual_drop == 0.1 and m.head_dims == 16
+    assert {k: tuple(v.shape) for k, v in m.state_dict().items() if 'lambda' in k or 'k_proj.w' in k} == {
+        'lambda_a': (2, 8), 'lambda_b': (2, 8), 'k_proj.weight': (32, 64)}
+    with torch.no_grad():
+        m.lambda_a.zero_()
+    assert m.lam().item() == pytest.approx(0.8)
+    for bad in (dict(num_heads=3), dict(num_heads=64), dict(num_heads=4, num_kv_heads=3)):
+        with pytest.raises(ValueError):
+            build_attention(dict(type='DifferentialAttention', embed_dims=64, **bad))

@@ -1,0 +1,801 @@
+"""Dropout, layer norm, differential attention and the module that runs them together, against plain 64-bit implementations.
+
+Tolerances are bounds, not fits: a result may be off by half a step of its type plus the error that the operands' roundings and
+the f32 operations can add, u = 2^-24 each, computed from the reference's own magnitudes.  (Half a step near zero is absolute:
+half the smallest positive number of the type.)"""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DEV = 'cuda'
+U = 2.0 ** -24
+TYPES = [torch.float32, torch.float16, torch.bfloat16]
+M64 = (1 << 64) - 1
+
+
+def UF():
+    from unibev_amd import functional
+    return functional
+
+
+def half(dt):
+    return torch.finfo(dt).eps / 2
+
+
+def tiny(dt):
+    """half the smallest positive number of the type (f32 products of the kernels may flush theirs: 2^-126)"""
+    return {torch.float32: 2.0 ** -126, torch.float16: 2.0 ** -25, torch.bfloat16: 2.0 ** -126}[dt]
+
+
+def within(x, ref, bound, what):
+    """every element of x inside ref +- (half a step + bound)"""
+    x, ref = x.detach().double().cpu(), ref.double().cpu()
+    assert x.shape == ref.shape, (what, x.shape, ref.shape)
+    return _within(x, ref, bound, what)
+
+
+def _within(x, ref, bound, what):
+    off = (x - ref).abs() - bound
+    assert not torch.isnan(off).any(), f'{what}: NaN'
+    worst = off.max().item() if off.numel() else -1.0
+    assert worst <= 0, f'{what}: {worst:.3e} over the bound (largest value {ref.abs().max().item():.3e})'
+
+
+def rand(shape, dt, seed, std=1.0):
+    return (torch.randn(*shape, generator=torch.Generator().manual_seed(seed)) * std).to(dt)
+
+
+def fields(seed, first, groups):
+    """4 groups fields of the counter-based generator, in unsigned integer arithmetic"""
+    with np.errstate(over='ignore'):
+        z = np.arange(first, first + groups, dtype=np.uint64) + np.uint64((seed * 0x9E3779B97F4A7C15 + 0x632BE59BD9B4E019) & M64)
+        z = (z ^ (z >> np.uint64(30))) * np.uint64(0xBF58476D1CE4E5B9)
+        z = (z ^ (z >> np.uint64(27))) * np.uint64(0x94D049BB133111EB)
+        z = z ^ (z >> np.uint64(31))
+    return torch.from_numpy(z.astype('<u8').view('<u2').astype(np.int64))
+
+
+def drop_mask(seed, n, p, first=0):
+    t = int(p * 65536 + 0.5)
+    keep = fields(seed, first // 4, (n + 3) // 4)[:n] >= t
+    return keep.double() * (65536 / (65536 - t) if t < 65536 else 0.0)
+
+
+# ------------------------------------------------------------------------------------------------------------------ dropout
+@pytest.mark.parametrize('n', [1, 3, 7, 8, 9, 63, 1000, 4099, 65536])
+@pytest.mark.parametrize('dt', TYPES)
+@pytest.mark.parametrize('with_identity', [False, True])
+def test_dropout(n, dt, with_identity):
+    p, seed = 0.3, 1234567
+    x = rand((n,), dt, 1)
+    idn = rand((n,), dt, 2) if with_identity else None
+    g = rand((n,), dt, 3)
+    xd = x.to(DEV).requires_grad_()
+    idd = idn.to(DEV).requires_grad_() if with_identity else None
+    y = UF().dropout(xd, p, True, identity=idd, seed=seed)
+    D = drop_mask(seed, n, p)
+    ref = x.double() * D + (idn.double() if with_identity else 0.0)
+    mag = (x.double() * D).abs()
+    within(y, ref, half(dt) * ref.abs() + tiny(dt) + 2 * U * (mag + ref.abs()), 'y')       # a product, a sum, the scale's rounding
+    y.backward(g.to(DEV))
+    rg = g.double() * D
+    within(xd.grad, rg, half(dt) * rg.abs() + tiny(dt) + 2 * U * rg.abs(), 'grad_x')
+    assert torch.equal(xd.grad == 0, ((D == 0) | (g == 0)).to(DEV))
+    if with_identity:
+        assert torch.equal(idd.grad.cpu(), g)
+
+
+@pytest.mark.parametrize('dt', [torch.float16, torch.bfloat16])
+def test_dropout_16bit_branch_f32_residual(dt):
+    x, idn, g = rand((37, 50), dt, 1), rand((37, 50), torch.float32, 2), rand((37, 50), torch.float32, 3)
+    xd, idd = x.to(DEV).requires_grad_(), idn.to(DEV).requires_grad_()
+    y = UF().dropout(xd, 0.1, True, identity=idd, seed=5)
+    D = drop_mask(5, x.numel(), 0.1).view(x.shape)
+    ref = x.double() * D + idn.double()
+    assert y.dtype == torch.float32
+    within(y, ref, 3 * U * (ref.abs() + (x.double() * D).abs()), 'y')
+    y.backward(g.to(DEV))
+    rg = g.double() * D
+    assert xd.grad.dtype == dt and torch.equal(idd.grad.cpu(), g)
+    within(xd.grad, rg, (half(dt) + 2 * U) * rg.abs() + tiny(dt), 'grad_x')
+
+
+def test_dropout_rates_seeds_and_borders():
+    F = UF()
+    x = torch.ones(400000, device=DEV)
+    for p in (0.1, 0.5, 0.9):
+        y = F.dropout(x, p, True)
+        q = int(p * 65536 + 0.5) / 65536
+        dropped = (y == 0).double().mean().item()
+        assert abs(dropped - q) < 6 * math.sqrt(q * (1 - q) / x.numel())              # six standard deviations
+    assert F.dropout(x, 0.3, False) is x and F.dropout(x, 0.0, True) is x
+    assert F.dropout(x, 1.0, True).abs().max().item() == 0.0
+    assert torch.equal(F.dropout(x, 0.0, True, identity=x), x + x)
+    a, b, c = F.dropout(x, 0.5, True, seed=1), F.dropout(x, 0.5, True, seed=1), F.dropout(x, 0.5, True, seed=2)
+    assert torch.equal(a, b) and not torch.equal(a, c)
+    assert not torch.equal(F.dropout(x, 0.5, True), F.dropout(x, 0.5, True))
+    assert F.dropout(x[:0], 0.5, True).shape == (0,)
+
+
+@pytest.mark.parametrize('off', [1, 3, 4])
+@pytest.mark.parametrize('dt', TYPES)
+def test_dropout_buffers_off_a_16_byte_border(off, dt):
+    n = 1003
+    x = torch.zeros(n + off, dtype=dt, device=DEV)[off:]
+    x.copy_(rand((n,), dt, 1))
+    y = UF().dropout(x, 0.3, True, identity=x, seed=9)
+    assert torch.equal(y, UF().dropout(x.clone(), 0.3, True, identity=x.clone(), seed=9))
+
+
+def test_dropout_takes_views_and_refuses():
+    F = UF()
+    x = torch.randn(6, 10, device=DEV)
+    assert torch.equal(F.dropout(x.t(), 0.5, True, seed=3), F.dropout(x.t().contiguous(), 0.5, True, seed=3))
+    e = torch.randn(1, 10, device=DEV, requires_grad=True)
+    D = drop_mask(3, 40, 0.5).view(4, 10).float().to(DEV)
+    F.dropout(e.expand(4, 10), 0.5, True, seed=3).sum().backward()                    # the sum over a broadcast input's copies
+    torch.testing.assert_close(e.grad[0], D.sum(0))
+    with pytest.raises(ValueError, match='must be in'):
+        F.dropout(x, 1.5, True)
+    with pytest.raises(ValueError, match='seed'):
+        F.dropout(x, 0.5, True, seed=-1)
+    with pytest.raises(ValueError, match='shape'):
+        F.dropout(x, 0.5, True, identity=x[:1])
+    with pytest.raises(TypeError):
+        F.dropout(x, 0.5, True, identity=x.half())
+    with pytest.raises(TypeError):
+        F.dropout(x.double(), 0.5, True)
+    with pytest.raises(TypeError):
+        F.dropout(x.half(), 0.5, True, identity=x.bfloat16())
+    with pytest.raises(RuntimeError, match='GPU only'):
+        F.dropout(x, 0.5, True, identity=x.cpu())
+
+
+def test_dropout_past_32_bit_offsets():
+    """more than 2^32 elements: the tail's mask counts on where the 32-bit part wraps"""
+    n = (1 << 32) + 1003
+    x = torch.ones(n, dtype=torch.float16, device=DEV)
+    y = UF().dropout(x, 0.5, True, seed=11)
+    first = n - 1003
+    assert torch.equal(y[first:].double().cpu(), drop_mask(11, 1003, 0.5, first=first))
+    assert torch.equal(y[:4096].double().cpu(), drop_mask(11, 4096, 0.5))
+
+
+# --------------------------------------------------------------------------------------------------------------- layer norm
+def norm_case(R, C, dt, seed=0, mean=0.7):
+    x, g = rand((R, C), dt, seed, 2.0) + torch.tensor(mean, dtype=dt), rand((R, C), dt, seed + 1)
+    return x, rand((C,), torch.float32, seed + 2, 0.3) + 1.0, rand((C,), torch.float32, seed + 3, 0.3), g
+
+
+def norm_check(x, gamma, beta, g, y, gx, dg, db, dt, eps=1e-5):
+    """K roundings in a row at most on any chain of sums: 32 in a thread, 10 over threads, and those of single operations; streamed
+    rows add C / 8192 more"""
+    R, C = x.shape
+    K = (64 + C / 4096) * U
+    X, G = x.double(), g.double()
+    w = torch.ones(C).double() if gamma is None else gamma.double()
+    b = torch.zeros(C).double() if beta is None else beta.double()
+    mu = X.mean(-1, keepdim=True)
+    rs = ((X - mu).pow(2).mean(-1, keepdim=True) + eps).rsqrt()
+    h = (X - mu) * rs
+    ref = h * w + b
+    big = X.abs().mean(-1, keepdim=True)
+    eh = K * (h.abs() * 2 + rs * (big + X.abs()))                                 # of h: the mean's error, the difference's, rstd's
+    within(y, ref, half(dt) * ref.abs() + tiny(dt) + eh * w.abs() + K * (ref.abs() + b.abs()), 'y')
+    u = G * w
+    s1, s2 = u.mean(-1, keepdim=True), (u * h).mean(-1, keepdim=True)
+    r = rs * (u - s1 - h * s2)
+    e = rs * K * (u.abs() + u.abs().mean(-1, keepdim=True) + h.abs() * (u * h).abs().mean(-1, keepdim=True)) * 2 + \
+        rs * (eh * s2.abs() + h.abs() * (u.abs() * eh).mean(-1, keepdim=True)) + K * r.abs()
+    if gx is not None:
+        within(gx, r, half(dt) * r.abs() + tiny(dt) + e, 'grad_x')
+    KR = (64 + R / 64) * U                                                         # a thread's rows in a row, then the blocks'
+    if dg is not None:
+        t = G * h
+        within(dg, t.sum(0), (G.abs() * eh).sum(0) + KR * t.abs().sum(0), 'grad_gamma')
+    if db is not None:
+        within(db, G.sum(0), KR * G.abs().sum(0), 'grad_beta')
+
+
+@pytest.mark.parametrize('R,C', [(1, 1), (3, 1), (1, 7), (5, 8), (70, 16), (33, 17), (300, 64), (9, 255), (257, 256), (13, 257),
+                                 (40, 512), (21, 1021), (11, 1500), (6, 2056), (5, 4100), (3, 8192), (2, 8200), (3, 20011)])
+@pytest.mark.parametrize('dt', TYPES)
+def test_layer_norm(R, C, dt):
+    x, gamma, beta, g = norm_case(R, C, dt)
+    xd, wd, bd = (t.to(DEV).requires_grad_() for t in (x, gamma, beta))
+    y = UF().layer_norm(xd, wd, bd)
+    y.backward(g.to(DEV))
+    norm_check(x, gamma, beta, g, y, xd.grad, wd.grad, bd.grad, dt)
+
+
+def test_layer_norm_many_rows_is_deterministic():
+    x, gamma, beta, g = norm_case(20011, 96, torch.bfloat16)
+    outs = []
+    for _ in range(2):
+        xd, wd, bd = (t.to(DEV).requires_grad_() for t in (x, gamma, beta))
+        y = UF().layer_norm(xd, wd, bd)
+        y.backward(g.to(DEV))
+        outs.append((y.detach(), xd.grad, wd.grad, bd.grad))
+    assert all(torch.equal(a, b) for a, b in zip(*outs))
+    norm_check(x, gamma, beta, g, *outs[0], torch.bfloat16)
+
+
+@pytest.mark.parametrize('dt', TYPES)
+def test_layer_norm_without_weights_views_and_borders(dt):
+    x, gamma, beta, g = norm_case(12, 40, dt)
+    xd = x.to(DEV).requires_grad_()
+    y = UF().layer_norm(xd)
+    y.backward(g.to(DEV))
+    norm_check(x, None, None, g, y, xd.grad, None, None, dt)
+    y2 = UF().layer_norm(x.to(DEV), gamma.to(DEV))
+    norm_check(x, gamma, None, g, y2, None, None, None, dt)
+    buf = torch.zeros(12 * 40 + 3, dtype=dt, device=DEV)
+    v = buf[3:].view(12, 40)
+    v.copy_(x)
+    assert torch.equal(UF().layer_norm(v), y)                                       # off a 16-byte border
+    wide = torch.zeros(12, 80, dtype=dt, device=DEV)
+    wide[:, ::2].copy_(x)
+    assert torch.equal(UF().layer_norm(wide[:, ::2]), y)                            # a strided view
+    wd = gamma.to(DEV).requires_grad_()                                             # the weight alone wants a gradient
+    UF().layer_norm(x.to(DEV), wd).backward(g.to(DEV))
+    norm_check(x, gamma, None, g, y2, None, wd.grad, None, dt)
+
+
+def test_layer_norm_far_from_zero_and_constant_rows():
+    """|mean| = 1000 standard deviations: the variance is taken around the mean; a constant row gives beta exactly"""
+    x = rand((50, 256), torch.float32, 1) + 1000.0
+    g = rand((50, 256), torch.float32, 2)
+    xd = x.to(DEV).requires_grad_()
+    y = UF().layer_norm(xd)
+    y.backward(g.to(DEV))
+    norm_check(x, None, None, g, y, xd.grad, None, None, torch.float32)
+    beta = rand((64,), torch.float32, 3).to(DEV)
+    c = UF().layer_norm(torch.full((3, 64), 0.25, device=DEV), torch.ones(64, device=DEV), beta)
+    assert torch.equal(c, beta.expand(3, 64))
+
+
+def test_layer_norm_empty_and_refusals():
+    F = UF()
+    x = torch.randn(0, 32, device=DEV, requires_grad=True)
+    w = torch.ones(32, device=DEV, requires_grad=True)
+    y = F.layer_norm(x, w)
+    y.sum().backward()
+    assert y.shape == (0, 32) and x.grad.shape == (0, 32) and torch.equal(w.grad, torch.zeros(32, device=DEV))
+    z = torch.randn(4, 32, device=DEV)
+    with pytest.raises(ValueError, match='gamma'):
+        F.layer_norm(z, torch.ones(31, device=DEV))
+    with pytest.raises(ValueError, match='beta'):
+        F.layer_norm(z, None, torch.ones(1, device=DEV))
+    with pytest.raises(ValueError, match='last axis'):
+        F.layer_norm(z[:, :0])
+    with pytest.raises(TypeError):
+        F.layer_norm(z.double())
+    with pytest.raises(RuntimeError, match='GPU only'):
+        F.layer_norm(z, torch.ones(32))
+
+
+# ---------------------------------------------------------------------------------------------------- differential attention
+class Ref:
+    """The definition in 64 bits on the CPU, its gradients by the formulas, and bounds of what the kernels' arithmetic may add."""
+
+    def __init__(self, q, k, v, lam, go, dt, hidden=None, bias=None, D=None, scale=None):
+        B, Nq, H, _, Dh = q.shape
+        _, Nk, Hk, Dv = v.shape
+        G = H // Hk
+        q, k, v, go = (t.double() for t in (q, k, v, go))
+        lam = lam.double().view(1, H, 1, 1)
+        scale = Dh ** -0.5 if scale is None else scale
+        e = half(dt) if dt != torch.float32 else 0.0                                # rounding of a matrix operand
+        Q, K = q.permute(0, 2, 3, 1, 4), k.permute(0, 2, 3, 1, 4).repeat_interleave(G, 1)      # B H 2 N Dh
+        V, O = v.permute(0, 2, 1, 3).repeat_interleave(G, 1), go.permute(0, 2, 1, 3)
+        D = torch.ones(B, H, Nq, Nk).double() if D is None else D
+        hid = torch.zeros(B, H, Nq, Nk, dtype=torch.bool) if hidden is None else hidden.expand(B, H, Nq, Nk)
+        live = (~hid).any(-1, keepdim=True)
+        A, rho = [], []
+        for m in (0, 1):
+            s = scale * Q[:, :, m] @ K[:, :, m].transpose(-1, -2)
+            size = scale * Q[:, :, m].abs() @ K[:, :, m].abs().transpose(-1, -2)
+            if bias is not None:
+                s, size = s + bias, size + bias.abs().clamp_max(3e38)
+            s = torch.where(hid & live, torch.full_like(s, -math.inf), s)
+            a = torch.softmax(s, -1) * live
+            # of a probability, relative: its score's and its row's largest (Dh products each, the scale, the mask, the base),
+            # the exponential's and the sum's
+            far = torch.where(a > 0, size, torch.zeros_like(size)).amax(-1, keepdim=True)
+            A.append(a)
+            rho.append(U * ((Dh + 12) * (torch.where(a > 0, size, torch.zeros_like(size)) + far) + Nk / 16 + 48))
+        acc = U * (Nk / 4 + 64)
+        # f16: a probability is rounded as 2^8 p, to a multiple of 2^-24 where that is below 2^-14: at most 2^-25 / 2^8 off (p is
+        # of the row's largest, so at least that of its normalised value)
+        sub = 2.0 ** -33 if dt == torch.float16 else 0.0
+        A1, A2 = A
+        la = lam.abs()
+        self.out = (D * (A1 - lam * A2)) @ V
+        eo = [(D * (a * (e + r + acc) + sub * (a > 0))) @ V.abs() for a, r in zip(A, rho)]
+        self.e_out = half(dt) * self.out.abs() + tiny(dt) + eo[0] + la * eo[1] + 4 * U * ((D * (A1 + la * A2)) @ V.abs())
+        P = D * (A1 - lam * A2)
+        eP = D * (A1 * rho[0] + la * A2 * rho[1] + 4 * U * (A1 + la * A2) + sub) + e * P.abs()
+        accq = U * (Nq * G / 4 + 64)
+        gv = P.transpose(-1, -2) @ O
+        egv = (eP + accq * P.abs()).transpose(-1, -2) @ O.abs()
+        T = D * (O @ V.transpose(-1, -2))
+        eT = U * (Dv + 8) * D * (O.abs() @ V.abs().transpose(-1, -2))
+        gq, gk, egq, egk, dl = [], [], [], [], None
+        for m, (a, r) in enumerate(zip(A, rho)):
+            d = (a * T).sum(-1, keepdim=True)
+            ed = (O.abs() * (eo[m] + U * (Dv + 8) * ((D * a) @ V).abs())).sum(-1, keepdim=True)
+            f = 1.0 if m == 0 else -lam
+            s = a * (T - d) * f
+            es = f.abs() * a * (r * (T - d).abs() + eT + ed + 4 * U * (T.abs() + d.abs())) if m else \
+                a * (r * (T - d).abs() + eT + ed + 4 * U * (T.abs() + d.abs()))
+            es = es + (e + 4 * U) * s.abs() + (tiny(dt) if dt == torch.float16 else 0.0)
+            gq.append(scale * s @ K[:, :, m])
+            egq.append(scale * (es + acc * s.abs()) @ K[:, :, m].abs())
+            gk.append(scale * s.transpose(-1, -2) @ Q[:, :, m])
+            egk.append(scale * (es + accq * s.abs()).transpose(-1, -2) @ Q[:, :, m].abs())
+            if m == 1:
+                t = a * T
+                self.lam = -t.sum((0, 2, 3))
+                self.e_lam = (t.abs() * (r + acc + accq * B) + a * eT).sum((0, 2, 3)) + half(torch.float32) * self.lam.abs()
+
+        def heads(x):
+            return x.view(B, Hk, G, *x.shape[2:]).sum(2)
+
+        def own(x, ex):
+            return x, half(dt) * x.abs() + tiny(dt) + ex + 4 * U * x.abs()
+        self.out, self.e_out = self.out.permute(0, 2, 1, 3), self.e_out.permute(0, 2, 1, 3)
+        self.q, self.eq = own(torch.stack(gq, 2).permute(0, 3, 1, 2, 4), torch.stack(egq, 2).permute(0, 3, 1, 2, 4))
+        self.k, self.ek = own(heads(torch.stack(gk, 2)).permute(0, 3, 1, 2, 4), heads(torch.stack(egk, 2)).permute(0, 3, 1, 2, 4))
+        self.v, self.ev = own(heads(gv).permute(0, 2, 1, 3), heads(egv).permute(0, 2, 1, 3))
+
+
+def attn_inputs(B, H, Hk, Nq, Nk, Dh, Dv, dt, seed=0):
+    return (rand((B, Nq, H, 2, Dh), dt, seed, 1.5), rand((B, Nk, Hk, 2, Dh), dt, seed + 1), rand((B, Nk, Hk, Dv), dt, seed + 2),
+            rand((H,), torch.float32, seed + 3, 0.2) + 0.5, rand((B, Nq, H, Dv), dt, seed + 4))
+
+
+def attn_drop(seed, B, H, Nq, Nk, p):
+    if p == 0:
+        return None
+    n4 = (Nk + 3) // 4
+    t = int(p * 65536 + 0.5)
+    keep = (fields(seed, 0, B * H * Nq * n4).view(B, H, Nq, 4 * n4)[..., :Nk] >= t).double()
+    return keep * (65536 / (65536 - t) if t < 65536 else 0.0)
+
+
+def attn_check(q, k, v, lam, go, dt, hidden=None, bias=None, p=0.0, scale=None, seed=77, **kw):
+    leaves = [t.to(DEV).requires_grad_() for t in (q, k, v, lam)]
+    y = UF().diff_attention(*leaves, p=p, training=True, seed=seed, scale=scale, **kw)
+    B, Nq, H = q.shape[:3]
+    r = Ref(q, k, v, lam, go, dt, hidden, bias, attn_drop(seed, B, H, Nq, k.shape[1], p), scale)
+    within(y, r.out, r.e_out, 'out')
+    with torch.no_grad():
+        again = UF().diff_attention(*leaves, p=p, training=True, seed=seed, scale=scale, **kw)
+    within(again, r.out, r.e_out, 'out without gradients')
+    y.backward(go.to(DEV))
+    for name, t, ref, e in (('grad_q', leaves[0], r.q, r.eq), ('grad_k', leaves[1], r.k, r.ek), ('grad_v', leaves[2], r.v, r.ev),
+                            ('grad_lam', leaves[3], r.lam, r.e_lam)):
+        assert t.grad.dtype == t.dtype
+        within(t.grad, ref, e, name)
+    return y, leaves
+
+
+SHAPES = [(1, 1, 1, 1, 1, 1, 1), (2, 2, 1, 1, 1, 16, 32), (2, 4, 2, 33, 70, 20, 40), (1, 2, 1, 64, 64, 16, 32), (1, 3, 3, 5, 300, 32, 64),
+          (2, 2, 2, 130, 31, 64, 64), (1, 4, 2, 40, 65, 64, 128), (1, 1, 1, 33, 129, 128, 128), (1, 2, 1, 17, 90, 128, 256),
+          (1, 1, 1, 3, 3, 7, 13), (1, 2, 2, 31, 33, 96, 192), (1, 6, 2, 50, 257, 24, 24)]
+
+
+@pytest.mark.parametrize('shape', SHAPES)
+@pytest.mark.parametrize('dt', TYPES)
+def test_attention(shape, dt):
+    attn_check(*attn_inputs(*shape, dt), dt)
+
+
+@pytest.mark.parametrize('shape', SHAPES[2:8])
+@pytest.mark.parametrize('dt', [torch.float32, torch.bfloat16])
+def test_attention_dropout(shape, dt):
+    attn_check(*attn_inputs(*shape, dt), dt, p=0.2)
+
+
+def causal(Nq, Nk):
+    return torch.arange(Nk)[None] - torch.arange(Nq)[:, None] > Nk - Nq
+
+
+@pytest.mark.parametrize('Nq,Nk', [(1, 1), (1, 200), (200, 1), (70, 70), (40, 130), (130, 40), (97, 96)])
+@pytest.mark.parametrize('dt', TYPES)
+def test_attention_causal(Nq, Nk, dt):
+    attn_check(*attn_inputs(2, 4, 2, Nq, Nk, 32, 64, dt), dt, hidden=causal(Nq, Nk), causal=True)
+
+
+@pytest.mark.parametrize('kind', ['bool', 'rows', 'heads', 'float', 'slopes', 'lowest', 'inf', 'padding', 'padding+causal', 'all'])
+@pytest.mark.parametrize('dt', TYPES)
+def test_attention_masks(kind, dt):
+    """rows that see nothing, masks of the type's lowest value, whole samples hidden, masks broadcast over batch and heads"""
+    B, H, Hk, Nq, Nk = 2, 4, 2, 45, 77
+    q, k, v, lam, go = attn_inputs(B, H, Hk, Nq, Nk, 32, 64, dt)
+    gen = torch.Generator().manual_seed(5)
+    m = torch.rand(Nq, Nk, generator=gen) < 0.4
+    m[::9] = True
+    kw, hidden, bias = {}, None, None
+    if kind == 'bool':
+        kw, hidden = dict(attn_mask=m), m
+    elif kind == 'rows':
+        m = torch.rand(B, 1, Nq, 1, generator=gen) < 0.5
+        kw, hidden = dict(attn_mask=m), m
+    elif kind == 'heads':
+        m = torch.rand(B * H, Nq, Nk, generator=gen) < 0.5
+        kw, hidden = dict(attn_mask=m), m.view(B, H, Nq, Nk)
+    elif kind == 'float':
+        bias = torch.randn(Nq, Nk, generator=gen).to(dt).float()
+        kw = dict(attn_mask=bias.to(dt))
+    elif kind == 'slopes':
+        bias = -torch.rand(1, H, Nq, Nk, generator=gen) * 20
+        kw = dict(attn_mask=bias)
+    elif kind == 'lowest':                              # finite: a row of it alone is a uniform row, beside others it is nothing
+        low = torch.finfo(torch.float32).min
+        bias = torch.where(m, torch.tensor(low), torch.tensor(0.0))
+        kw = dict(attn_mask=bias)
+    elif kind == 'inf':
+        f = torch.where(m, torch.tensor(-math.inf), torch.randn(Nq, Nk, generator=gen))
+        kw, hidden, bias = dict(attn_mask=f), m, torch.where(m, torch.tensor(0.0), f)
+    else:
+        pad = torch.arange(Nk)[None] >= torch.tensor([[Nk], [0 if kind == 'all' else 50]])
+        kw, hidden = dict(key_padding_mask=pad), pad[:, None, None]
+        if kind == 'padding+causal':
+            kw['causal'], hidden = True, hidden | causal(Nq, Nk)
+    if kind == 'lowest':                                # its reference: scores vanish beside it in f32
+        q64 = Ref(q, k, v, lam, go, dt, hidden=m & ~m.all(-1, keepdim=True))
+        y = UF().diff_attention(*(t.to(DEV) for t in (q, k, v, lam)), attn_mask=kw['attn_mask'].to(DEV))
+        rows = ~m.all(-1)
+        _within(y.double().cpu()[:, rows], q64.out[:, rows], q64.e_out[:, rows], 'rows with a key')
+        flat = (1 - lam.double()).view(1, 1, H, 1) * v.double().mean(1, keepdim=True).repeat_interleave(H // Hk, 2)
+        e = (half(dt) + 80 * U) * (1 + lam.double().abs()).view(1, 1, H, 1) * v.double().abs().mean(1, keepdim=True).repeat_interleave(H // Hk, 2)
+        _within(y.double().cpu()[:, ~rows], flat.expand(B, int((~rows).sum()), H, -1), (e + half(dt) * flat.abs()).expand(B, int((~rows).sum()), H, -1),
+                'rows of the lowest value')
+        return
+    kw = {n: t.to(DEV) if torch.is_tensor(t) else t for n, t in kw.items()}
+    y, leaves = attn_check(q, k, v, lam, go, dt, hidden=hidden, bias=bias, p=0.1, **kw)
+    if hidden is not None:
+        dead = hidden.expand(B, H, Nq, Nk).all(-1)
+        assert dead.any() or kind in ('padding', 'heads', 'padding+causal')
+        assert (y.detach().cpu().permute(0, 2, 1, 3)[dead] == 0).all()
+        assert (leaves[0].grad.cpu().permute(0, 2, 1, 3, 4)[dead] == 0).all()
+
+
+@pytest.mark.parametrize('dt', TYPES)
+def test_attention_hidden_keys_may_hold_anything(dt):
+    """NaN and infinity in the padded keys reach nothing; their gradients are zero"""
+    q, k, v, lam, go = attn_inputs(2, 2, 1, 20, 90, 32, 64, dt)
+    pad = torch.zeros(2, 90, dtype=torch.bool)
+    pad[0, 10:40], pad[1, 64:] = True, True
+    bad_k, bad_v = k.clone(), v.clone()
+    bad_k[pad], bad_v[pad] = math.nan, math.inf
+    outs = []
+    for kk, vv in ((k, v), (bad_k, bad_v)):
+        leaves = [t.to(DEV).requires_grad_() for t in (q, kk, vv, lam)]
+        y = UF().diff_attention(*leaves, key_padding_mask=pad.to(DEV))
+        y.backward(go.to(DEV))
+        outs.append([y.detach()] + [t.grad for t in leaves])
+    assert all(torch.equal(a, b) for a, b in zip(*outs))
+    assert (outs[1][2][pad.to(DEV)] == 0).all() and (outs[1][3][pad.to(DEV)] == 0).all()
+
+
+@pytest.mark.parametrize('dt', TYPES)
+def test_attention_many_heads_takes_the_wide_tiling(dt):
+    """enough blocks of 128 own items that no two waves share a row: the other arrangement of the same kernels"""
+    B, H, Nq, Nk = 8, 64, 5, 70
+    attn_check(*attn_inputs(B, H, H, Nq, Nk, 16, 32, dt), dt, hidden=causal(Nq, Nk), causal=True, p=0.1)
+
+
+@pytest.mark.parametrize('Nq,H,Hk', [(1, 4, 4), (1, 8, 2), (3, 4, 1), (7, 2, 2)])
+@pytest.mark.parametrize('dt', TYPES)
+def test_attention_few_queries_many_keys(Nq, H, Hk, dt):
+    q, k, v, lam, go = attn_inputs(2, H, Hk, Nq, 5003, 32, 64, dt)
+    pad = torch.arange(5003)[None] >= torch.tensor([[5003], [1234]])
+    attn_check(q, k, v, lam, go, dt, hidden=pad[:, None, None], key_padding_mask=pad.to(DEV))
+
+
+def test_attention_large_scores():
+    """scores far beyond f32's exponent range: the row's largest is subtracted first"""
+    q, k, v, lam, go = attn_inputs(1, 2, 2, 20, 50, 32, 64, torch.float32)
+    y = UF().diff_attention((q * 100).to(DEV), k.to(DEV), v.to(DEV), lam.to(DEV))
+    r = Ref(q * 100, k, v, lam, go, torch.float32)
+    assert torch.isfinite(y).all()
+    within(y, r.out, r.e_out, 'out')
+
+
+@pytest.mark.parametrize('dt', TYPES)
+def test_attention_strides(dt):
+    """token-major operands, one projection cut into q, k and v, rows off a 16-byte border, expanded batches, a padded last axis"""
+    B, H, N, Dh, Dv = 2, 2, 37, 16, 32
+    F = UF()
+    q, k, v, lam, go = (t.to(DEV) for t in attn_inputs(B, H, H, N, N, Dh, Dv, dt))
+    want = F.diff_attention(q, k, v, lam)
+    tok = [t.transpose(0, 1).contiguous().transpose(0, 1) for t in (q, k, v)]
+    assert torch.equal(F.diff_attention(*tok, lam), want)
+    qkv = torch.cat([q.flatten(2), k.flatten(2), v.flatten(2)], -1)
+    cut = qkv.split([q[0, 0].numel(), k[0, 0].numel(), v[0, 0].numel()], -1)
+    assert torch.equal(F.diff_attention(cut[0].view(q.shape), cut[1].view(k.shape), cut[2].view(v.shape), lam), want)
+    off = []
+    for t in (q, k, v):
+        b = torch.empty(t.numel() + 1, dtype=dt, device=DEV)
+        off.append(b[1:].view(t.shape))
+        off[-1].copy_(t)
+    assert torch.equal(F.diff_attention(*off, lam), want)
+    last = [t.transpose(-1, -2).contiguous().transpose(-1, -2) for t in (q, k, v)]
+    assert torch.equal(F.diff_attention(*last, lam), want)
+    one = F.diff_attention(q, k[:1].expand(B, -1, -1, -1, -1), v[:1].expand(B, -1, -1, -1), lam)
+    assert torch.equal(one[1], F.diff_attention(q[1:], k[:1], v[:1], lam)[0])
+    kk = k[:1].clone().requires_grad_()                                             # a broadcast input's gradient is the sum
+    F.diff_attention(q, kk.expand(B, -1, -1, -1, -1), v, lam).backward(go)
+    parts = []
+    for b in range(B):
+        kb = k[:1].clone().requires_grad_()
+        F.diff_attention(q[b:b + 1], kb, v[b:b + 1], lam).backward(go[b:b + 1])
+        parts.append(kb.grad)
+    assert torch.equal(kk.grad, parts[0] + parts[1])
+    s = lam[:1].clone().requires_grad_()                                            # one lam for all heads
+    F.diff_attention(q, k, v, s).backward(go)
+    l = s.detach().expand(H).clone().requires_grad_()
+    F.diff_attention(q, k, v, l).backward(go)
+    torch.testing.assert_close(s.grad, l.grad.sum(0, keepdim=True), rtol=4 * U, atol=0)
+    leaf = q.clone().requires_grad_()                                               # grad_out expanded from one value
+    F.diff_attention(leaf, k, v, lam).sum().backward()
+    leaf2 = q.clone().requires_grad_()
+    F.diff_attention(leaf2, k, v, lam).backward(torch.ones_like(go))
+    assert torch.equal(leaf.grad, leaf2.grad)
+
+
+@pytest.mark.parametrize('wants', [(0,), (1,), (2,), (3,), (0, 3), (1, 2)])
+def test_attention_gradients_of_some_inputs(wants):
+    ins = [t.to(DEV) for t in attn_inputs(1, 2, 1, 30, 40, 16, 32, torch.float32)]
+    full = [t.clone().requires_grad_() for t in ins[:4]]
+    UF().diff_attention(*full).backward(ins[4])
+    some = [t.clone().requires_grad_(i in wants) for i, t in enumerate(ins[:4])]
+    UF().diff_attention(*some).backward(ins[4])
+    for i in range(4):
+        assert (some[i].grad is None) == (i not in wants)
+        if i in wants:
+            assert torch.equal(some[i].grad, full[i].grad)
+
+
+def test_attention_gradients_against_differences():
+    """<grad, d> against the difference of two forward calls, and both against the reference's own difference"""
+    dt = torch.float32
+    q, k, v, lam, go = attn_inputs(1, 2, 1, 21, 34, 16, 32, dt)
+    ds = [rand(t.shape, torch.float32, 50 + i) for i, t in enumerate((q, k, v, lam))]
+    _, leaves = attn_check(q, k, v, lam, go, dt)
+    eps = 2.0 ** -7
+    for i in range(4):
+        val, ref, err = [], [], []
+        for s in (1, -1):
+            ins = [t + s * eps * ds[i] if j == i else t for j, t in enumerate((q, k, v, lam))]
+            y = UF().diff_attention(*(t.to(DEV) for t in ins))
+            r = Ref(*ins, go, dt)
+            val.append((y.double().cpu() * go.double()).sum().item())
+            ref.append((r.out * go.double()).sum().item())
+            err.append((r.e_out * go.double().abs()).sum().item())
+        assert abs((val[0] - val[1]) - (ref[0] - ref[1])) <= err[0] + err[1]
+        slope = (leaves[i].grad.double().cpu() * ds[i].double()).sum().item() * 2 * eps
+        curve = abs((ref[0] - ref[1]) - slope)                                      # third order in eps: shrinks by 8 when eps halves
+        ins = [[t + s * eps / 2 * ds[i] if j == i else t for j, t in enumerate((q, k, v, lam))] for s in (1, -1)]
+        halfway = [(Ref(*x, go, dt).out * go.double()).sum().item() for x in ins]
+        curve2 = abs((halfway[0] - halfway[1]) - slope / 2)
+        assert curve2 <= curve / 4 + 1e-5 * abs(slope) + 1e-6
+
+
+def test_attention_empty_calls():
+    F = UF()
+    for B, Nq, Nk in ((0, 3, 4), (2, 0, 4), (2, 3, 0)):
+        q, k, v, lam, _ = attn_inputs(B, 2, 1, Nq, Nk, 16, 32, torch.float32)
+        leaves = [t.to(DEV).requires_grad_() for t in (q, k, v, lam)]
+        y = F.diff_attention(*leaves)
+        assert y.shape == (B, Nq, 2, 32) and (y == 0).all()
+        y.sum().backward()
+        assert all(t.grad.shape == t.shape and (t.grad == 0).all() for t in leaves)
+
+
+def test_attention_refusals():
+    F = UF()
+    q, k, v, lam, _ = (t.to(DEV) for t in attn_inputs(2, 4, 2, 9, 11, 16, 32, torch.float32))
+    ok = torch.zeros(9, 11, dtype=torch.bool, device=DEV)
+    for err, kw in ((ValueError, dict(q=q[0])), (ValueError, dict(k=k[:1])), (ValueError, dict(v=v[:, :5])), (ValueError, dict(q=q[:, :, :3])),
+                    (TypeError, dict(q=q.half())), (TypeError, dict(q=q.double(), k=k.double(), v=v.double())),
+                    (ValueError, dict(lam=lam[:3])), (ValueError, dict(lam=lam.long())), (ValueError, dict(attn_mask=ok[:5])),
+                    (ValueError, dict(attn_mask=ok[0])), (TypeError, dict(attn_mask=ok.long())),
+                    (ValueError, dict(attn_mask=ok.float().requires_grad_())), (ValueError, dict(key_padding_mask=ok[:3])),
+                    (ValueError, dict(key_padding_mask=torch.zeros(2, 11, device=DEV))), (ValueError, dict(p=2.0)),
+                    (ValueError, dict(p=0.1, training=True, seed=1 << 63)), (RuntimeError, dict(q=q.cpu())),
+                    (RuntimeError, dict(key_padding_mask=torch.zeros(2, 11, dtype=torch.bool)))):
+        args = dict(dict(q=q, k=k, v=v, lam=lam), **kw)
+        with pytest.raises(err):
+            F.diff_attention(**args)
+    with pytest.raises(ValueError, match='widths'):
+        F.diff_attention(torch.zeros(1, 2, 1, 2, 136, device=DEV), torch.zeros(1, 2, 1, 2, 136, device=DEV), torch.zeros(1, 2, 1, 8, device=DEV), lam[:1])
+
+
+def test_attention_past_32_bit_offsets():
+    """a cache whose second sample and last head begin more than 2^32 elements into the buffer"""
+    B, H, N, Dh, Dv = 2, 2, 300, 16, 32
+    q, k, v, lam, _ = attn_inputs(B, H, H, 4, N, Dh, Dv, torch.bfloat16)
+    want = UF().diff_attention(*(t.to(DEV) for t in (q, k, v, lam)))
+    buf = torch.empty((1 << 32) + (1 << 24), dtype=torch.bfloat16, device=DEV)
+    big = 1 << 32
+    ck = buf.as_strided(k.shape, (big, H * 2 * Dh, 2 * Dh, Dh, 1), 64)
+    cv = buf.as_strided(v.shape, (big, H * Dv, Dv, 1), 1 << 20)
+    ck.copy_(k), cv.copy_(v)
+    assert torch.equal(UF().diff_attention(q.to(DEV), ck, cv, lam.to(DEV)), want)
+
+
+# ------------------------------------------------------------------------------------------------- streams, graphs, the module
+def test_operators_on_another_stream():
+    F = UF()
+    ins = [t.to(DEV) for t in attn_inputs(2, 4, 2, 50, 60, 32, 64, torch.bfloat16)]
+    want = F.diff_attention(*ins[:4], p=0.1, training=True, seed=4)
+    wn = F.dropout(F.layer_norm(want), 0.3, True, identity=want, seed=4)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        got = F.diff_attention(*ins[:4], p=0.1, training=True, seed=4)
+        gn = F.dropout(F.layer_norm(got), 0.3, True, identity=got, seed=4)
+    side.synchronize()
+    assert torch.equal(got, want) and torch.equal(gn, wn)
+
+
+def block(x, w, lam, seed=None):
+    """a decoder block by the operators: attention, head-wise norm, residual dropout, norm"""
+    F = UF()
+    B, N, C = x.shape
+    qkv = (x @ w).view(B, N, 3, 4, C // 4)
+    o = F.diff_attention(qkv[:, :, 0].unflatten(-1, (2, -1)), qkv[:, :, 1].unflatten(-1, (2, -1)), qkv[:, :, 2], lam, p=0.1, training=True,
+                         seed=seed)
+    o = F.layer_norm(o).flatten(2)
+    return F.layer_norm(F.dropout(o, 0.2, True, identity=x, seed=seed))
+
+
+def test_two_captured_graphs_replay_like_the_eager_pass():
+    """forward and backward captured twice; replays of both, with eager work between, give the eager results every time"""
+    gen = torch.Generator().manual_seed(3)
+    data = [torch.randn(2, 33, 64, generator=gen).to(DEV) for _ in range(3)]
+    w0 = (torch.randn(64, 192, generator=gen) / 8).to(DEV)
+    lam0 = torch.full((4,), 0.5, device=DEV)
+    go = torch.randn(2, 33, 64, generator=gen).to(DEV)
+
+    def eager(x):
+        w, lam = w0.clone().requires_grad_(), lam0.clone().requires_grad_()
+        y = block(x, w, lam, seed=6)
+        return [y.detach()] + list(torch.autograd.grad(y, (w, lam), go))
+    want = [eager(x) for x in data]
+    graphs = []
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        eager(data[0])
+    torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    for _ in range(2):
+        x = data[0].clone()
+        w, lam = w0.clone().requires_grad_(), lam0.clone().requires_grad_()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            y = block(x, w, lam, seed=6)
+            grads = torch.autograd.grad(y, (w, lam), go)
+        graphs.append((g, x, [y] + list(grads)))
+    for step in range(6):
+        for i, (g, x, outs) in enumerate(graphs):
+            n = (step + i) % 3
+            x.copy_(data[n])
+            g.replay()
+            torch.cuda.synchronize()
+            for a, b in zip(outs, want[n]):
+                assert torch.equal(a, b), (step, i)
+        again = eager(data[step % 3])
+        assert all(torch.equal(a, b) for a, b in zip(again, want[step % 3]))
+
+
+def test_captured_dropout_follows_the_device_seed_base():
+    F = UF()
+    base = torch.zeros(1, dtype=torch.int64, device=DEV)
+    x = torch.ones(4096, device=DEV)
+    F.set_seed_base(base)
+    try:
+        F.dropout(x, 0.5, True)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            a = F.dropout(x, 0.5, True)
+            b = F.dropout(x, 0.5, True, seed=8)
+        seen = []
+        for n in range(3):
+            base.fill_(n)
+            g.replay()
+            torch.cuda.synchronize()
+            seen.append(a.clone())
+            assert torch.equal(b.double().cpu(), drop_mask(8, 4096, 0.5))             # a given seed stands by itself
+        assert not torch.equal(seen[0], seen[1]) and not torch.equal(seen[1], seen[2])
+        base.fill_(1)
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(a, seen[1])
+    finally:
+        F.set_seed_base(None)
+
+
+def module_reference(m, query, pos, mask, dt=torch.float64):
+    """the module's forward pass in 64 bits on the CPU from its parameters (eval mode)"""
+    P = {n: t.detach().to(dt).cpu() for n, t in m.state_dict().items()}
+    x, xp = query.to(dt), (query + pos).to(dt)
+    if not m.batch_first:
+        x, xp = x.transpose(0, 1), xp.transpose(0, 1)
+    lin = torch.nn.functional.linear
+    B, N, C = x.shape
+    H, dv = m.num_heads, m.head_dims
+    q = lin(xp, P['q_proj.weight'], P['q_proj.bias']).view(B, N, H, 2, dv // 2)
+    k = lin(xp, P['k_proj.weight'], P['k_proj.bias']).view(B, N, -1, 2, dv // 2)
+    v = lin(x, P['v_proj.weight'], P['v_proj.bias']).view(B, N, -1, dv)
+    G = H // k.shape[2]
+    k, v = k.repeat_interleave(G, 2), v.repeat_interleave(G, 2)
+    e = (P['lambda_a'] * P['lambda_b']).sum(-1).exp()
+    lam = e[0] - e[1] + m.lambda_init
+    A = []
+    for i in (0, 1):
+        s = torch.einsum('bqhd,bkhd->bhqk', q[:, :, :, i], k[:, :, :, i]) / math.sqrt(dv // 2)
+        if mask is not None:
+            s = s.masked_fill(mask, -math.inf)
+        A.append(s.softmax(-1))
+    o = torch.einsum('bhqk,bkhd->bqhd', A[0] - lam * A[1], v)
+    o = torch.nn.functional.layer_norm(o, (dv,), P['head_norm.weight'], P['head_norm.bias'], m.head_norm.eps) * (1 - m.lambda_init)
+    out = lin(o.flatten(2), P['out_proj.weight'], P['out_proj.bias']) + (query.to(dt) if m.batch_first else query.to(dt).transpose(0, 1))
+    return out if m.batch_first else out.transpose(0, 1)
+
+
+@pytest.mark.parametrize('batch_first,kv,masked', [(False, None, False), (True, 2, True)])
+def test_module_matches_its_definition(batch_first, kv, masked):
+    """the whole block in f32; its Linears are split-bf16 products (2^-16 of the products' magnitudes each, four in a row), which
+    a head-wise norm of unit variance passes on: 1e-3 of the output's scale"""
+    from unibev_amd import build_attention
+    torch.manual_seed(0)
+    m = build_attention(dict(type='DifferentialAttention', embed_dims=128, num_heads=4, num_kv_heads=kv, dropout=0.1,
+                             batch_first=batch_first)).to(DEV).eval()
+    with torch.no_grad():
+        m.head_norm.weight.uniform_(0.5, 1.5)
+        m.head_norm.bias.uniform_(-0.5, 0.5)
+    shape = (2, 90, 128) if batch_first else (90, 2, 128)
+    x, pos = torch.randn(shape), torch.randn(shape)
+    mask = torch.rand(90, 90) < 0.3 if masked else None
+    y = m(x.to(DEV), query_pos=pos.to(DEV), attn_mask=None if mask is None else mask.to(DEV))
+    ref = module_reference(m, x, pos, mask)
+    assert y.shape == x.shape
+    assert (y.double().cpu() - ref).abs().max().item() <= 1e-3 * ref.abs().max().item()
+
+
+@pytest.mark.parametrize('autocast', [None, torch.bfloat16, torch.float16])
+def test_decoder_runs_with_differential_attention(autocast):
+    """the shipped decoder with the operator in its self-attention slot: a training pass, finite gradients everywhere"""
+    import copy
+    from unibev_amd import configs
+    from unibev_amd.registry import build_transformer_layer_sequence
+    cfg = copy.deepcopy(configs.decoder_cfg(embed_dims=64, num_layers=2))
+    cfg['transformerlayers']['attn_cfgs'][0] = dict(type='DifferentialAttention', embed_dims=64, num_heads=4, dropout=0.1)
+    torch.manual_seed(1)
+    dec = build_transformer_layer_sequence(cfg).to(DEV).train()
+    nq, bs, h, w = 50, 2, 12, 10
+    query, pos = torch.randn(nq, bs, 64, device=DEV), torch.randn(nq, bs, 64, device=DEV)
+    value = torch.randn(h * w, bs, 64, device=DEV)
+    ref = torch.rand(bs, nq, 3, device=DEV)
+    kw = dict(key=None, value=value, query_pos=pos, reference_points=ref, spatial_shapes=torch.tensor([[h, w]], device=DEV),
+              level_start_index=torch.tensor([0], device=DEV))
+    cot = torch.randn(2, nq, bs, 64, device=DEV)
+    for _ in range(2):
+        torch.manual_seed(7)
+        UF().new_step()
+        dec.zero_grad()
+        with torch.autocast('cuda', dtype=autocast, enabled=autocast is not None):
+            states, _ = dec(query, **kw)
+        (states.float() * cot).sum().backward()                                    # (a loss whose gradients f16 can hold)
+        got = {n: p.grad.clone() for n, p in dec.named_parameters() if 'attentions.0' in n}
+        assert got and all(torch.isfinite(g).all() for g in got.values())
+        assert all(g.abs().max() > 0 for n, g in got.items() if 'k_proj.bias' not in n)

@@ -1,0 +1,148 @@
+// Differential attention: what the host passes to the kernels, and the pieces they share.
+//
+//   A_m = softmax_j(scale q_m . k_m + mask), m = 1, 2;     out = (D o (A_1 - lam_h A_2)) v;     a row that sees no key gives 0
+//
+// Rows: the G = H / Hk query heads that share a key / value head are walked as one list of G Nq rows (row r = head r / Nq of
+// the group, query r % Nq), so that shared heads read their keys once and their gradients are sums inside one block.
+//
+// All products run on 32 x 32 MFMA tiles whose output gives a lane ONE item of its own (column lane & 31) and 16 items of
+// the staged tile, rows 8 (i >> 2) + 4 (lane >> 5) + (i & 3).  Forward and grad_q: own = rows, staged = keys; grad_k / grad_v:
+// own = keys, staged = rows.  The second product of each pair contracts over the staged items, whose order does not
+// matter: registers 8 s .. 8 s + 7 of the tile, rounded, ARE its B operand for the 16 staged items of step s (f32: eight
+// operands of one), and the A operand is read transposed from the same staged rows (ds_read_b64_tr_b16).  So no score ever
+// goes through memory or LDS, and the softmax of a row is arithmetic of its own lane and the one 32 lanes away.
+#pragma once
+#include <type_traits>
+
+#include "ubv_common.h"
+
+namespace ubv {
+
+struct DiffAttnArgs {
+  const void *q, *k, *v, *go;              // [B, N, heads, (2,) D] with element strides below, D contiguous
+  int64_t qs[4], ks[4], vs[3], gs[3];      // batch, token, head, map
+  const float* lam;                        // [H]
+  const uint8_t* kpm;                      // [B, Nk] contiguous, nonzero hides the key; or null
+  const void* mask;                        // element strides ms; kind 0: none, 1: bytes (nonzero hides), 2: f32 (added)
+  int64_t ms[4];
+  int mask_kind, causal;
+  int B, H, Hk, G, Nq, Nk, Dh, Dv, R;      // R = G Nq rows of a group
+  float scale;
+  uint32_t t16;                            // dropout threshold of a 16-bit field, 0: none
+  float up;
+  uint64_t seed;
+  const uint64_t* seed_dev;
+  int n4;                                  // ceil(Nk / 4) field groups per row
+  void* out;                               // [B, Nq, H, Dv] contiguous
+  float* lse;                              // [2][B H Nq] log2-sum-exp2 of the scores in units of log 2; -inf: empty row
+  float* o;                                // [2][B H Nq][Dv] the two maps' normalised products (D's scale included)
+  float* del;                              // [2][B H Nq] grad_out . o_m
+  float* dlrow;                            // [B H Nq] sum_j A_2 G
+  void *gq, *gk, *gv;                      // contiguous gradients
+};
+
+// f16 holds nothing below 2^-24 and loses bits below 2^-14, which the probabilities of a long row reach: they enter the matrix
+// instructions 2^8 larger and their products leave 2^8 smaller (|lam| up to 255 stays in range)
+template <typename T> constexpr float kProbShift = std::is_same<T, f16_t>::value ? 8.0f : 0.0f;
+template <typename T> constexpr float kProbScale = std::is_same<T, f16_t>::value ? 256.0f : 1.0f;
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kNegInf = -__builtin_inff();
+
+typedef __attribute__((ext_vector_type(16))) float af32x16_t;
+typedef __attribute__((ext_vector_type(4))) uint32_t au32x4_t;
+typedef __attribute__((ext_vector_type(2))) uint32_t au32x2_t;
+typedef __attribute__((ext_vector_type(8))) __bf16 abf16x8_t;
+typedef __attribute__((ext_vector_type(8))) _Float16 af16x8_t;
+typedef __attribute__((ext_vector_type(4))) short ai16x4_t;
+
+// ---- one 16-deep step of a 32 x 32 product: a lane holds items 8 (lane >> 5) + 0 .. 7 of the contraction -------------------
+template <typename T> struct amma {                       // 16-bit types: one MFMA
+  struct frag { au32x4_t d; };
+  static __device__ __forceinline__ af32x16_t mul(const frag& a, const frag& b, af32x16_t c) {
+    if constexpr (std::is_same<T, f16_t>::value)
+      return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(af16x8_t, a.d), __builtin_bit_cast(af16x8_t, b.d), c, 0, 0, 0);
+    else
+      return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(abf16x8_t, a.d), __builtin_bit_cast(abf16x8_t, b.d), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ frag load(const T* p) { return {*reinterpret_cast<const au32x4_t*>(p)}; }   // 16-byte aligned
+  // rounding to the inputs' type: the matrix instruction takes no wider operand; half a step of each probability, random
+  static __device__ __forceinline__ frag pack(const float* p) {
+    frag f;
+    if constexpr (std::is_same<T, f16_t>::value) {
+      af16x8_t h;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) h[i] = (_Float16)p[i];
+      f.d = __builtin_bit_cast(au32x4_t, h);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) f.d[i] = cvt_pk_bf16(p[2 * i], p[2 * i + 1]);
+    }
+    return f;
+  }
+  // column n0 + (lane & 31) of staged rows k0 + 8 (j >> 2) + 4 (lane >> 5) + (j & 3), j = 0 .. 7
+  template <int LD> static __device__ __forceinline__ frag load_tr(const T* tile, int k0, int n0, int lane) {
+    typedef __attribute__((address_space(3))) ai16x4_t lds_v4;
+    const T* p = tile + (k0 + 4 * (lane >> 5) + ((lane & 15) >> 2)) * LD + n0 + (lane & 16) + 4 * (lane & 3);
+    const ai16x4_t a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4*)p);
+    const ai16x4_t b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4*)(p + 8 * LD));
+    const au32x2_t ua = __builtin_bit_cast(au32x2_t, a), ub = __builtin_bit_cast(au32x2_t, b);
+    return {au32x4_t{ua.x, ua.y, ub.x, ub.y}};
+  }
+};
+template <> struct amma<float> {                          // f32: eight MFMAs of depth 2 (lane halves), IEEE products
+  struct frag { float d[8]; };
+  static __device__ __forceinline__ af32x16_t mul(const frag& a, const frag& b, af32x16_t c) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a.d[j], b.d[j], c, 0, 0, 0);
+    return c;
+  }
+  static __device__ __forceinline__ frag load(const float* p) {
+    frag f;
+    *reinterpret_cast<float4*>(f.d) = *reinterpret_cast<const float4*>(p);
+    *reinterpret_cast<float4*>(f.d + 4) = *reinterpret_cast<const float4*>(p + 4);
+    return f;
+  }
+  static __device__ __forceinline__ frag pack(const float* p) {
+    frag f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f.d[i] = p[i];
+    return f;
+  }
+  template <int LD> static __device__ __forceinline__ frag load_tr(const float* tile, int k0, int n0, int lane) {
+    frag f;
+    const float* p = tile + (k0 + 4 * (lane >> 5)) * LD + n0 + (lane & 31);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f.d[j] = p[(8 * (j >> 2) + (j & 3)) * LD];
+    return f;
+  }
+};
+
+__device__ __forceinline__ int tile_item(int i, int lane) { return 8 * (i >> 2) + 4 * (lane >> 5) + (i & 3); }
+
+__device__ __forceinline__ float aexp2(float x) { return __builtin_amdgcn_exp2f(x); }      // v_exp_f32: 1 ulp, 0 below 2^-126
+
+// value of the lane of the other half (lane ^ 32)
+__device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32, 64); }
+
+// registers of a 16-byte row piece from global memory, 0 where !ok
+__device__ __forceinline__ au32x4_t piece(const void* p, bool ok) {
+  au32x4_t z = {0u, 0u, 0u, 0u};
+  return ok ? *reinterpret_cast<const au32x4_t*>(p) : z;
+}
+
+// additive mask value in log2 units: a finite value stays finite (the type's lowest value hides nothing by itself: a row of
+// it alone is a uniform row), -inf hides
+__device__ __forceinline__ float mask_log2(float m) { return m == kNegInf ? kNegInf : fmaxf(m * kLog2e, -3.0e38f); }
+
+// what the call's masks add to the score (log2 units) of query i of head h against key j: -inf hides; `j` in range
+__device__ __forceinline__ float mask_bias(const DiffAttnArgs& a, int b, int h, int i, int j) {
+  if (a.causal && j > i + (a.Nk - a.Nq)) return kNegInf;
+  if (a.kpm != nullptr && a.kpm[(int64_t)b * a.Nk + j]) return kNegInf;
+  if (a.mask_kind == 0) return 0.0f;
+  const int64_t o = b * a.ms[0] + h * a.ms[1] + i * a.ms[2] + j * a.ms[3];
+  if (a.mask_kind == 1) return ((const uint8_t*)a.mask)[o] ? kNegInf : 0.0f;
+  return mask_log2(((const float*)a.mask)[o]);
+}
+
+}  // namespace ubv

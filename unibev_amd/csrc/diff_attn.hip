@@ -1,0 +1,91 @@
+// C entries of differential attention: argument checks and the dispatch by element type (kernels: diff_attn.inl).
+#include "diff_attn.h"
+
+namespace ubv {
+int diff_attn_forward_f32(const DiffAttnArgs&, hipStream_t);
+int diff_attn_forward_f16(const DiffAttnArgs&, hipStream_t);
+int diff_attn_forward_bf16(const DiffAttnArgs&, hipStream_t);
+int diff_attn_backward_f32(const DiffAttnArgs&, float*, hipStream_t);
+int diff_attn_backward_f16(const DiffAttnArgs&, float*, hipStream_t);
+int diff_attn_backward_bf16(const DiffAttnArgs&, float*, hipStream_t);
+
+// what forward and backward share: shapes, strides (in elements: q 4, k 4, v 3, grad_out 3, mask 4), masks, dropout
+static int attn_args(DiffAttnArgs& a, const void* q, const void* k, const void* v, const float* lam, const uint8_t* kpm,
+                     const void* mask, int mask_kind, const int64_t* strides, int B, int H, int Hk, int Nq, int Nk, int Dh, int Dv,
+                     float scale, int causal, float p, uint64_t seed, const uint64_t* seed_dev, int dtype, const char* who) {
+  UBV_CHECK_ARG(q && k && v && lam && strides, "%s: null pointer", who);
+  UBV_CHECK_ARG(dtype >= 0 && dtype <= 2, "%s: unknown dtype %d", who, dtype);
+  UBV_CHECK_ARG(B > 0 && H > 0 && Hk > 0 && Nq > 0 && Nk > 0, "%s: empty shape B=%d H=%d Hk=%d Nq=%d Nk=%d", who, B, H, Hk, Nq, Nk);
+  UBV_CHECK_ARG(H % Hk == 0, "%s: %d query heads do not share %d key heads evenly", who, H, Hk);
+  UBV_CHECK_ARG(Dh > 0 && Dh <= 128 && Dv > 0 && Dv <= 256, "%s: head widths %d (at most 128) and %d (at most 256)", who, Dh, Dv);
+  UBV_CHECK_ARG((int64_t)(H / Hk) * Nq < (int64_t(1) << 31) - 256 && Nk < (1 << 31) - 256 && (int64_t)B * H < (int64_t(1) << 31),
+                "%s: Nq=%d x %d heads or Nk=%d out of range", who, Nq, H / Hk, Nk);
+  UBV_CHECK_ARG(p >= 0.0f && p <= 1.0f, "%s: p = %g must be in [0, 1]", who, (double)p);
+  UBV_CHECK_ARG(mask_kind >= 0 && mask_kind <= 2 && (mask_kind == 0) == (mask == nullptr), "%s: mask kind %d", who, mask_kind);
+  const int vec = dtype == UBV_F32 ? 4 : 8;
+  for (int n = 0; n < 14; ++n)
+    UBV_CHECK_ARG(strides[n] % vec == 0, "%s: stride %ld is no multiple of 16 bytes", who, (long)strides[n]);
+  UBV_CHECK_ARG(((uintptr_t)q | (uintptr_t)k | (uintptr_t)v) % 16 == 0, "%s: operands must be 16-byte aligned", who);
+  a = DiffAttnArgs{};
+  a.q = q; a.k = k; a.v = v; a.lam = lam; a.kpm = kpm; a.mask = mask; a.mask_kind = mask_kind;
+  for (int n = 0; n < 4; ++n) { a.qs[n] = strides[n]; a.ks[n] = strides[4 + n]; a.ms[n] = strides[14 + n]; }
+  for (int n = 0; n < 3; ++n) { a.vs[n] = strides[8 + n]; a.gs[n] = strides[11 + n]; }
+  a.B = B; a.H = H; a.Hk = Hk; a.G = H / Hk; a.Nq = Nq; a.Nk = Nk; a.Dh = Dh; a.Dv = Dv; a.R = a.G * Nq;
+  a.scale = scale; a.causal = causal != 0; a.n4 = (Nk + 3) / 4;
+  drop_params16(p, a.t16, a.up);
+  a.seed = seed; a.seed_dev = seed_dev;
+  return UBV_OK;
+}
+}  // namespace ubv
+
+extern "C" int ubv_diff_attention_forward(const void* q, const void* k, const void* v, const float* lam, const uint8_t* key_padding_mask,
+                                          const void* mask, int mask_kind, void* out, float* lse, float* maps,
+                                          const int64_t* strides, int B, int H, int Hk, int Nq, int Nk, int Dh, int Dv, float scale,
+                                          int causal, float p, uint64_t seed, const uint64_t* seed_dev, int dtype, void* stream) {
+  using namespace ubv;
+  DiffAttnArgs a;
+  const int rc = attn_args(a, q, k, v, lam, key_padding_mask, mask, mask_kind, strides, B, H, Hk, Nq, Nk, Dh, Dv, scale, causal, p, seed,
+                           seed_dev, dtype, "diff_attention_forward");
+  if (rc) return rc;
+  UBV_CHECK_ARG(out && (uintptr_t)out % 16 == 0 && (uintptr_t)maps % 16 == 0 && (lse == nullptr) == (maps == nullptr),
+                "diff_attention_forward: out, or lse without maps");
+  a.out = out; a.lse = lse; a.o = maps;
+  hipStream_t st = as_stream(stream);
+  switch (dtype) {
+    case UBV_F32: return diff_attn_forward_f32(a, st);
+    case UBV_F16: return diff_attn_forward_f16(a, st);
+    default: return diff_attn_forward_bf16(a, st);
+  }
+}
+
+extern "C" int64_t ubv_diff_attention_backward_workspace(int B, int H, int Nq) {
+  return B <= 0 || H <= 0 || Nq <= 0 ? 0 : 3 * (int64_t)B * H * Nq * 4;
+}
+
+extern "C" int ubv_diff_attention_backward(const void* grad_out, const void* q, const void* k, const void* v, const float* lam,
+                                           const uint8_t* key_padding_mask, const void* mask, int mask_kind, const float* lse,
+                                           const float* maps, void* grad_q, void* grad_k, void* grad_v, float* grad_lam,
+                                           const int64_t* strides, int B, int H, int Hk, int Nq, int Nk, int Dh, int Dv, float scale,
+                                           int causal, float p, uint64_t seed, const uint64_t* seed_dev, int dtype, void* workspace,
+                                           int64_t workspace_bytes, void* stream) {
+  using namespace ubv;
+  DiffAttnArgs a;
+  const int rc = attn_args(a, q, k, v, lam, key_padding_mask, mask, mask_kind, strides, B, H, Hk, Nq, Nk, Dh, Dv, scale, causal, p, seed,
+                           seed_dev, dtype, "diff_attention_backward");
+  if (rc) return rc;
+  UBV_CHECK_ARG(grad_out && lse && maps && (uintptr_t)grad_out % 16 == 0, "diff_attention_backward: grad_out, lse or maps");
+  UBV_CHECK_ARG((grad_k == nullptr) == (grad_v == nullptr), "diff_attention_backward: grad_k and grad_v come together");
+  UBV_CHECK_ARG(((uintptr_t)grad_q | (uintptr_t)grad_k | (uintptr_t)grad_v) % 16 == 0, "diff_attention_backward: gradients must be 16-byte aligned");
+  UBV_CHECK_ARG(workspace && (uintptr_t)workspace % 4 == 0 && workspace_bytes >= ubv_diff_attention_backward_workspace(B, H, Nq),
+                "diff_attention_backward: the workspace is too small (%ld bytes)", (long)workspace_bytes);
+  const int64_t rows = (int64_t)B * H * Nq;
+  a.go = grad_out; a.lse = const_cast<float*>(lse); a.o = const_cast<float*>(maps);
+  a.gq = grad_q; a.gk = grad_k; a.gv = grad_v;
+  a.del = (float*)workspace; a.dlrow = a.del + 2 * rows;
+  hipStream_t st = as_stream(stream);
+  switch (dtype) {
+    case UBV_F32: return diff_attn_backward_f32(a, grad_lam, st);
+    case UBV_F16: return diff_attn_backward_f16(a, grad_lam, st);
+    default: return diff_attn_backward_bf16(a, grad_lam, st);
+  }
+}

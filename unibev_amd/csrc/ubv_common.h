@@ -259,4 +259,10 @@ static inline void drop_params(float p, uint32_t& thresh, float& scale) {
   scale = 1.0f / (1.0f - p);
 }
 
+// p as a 16-bit threshold (rounded) and the scale that keeps E[mask] = 1 at this resolution; p = 1 keeps nothing
+static inline void drop_params16(float p, uint32_t& t16, float& scale) {
+  t16 = (uint32_t)((double)p * 65536.0 + 0.5);
+  scale = t16 >= 65536u ? 0.0f : (float)(65536.0 / (65536.0 - (double)t16));
+}
+
 }  // namespace ubv

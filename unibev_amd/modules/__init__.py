@@ -3,6 +3,7 @@ from .bricks import (FFN, BaseModule, BaseTransformerLayer, DetrTransformerDecod
 from .decoder import DetectionTransformerDecoder  # noqa
 from .deform_attn import (CustomMSDeformableAttention, MSDeformableAttention3DImg,  # noqa
                           MSDeformableAttention3DPts, MultiScaleDeformableAttention)
+from .diff_attn import DifferentialAttention  # noqa
 from .head import UniBEV_Head, inverse_sigmoid  # noqa
 from .encoders import ImgEncoder, ImgLayer, PtsEncoder, PtsLayer  # noqa
 from .sca import SpatialCrossAttentionImg, SpatialCrossAttentionPts  # noqa
