@@ -702,24 +702,26 @@ int ubv_layer_norm_backward(const void* grad_y, const void* x, const float* gamm
  * key gives a zero row (and zero gradients).
  *   q [B, Nq, H, 2, Dh], k [B, Nk, Hk, 2, Dh], v [B, Nk, Hk, Dv] of dtype, lam [H] f32.  Query head h reads key / value head
  *   h / (H / Hk).  Dh <= 128, Dv <= 256, the last axis contiguous and readable up to the next multiple of 16 bytes (zeros there);
- *   16-byte aligned, other strides multiples of 16 bytes.
+ *   16-byte aligned, other strides multiples of 16 bytes, token strides below 16 MiB, map strides below 256 MiB.  scale > 0.
  *   strides (HOST, elements): q batch, token, head, map | k the same | v batch, token, head | grad_out batch, token, head
  *   (forward: 0) | mask batch, head, query, key.
  *   key_padding_mask [B, Nk] bytes or NULL: nonzero hides the key from every query; what k and v hold there is never used.
  *   mask_kind 0: mask NULL; 1: bytes, nonzero hides; 2: f32, added to the scaled scores (-inf hides).
  *   causal: query i sees keys j <= i + Nk - Nq.
  *   D as in ubv_dropout over the map: key j of row r = (b H + h) Nq + i is field j % 4 of group r ceil(Nk / 4) + j / 4.
- *   out [B, Nq, H, Dv] contiguous; lse f32 [2, B, H, Nq] and maps f32 [2, B, H, Nq, Dv] (the two maps' products) are written for
- *   the backward pass, or both NULL.
+ *   out [B, Nq, H, Dv] contiguous; stat f32 [B, H, Nq, 4] (the softmax sums) and maps f32 [2, B, H, Nq, Dv] (the two maps'
+ *   products) are written for the backward pass, or both NULL.  workspace: ubv_diff_attention_forward_workspace bytes let few
+ *   queries share many keys' blocks; with less (or NULL) fewer blocks do.
  * Backward: grad_q / grad_k / grad_v contiguous in the shapes of q, k, v, grad_lam f32 [H]; grad_q and grad_lam each or NULL,
  * grad_k and grad_v both or neither.  No atomics: the same bits on every run. */
 int ubv_diff_attention_forward(const void* q, const void* k, const void* v, const float* lam, const uint8_t* key_padding_mask,
-                               const void* mask, int mask_kind, void* out, float* lse, float* maps, const int64_t* strides, int B,
+                               const void* mask, int mask_kind, void* out, float* stat, float* maps, const int64_t* strides, int B,
                                int H, int Hk, int Nq, int Nk, int Dh, int Dv, float scale, int causal, float p, uint64_t seed,
-                               const uint64_t* seed_dev, int dtype, void* stream);
+                               const uint64_t* seed_dev, int dtype, void* workspace, int64_t workspace_bytes, void* stream);
+int64_t ubv_diff_attention_forward_workspace(int B, int H, int Hk, int Nq, int Nk, int Dv);
 int64_t ubv_diff_attention_backward_workspace(int B, int H, int Nq);
 int ubv_diff_attention_backward(const void* grad_out, const void* q, const void* k, const void* v, const float* lam,
-                                const uint8_t* key_padding_mask, const void* mask, int mask_kind, const float* lse,
+                                const uint8_t* key_padding_mask, const void* mask, int mask_kind, const float* stat,
                                 const float* maps, void* grad_q, void* grad_k, void* grad_v, float* grad_lam,
                                 const int64_t* strides, int B, int H, int Hk, int Nq, int Nk, int Dh, int Dv, float scale, int causal,
                                 float p, uint64_t seed, const uint64_t* seed_dev, int dtype, void* workspace,

@@ -42,17 +42,18 @@ def test_layer_norm_entries_refuse():
     refused(b(P, P, None, P, P, P, P, P, 4, 4, 0, P, need - 1, None), 'workspace')
 
 
-def attn_call(q=P, k=P, v=P, lam=P, mask=None, kind=0, out=P, lse=None, maps=None, strides=None, B=1, H=4, Hk=2, Nq=8, Nk=8, Dh=32,
-              Dv=64, p=0.0, dtype=0):
+def attn_call(q=P, k=P, v=P, lam=P, mask=None, kind=0, out=P, stat=None, maps=None, strides=None, B=1, H=4, Hk=2, Nq=8, Nk=8, Dh=32,
+              Dv=64, p=0.0, dtype=0, scale=0.1):
     s = strides if strides is not None else [0] * 18
-    return _lib.lib().ubv_diff_attention_forward(q, k, v, lam, None, mask, kind, out, lse, maps, (ctypes.c_int64 * 18)(*s), B, H, Hk, Nq,
-                                                 Nk, Dh, Dv, 0.1, 0, p, 0, None, dtype, None)
+    return _lib.lib().ubv_diff_attention_forward(q, k, v, lam, None, mask, kind, out, stat, maps, (ctypes.c_int64 * 18)(*s), B, H, Hk, Nq,
+                                                 Nk, Dh, Dv, scale, 0, p, 0, None, dtype, None, 0, None)
 
 
 @pytest.mark.parametrize('kw,word', [(dict(q=None), 'null'), (dict(lam=None), 'null'), (dict(dtype=3), 'dtype'), (dict(Nq=0), 'empty'),
                                      (dict(Hk=3), 'share'), (dict(Dh=129), 'widths'), (dict(Dv=257), 'widths'), (dict(p=-0.1), 'p = '),
                                      (dict(kind=1), 'mask kind'), (dict(mask=P, kind=3), 'mask kind'), (dict(out=None), 'out'),
-                                     (dict(lse=P), 'maps'), (dict(q=ctypes.c_void_p((1 << 20) + 2)), 'aligned'),
+                                     (dict(stat=P), 'maps'), (dict(scale=0.0), 'scale'), (dict(scale=float('nan')), 'scale'),
+                                     (dict(strides=[0, 1 << 22] + [0] * 16), 'token stride'), (dict(strides=[0] * 7 + [1 << 26] + [0] * 10), 'map stride'), (dict(q=ctypes.c_void_p((1 << 20) + 2)), 'aligned'),
                                      (dict(strides=[0] * 5 + [6] + [0] * 12), '16 bytes'), (dict(Nq=1 << 30, H=8, Hk=2), 'out of range')])
 def test_attention_forward_entry_refuses(kw, word):
     refused(attn_call(**kw), word)
@@ -63,12 +64,12 @@ def test_attention_backward_entry_refuses():
     need = _lib.lib().ubv_diff_attention_backward_workspace(1, 4, 8)
     s = (ctypes.c_int64 * 18)()
 
-    def call(go=P, lse=P, gq=P, gk=P, gv=P, ws=P, n=need):
-        return f(go, P, P, P, P, None, None, 0, lse, P, gq, gk, gv, P, s, 1, 4, 2, 8, 8, 32, 64, 0.1, 0, 0.0, 0, None, 0, ws, n, None)
+    def call(go=P, stat=P, gq=P, gk=P, gv=P, ws=P, n=need):
+        return f(go, P, P, P, P, None, None, 0, stat, P, gq, gk, gv, P, s, 1, 4, 2, 8, 8, 32, 64, 0.1, 0, 0.0, 0, None, 0, ws, n, None)
 
     assert need > 0 and _lib.lib().ubv_diff_attention_backward_workspace(0, 4, 8) == 0
     refused(call(go=None), 'grad_out')
-    refused(call(lse=None), 'lse')
+    refused(call(stat=None), 'stat')
     refused(call(gv=None), 'come together')
     refused(call(gq=ctypes.c_void_p((1 << 20) + 4)), 'aligned')
     refused(call(n=need - 1), 'workspace')

@@ -451,6 +451,11 @@ def test_attention_masks(kind, dt):
         y = UF().diff_attention(*(t.to(DEV) for t in (q, k, v, lam)), attn_mask=kw['attn_mask'].to(DEV))
         rows = ~m.all(-1)
         _within(y.double().cpu()[:, rows], q64.out[:, rows], q64.e_out[:, rows], 'rows with a key')
+        # and behind such rows: A is 1 / Nk exactly, del = G's mean; grad_q is far from zero where a probability would be lost
+        leaves = [t.to(DEV).requires_grad_() for t in (q, k, v, lam)]
+        UF().diff_attention(*leaves, attn_mask=kw['attn_mask'].to(DEV)).backward(go.to(DEV))
+        free = Ref(torch.zeros_like(q), k, v, lam, go, dt)                                   # equal scores: the same uniform rows
+        _within(leaves[0].grad.double().cpu()[:, ~rows], free.q[:, ~rows], free.eq[:, ~rows], 'grad_q of rows of the lowest value')
         flat = (1 - lam.double()).view(1, 1, H, 1) * v.double().mean(1, keepdim=True).repeat_interleave(H // Hk, 2)
         e = (half(dt) + 80 * U) * (1 + lam.double().abs()).view(1, 1, H, 1) * v.double().abs().mean(1, keepdim=True).repeat_interleave(H // Hk, 2)
         _within(y.double().cpu()[:, ~rows], flat.expand(B, int((~rows).sum()), H, -1), (e + half(dt) * flat.abs()).expand(B, int((~rows).sum()), H, -1),

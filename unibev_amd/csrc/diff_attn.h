@@ -27,18 +27,21 @@ struct DiffAttnArgs {
   int64_t ms[4];
   int mask_kind, causal;
   int B, H, Hk, G, Nq, Nk, Dh, Dv, R;      // R = G Nq rows of a group
-  float scale;
+  float scale;                             // > 0
   uint32_t t16;                            // dropout threshold of a 16-bit field, 0: none
-  float up;
+  float up;                                // scale of what dropout keeps
   uint64_t seed;
   const uint64_t* seed_dev;
   int n4;                                  // ceil(Nk / 4) field groups per row
   void* out;                               // [B, Nq, H, Dv] contiguous
-  float* lse;                              // [2][B H Nq] log2-sum-exp2 of the scores in units of log 2; -inf: empty row
+  float4* stat;                            // [B H Nq] {a_1, l_1, a_2, l_2}: see row_probability
   float* o;                                // [2][B H Nq][Dv] the two maps' normalised products (D's scale included)
-  float* del;                              // [2][B H Nq] grad_out . o_m
-  float* dlrow;                            // [B H Nq] sum_j A_2 G
+  float4* row;                             // [B H Nq] {A_1, A_2, del_1, del_2}, del_m = grad_out . o_m
+  float2* rowl;                            // [B H Nq] {l_1, l_2}, with a float mask only
+  float* dlrow;                            // [B H Nq] - sum_j A_2 G
   void *gq, *gk, *gv;                      // contiguous gradients
+  int splits;                              // forward: blocks that share a row tile's keys, 1: none
+  float* part;                             // forward, splits > 1: [splits][tiles][(4 + DV) 64] maxima, sums, products
 };
 
 // f16 holds nothing below 2^-24 and loses bits below 2^-14, which the probabilities of a long row reach: they enter the matrix
@@ -122,27 +125,47 @@ __device__ __forceinline__ int tile_item(int i, int lane) { return 8 * (i >> 2) 
 
 __device__ __forceinline__ float aexp2(float x) { return __builtin_amdgcn_exp2f(x); }      // v_exp_f32: 1 ulp, 0 below 2^-126
 
-// value of the lane of the other half (lane ^ 32)
-__device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32, 64); }
-
-// registers of a 16-byte row piece from global memory, 0 where !ok
-__device__ __forceinline__ au32x4_t piece(const void* p, bool ok) {
-  au32x4_t z = {0u, 0u, 0u, 0u};
-  return ok ? *reinterpret_cast<const au32x4_t*>(p) : z;
+// v and the value of the lane 32 away, joined
+__device__ __forceinline__ float half_max(float v) {
+  const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+}
+__device__ __forceinline__ float half_sum(float v) {
+  const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(s[0]) + __uint_as_float(s[1]);
 }
 
-// additive mask value in log2 units: a finite value stays finite (the type's lowest value hides nothing by itself: a row of
-// it alone is a uniform row), -inf hides
-__device__ __forceinline__ float mask_log2(float m) { return m == kNegInf ? kNegInf : fmaxf(m * kLog2e, -3.0e38f); }
-
-// what the call's masks add to the score (log2 units) of query i of head h against key j: -inf hides; `j` in range
-__device__ __forceinline__ float mask_bias(const DiffAttnArgs& a, int b, int h, int i, int j) {
-  if (a.causal && j > i + (a.Nk - a.Nq)) return kNegInf;
-  if (a.kpm != nullptr && a.kpm[(int64_t)b * a.Nk + j]) return kNegInf;
-  if (a.mask_kind == 0) return 0.0f;
-  const int64_t o = b * a.ms[0] + h * a.ms[1] + i * a.ms[2] + j * a.ms[3];
-  if (a.mask_kind == 1) return ((const uint8_t*)a.mask)[o] ? kNegInf : 0.0f;
-  return mask_log2(((const float*)a.mask)[o]);
+// 16 bytes at base + off + soff; 0 from an offset past 2^31 (the buffer descriptor's bound), which kOutside is
+constexpr uint32_t kOutside = 0x80000000u;
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t attn_rsrc(const void* base) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, 0x7fffffff, 0x00027000);
 }
+__device__ __forceinline__ au32x4_t attn_piece(__amdgpu_buffer_rsrc_t r, uint32_t off, uint32_t soff) {
+  return __builtin_bit_cast(au32x4_t, __builtin_amdgcn_raw_buffer_load_b128(r, off, soff, 0));
+}
+
+// A row's probability of raw score x (q . k, a float mask added over scale), c = scale log2 e.  Without a float mask
+// a = log2 of the row's sum (its reference included) and one fma serves.  A float mask may hold the type's lowest value, beside
+// which a f32 product loses the score: there the reference a is subtracted first (raw) and l is log2 of the sum.
+// A row that sees no key: without a float mask a = +inf, with one a = 0 and l = +inf; both give 0.
+__device__ __forceinline__ float row_probability(bool fm, float x, float c, float a, float l) {
+  return fm ? aexp2(fmaf(x - a, c, -l)) : aexp2(fmaf(x, c, -a));
+}
+
+// what a float mask adds to a raw score: a finite value stays finite (the lowest value alone hides nothing: a row of it is a
+// uniform row), -inf hides
+__device__ __forceinline__ float mask_raw(float m, float rscale) {
+  const float v = m * rscale;
+  return m == kNegInf ? kNegInf : v < -3.0e38f ? -3.0e38f : v > 3.0e38f ? 3.0e38f : v;
+}
+__device__ __forceinline__ float mask_add(float x, float bias) { return bias == kNegInf ? kNegInf : x + bias; }
+
+// 64 bits of the dropout generator from seed's part and a group's number (drop_mix64 of the two)
+__device__ __forceinline__ uint64_t attn_seed(uint64_t seed, const uint64_t* dev) {
+  return (seed + (dev != nullptr ? *dev : 0)) * 0x9E3779B97F4A7C15ull;
+}
+__device__ __forceinline__ uint64_t attn_mix(uint64_t z) { return drop_mix64(0, z); }
+// field e of a group's bits against the threshold in the upper half of a word
+__device__ __forceinline__ bool attn_keep(uint32_t word, int odd, uint32_t t32) { return (odd ? word : word << 16) >= t32; }
 
 }  // namespace ubv

@@ -2,9 +2,9 @@
 #include "diff_attn.h"
 
 namespace ubv {
-int diff_attn_forward_f32(const DiffAttnArgs&, hipStream_t);
-int diff_attn_forward_f16(const DiffAttnArgs&, hipStream_t);
-int diff_attn_forward_bf16(const DiffAttnArgs&, hipStream_t);
+int diff_attn_forward_f32(const DiffAttnArgs&, void*, int64_t, hipStream_t);
+int diff_attn_forward_f16(const DiffAttnArgs&, void*, int64_t, hipStream_t);
+int diff_attn_forward_bf16(const DiffAttnArgs&, void*, int64_t, hipStream_t);
 int diff_attn_backward_f32(const DiffAttnArgs&, float*, hipStream_t);
 int diff_attn_backward_f16(const DiffAttnArgs&, float*, hipStream_t);
 int diff_attn_backward_bf16(const DiffAttnArgs&, float*, hipStream_t);
@@ -21,10 +21,16 @@ static int attn_args(DiffAttnArgs& a, const void* q, const void* k, const void* 
   UBV_CHECK_ARG((int64_t)(H / Hk) * Nq < (int64_t(1) << 31) - 256 && Nk < (1 << 31) - 256 && (int64_t)B * H < (int64_t(1) << 31),
                 "%s: Nq=%d x %d heads or Nk=%d out of range", who, Nq, H / Hk, Nk);
   UBV_CHECK_ARG(p >= 0.0f && p <= 1.0f, "%s: p = %g must be in [0, 1]", who, (double)p);
+  UBV_CHECK_ARG(scale > 0.0f && scale < 1.0e30f, "%s: scale %g must be positive and finite", who, (double)scale);
   UBV_CHECK_ARG(mask_kind >= 0 && mask_kind <= 2 && (mask_kind == 0) == (mask == nullptr), "%s: mask kind %d", who, mask_kind);
   const int vec = dtype == UBV_F32 ? 4 : 8;
   for (int n = 0; n < 14; ++n)
     UBV_CHECK_ARG(strides[n] % vec == 0, "%s: stride %ld is no multiple of 16 bytes", who, (long)strides[n]);
+  const int size = 16 / vec;                 // a staged tile is reached with 32-bit offsets from its first row
+  for (int n : {1, 5, 9, 12})
+    UBV_CHECK_ARG(strides[n] >= 0 && strides[n] * size < (1 << 24), "%s: token stride %ld is negative or over 16 MiB", who, (long)strides[n]);
+  for (int n : {3, 7})
+    UBV_CHECK_ARG(strides[n] >= 0 && strides[n] * size < (1 << 28), "%s: map stride %ld is negative or over 256 MiB", who, (long)strides[n]);
   UBV_CHECK_ARG(((uintptr_t)q | (uintptr_t)k | (uintptr_t)v) % 16 == 0, "%s: operands must be 16-byte aligned", who);
   a = DiffAttnArgs{};
   a.q = q; a.k = k; a.v = v; a.lam = lam; a.kpm = kpm; a.mask = mask; a.mask_kind = mask_kind;
@@ -38,32 +44,42 @@ static int attn_args(DiffAttnArgs& a, const void* q, const void* k, const void* 
 }
 }  // namespace ubv
 
+extern "C" int64_t ubv_diff_attention_forward_workspace(int B, int H, int Hk, int Nq, int Nk, int Dv) {
+  // the partial sums of the most splits that attn_forward takes: 2 kAttnFill blocks of 32 rows' (4 + width) floats
+  if (B <= 0 || Hk <= 0 || H % Hk != 0 || Nq <= 0 || Nk < 256) return 0;
+  const int64_t blocks = (int64_t)B * Hk * (((int64_t)(H / Hk) * Nq + 31) / 32), splits = (1024 + blocks - 1) / blocks;
+  const int64_t most = (Nk + 31) / 32 / 4, width = Dv <= 32 ? 32 : Dv <= 64 ? 64 : Dv <= 128 ? 128 : 256;
+  return blocks >= 256 ? 0 : blocks * (splits < most ? splits : most) * (4 + width) * 64 * 4;
+}
+
 extern "C" int ubv_diff_attention_forward(const void* q, const void* k, const void* v, const float* lam, const uint8_t* key_padding_mask,
-                                          const void* mask, int mask_kind, void* out, float* lse, float* maps,
+                                          const void* mask, int mask_kind, void* out, float* stat, float* maps,
                                           const int64_t* strides, int B, int H, int Hk, int Nq, int Nk, int Dh, int Dv, float scale,
-                                          int causal, float p, uint64_t seed, const uint64_t* seed_dev, int dtype, void* stream) {
+                                          int causal, float p, uint64_t seed, const uint64_t* seed_dev, int dtype, void* workspace,
+                                          int64_t workspace_bytes, void* stream) {
   using namespace ubv;
   DiffAttnArgs a;
   const int rc = attn_args(a, q, k, v, lam, key_padding_mask, mask, mask_kind, strides, B, H, Hk, Nq, Nk, Dh, Dv, scale, causal, p, seed,
                            seed_dev, dtype, "diff_attention_forward");
   if (rc) return rc;
-  UBV_CHECK_ARG(out && (uintptr_t)out % 16 == 0 && (uintptr_t)maps % 16 == 0 && (lse == nullptr) == (maps == nullptr),
-                "diff_attention_forward: out, or lse without maps");
-  a.out = out; a.lse = lse; a.o = maps;
+  UBV_CHECK_ARG(out && (uintptr_t)out % 16 == 0 && ((uintptr_t)maps | (uintptr_t)stat | (uintptr_t)workspace) % 16 == 0 &&
+                    (stat == nullptr) == (maps == nullptr),
+                "diff_attention_forward: out, or stat without maps");
+  a.out = out; a.stat = (float4*)stat; a.o = maps;
   hipStream_t st = as_stream(stream);
   switch (dtype) {
-    case UBV_F32: return diff_attn_forward_f32(a, st);
-    case UBV_F16: return diff_attn_forward_f16(a, st);
-    default: return diff_attn_forward_bf16(a, st);
+    case UBV_F32: return diff_attn_forward_f32(a, workspace, workspace_bytes, st);
+    case UBV_F16: return diff_attn_forward_f16(a, workspace, workspace_bytes, st);
+    default: return diff_attn_forward_bf16(a, workspace, workspace_bytes, st);
   }
 }
 
 extern "C" int64_t ubv_diff_attention_backward_workspace(int B, int H, int Nq) {
-  return B <= 0 || H <= 0 || Nq <= 0 ? 0 : 3 * (int64_t)B * H * Nq * 4;
+  return B <= 0 || H <= 0 || Nq <= 0 ? 0 : 28 * (int64_t)B * H * Nq;
 }
 
 extern "C" int ubv_diff_attention_backward(const void* grad_out, const void* q, const void* k, const void* v, const float* lam,
-                                           const uint8_t* key_padding_mask, const void* mask, int mask_kind, const float* lse,
+                                           const uint8_t* key_padding_mask, const void* mask, int mask_kind, const float* stat,
                                            const float* maps, void* grad_q, void* grad_k, void* grad_v, float* grad_lam,
                                            const int64_t* strides, int B, int H, int Hk, int Nq, int Nk, int Dh, int Dv, float scale,
                                            int causal, float p, uint64_t seed, const uint64_t* seed_dev, int dtype, void* workspace,
@@ -73,15 +89,15 @@ extern "C" int ubv_diff_attention_backward(const void* grad_out, const void* q, 
   const int rc = attn_args(a, q, k, v, lam, key_padding_mask, mask, mask_kind, strides, B, H, Hk, Nq, Nk, Dh, Dv, scale, causal, p, seed,
                            seed_dev, dtype, "diff_attention_backward");
   if (rc) return rc;
-  UBV_CHECK_ARG(grad_out && lse && maps && (uintptr_t)grad_out % 16 == 0, "diff_attention_backward: grad_out, lse or maps");
+  UBV_CHECK_ARG(grad_out && stat && maps && ((uintptr_t)grad_out | (uintptr_t)stat) % 16 == 0, "diff_attention_backward: grad_out, stat or maps");
   UBV_CHECK_ARG((grad_k == nullptr) == (grad_v == nullptr), "diff_attention_backward: grad_k and grad_v come together");
   UBV_CHECK_ARG(((uintptr_t)grad_q | (uintptr_t)grad_k | (uintptr_t)grad_v) % 16 == 0, "diff_attention_backward: gradients must be 16-byte aligned");
-  UBV_CHECK_ARG(workspace && (uintptr_t)workspace % 4 == 0 && workspace_bytes >= ubv_diff_attention_backward_workspace(B, H, Nq),
+  UBV_CHECK_ARG(workspace && (uintptr_t)workspace % 16 == 0 && workspace_bytes >= ubv_diff_attention_backward_workspace(B, H, Nq),
                 "diff_attention_backward: the workspace is too small (%ld bytes)", (long)workspace_bytes);
   const int64_t rows = (int64_t)B * H * Nq;
-  a.go = grad_out; a.lse = const_cast<float*>(lse); a.o = const_cast<float*>(maps);
+  a.go = grad_out; a.stat = (float4*)const_cast<float*>(stat); a.o = const_cast<float*>(maps);
   a.gq = grad_q; a.gk = grad_k; a.gv = grad_v;
-  a.del = (float*)workspace; a.dlrow = a.del + 2 * rows;
+  a.row = (float4*)workspace; a.rowl = (float2*)(a.row + rows); a.dlrow = (float*)(a.rowl + rows);
   hipStream_t st = as_stream(stream);
   switch (dtype) {
     case UBV_F32: return diff_attn_backward_f32(a, grad_lam, st);

@@ -1,5 +1,12 @@
 // Kernels and launchers of differential attention for one element type: included once per type (diff_attn_f32.hip, ...),
 // UBV_ATTN_T names it.
+//
+// Two arrangements of the same wave program (a wave: 32 own items against a stream of 32-item tiles):
+//   shared   the block's four waves have 128 own items and share each staged tile (two LDS buffers, one barrier a tile)
+//   private  the block's waves have the SAME 32 own items, every wave stages tiles of its own (one buffer, no barrier: a wave's
+//            LDS accesses are in order) and the waves' sums are joined through LDS at the end: four times the blocks
+// In both the next tile's global loads are issued before the present tile is worked on.  Loads are buffer loads whose offset is
+// sent out of bounds where a zero is wanted: items past the end, hidden keys, columns past the head's width.
 #include "diff_attn.h"
 
 namespace ubv {
@@ -9,44 +16,75 @@ template <typename T, int DH, int DV> struct AttnTile {
   static constexpr int LDK = DH + VEC, LDV = DV + VEC;      // 16 bytes of padding: fragment reads of 32 rows hit all banks alike
   static constexpr int KB = DH / 16, VB = DV / 16;          // 16-deep steps over a head's width
   static constexpr int KO = (DH + 31) / 32, VO = DV / 32;   // 32-wide output blocks
-  static constexpr int bytes(int n) { return (n * (2 * LDK + LDV) + 32) * elem<T>::kBytes; }   // (+ 32: a 16-wide head's transposed reads)
-  static constexpr int WK = bytes(128) <= 150 * 1024 ? 4 : 2;       // most waves that share one set of own items
+  // a staged tile of n items: x of two maps, y, and the rows' statistics of the backward pass (float4 + float2 each)
+  static constexpr int elems(int n) { return n * (2 * LDK + LDV); }
+  static constexpr int bytes(int n) { return elems(n) * elem<T>::kBytes + 24 * n; }
+  static constexpr int WK = 4 * bytes(32) <= 150 * 1024 ? 4 : 2;                 // waves of a private block
+  static constexpr int NS = 2 * bytes(64) <= 76 * 1024 ? 64 : 32;                // items of a shared tile
 };
 
-// ---- staging: `n` items of 2 x DH (x) and DV (y) elements into LDS -----------------------------------------------------------
-// the block's threads take 16-byte pieces; items past `valid`, hidden keys and columns past the head's width become zeros
-template <typename T, int DH, int DV, int N> struct AttnStage {
+template <typename T, int DH, int DV, bool SHARED> struct AttnPlan {
   using S = AttnTile<T, DH, DV>;
-  static constexpr int PX = 2 * DH / S::VEC, PY = DV / S::VEC, NX = N * PX / 256, NY = N * PY / 256;
-  static_assert(N * PX % 256 == 0 && N * PY % 256 == 0, "pieces per thread");
-  au32x4_t x[NX], y[NY];
+  static constexpr int WK = SHARED ? 1 : S::WK, WQ = SHARED ? 4 : 1;             // waves per own items / groups of own items
+  static constexpr int NW = WK * WQ, NT = 64 * NW;
+  static constexpr int N = SHARED ? S::NS : 32;                                  // items of a staged tile
+  static constexpr int LT = SHARED ? NT : 64;                                    // threads that stage a tile
+  static constexpr int LDS = (SHARED ? 2 : WK) * S::bytes(N);
+  static constexpr int merge(int floats) { return SHARED ? 0 : (WK / 2) * floats * 64 * 4; }     // joining `floats` per lane
+  static constexpr int lds(int floats) { return LDS > merge(floats) ? LDS : merge(floats); }
+  // registers for two waves a SIMD where accumulators, operands and a tile in flight fit into half of them
+  static constexpr int MINW = (elem<T>::kBytes == 2 ? DH <= 64 && DV <= 128 : DH <= 32 && DV <= 64) ? 2 : 1;
+};
 
-  template <typename F> __device__ __forceinline__ void load(F&& item, int tid, int Dh, int Dv) {
+// ---- staging ------------------------------------------------------------------------------------------------------------------
+template <typename T, int DH, int DV, int N, int LT> struct AttnStage {
+  using S = AttnTile<T, DH, DV>;
+  static constexpr int PX = 2 * DH / S::VEC, PY = DV / S::VEC, NX = N * PX / LT, NY = N * PY / LT;
+  static_assert(N * PX % LT == 0 && N * PY % LT == 0 && LT % PX == 0 && LT % PY == 0, "a thread keeps its column");
+  au32x4_t x[NX], y[NY];
+  uint32_t xoff, yoff;               // this thread's byte offset inside a tile, kOutside past the head's width
+
+  __device__ __forceinline__ void init(int t, uint32_t xrow, uint32_t xmap, uint32_t yrow, int Dh, int Dv) {
+    const int pc = t % PX, m = pc / (PX / 2), dx = (pc % (PX / 2)) * S::VEC, dy = (t % PY) * S::VEC;
+    xoff = dx < Dh ? (t / PX) * xrow + m * xmap + dx * elem<T>::kBytes : kOutside;
+    yoff = dy < Dv ? (t / PY) * yrow + dy * elem<T>::kBytes : kOutside;
+  }
+  // `hid`: bit i set: item i becomes zeros
+  __device__ __forceinline__ void load(const char* xb, uint32_t xrow, const char* yb, uint32_t yrow, uint64_t hid, int t) {
+    const __amdgpu_buffer_rsrc_t rx = attn_rsrc(xb), ry = attn_rsrc(yb);
+    if (hid == 0) {
 #pragma unroll
-    for (int c = 0; c < NX; ++c) {
-      const int id = tid + 256 * c, it = id / PX, pc = id % PX, m = pc / (PX / 2), d = (pc % (PX / 2)) * S::VEC;
-      x[c] = item(it, m, d, d < Dh);
-    }
+      for (int c = 0; c < NX; ++c) x[c] = attn_piece(rx, xoff, c * (LT / PX) * xrow);
 #pragma unroll
-    for (int c = 0; c < NY; ++c) {
-      const int id = tid + 256 * c, it = id / PY, d = (id % PY) * S::VEC;
-      y[c] = item(it, 2, d, d < Dv);
+      for (int c = 0; c < NY; ++c) y[c] = attn_piece(ry, yoff, c * (LT / PY) * yrow);
+    } else {
+#pragma unroll
+      for (int c = 0; c < NX; ++c)
+        x[c] = attn_piece(rx, (hid >> (t / PX + c * (LT / PX))) & 1 ? kOutside : xoff, c * (LT / PX) * xrow);
+#pragma unroll
+      for (int c = 0; c < NY; ++c)
+        y[c] = attn_piece(ry, (hid >> (t / PY + c * (LT / PY))) & 1 ? kOutside : yoff, c * (LT / PY) * yrow);
     }
   }
-  __device__ __forceinline__ void store(T* lds, int tid) {
+  __device__ __forceinline__ void store(T* lds, int t) {
+    const int pc = t % PX, m = pc / (PX / 2);
+    T* lx = lds + (m * N + t / PX) * S::LDK + (pc % (PX / 2)) * S::VEC;
 #pragma unroll
-    for (int c = 0; c < NX; ++c) {
-      const int id = tid + 256 * c, it = id / PX, pc = id % PX, m = pc / (PX / 2), d = (pc % (PX / 2)) * S::VEC;
-      *reinterpret_cast<au32x4_t*>(lds + (m * N + it) * S::LDK + d) = x[c];
-    }
-    T* ly = lds + 2 * N * S::LDK;
+    for (int c = 0; c < NX; ++c) *reinterpret_cast<au32x4_t*>(lx + c * (LT / PX) * S::LDK) = x[c];
+    T* ly = lds + 2 * N * S::LDK + (t / PY) * S::LDV + (t % PY) * S::VEC;
 #pragma unroll
-    for (int c = 0; c < NY; ++c) {
-      const int id = tid + 256 * c, it = id / PY, d = (id % PY) * S::VEC;
-      *reinterpret_cast<au32x4_t*>(ly + it * S::LDV + d) = y[c];
-    }
+    for (int c = 0; c < NY; ++c) *reinterpret_cast<au32x4_t*>(ly + c * (LT / PY) * S::LDV) = y[c];
   }
 };
+
+// the staged tile is there for every lane that reads it
+template <bool SHARED> __device__ __forceinline__ void tile_ready() {
+  if constexpr (SHARED) __syncthreads();
+  else {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  }
+}
 
 // a lane's own item as B operands: 8 elements at 16 s + 8 (lane >> 5) of step s
 template <typename T, int NB>
@@ -57,13 +95,16 @@ __device__ __forceinline__ void own_frags(typename amma<T>::frag (&f)[NB], const
     const int d = 16 * s + 8 * (lane >> 5);
     T t[8];
 #pragma unroll
-    for (int w = 0; w < 8 / VEC; ++w)
-      *reinterpret_cast<au32x4_t*>(t + w * VEC) = piece(p + d + w * VEC, ok && d + w * VEC < D);
+    for (int w = 0; w < 8 / VEC; ++w) {
+      au32x4_t z = {0u, 0u, 0u, 0u};
+      if (ok && d + w * VEC < D) z = *reinterpret_cast<const au32x4_t*>(p + d + w * VEC);
+      *reinterpret_cast<au32x4_t*>(t + w * VEC) = z;
+    }
     f[s] = amma<T>::load(t);
   }
 }
 
-// 16 scores of own item (lane & 31) against staged items it0 .. it0 + 31
+// 16 dot products of own item (lane & 31) with staged items it0 .. it0 + 31
 template <typename T, int NB, int LD>
 __device__ __forceinline__ af32x16_t tile_dot(const T* tile, int it0, const typename amma<T>::frag (&own)[NB], int lane) {
   af32x16_t c = {0.0f};
@@ -84,201 +125,368 @@ template <typename T> __device__ __forceinline__ void store_quad(T* row, int d, 
   }
 }
 
-// fields of the four staged rows 8 q + 4 (lane >> 5) + t of this lane's key: the four lanes of a key group each mix one row
-// and hand it round
-__device__ __forceinline__ void quad_fields(uint64_t mix, int lane, uint32_t (&f)[4]) {
+// words (lower field row t even, ...) of the four staged rows 8 q + 4 (lane >> 5) + t of this lane's key: the four lanes of a key
+// group each mix one row and hand it round; w[t] is the word that holds this key's field
+__device__ __forceinline__ void quad_words(uint64_t mix, int lane, uint32_t (&w)[4]) {
   const int lo = (int)(uint32_t)mix, hi = (int)(uint32_t)(mix >> 32);
-#define UBV_QUAD(t)                                                                             \
-  {                                                                                             \
-    const uint32_t a = (uint32_t)__builtin_amdgcn_mov_dpp(lo, (t) * 0x55, 0xf, 0xf, true);     \
-    const uint32_t b = (uint32_t)__builtin_amdgcn_mov_dpp(hi, (t) * 0x55, 0xf, 0xf, true);     \
-    f[t] = (((lane & 2) ? b : a) >> (16 * (lane & 1))) & 0xffffu;                              \
+#define UBV_QUAD(t)                                                                           \
+  {                                                                                           \
+    const uint32_t a = (uint32_t)__builtin_amdgcn_mov_dpp(lo, (t) * 0x55, 0xf, 0xf, true);   \
+    const uint32_t b = (uint32_t)__builtin_amdgcn_mov_dpp(hi, (t) * 0x55, 0xf, 0xf, true);   \
+    w[t] = (lane & 2) ? b : a;                                                                \
   }
   UBV_QUAD(0) UBV_QUAD(1) UBV_QUAD(2) UBV_QUAD(3)
 #undef UBV_QUAD
 }
 
-// ---- forward -----------------------------------------------------------------------------------------------------------------
-template <typename T, int DH, int DV, int WQ, int WK>
-__global__ __launch_bounds__(256) void diff_attn_fwd_kernel(const DiffAttnArgs a) {
-  using S = AttnTile<T, DH, DV>;
-  using M = amma<T>;
-  constexpr int BK = WK == 1 ? 64 : 32 * WK, SUB = BK / (32 * WK);
-  extern __shared__ __attribute__((aligned(16))) char smem[];
-  T* lds = reinterpret_cast<T*>(smem);
-  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, wq = wv / WK, wk = wv % WK;
-  const int tiles = (a.R + 32 * WQ - 1) / (32 * WQ);
-  const int bh = blockIdx.x / tiles, rb = (blockIdx.x % tiles) * 32 * WQ;
-  const int b = bh / a.Hk, hk = bh % a.Hk;
-  const int r = rb + 32 * wq + (lane & 31);
-  const bool ok = r < a.R;
-  const int rc = ok ? r : a.R - 1, h = hk * a.G + rc / a.Nq, i = rc % a.Nq;
-  const int64_t rows = (int64_t)a.B * a.H * a.Nq, rowid = ((int64_t)b * a.H + hk * a.G) * a.Nq + rc;
-  const uint64_t seed = a.seed + (a.seed_dev != nullptr ? *a.seed_dev : 0);
+// keys j0 .. j0 + n - 1 that no row may see: past the end or padded (this lane's part; the wave's ballot is the tile's)
+__device__ __forceinline__ bool key_hidden(const DiffAttnArgs& a, int b, int j0, int n, int lane) {
+  const int j = j0 + lane;
+  if (lane >= n) return false;
+  return j >= a.Nk || (a.kpm != nullptr && a.kpm[(int64_t)b * a.Nk + j] != 0);
+}
 
-  typename M::frag qf[2][S::KB];
+// hides keys of a tile from the lane's row (query i of head h): `hid` bits of the 32 keys from j0, causal, the call's mask
+__device__ __forceinline__ void mask_tile(const DiffAttnArgs& a, af32x16_t (&x)[2], uint32_t hid, int b, int h, int i, int j0, float rscale,
+                                          int lane) {
+  const int half = 4 * (lane >> 5);
+  if (hid != 0) {
+    const uint32_t w = hid >> half;
 #pragma unroll
-  for (int m = 0; m < 2; ++m)
-    own_frags<T, S::KB>(qf[m], (const T*)a.q + b * a.qs[0] + i * a.qs[1] + h * a.qs[2] + m * a.qs[3], ok, a.Dh, lane);
-  af32x16_t acc[2][S::VO];
-  float mx[2] = {kNegInf, kNegInf}, l[2] = {0.0f, 0.0f};
-#pragma unroll
-  for (int m = 0; m < 2; ++m)
-#pragma unroll
-    for (int d = 0; d < S::VO; ++d) acc[m][d] = af32x16_t{0.0f};
-
-  // keys that any row of the block sees
-  int kend = a.Nk;
+    for (int e = 0; e < 16; ++e)
+      if (w & (1u << (8 * (e >> 2) + (e & 3)))) { x[0][e] = kNegInf; x[1][e] = kNegInf; }
+  }
   if (a.causal) {
-    const int last = min(rb + 32 * WQ, a.R) - 1;
-    const int imax = rb / a.Nq == last / a.Nq ? last % a.Nq : a.Nq - 1;
-    kend = max(0, min(a.Nk, imax + a.Nk - a.Nq + 1));
-  }
-  const T* kbase = (const T*)a.k + b * a.ks[0] + hk * a.ks[2];
-  const T* vbase = (const T*)a.v + b * a.vs[0] + hk * a.vs[2];
-  const float c = a.scale * kLog2e;
-  AttnStage<T, DH, DV, BK> st;
-  for (int k0 = 0; k0 < kend; k0 += BK) {
-    st.load([&](int it, int m, int d, bool in) {
-      const int j = k0 + it;
-      const bool use = in && j < a.Nk && !(a.kpm != nullptr && a.kpm[(int64_t)b * a.Nk + min(j, a.Nk - 1)]);
-      return m < 2 ? piece(kbase + j * a.ks[1] + m * a.ks[3] + d, use) : piece(vbase + j * a.vs[1] + d, use);
-    }, tid, a.Dh, a.Dv);
-    __syncthreads();
-    st.store(lds, tid);
-    __syncthreads();
-#pragma unroll 1
-    for (int sub = 0; sub < SUB; ++sub) {
-      const int it0 = (sub * WK + wk) * 32, j0 = k0 + it0;
-      if (j0 >= kend) break;
-      af32x16_t x[2];
+    const int lim = i + a.Nk - a.Nq - j0 - half;
+    if (__any(lim < 31 - half)) {
 #pragma unroll
-      for (int m = 0; m < 2; ++m) x[m] = tile_dot<T, S::KB, S::LDK>(lds + m * BK * S::LDK, it0, qf[m], lane);
-#pragma unroll
-      for (int m = 0; m < 2; ++m)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) x[m][e] *= c;
-      if (a.causal || a.kpm != nullptr || a.mask_kind != 0 || j0 + 32 > a.Nk) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int j = j0 + tile_item(e, lane);
-          const float bias = j < a.Nk ? mask_bias(a, b, h, i, j) : kNegInf;
-#pragma unroll
-          for (int m = 0; m < 2; ++m) x[m][e] = bias == kNegInf ? kNegInf : x[m][e] + bias;
-        }
-      }
-      float p[2][16];
-#pragma unroll
-      for (int m = 0; m < 2; ++m) {
-        float top = x[m][0];
-#pragma unroll
-        for (int e = 1; e < 16; ++e) top = fmaxf(top, x[m][e]);
-        top = fmaxf(mx[m], fmaxf(top, other_half(top)));
-        if (__any(top > mx[m])) {                   // a larger maximum: what is summed so far shrinks (wave-uniform branch)
-          const float al = aexp2(mx[m] - (top == kNegInf ? 0.0f : top));
-          l[m] *= al;
-#pragma unroll
-          for (int d = 0; d < S::VO; ++d)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) acc[m][d][e] *= al;
-          mx[m] = top;
-        }
-        const float mu = mx[m] == kNegInf ? 0.0f : mx[m] - kProbShift<T>;
-#pragma unroll
-        for (int e = 0; e < 16; ++e) { p[m][e] = aexp2(x[m][e] - mu); l[m] += p[m][e]; }
-      }
-      if (a.t16 != 0) {
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const uint64_t mix = drop_mix64(seed, (uint64_t)(rowid * a.n4 + ((j0 + tile_item(4 * q, lane)) >> 2)));
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const bool keep = (uint32_t)((mix >> (16 * e)) & 0xffffull) >= a.t16;
-#pragma unroll
-            for (int m = 0; m < 2; ++m) p[m][4 * q + e] = keep ? p[m][4 * q + e] : 0.0f;
-          }
-        }
-      }
-      const T* vt = lds + 2 * BK * S::LDK;
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const typename M::frag f0 = M::pack(p[0] + 8 * s), f1 = M::pack(p[1] + 8 * s);
-#pragma unroll
-        for (int d = 0; d < S::VO; ++d) {
-          const typename M::frag vf = M::template load_tr<S::LDV>(vt, it0 + 16 * s, 32 * d, lane);
-          acc[0][d] = M::mul(vf, f0, acc[0][d]);
-          acc[1][d] = M::mul(vf, f1, acc[1][d]);
-        }
-      }
+      for (int e = 0; e < 16; ++e)
+        if (8 * (e >> 2) + (e & 3) > lim) { x[0][e] = kNegInf; x[1][e] = kNegInf; }
     }
   }
-#pragma unroll
-  for (int m = 0; m < 2; ++m) l[m] += other_half(l[m]);
-  if constexpr (WK > 1) {                            // join the waves that walked other keys of the same rows
-    float* mrg = reinterpret_cast<float*>(smem);
-    constexpr int SLOT = (4 + DV) * 64;
-#pragma unroll 1
-    for (int half = WK / 2; half >= 1; half >>= 1) {
-      __syncthreads();
-      float* slot = mrg + (wq * (WK / 2) + wk % half) * SLOT + lane;
-      if (wk >= half && wk < 2 * half) {
-#pragma unroll
-        for (int m = 0; m < 2; ++m) {
-          slot[(2 * m) * 64] = mx[m]; slot[(2 * m + 1) * 64] = l[m];
-#pragma unroll
-          for (int d = 0; d < S::VO; ++d)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) slot[(4 + (m * S::VO + d) * 16 + e) * 64] = acc[m][d][e];
-        }
-      }
-      __syncthreads();
-      if (wk < half) {
-#pragma unroll
-        for (int m = 0; m < 2; ++m) {
-          const float mo = slot[(2 * m) * 64], top = fmaxf(mx[m], mo), mu = top == kNegInf ? 0.0f : top;
-          const float f0 = aexp2(mx[m] - mu), f1 = aexp2(mo - mu);
-          l[m] = l[m] * f0 + slot[(2 * m + 1) * 64] * f1;
-          mx[m] = top;
-#pragma unroll
-          for (int d = 0; d < S::VO; ++d)
-#pragma unroll
-            for (int e = 0; e < 16; ++e)
-              acc[m][d][e] = acc[m][d][e] * f0 + slot[(4 + (m * S::VO + d) * 16 + e) * 64] * f1;
-        }
-      }
-    }
-    if (wk != 0) return;
-  }
-  if (!ok) return;
-  const float lam = a.lam[h];
-  float inv[2];
-#pragma unroll
-  for (int m = 0; m < 2; ++m) {
-    inv[m] = l[m] == 0.0f ? 0.0f : a.up / l[m];
-    if (a.lse != nullptr && lane < 32) a.lse[m * rows + rowid] = mx[m] - kProbShift<T> + log2f(l[m]);
-  }
-  T* orow = (T*)a.out + (((int64_t)b * a.Nq + i) * a.H + h) * a.Dv;
-#pragma unroll
-  for (int d = 0; d < S::VO; ++d)
+  if (a.mask_kind == 0) return;
+  const int64_t o = b * a.ms[0] + h * a.ms[1] + i * a.ms[2] + (j0 + half) * a.ms[3];
+  const bool whole = j0 + 32 <= a.Nk;
+  if (a.mask_kind == 1) {
+    const uint8_t* m = (const uint8_t*)a.mask + o;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      const int dv = 32 * d + tile_item(4 * q, lane);
+      uint32_t w = 0;
+      if (whole && a.ms[3] == 1) __builtin_memcpy(&w, m + 8 * q, 4);
+      else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (j0 + half + 8 * q + e < a.Nk) w |= (uint32_t)m[(8 * q + e) * a.ms[3]] << (8 * e);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (w & (0xffu << (8 * e))) { x[0][4 * q + e] = kNegInf; x[1][4 * q + e] = kNegInf; }
+    }
+  } else {
+    const float* m = (const float*)a.mask + o;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      float w[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      if (whole && a.ms[3] == 1) __builtin_memcpy(w, m + 8 * q, 16);
+      else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (j0 + half + 8 * q + e < a.Nk) w[e] = m[(8 * q + e) * a.ms[3]];
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float bias = mask_raw(w[e], rscale);
+        x[0][4 * q + e] = mask_add(x[0][4 * q + e], bias);
+        x[1][4 * q + e] = mask_add(x[1][4 * q + e], bias);
+      }
+    }
+  }
+}
+
+// what forward and grad_q share: own = rows
+struct RowWave {
+  int wave, lane, wq, wk, b, hk, rb, r, h, i;
+  bool ok;
+  int64_t rowid;
+  int kend;                            // keys that some row of the block sees: [0, kend)
+
+  template <int WQ, int WK> __device__ __forceinline__ void init(const DiffAttnArgs& a, int tile) {
+    wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    lane = threadIdx.x & 63;
+    wq = wave / WK; wk = wave % WK;
+    const int tiles = (a.R + 32 * WQ - 1) / (32 * WQ), bh = tile / tiles;
+    rb = (tile - bh * tiles) * 32 * WQ;
+    b = bh / a.Hk; hk = bh - b * a.Hk;
+    r = rb + 32 * wq + (lane & 31);
+    ok = r < a.R;
+    const int rc = ok ? r : a.R - 1, g = rc / a.Nq;
+    h = hk * a.G + g; i = rc - g * a.Nq;
+    rowid = ((int64_t)b * a.H + hk * a.G) * a.Nq + rc;
+    kend = a.Nk;
+    if (a.causal) {
+      const int last = min(rb + 32 * WQ, a.R) - 1;
+      const int imax = rb / a.Nq == last / a.Nq ? last % a.Nq : a.Nq - 1;
+      kend = max(0, min(a.Nk, imax + a.Nk - a.Nq + 1));
+    }
+  }
+};
+
+// the stream of staged key tiles: f(tile of T, it0, hid of its 32 keys, j0) for every 32 keys that are not all hidden
+template <typename T, int DH, int DV, bool SHARED, typename F>
+__device__ __forceinline__ void key_tiles(const DiffAttnArgs& a, const RowWave& w, int t0, int t1, char* smem, F&& f) {
+  using S = AttnTile<T, DH, DV>;
+  using P = AttnPlan<T, DH, DV, SHARED>;
+  constexpr int N = P::N, STEP = P::WK;
+  constexpr uint64_t ALL = N == 64 ? ~0ull : 0xffffffffull;
+  const int st = SHARED ? threadIdx.x : w.lane;
+  AttnStage<T, DH, DV, N, P::LT> sg;
+  const uint32_t xrow = (uint32_t)(a.ks[1] * elem<T>::kBytes), yrow = (uint32_t)(a.vs[1] * elem<T>::kBytes);
+  sg.init(st, xrow, (uint32_t)(a.ks[3] * elem<T>::kBytes), yrow, a.Dh, a.Dv);
+  const char* kb = (const char*)a.k + (w.b * a.ks[0] + w.hk * a.ks[2]) * elem<T>::kBytes;
+  const char* vb = (const char*)a.v + (w.b * a.vs[0] + w.hk * a.vs[2]) * elem<T>::kBytes;
+  int t = t0 + w.wk;
+  if (t >= t1) return;                                       // (private waves only: no barrier inside)
+  auto load = [&](int tt, uint64_t hid) {
+    const int64_t j0 = (int64_t)tt * N;
+    if (hid != ALL) sg.load(kb + j0 * xrow, xrow, vb + j0 * yrow, yrow, hid, st);
+  };
+  uint64_t hid = __ballot(key_hidden(a, w.b, t * N, N, w.lane));
+  load(t, hid);
+  T* buf = reinterpret_cast<T*>(smem + (SHARED ? 0 : w.wk * S::bytes(N)));
+  sg.store(buf, st);
+  tile_ready<SHARED>();
+  bool nb = t + STEP < t1 && key_hidden(a, w.b, (t + STEP) * N, N, w.lane);
+  int cur = 0;
+#pragma unroll 1
+  for (; t < t1; t += STEP) {
+    const bool more = t + STEP < t1;
+    const uint64_t nhid = __ballot(nb);
+    if (more) load(t + STEP, nhid);
+    nb = t + 2 * STEP < t1 && key_hidden(a, w.b, (t + 2 * STEP) * N, N, w.lane);
+    const T* tile = SHARED ? reinterpret_cast<T*>(smem + cur * S::bytes(N)) : buf;
+#pragma unroll 1
+    for (int it0 = 0; it0 < N; it0 += 32) {
+      const uint32_t h32 = (uint32_t)(hid >> it0);
+      if (h32 != 0xffffffffu && t * N + it0 < w.kend) f(tile, it0, h32, t * N + it0);
+    }
+    if (more) {
+      if constexpr (SHARED) cur ^= 1;
+      else tile_ready<false>();
+      sg.store(SHARED ? reinterpret_cast<T*>(smem + cur * S::bytes(N)) : buf, st);
+      tile_ready<SHARED>();
+    }
+    hid = nhid;
+  }
+}
+
+// ---- forward ------------------------------------------------------------------------------------------------------------------
+template <typename T, int DV> struct FwdState {
+  static constexpr int VO = DV / 32;
+  af32x16_t acc[2][VO];
+  float top[2], l[2];              // the row's reference (raw score) and this lane half's sum beside it
+
+  __device__ __forceinline__ void init() {
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      top[m] = kNegInf; l[m] = 0.0f;
+#pragma unroll
+      for (int d = 0; d < VO; ++d) acc[m][d] = af32x16_t{0.0f};
+    }
+  }
+  __device__ __forceinline__ void scale(int m, float f) {
+    l[m] *= f;
+#pragma unroll
+    for (int d = 0; d < VO; ++d)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[m][d][e] *= f;
+  }
+  static constexpr int FLOATS = 4 + DV;
+  __device__ __forceinline__ void put(float* slot) const {
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      slot[(2 * m) * 64] = top[m]; slot[(2 * m + 1) * 64] = l[m];
+#pragma unroll
+      for (int d = 0; d < VO; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) slot[(4 + (m * VO + d) * 16 + e) * 64] = acc[m][d][e];
+    }
+  }
+  // joins what another wave put for the same rows
+  __device__ __forceinline__ void join(const float* slot, float c) {
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      const float to = slot[(2 * m) * 64], t = fmaxf(top[m], to);
+      const float f0 = top[m] == kNegInf ? 0.0f : aexp2((top[m] - t) * c), f1 = to == kNegInf ? 0.0f : aexp2((to - t) * c);
+      scale(m, f0);
+      l[m] = fmaf(slot[(2 * m + 1) * 64], f1, l[m]);
+      top[m] = t;
+#pragma unroll
+      for (int d = 0; d < VO; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[m][d][e] = fmaf(slot[(4 + (m * VO + d) * 16 + e) * 64], f1, acc[m][d][e]);
+    }
+  }
+};
+
+// the rows' outputs and what the backward pass wants, from the joined state
+template <typename T, int DV>
+__device__ __forceinline__ void fwd_finish(const DiffAttnArgs& a, const FwdState<T, DV>& s, const RowWave& w, float c) {
+  if (!w.ok) return;
+  const bool fm = a.mask_kind == 2;
+  const int64_t rows = (int64_t)a.B * a.H * a.Nq;
+  const float lam = a.lam[w.h];
+  float inv[2], st[4];
+#pragma unroll
+  for (int m = 0; m < 2; ++m) {
+    const float l = half_sum(s.l[m]);
+    const bool dead = l == 0.0f;
+    inv[m] = dead ? 0.0f : a.up / l;
+    st[2 * m] = dead ? 0.0f : fm ? s.top[m] : s.top[m] * c - kProbShift<T>;
+    st[2 * m + 1] = dead ? -kNegInf : fm ? log2f(l) - kProbShift<T> : log2f(l);
+  }
+  if (a.stat != nullptr && w.lane < 32) a.stat[w.rowid] = make_float4(st[0], st[1], st[2], st[3]);
+  T* orow = (T*)a.out + (((int64_t)w.b * a.Nq + w.i) * a.H + w.h) * a.Dv;
+#pragma unroll
+  for (int d = 0; d < DV / 32; ++d)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int dv = 32 * d + tile_item(4 * q, w.lane);
       float o1[4], o2[4], o[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        o1[e] = acc[0][d][4 * q + e] * inv[0];
-        o2[e] = acc[1][d][4 * q + e] * inv[1];
+        o1[e] = s.acc[0][d][4 * q + e] * inv[0];
+        o2[e] = s.acc[1][d][4 * q + e] * inv[1];
         o[e] = fmaf(-lam, o2[e], o1[e]);
       }
       store_quad<T>(orow, dv, a.Dv, o);
       if (a.o != nullptr) {
-        store_quad<float>(a.o + rowid * a.Dv, dv, a.Dv, o1);
-        store_quad<float>(a.o + (rows + rowid) * a.Dv, dv, a.Dv, o2);
+        store_quad<float>(a.o + w.rowid * a.Dv, dv, a.Dv, o1);
+        store_quad<float>(a.o + (rows + w.rowid) * a.Dv, dv, a.Dv, o2);
       }
     }
 }
 
-// ---- backward: del_m = grad_out . o_m per row, 16 lanes a row -----------------------------------------------------------------
+template <typename T, int DH, int DV, bool SHARED>
+__global__ __launch_bounds__((AttnPlan<T, DH, DV, SHARED>::NT), (AttnPlan<T, DH, DV, SHARED>::MINW)) void diff_attn_fwd_kernel(
+    const DiffAttnArgs a) {
+  using S = AttnTile<T, DH, DV>;
+  using P = AttnPlan<T, DH, DV, SHARED>;
+  using M = amma<T>;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int tile = blockIdx.x / a.splits, split = blockIdx.x - tile * a.splits;
+  RowWave w;
+  w.init<P::WQ, P::WK>(a, tile);
+  typename M::frag qf[2][S::KB];
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+    own_frags<T, S::KB>(qf[m], (const T*)a.q + w.b * a.qs[0] + w.i * a.qs[1] + w.h * a.qs[2] + m * a.qs[3], w.ok, a.Dh, w.lane);
+  const float c = a.scale * kLog2e, rscale = 1.0f / a.scale, grow = 6.0f / c;
+  const bool fm = a.mask_kind == 2, drop = a.t16 != 0;
+  const uint32_t t32 = a.t16 << 16;
+  const uint64_t zrow = attn_seed(a.seed, a.seed_dev) + (uint64_t)(w.rowid * a.n4) + (w.lane >> 5);
+  FwdState<T, DV> s;
+  s.init();
+  float mu[2] = {0.0f, 0.0f};
+  const int tn = (w.kend + P::N - 1) / P::N, per = (tn + a.splits - 1) / a.splits;
+  key_tiles<T, DH, DV, SHARED>(a, w, split * per, min(tn, (split + 1) * per), smem,
+                               [&](const T* kt, int it0, uint32_t hid, int j0) {
+    af32x16_t x[2];
+#pragma unroll
+    for (int m = 0; m < 2; ++m) x[m] = tile_dot<T, S::KB, S::LDK>(kt + m * P::N * S::LDK, it0, qf[m], w.lane);
+    if (hid != 0 || a.causal || a.mask_kind != 0) mask_tile(a, x, hid, w.b, w.h, w.i, j0, rscale, w.lane);
+    float p[2][16];
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      float t = x[m][0];
+#pragma unroll
+      for (int e = 1; e < 16; ++e) t = fmaxf(t, x[m][e]);
+      t = half_max(t);
+      // the reference moves, and what is summed so far shrinks, only where a score is over it by 2^6: the sums have room for
+      // that, and after a row's first tiles this (wave-uniform) branch is hardly taken
+      if (__any(t > s.top[m] + grow)) {
+        t = fmaxf(t, s.top[m]);
+        s.scale(m, s.top[m] == kNegInf ? 0.0f : aexp2((s.top[m] - t) * c));
+        s.top[m] = t;
+        mu[m] = t == kNegInf ? 0.0f : fm ? t : t * c - kProbShift<T>;
+      }
+      if (fm) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) p[m][e] = aexp2(fmaf(x[m][e] - mu[m], c, kProbShift<T>));
+      } else {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) p[m][e] = aexp2(fmaf(x[m][e], c, -mu[m]));
+      }
+      float t0 = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) t0 += p[m][e];
+      s.l[m] += t0;
+    }
+    if (drop) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const uint64_t mix = attn_mix(zrow + (uint64_t)((j0 >> 2) + 2 * q));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const bool keep = attn_keep((uint32_t)(e < 2 ? mix : mix >> 32), e & 1, t32);
+#pragma unroll
+          for (int m = 0; m < 2; ++m) p[m][4 * q + e] = keep ? p[m][4 * q + e] : 0.0f;
+        }
+      }
+    }
+    const T* vt = kt + 2 * P::N * S::LDK;
+#pragma unroll
+    for (int st = 0; st < 2; ++st) {
+      const typename M::frag f0 = M::pack(p[0] + 8 * st), f1 = M::pack(p[1] + 8 * st);
+#pragma unroll
+      for (int d = 0; d < S::VO; ++d) {
+        const typename M::frag vf = M::template load_tr<S::LDV>(vt, it0 + 16 * st, 32 * d, w.lane);
+        s.acc[0][d] = M::mul(vf, f0, s.acc[0][d]);
+        s.acc[1][d] = M::mul(vf, f1, s.acc[1][d]);
+      }
+    }
+  });
+  if constexpr (!SHARED) {                            // join the waves that walked other keys of the same rows
+    float* slots = reinterpret_cast<float*>(smem);
+#pragma unroll 1
+    for (int half = P::WK / 2; half >= 1; half >>= 1) {
+      __syncthreads();
+      float* slot = slots + (w.wk % half) * (s.FLOATS * 64) + w.lane;
+      if (w.wk >= half && w.wk < 2 * half) s.put(slot);
+      __syncthreads();
+      if (w.wk < half) s.join(slot, c);
+    }
+    if (w.wk != 0) return;
+  }
+  if (a.splits > 1) {
+    s.put(a.part + ((int64_t)blockIdx.x * P::WQ + w.wq) * (s.FLOATS * 64) + w.lane);
+    return;
+  }
+  fwd_finish<T, DV>(a, s, w, c);
+}
+
+// joins the splits of a row tile in split order, one wave a tile of 32 rows
+template <typename T, int DV, int WQ>
+__global__ __launch_bounds__(64) void diff_attn_join_kernel(const DiffAttnArgs a) {
+  const float c = a.scale * kLog2e;
+  RowWave w;
+  const int tile = blockIdx.x / WQ;
+  w.init<WQ, 1>(a, tile);
+  w.wq = blockIdx.x % WQ;
+  if (WQ > 1) {                                       // (the wave is that group's)
+    w.r = w.rb + 32 * w.wq + (w.lane & 31);
+    w.ok = w.r < a.R;
+    const int rc = w.ok ? w.r : a.R - 1, g = rc / a.Nq;
+    w.h = w.hk * a.G + g; w.i = rc - g * a.Nq;
+    w.rowid = ((int64_t)w.b * a.H + w.hk * a.G) * a.Nq + rc;
+  }
+  FwdState<T, DV> s;
+  s.init();
+  for (int n = 0; n < a.splits; ++n)
+    s.join(a.part + (((int64_t)tile * a.splits + n) * WQ + w.wq) * (s.FLOATS * 64) + w.lane, c);
+  fwd_finish<T, DV>(a, s, w, c);
+}
+
+// ---- backward: del_m = grad_out . o_m per row, 16 lanes a row; the statistics as row_probability takes them -------------------
 template <typename T>
 __global__ __launch_bounds__(256) void diff_attn_del_kernel(const DiffAttnArgs a) {
   const int64_t rows = (int64_t)a.B * a.H * a.Nq, rowid = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
@@ -296,16 +504,24 @@ __global__ __launch_bounds__(256) void diff_attn_del_kernel(const DiffAttnArgs a
   }
 #pragma unroll
   for (int m = 8; m >= 1; m >>= 1) { s1 += __shfl_xor(s1, m, 64); s2 += __shfl_xor(s2, m, 64); }
-  if (t == 0 && rowid < rows) { a.del[rowid] = s1; a.del[rows + rowid] = s2; }
+  if (t == 0 && rowid < rows) {
+    const float4 st = a.stat[rr];
+    if (a.mask_kind == 2) {
+      a.row[rr] = make_float4(st.x, st.z, s1, s2);
+      a.rowl[rr] = make_float2(st.y, st.w);
+    } else {
+      a.row[rr] = make_float4(st.x + st.y, st.z + st.w, s1, s2);
+    }
+  }
 }
 
-// sums over the waves of a block that walked other staged items of the same own items; the result is in the waves wk == 0
-template <int WQ, int WK, int NB>
-__device__ __forceinline__ void join_waves(af32x16_t* const (&acc)[NB], float* mrg, int wq, int wk, int lane) {
+// sums over the waves of a private block; the result is in wave 0
+template <int WK, int NB>
+__device__ __forceinline__ void join_waves(af32x16_t* const (&acc)[NB], float* slots, int wk, int lane) {
 #pragma unroll 1
   for (int half = WK / 2; half >= 1; half >>= 1) {
     __syncthreads();
-    float* slot = mrg + (wq * (WK / 2) + wk % half) * (NB * 16 * 64) + lane;
+    float* slot = slots + (wk % half) * (NB * 16 * 64) + lane;
     if (wk >= half && wk < 2 * half) {
 #pragma unroll
       for (int n = 0; n < NB; ++n)
@@ -322,127 +538,89 @@ __device__ __forceinline__ void join_waves(af32x16_t* const (&acc)[NB], float* m
   }
 }
 
-// ---- backward: grad_q and the rows' parts of grad_lam; own = rows, staged = keys ---------------------------------------------
-template <typename T, int DH, int DV, int WQ, int WK>
-__global__ __launch_bounds__(256) void diff_attn_bwd_q_kernel(const DiffAttnArgs a) {
+// ---- backward: grad_q and the rows' parts of grad_lam; own = rows, staged = keys -----------------------------------------------
+template <typename T, int DH, int DV, bool SHARED>
+__global__ __launch_bounds__((AttnPlan<T, DH, DV, SHARED>::NT), (AttnPlan<T, DH, DV, SHARED>::MINW)) void diff_attn_bwd_q_kernel(
+    const DiffAttnArgs a) {
   using S = AttnTile<T, DH, DV>;
+  using P = AttnPlan<T, DH, DV, SHARED>;
   using M = amma<T>;
-  constexpr int BK = WK == 1 ? 64 : 32 * WK, SUB = BK / (32 * WK);
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  T* lds = reinterpret_cast<T*>(smem);
-  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, wq = wv / WK, wk = wv % WK;
-  const int tiles = (a.R + 32 * WQ - 1) / (32 * WQ);
-  const int bh = blockIdx.x / tiles, rb = (blockIdx.x % tiles) * 32 * WQ;
-  const int b = bh / a.Hk, hk = bh % a.Hk;
-  const int r = rb + 32 * wq + (lane & 31);
-  const bool ok = r < a.R;
-  const int rc = ok ? r : a.R - 1, h = hk * a.G + rc / a.Nq, i = rc % a.Nq;
-  const int64_t rows = (int64_t)a.B * a.H * a.Nq, rowid = ((int64_t)b * a.H + hk * a.G) * a.Nq + rc;
-  const uint64_t seed = a.seed + (a.seed_dev != nullptr ? *a.seed_dev : 0);
-
+  RowWave w;
+  w.init<P::WQ, P::WK>(a, blockIdx.x);
+  const bool fm = a.mask_kind == 2, drop = a.t16 != 0;
   typename M::frag qf[2][S::KB], gf[S::VB];
-  float lse[2], del[2];
 #pragma unroll
-  for (int m = 0; m < 2; ++m) {
-    own_frags<T, S::KB>(qf[m], (const T*)a.q + b * a.qs[0] + i * a.qs[1] + h * a.qs[2] + m * a.qs[3], ok, a.Dh, lane);
-    const float v = a.lse[m * rows + rowid];
-    lse[m] = !ok || v == kNegInf ? -kNegInf : v;     // no key seen: every probability is exp2(x - inf) = 0
-    del[m] = a.del[m * rows + rowid];
-  }
-  own_frags<T, S::VB>(gf, (const T*)a.go + b * a.gs[0] + i * a.gs[1] + h * a.gs[2], ok, a.Dv, lane);
+  for (int m = 0; m < 2; ++m)
+    own_frags<T, S::KB>(qf[m], (const T*)a.q + w.b * a.qs[0] + w.i * a.qs[1] + w.h * a.qs[2] + m * a.qs[3], w.ok, a.Dh, w.lane);
+  own_frags<T, S::VB>(gf, (const T*)a.go + w.b * a.gs[0] + w.i * a.gs[1] + w.h * a.gs[2], w.ok, a.Dv, w.lane);
+  const float4 rw = a.row[w.rowid];
+  const float2 rl = fm ? a.rowl[w.rowid] : make_float2(0.0f, 0.0f);
+  const float c = a.scale * kLog2e, rscale = 1.0f / a.scale;
+  const uint32_t t32 = a.t16 << 16;
+  const uint64_t zrow = attn_seed(a.seed, a.seed_dev) + (uint64_t)(w.rowid * a.n4) + (w.lane >> 5);
   af32x16_t acc[2][S::KO];
   float dl = 0.0f;
 #pragma unroll
   for (int m = 0; m < 2; ++m)
 #pragma unroll
     for (int d = 0; d < S::KO; ++d) acc[m][d] = af32x16_t{0.0f};
-  int kend = a.Nk;
-  if (a.causal) {
-    const int last = min(rb + 32 * WQ, a.R) - 1;
-    const int imax = rb / a.Nq == last / a.Nq ? last % a.Nq : a.Nq - 1;
-    kend = max(0, min(a.Nk, imax + a.Nk - a.Nq + 1));
-  }
-  const T* kbase = (const T*)a.k + b * a.ks[0] + hk * a.ks[2];
-  const T* vbase = (const T*)a.v + b * a.vs[0] + hk * a.vs[2];
-  const float c = a.scale * kLog2e;
-  AttnStage<T, DH, DV, BK> st;
-  for (int k0 = 0; k0 < kend; k0 += BK) {
-    st.load([&](int it, int m, int d, bool in) {
-      const int j = k0 + it;
-      const bool use = in && j < a.Nk && !(a.kpm != nullptr && a.kpm[(int64_t)b * a.Nk + min(j, a.Nk - 1)]);
-      return m < 2 ? piece(kbase + j * a.ks[1] + m * a.ks[3] + d, use) : piece(vbase + j * a.vs[1] + d, use);
-    }, tid, a.Dh, a.Dv);
-    __syncthreads();
-    st.store(lds, tid);
-    __syncthreads();
-#pragma unroll 1
-    for (int sub = 0; sub < SUB; ++sub) {
-      const int it0 = (sub * WK + wk) * 32, j0 = k0 + it0;
-      if (j0 >= kend) break;
-      af32x16_t x[2];
+  key_tiles<T, DH, DV, SHARED>(a, w, 0, (w.kend + P::N - 1) / P::N, smem, [&](const T* kt, int it0, uint32_t hid, int j0) {
+    af32x16_t x[2];
+#pragma unroll
+    for (int m = 0; m < 2; ++m) x[m] = tile_dot<T, S::KB, S::LDK>(kt + m * P::N * S::LDK, it0, qf[m], w.lane);
+    af32x16_t g = tile_dot<T, S::VB, S::LDV>(kt + 2 * P::N * S::LDK, it0, gf, w.lane);
+    if (hid != 0 || a.causal || a.mask_kind != 0) mask_tile(a, x, hid, w.b, w.h, w.i, j0, rscale, w.lane);
+    if (drop) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const uint64_t mix = attn_mix(zrow + (uint64_t)((j0 >> 2) + 2 * q));
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          g[4 * q + e] = attn_keep((uint32_t)(e < 2 ? mix : mix >> 32), e & 1, t32) ? g[4 * q + e] * a.up : 0.0f;
+      }
+    }
+    float dt = 0.0f;                                  // (the tile's own sum first: 16 times fewer additions to the long one)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const float p1 = row_probability(fm, x[0][e], c, rw.x, rl.x), p2 = row_probability(fm, x[1][e], c, rw.y, rl.y);
+      dt = fmaf(p2, g[e], dt);
+      x[0][e] = p1 * (g[e] - rw.z);
+      x[1][e] = p2 * (g[e] - rw.w);
+    }
+    dl += dt;
+#pragma unroll
+    for (int st = 0; st < 2; ++st)
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
-        x[m] = tile_dot<T, S::KB, S::LDK>(lds + m * BK * S::LDK, it0, qf[m], lane);
+        float ds[8];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) x[m][e] *= c;
+        for (int e = 0; e < 8; ++e) ds[e] = x[m][8 * st + e];
+        const typename M::frag f = M::pack(ds);
+#pragma unroll
+        for (int d = 0; d < S::KO; ++d)
+          acc[m][d] = M::mul(M::template load_tr<S::LDK>(kt + m * P::N * S::LDK, it0 + 16 * st, 32 * d, w.lane), f, acc[m][d]);
       }
-      if (a.causal || a.kpm != nullptr || a.mask_kind != 0 || j0 + 32 > a.Nk) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int j = j0 + tile_item(e, lane);
-          const float bias = j < a.Nk ? mask_bias(a, b, h, i, j) : kNegInf;
-#pragma unroll
-          for (int m = 0; m < 2; ++m) x[m][e] = bias == kNegInf ? kNegInf : x[m][e] + bias;
-        }
-      }
-      af32x16_t g = tile_dot<T, S::VB, S::LDV>(lds + 2 * BK * S::LDK, it0, gf, lane);
-      if (a.t16 != 0) {
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const uint64_t mix = drop_mix64(seed, (uint64_t)(rowid * a.n4 + ((j0 + tile_item(4 * q, lane)) >> 2)));
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            g[4 * q + e] = (uint32_t)((mix >> (16 * e)) & 0xffffull) >= a.t16 ? g[4 * q + e] * a.up : 0.0f;
-        }
-      }
-      float ds[2][16], dt = 0.0f;                     // (the tile's own sum first: 16 times fewer additions to the long one)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const float p1 = aexp2(x[0][e] - lse[0]), p2 = aexp2(x[1][e] - lse[1]);
-        dt = fmaf(p2, g[e], dt);
-        ds[0][e] = p1 * (g[e] - del[0]);
-        ds[1][e] = p2 * (g[e] - del[1]);
-      }
-      dl += dt;
-#pragma unroll
-      for (int s = 0; s < 2; ++s)
-#pragma unroll
-        for (int m = 0; m < 2; ++m) {
-          const typename M::frag f = M::pack(ds[m] + 8 * s);
-#pragma unroll
-          for (int d = 0; d < S::KO; ++d)
-            acc[m][d] = M::mul(M::template load_tr<S::LDK>(lds + m * BK * S::LDK, it0 + 16 * s, 32 * d, lane), f, acc[m][d]);
-        }
-    }
-  }
-  dl += other_half(dl);
-  if constexpr (WK > 1) {
+  });
+  if constexpr (!SHARED) {
     af32x16_t dlv = {dl};
     af32x16_t* ptr[2 * S::KO + 1];
 #pragma unroll
     for (int d = 0; d < S::KO; ++d) { ptr[d] = &acc[0][d]; ptr[S::KO + d] = &acc[1][d]; }
     ptr[2 * S::KO] = &dlv;
-    join_waves<WQ, WK>(ptr, reinterpret_cast<float*>(smem), wq, wk, lane);
-    if (wk != 0) return;
+    join_waves<P::WK>(ptr, reinterpret_cast<float*>(smem), w.wk, w.lane);
+    if (w.wk != 0) return;
     dl = dlv[0];
   }
-  if (!ok) return;
-  if (lane < 32) a.dlrow[rowid] = -dl;
+  dl = half_sum(dl);
+  if (!w.ok) return;
+  if (w.lane < 32) a.dlrow[w.rowid] = -dl;
   if (a.gq == nullptr) return;
-  const float f[2] = {a.scale, -a.lam[h] * a.scale};
+  // a single key has probability 1 whatever its score: its gradient is zero, not the rounding of G - del
+  const float one = a.Nk > 1 ? a.scale : 0.0f, f[2] = {one, -a.lam[w.h] * one};
 #pragma unroll
   for (int m = 0; m < 2; ++m) {
-    T* row = (T*)a.gq + ((((int64_t)b * a.Nq + i) * a.H + h) * 2 + m) * a.Dh;
+    T* row = (T*)a.gq + ((((int64_t)w.b * a.Nq + w.i) * a.H + w.h) * 2 + m) * a.Dh;
 #pragma unroll
     for (int d = 0; d < S::KO; ++d)
 #pragma unroll
@@ -450,7 +628,7 @@ __global__ __launch_bounds__(256) void diff_attn_bwd_q_kernel(const DiffAttnArgs
         float o[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[e] = acc[m][d][4 * q + e] * f[m];
-        store_quad<T>(row, 32 * d + tile_item(4 * q, lane), a.Dh, o);
+        store_quad<T>(row, 32 * d + tile_item(4 * q, w.lane), a.Dh, o);
       }
   }
 }
@@ -470,25 +648,24 @@ __global__ __launch_bounds__(256) static void diff_attn_lam_kernel(const float* 
   if (threadIdx.x == 0) glam[h] = (red[0] + red[1]) + (red[2] + red[3]);
 }
 
-// ---- backward: grad_k and grad_v; own = keys, staged = the rows of every head that shares them --------------------------------
-template <typename T, int DH, int DV, int WQ, int WK>
-__global__ __launch_bounds__(256) void diff_attn_bwd_kv_kernel(const DiffAttnArgs a) {
+// ---- backward: grad_k and grad_v; own = keys, staged = the rows of every head that shares them ----------------------------------
+// A tile of rows stays inside one head (its rows are one stretch of queries), heads one after the other.
+template <typename T, int DH, int DV, bool SHARED>
+__global__ __launch_bounds__((AttnPlan<T, DH, DV, SHARED>::NT), (AttnPlan<T, DH, DV, SHARED>::MINW)) void diff_attn_bwd_kv_kernel(
+    const DiffAttnArgs a) {
   using S = AttnTile<T, DH, DV>;
+  using P = AttnPlan<T, DH, DV, SHARED>;
   using M = amma<T>;
-  constexpr int BK = WK == 1 ? 64 : 32 * WK, SUB = BK / (32 * WK);
+  constexpr int N = P::N;
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  __shared__ __attribute__((aligned(16))) float stat[5][BK];     // lse_1, lse_2, del_1, del_2, lam of the staged rows
-  T* lds = reinterpret_cast<T*>(smem);
-  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, wq = wv / WK, wk = wv % WK;
-  const int tiles = (a.Nk + 32 * WQ - 1) / (32 * WQ);
-  const int bh = blockIdx.x / tiles, jb = (blockIdx.x % tiles) * 32 * WQ;
-  const int b = bh / a.Hk, hk = bh % a.Hk;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, wq = wave / P::WK, wk = wave % P::WK;
+  const int tiles = (a.Nk + 32 * P::WQ - 1) / (32 * P::WQ), bh = blockIdx.x / tiles, jb = (blockIdx.x - bh * tiles) * 32 * P::WQ;
+  const int b = bh / a.Hk, hk = bh - b * a.Hk;
   const int j = jb + 32 * wq + (lane & 31);
   // a hidden key's column is computed from zeros and its gradients are stored as zeros: no masking needed for it
   const bool in = j < a.Nk, ok = in && !(a.kpm != nullptr && a.kpm[(int64_t)b * a.Nk + (in ? j : 0)]);
-  const int jc = in ? j : a.Nk - 1;
-  const int64_t rows = (int64_t)a.B * a.H * a.Nq, row0 = ((int64_t)b * a.H + hk * a.G) * a.Nq;
-  const uint64_t seed = a.seed + (a.seed_dev != nullptr ? *a.seed_dev : 0);
+  const int jc = in ? j : a.Nk - 1, off = a.Nk - a.Nq;
+  const bool fm = a.mask_kind == 2, drop = a.t16 != 0;
 
   typename M::frag kf[2][S::KB], vf[S::VB];
 #pragma unroll
@@ -500,109 +677,142 @@ __global__ __launch_bounds__(256) void diff_attn_bwd_kv_kernel(const DiffAttnArg
   for (int d = 0; d < S::KO; ++d) { ak[0][d] = af32x16_t{0.0f}; ak[1][d] = af32x16_t{0.0f}; }
 #pragma unroll
   for (int d = 0; d < S::VO; ++d) av[d] = af32x16_t{0.0f};
-  const float c = a.scale * kLog2e;
-  AttnStage<T, DH, DV, BK> st;
-  for (int r0 = 0; r0 < a.R; r0 += BK) {
-    if (a.causal) {                                   // no row of the tile sees a key of the block
-      const int last = min(r0 + BK, a.R) - 1;
-      const int imax = r0 / a.Nq == last / a.Nq ? last % a.Nq : a.Nq - 1;
-      if (imax + a.Nk - a.Nq < jb) continue;
+  const float c = a.scale * kLog2e, rscale = 1.0f / a.scale;
+  const uint32_t t32 = a.t16 << 16;
+  const uint64_t zseed = attn_seed(a.seed, a.seed_dev) + (uint64_t)(j >> 2);
+
+  // tiles of a head from the first whose rows may see a key of the block
+  const int first = a.causal ? max(0, jb - off) / N : 0, per = max(0, (a.Nq + N - 1) / N - first), total = per * a.G;
+  const int st = SHARED ? threadIdx.x : lane;
+  AttnStage<T, DH, DV, N, P::LT> sg;
+  const uint32_t xrow = (uint32_t)(a.qs[1] * elem<T>::kBytes), yrow = (uint32_t)(a.gs[1] * elem<T>::kBytes);
+  sg.init(st, xrow, (uint32_t)(a.qs[3] * elem<T>::kBytes), yrow, a.Dh, a.Dv);
+  float4 srow;
+  float2 srowl = make_float2(0.0f, 0.0f);
+  auto load = [&](int t) {
+    const int g = t / per, i0 = (first + t - g * per) * N, h = hk * a.G + g, left = a.Nq - i0;
+    const char* xb = (const char*)a.q + (b * a.qs[0] + (int64_t)i0 * a.qs[1] + h * a.qs[2]) * elem<T>::kBytes;
+    const char* yb = (const char*)a.go + (b * a.gs[0] + (int64_t)i0 * a.gs[1] + h * a.gs[2]) * elem<T>::kBytes;
+    sg.load(xb, xrow, yb, yrow, left >= N ? 0ull : ~0ull << left, st);
+    if (st < N) {
+      const int64_t rid = ((int64_t)b * a.H + h) * a.Nq + i0 + min(st, left - 1);
+      srow = a.row[rid];
+      if (fm) srowl = a.rowl[rid];
+      if (st >= left) { srow = fm ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : make_float4(-kNegInf, -kNegInf, 0.0f, 0.0f); srowl = make_float2(-kNegInf, -kNegInf); }
     }
-    st.load([&](int it, int m, int d, bool use) {
-      const int r = r0 + it, rc = r < a.R ? r : a.R - 1, h = hk * a.G + rc / a.Nq, i = rc % a.Nq;
-      use = use && r < a.R;
-      return m < 2 ? piece((const T*)a.q + b * a.qs[0] + i * a.qs[1] + h * a.qs[2] + m * a.qs[3] + d, use)
-                   : piece((const T*)a.go + b * a.gs[0] + i * a.gs[1] + h * a.gs[2] + d, use);
-    }, tid, a.Dh, a.Dv);
-    float sv[5] = {-kNegInf, -kNegInf, 0.0f, 0.0f, 0.0f};
-    if (tid < BK && r0 + tid < a.R) {
-      const int64_t rid = row0 + r0 + tid;
-#pragma unroll
-      for (int m = 0; m < 2; ++m) {
-        const float v = a.lse[m * rows + rid];
-        sv[m] = v == kNegInf ? -kNegInf : v;
-        sv[2 + m] = a.del[m * rows + rid];
-      }
-      sv[4] = a.lam[hk * a.G + (r0 + tid) / a.Nq];
+  };
+  auto store = [&](char* at) {
+    sg.store(reinterpret_cast<T*>(at), st);
+    if (st < N) {
+      reinterpret_cast<float4*>(at + S::elems(N) * elem<T>::kBytes)[st] = srow;
+      if (fm) reinterpret_cast<float2*>(at + S::elems(N) * elem<T>::kBytes + 16 * N)[st] = srowl;
     }
-    __syncthreads();
-    st.store(lds, tid);
-    if (tid < BK) {
-#pragma unroll
-      for (int n = 0; n < 5; ++n) stat[n][tid] = sv[n];
-    }
-    __syncthreads();
+  };
+  char* const own = smem + (SHARED ? 0 : wk * S::bytes(N));
+  int cur = 0;
+  if (wk < total) {
+    load(wk);
+    store(own);
+    tile_ready<SHARED>();
+  }
 #pragma unroll 1
-    for (int sub = 0; sub < SUB; ++sub) {
-      const int it0 = (sub * WK + wk) * 32;
-      if (r0 + it0 >= a.R) break;
+  for (int t = wk; t < total; t += P::WK) {
+    const bool more = t + P::WK < total;
+    if (more) load(t + P::WK);
+    const char* at = SHARED ? smem + cur * S::bytes(N) : own;
+    const T* qt = reinterpret_cast<const T*>(at);
+    const T* gt = qt + 2 * N * S::LDK;
+    const float4* rows = reinterpret_cast<const float4*>(at + S::elems(N) * elem<T>::kBytes);
+    const float2* rowl = reinterpret_cast<const float2*>(rows + N);
+    const int g = t / per, h = hk * a.G + g, i00 = (first + t - g * per) * N;
+    const float lam = a.lam[h];
+#pragma unroll 1
+    for (int it0 = 0; it0 < N; it0 += 32) {
+      const int i0 = i00 + it0;
+      if (i0 >= a.Nq) break;
       af32x16_t x[2];
 #pragma unroll
-      for (int m = 0; m < 2; ++m) {
-        x[m] = tile_dot<T, S::KB, S::LDK>(lds + m * BK * S::LDK, it0, kf[m], lane);
+      for (int m = 0; m < 2; ++m) x[m] = tile_dot<T, S::KB, S::LDK>(qt + m * N * S::LDK, it0, kf[m], lane);
+      af32x16_t gm = tile_dot<T, S::VB, S::LDV>(gt, it0, vf, lane);
+      if (a.causal) {
+        const int lim = jc - off - i0 - 4 * (lane >> 5);                // rows before it do not see the key
+        if (__any(lim > -4 * (lane >> 5))) {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) x[m][e] *= c;
-      }
-      if (a.causal || a.mask_kind != 0) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int r = min(r0 + it0 + tile_item(e, lane), a.R - 1);
-          const float bias = mask_bias(a, b, hk * a.G + r / a.Nq, r % a.Nq, jc);
-#pragma unroll
-          for (int m = 0; m < 2; ++m) x[m][e] = bias == kNegInf ? kNegInf : x[m][e] + bias;
+          for (int e = 0; e < 16; ++e)
+            if (8 * (e >> 2) + (e & 3) < lim) { x[0][e] = kNegInf; x[1][e] = kNegInf; }
         }
       }
-      const af32x16_t g = tile_dot<T, S::VB, S::LDV>(lds + 2 * BK * S::LDK, it0, vf, lane);
-      float pc[16], ds[2][16];
+      if (a.mask_kind != 0) {
+        const int64_t o = b * a.ms[0] + h * a.ms[1] + jc * a.ms[3];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int64_t oi = o + min(i0 + tile_item(e, lane), a.Nq - 1) * a.ms[2];
+          float bias;
+          if (fm) bias = mask_raw(((const float*)a.mask)[oi], rscale);
+          else bias = ((const uint8_t*)a.mask)[oi] ? kNegInf : 0.0f;
+          x[0][e] = mask_add(x[0][e], bias);
+          x[1][e] = mask_add(x[1][e], bias);
+        }
+      }
+      const uint64_t zt = zseed + (uint64_t)((((int64_t)b * a.H + h) * a.Nq + i0 + 4 * (lane >> 5) + (lane & 3)) * a.n4);
+      float pc[16];
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const int t0 = it0 + tile_item(4 * q, lane);
-        uint32_t fld[4];
-        if (a.t16 != 0) quad_fields(drop_mix64(seed, (uint64_t)((row0 + r0 + t0 + (lane & 3)) * a.n4 + (j >> 2))), lane, fld);
-        float s[5][4];
-#pragma unroll
-        for (int n = 0; n < 5; ++n) *reinterpret_cast<float4*>(s[n]) = *reinterpret_cast<const float4*>(&stat[n][t0]);
+        const int r0 = it0 + tile_item(4 * q, lane);
+        uint32_t word[4];
+        if (drop) quad_words(attn_mix(zt + (uint64_t)(8 * q * (int64_t)a.n4)), lane, word);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int n = 4 * q + e;
-          const float p1 = aexp2(x[0][n] - s[0][e]), p2 = s[4][e] * aexp2(x[1][n] - s[1][e]);
-          float gn = g[n], pn = p1 - p2;
-          if (a.t16 != 0) {
-            const bool keep = fld[e] >= a.t16;
+          const float4 rw = rows[r0 + e];
+          const float2 rl = fm ? rowl[r0 + e] : make_float2(0.0f, 0.0f);
+          const float p1 = row_probability(fm, x[0][n], c, rw.x, rl.x), p2 = lam * row_probability(fm, x[1][n], c, rw.y, rl.y);
+          float gn = gm[n], pn = p1 - p2;
+          if (drop) {
+            const bool keep = attn_keep(word[e], lane & 1, t32);
             gn = keep ? gn * a.up : 0.0f;
             pn = keep ? pn : 0.0f;
           }
           pc[n] = kProbScale<T> == 1.0f ? pn : pn * kProbScale<T>;
-          ds[0][n] = p1 * (gn - s[2][e]);
-          ds[1][n] = p2 * (s[3][e] - gn);
+          x[0][n] = p1 * (gn - rw.z);
+          x[1][n] = p2 * (rw.w - gn);
         }
       }
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         const typename M::frag fp = M::pack(pc + 8 * s);
 #pragma unroll
-        for (int d = 0; d < S::VO; ++d)
-          av[d] = M::mul(M::template load_tr<S::LDV>(lds + 2 * BK * S::LDK, it0 + 16 * s, 32 * d, lane), fp, av[d]);
+        for (int d = 0; d < S::VO; ++d) av[d] = M::mul(M::template load_tr<S::LDV>(gt, it0 + 16 * s, 32 * d, lane), fp, av[d]);
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
-          const typename M::frag f = M::pack(ds[m] + 8 * s);
+          float ds[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) ds[e] = x[m][8 * s + e];
+          const typename M::frag f = M::pack(ds);
 #pragma unroll
           for (int d = 0; d < S::KO; ++d)
-            ak[m][d] = M::mul(M::template load_tr<S::LDK>(lds + m * BK * S::LDK, it0 + 16 * s, 32 * d, lane), f, ak[m][d]);
+            ak[m][d] = M::mul(M::template load_tr<S::LDK>(qt + m * N * S::LDK, it0 + 16 * s, 32 * d, lane), f, ak[m][d]);
         }
       }
     }
+    if (more) {
+      if constexpr (SHARED) cur ^= 1;
+      else tile_ready<false>();
+      store(SHARED ? smem + cur * S::bytes(N) : own);
+      tile_ready<SHARED>();
+    }
   }
-  if constexpr (WK > 1) {
+  if constexpr (!SHARED) {
     af32x16_t* ptr[2 * S::KO + S::VO];
 #pragma unroll
     for (int d = 0; d < S::KO; ++d) { ptr[d] = &ak[0][d]; ptr[S::KO + d] = &ak[1][d]; }
 #pragma unroll
     for (int d = 0; d < S::VO; ++d) ptr[2 * S::KO + d] = &av[d];
-    join_waves<WQ, WK>(ptr, reinterpret_cast<float*>(smem), wq, wk, lane);
+    join_waves<P::WK>(ptr, reinterpret_cast<float*>(smem), wk, lane);
     if (wk != 0) return;
   }
   if (!in) return;
+  const float fk = ok && a.Nk > 1 ? a.scale : 0.0f, fv = a.up / kProbScale<T>;        // (Nk = 1: as for grad_q)
 #pragma unroll
   for (int m = 0; m < 2; ++m) {
     T* row = (T*)a.gk + ((((int64_t)b * a.Nk + j) * a.Hk + hk) * 2 + m) * a.Dh;
@@ -612,11 +822,10 @@ __global__ __launch_bounds__(256) void diff_attn_bwd_kv_kernel(const DiffAttnArg
       for (int q = 0; q < 4; ++q) {
         float o[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = ok ? ak[m][d][4 * q + e] * a.scale : 0.0f;
+        for (int e = 0; e < 4; ++e) o[e] = fk != 0.0f ? ak[m][d][4 * q + e] * fk : 0.0f;
         store_quad<T>(row, 32 * d + tile_item(4 * q, lane), a.Dh, o);
       }
   }
-  const float fv = a.up / kProbScale<T>;
   T* row = (T*)a.gv + (((int64_t)b * a.Nk + j) * a.Hk + hk) * a.Dv;
 #pragma unroll
   for (int d = 0; d < S::VO; ++d)
@@ -631,58 +840,79 @@ __global__ __launch_bounds__(256) void diff_attn_bwd_kv_kernel(const DiffAttnArg
 
 // ---- launch -----------------------------------------------------------------------------------------------------------------------
 template <typename K>
-static int attn_launch(K kernel, int64_t blocks, int lds, const DiffAttnArgs& a, hipStream_t st, const char* who) {
+static int attn_launch(K kernel, int64_t blocks, int threads, int lds, const DiffAttnArgs& a, hipStream_t st, const char* who) {
   if (blocks >= (int64_t(1) << 31)) { set_error("%s: %ld blocks", who, (long)blocks); return UBV_ERR_UNSUPPORTED; }
   if (lds > 48 * 1024) (void)hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-  hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), (size_t)lds, st, a);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(threads), (size_t)lds, st, a);
   UBV_CHECK_LAUNCH(who);
   return UBV_OK;
 }
 
-constexpr int64_t kAttnFill = 512;      // blocks of 4 waves that keep the 256 CUs busy
+#ifndef UBV_ATTN_FILL
+#define UBV_ATTN_FILL 512
+#endif
+constexpr int64_t kAttnFill = UBV_ATTN_FILL;      // blocks that keep the 256 CUs busy
+
+// blocks of 32 own items a head, by the arrangement
+static inline int64_t attn_blocks(int64_t heads, int64_t items, int wq) { return heads * ((items + 32 * wq - 1) / (32 * wq)); }
 
 template <typename T, int DH, int DV>
-static int attn_forward(const DiffAttnArgs& a, hipStream_t st) {
-  using S = AttnTile<T, DH, DV>;
-  constexpr int WK = S::WK, WQ = 4 / WK, MRG = WQ * (WK / 2) * (4 + DV) * 64 * 4;
-  const int64_t heads = (int64_t)a.B * a.Hk, wide = heads * ((a.R + 127) / 128);
-  if (wide >= kAttnFill)
-    return attn_launch(diff_attn_fwd_kernel<T, DH, DV, 4, 1>, wide, S::bytes(64), a, st, "diff_attention_forward");
-  constexpr int lds = S::bytes(32 * WK) > MRG ? S::bytes(32 * WK) : MRG;
-  return attn_launch(diff_attn_fwd_kernel<T, DH, DV, WQ, WK>, heads * ((a.R + 32 * WQ - 1) / (32 * WQ)), lds, a, st, "diff_attention_forward");
+static int attn_forward(DiffAttnArgs a, void* ws, int64_t ws_bytes, hipStream_t st) {
+  const int64_t heads = (int64_t)a.B * a.Hk, wide = attn_blocks(heads, a.R, 4);
+  a.splits = 1;
+  auto run = [&](auto shared) {
+    constexpr bool SH = decltype(shared)::value;
+    using P = AttnPlan<T, DH, DV, SH>;
+    return attn_launch(diff_attn_fwd_kernel<T, DH, DV, SH>, attn_blocks(heads, a.R, P::WQ) * a.splits, P::NT,
+                       P::lds(FwdState<T, DV>::FLOATS), a, st, "diff_attention_forward");
+  };
+  if (wide >= kAttnFill) return run(std::true_type{});
+  // few rows, many keys: blocks share the keys of a row tile and a second launch joins their sums
+  const int64_t blocks = attn_blocks(heads, a.R, 1), tiles = (a.Nk + 31) / 32;
+  if (blocks < kAttnFill / 2 && ws != nullptr) {
+    constexpr int PER = 2 * AttnPlan<T, DH, DV, false>::WK;                          // at least two tiles a wave
+    int64_t splits = (2 * kAttnFill + blocks - 1) / blocks;
+    splits = splits < tiles / PER ? splits : tiles / PER;
+    const int64_t most = ws_bytes / (blocks * FwdState<T, DV>::FLOATS * 64 * 4);
+    splits = splits < most ? splits : most;
+    if (splits > 1) {
+      a.splits = (int)splits;
+      a.part = (float*)ws;
+      const int rc = run(std::false_type{});
+      if (rc != UBV_OK) return rc;
+      return attn_launch(diff_attn_join_kernel<T, DV, 1>, blocks, 64, 0, a, st, "diff_attention_forward");
+    }
+  }
+  return run(std::false_type{});
 }
 
 template <typename T, int DH, int DV>
 static int attn_backward(const DiffAttnArgs& a, float* glam, hipStream_t st) {
   using S = AttnTile<T, DH, DV>;
-  constexpr int WK = S::WK, WQ = 4 / WK;
-  constexpr int MQ = WQ * (WK / 2) * (2 * S::KO + 1) * 16 * 64 * 4, MKV = WQ * (WK / 2) * (2 * S::KO + S::VO) * 16 * 64 * 4;
-  constexpr int TL = S::bytes(32 * WK);
   const int64_t heads = (int64_t)a.B * a.Hk, rows = (int64_t)a.B * a.H * a.Nq;
   hipLaunchKernelGGL(diff_attn_del_kernel<T>, dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, st, a);
   UBV_CHECK_LAUNCH("diff_attention_backward");
+  auto run = [&](auto shared, auto which) {
+    constexpr bool SH = decltype(shared)::value;
+    using P = AttnPlan<T, DH, DV, SH>;
+    if constexpr (decltype(which)::value)
+      return attn_launch(diff_attn_bwd_q_kernel<T, DH, DV, SH>, attn_blocks(heads, a.R, P::WQ), P::NT, P::lds((2 * S::KO + 1) * 16), a, st,
+                         "diff_attention_backward");
+    else
+      return attn_launch(diff_attn_bwd_kv_kernel<T, DH, DV, SH>, attn_blocks(heads, a.Nk, P::WQ), P::NT, P::lds((2 * S::KO + S::VO) * 16), a,
+                         st, "diff_attention_backward");
+  };
   int rc = UBV_OK;
   if (a.gq != nullptr || glam != nullptr) {
-    const int64_t wide = heads * ((a.R + 127) / 128);
-    if (wide >= kAttnFill)
-      rc = attn_launch(diff_attn_bwd_q_kernel<T, DH, DV, 4, 1>, wide, S::bytes(64), a, st, "diff_attention_backward");
-    else
-      rc = attn_launch(diff_attn_bwd_q_kernel<T, DH, DV, WQ, WK>, heads * ((a.R + 32 * WQ - 1) / (32 * WQ)), TL > MQ ? TL : MQ, a, st,
-                       "diff_attention_backward");
+    rc = attn_blocks(heads, a.R, 4) >= kAttnFill ? run(std::true_type{}, std::true_type{}) : run(std::false_type{}, std::true_type{});
     if (rc != UBV_OK) return rc;
     if (glam != nullptr) {
       hipLaunchKernelGGL(diff_attn_lam_kernel, dim3((unsigned)a.H), dim3(256), 0, st, a.dlrow, glam, a.B, a.H, a.Nq);
       UBV_CHECK_LAUNCH("diff_attention_backward");
     }
   }
-  if (a.gk != nullptr) {
-    const int64_t wide = heads * ((a.Nk + 127) / 128);
-    if (wide >= kAttnFill)
-      rc = attn_launch(diff_attn_bwd_kv_kernel<T, DH, DV, 4, 1>, wide, S::bytes(64), a, st, "diff_attention_backward");
-    else
-      rc = attn_launch(diff_attn_bwd_kv_kernel<T, DH, DV, WQ, WK>, heads * ((a.Nk + 32 * WQ - 1) / (32 * WQ)), TL > MKV ? TL : MKV, a, st,
-                       "diff_attention_backward");
-  }
+  if (a.gk != nullptr)
+    rc = attn_blocks(heads, a.Nk, 4) >= kAttnFill ? run(std::true_type{}, std::false_type{}) : run(std::false_type{}, std::false_type{});
   return rc;
 }
 
@@ -695,8 +925,8 @@ static int attn_backward(const DiffAttnArgs& a, float* glam, hipStream_t st) {
   if (a.Dh <= 128 && a.Dv <= 128) DO(128, 128)                                                \
   DO(128, 256)
 
-int UBV_ATTN_NAME(forward)(const DiffAttnArgs& a, hipStream_t st) {
-#define UBV_DO(DH, DV) return attn_forward<UBV_ATTN_T, DH, DV>(a, st);
+int UBV_ATTN_NAME(forward)(const DiffAttnArgs& a, void* ws, int64_t ws_bytes, hipStream_t st) {
+#define UBV_DO(DH, DV) return attn_forward<UBV_ATTN_T, DH, DV>(a, ws, ws_bytes, st);
   UBV_ATTN_PAIRS(UBV_DO)
 #undef UBV_DO
 }

@@ -868,7 +868,9 @@ def _attn_operand(t):
     vec = 16 // t.element_size()
     if t.shape[-1] % vec:
         return torch.nn.functional.pad(t, (0, -t.shape[-1] % vec))
-    if t.stride(-1) != 1 or t.data_ptr() % 16 or any(s % vec for s, n in zip(t.stride()[:-1], t.shape) if n > 1):
+    if t.stride(-1) != 1 or t.data_ptr() % 16 or any(s % vec for s, n in zip(t.stride()[:-1], t.shape) if n > 1) or \
+            (t.shape[1] > 1 and t.stride(1) * t.element_size() >= 1 << 24) or \
+            (t.dim() == 5 and t.stride(3) * t.element_size() >= 1 << 28):
         return t.clone(memory_format=torch.contiguous_format)
     return t
 
@@ -885,13 +887,15 @@ def _attn_forward(q, k, v, lam, kpm, mask, sizes, scale, causal, drop, need):
     if not B * H * Nq * Nk:                           # no row, or nothing to see
         return q.new_zeros(B, Nq, H, Dv), None, None
     out = torch.empty(B, Nq, H, Dv, dtype=q.dtype, device=q.device)
-    lse = torch.empty(2, B, H, Nq, dtype=torch.float32, device=q.device) if need else None
+    stat = torch.empty(B, H, Nq, 4, dtype=torch.float32, device=q.device) if need else None
     maps = torch.empty(2, B, H, Nq, Dv, dtype=torch.float32, device=q.device) if need else None
     p, seed, base = drop
-    check(lib().ubv_diff_attention_forward(_p(q), _p(k), _p(v), _p(lam), _p(kpm), _p(mask), _mask_kind(mask), _p(out), _p(lse),
+    nws = int(lib().ubv_diff_attention_forward_workspace(B, H, Hk, Nq, Nk, Dv))
+    ws = torch.empty(nws, dtype=torch.uint8, device=q.device) if nws else None
+    check(lib().ubv_diff_attention_forward(_p(q), _p(k), _p(v), _p(lam), _p(kpm), _p(mask), _mask_kind(mask), _p(out), _p(stat),
                                            _p(maps), _attn_strides(q, k, v, None, mask), B, H, Hk, Nq, Nk, Dh, Dv, scale,
-                                           int(causal), p, seed, _p(base), _dt(q), _stream()), 'diff_attention_forward')
-    return out, lse, maps
+                                           int(causal), p, seed, _p(base), _dt(q), _p(ws), nws, _stream()), 'diff_attention_forward')
+    return out, stat, maps
 
 
 def _mask_kind(mask):
@@ -904,20 +908,20 @@ class _DiffAttention(Function):
         with _need_cuda(q, k, v, lam, kpm, mask):
             qc, kc, vc = _attn_operand(q), _attn_operand(k), _attn_operand(v)
             lc = lam.float().contiguous()
-            out, lse, maps = _attn_forward(qc, kc, vc, lc, kpm, mask, sizes, scale, causal, drop, True)
-            ctx.save_for_backward(qc, kc, vc, lc, kpm, mask, lse, maps)
+            out, stat, maps = _attn_forward(qc, kc, vc, lc, kpm, mask, sizes, scale, causal, drop, True)
+            ctx.save_for_backward(qc, kc, vc, lc, kpm, mask, stat, maps)
             ctx.args, ctx.lam_dtype = (sizes, scale, causal, drop), lam.dtype
             return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_out):
-        q, k, v, lam, kpm, mask, lse, maps = ctx.saved_tensors
+        q, k, v, lam, kpm, mask, stat, maps = ctx.saved_tensors
         (B, H, Hk, Nq, Nk, Dh, Dv), scale, causal, (p, seed, base) = ctx.args
         nq, nk, nv, nl = ctx.needs_input_grad[:4]
         with _need_cuda(grad_out, q):
             dev, dt = q.device, q.dtype
-            if lse is None:                           # an empty call
+            if stat is None:                           # an empty call
                 return (q.new_zeros(B, Nq, H, 2, Dh), q.new_zeros(B, Nk, Hk, 2, Dh), q.new_zeros(B, Nk, Hk, Dv),
                         torch.zeros(H, dtype=ctx.lam_dtype, device=dev), None, None, None, None, None, None)
             gq = torch.empty(B, Nq, H, 2, Dh, dtype=dt, device=dev) if nq else None
@@ -926,7 +930,7 @@ class _DiffAttention(Function):
             gl = torch.empty(H, dtype=torch.float32, device=dev) if nl else None
             go = _attn_operand(grad_out)
             ws = torch.empty(int(lib().ubv_diff_attention_backward_workspace(B, H, Nq)), dtype=torch.uint8, device=dev)
-            check(lib().ubv_diff_attention_backward(_p(go), _p(q), _p(k), _p(v), _p(lam), _p(kpm), _p(mask), _mask_kind(mask), _p(lse),
+            check(lib().ubv_diff_attention_backward(_p(go), _p(q), _p(k), _p(v), _p(lam), _p(kpm), _p(mask), _mask_kind(mask), _p(stat),
                                                     _p(maps), _p(gq), _p(gk), _p(gv), _p(gl), _attn_strides(q, k, v, go, mask), B, H,
                                                     Hk, Nq, Nk, Dh, Dv, scale, int(causal), p, seed, _p(base), _dt(q), _p(ws),
                                                     ws.numel(), _stream()), 'diff_attention_backward')
@@ -945,7 +949,7 @@ def diff_attention(q, k, v, lam, attn_mask=None, key_padding_mask=None, causal=F
     attn_mask: bool (True hides, as in ``torch.nn.MultiheadAttention``) or float (added; -inf hides), (Nq, Nk), (B H, Nq, Nk) or
     broadcastable to (B, H, Nq, Nk); it gets no gradient.  key_padding_mask: bool (B, Nk), True hides the key from every query;
     what k and v hold there is never used.  A key that only attn_mask or causal hides must be finite.  causal: query i sees keys
-    j <= i + Nk - Nq.  scale: default Dh ** -0.5.
+    j <= i + Nk - Nq.  scale: positive, default Dh ** -0.5.
 
     ``p``, ``training``, ``seed``: dropout D on the map, as in ``dropout`` (never stored)."""
     _need_cuda(q, k, v, lam, attn_mask, key_padding_mask)
@@ -985,6 +989,8 @@ def diff_attention(q, k, v, lam, attn_mask=None, key_padding_mask=None, causal=F
         key_padding_mask = key_padding_mask.contiguous()
     drop = _drop_args(p, training, seed, 'diff_attention')
     scale = float(Dh ** -0.5 if scale is None else scale)
+    if not 0.0 < scale < 1e30:
+        raise ValueError(f'diff_attention: scale {scale} must be positive and finite')
     sizes = (B, H, Hk, Nq, Nk, Dh, Dv)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or lam.requires_grad):
         return _DiffAttention.apply(q, k, v, lam, key_padding_mask, attn_mask, sizes, scale, causal, drop)
