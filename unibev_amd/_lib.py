@@ -12,6 +12,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get('UBV_LIB_PATH') or os.path.join(_HERE, 'libunibev_hip.so')
 
 _lib = None
+_native = None
 
 UBV_F32, UBV_F16, UBV_BF16 = 0, 1, 2
 
@@ -156,7 +157,26 @@ class _Hooked:
 def set_call_hook(fn):
     """Install (None: remove) a function called with the name of every C-ABI entry point about to be called."""
     prev, _CALL_HOOK[0] = _CALL_HOOK[0], fn
+    if _native is not None:
+        _native.set_hook(fn)
     return prev
+
+
+def native():
+    """Load (once) the tensor-level entries of csrc/torch_ops.cpp (``_native.so``) over the loaded library; raise loudly if
+    they are absent."""
+    global _native
+    if _native is None:
+        lib()
+        try:
+            from . import _native as ops
+        except ImportError as e:
+            raise UniBEVHipError(f'unibev_amd/_native.so cannot be loaded ({e}): build it with `python -c "import __graft_entry__ as g; '
+                                 'g.build()"` (or `make -C unibev_amd/csrc`). There is no CPU fallback.') from e
+        ops.bind({name: ctypes.cast(getattr(_lib, name), c_void_p).value for name in ops.entries()}, UniBEVHipError)
+        ops.set_hook(_CALL_HOOK[0])
+        _native = ops
+    return _native
 
 
 def lib():

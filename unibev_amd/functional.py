@@ -12,7 +12,7 @@ from torch.autograd import Function
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._lib import check, lib
+from ._lib import check, lib, native
 
 _DT = {torch.float32: _lib.UBV_F32, torch.float16: _lib.UBV_F16, torch.bfloat16: _lib.UBV_BF16}
 
@@ -759,185 +759,27 @@ def _drop_args(p, training, seed, who):
     return float(p), int(seed), None
 
 
-def _dropout_raw(x, identity, out, p, seed, base):
-    with _need_cuda(x, identity):
-        check(lib().ubv_dropout(_p(x), _p(identity), _p(out), x.numel(), p, seed, _p(base), _dt(x), _dt(out), _stream()), 'dropout')
-    return out
-
-
-class _Dropout(Function):
-    @staticmethod
-    def forward(ctx, x, identity, p, seed, base):
-        ctx.args, ctx.xdt = (p, seed, base), x.dtype
-        xc = x.contiguous()
-        idc = None if identity is None else identity.contiguous()
-        out = torch.empty(x.shape, dtype=x.dtype if idc is None else idc.dtype, device=x.device)
-        return _dropout_raw(xc, idc, out, p, seed, base)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad_y):
-        gx = None
-        if ctx.needs_input_grad[0]:
-            gy = grad_y.contiguous()
-            gx = _dropout_raw(gy, None, torch.empty(gy.shape, dtype=ctx.xdt, device=gy.device), *ctx.args)
-        return gx, grad_y if ctx.needs_input_grad[1] else None, None, None, None
-
-
 def dropout(x, p=0.0, training=False, identity=None, seed=None):
     """``identity + dropout(x, p)`` (without ``identity``: ``dropout(x, p)``) in one pass each way (``ubv_dropout``).  The mask is a
     function of the seed and the element's index and is never stored; ``p`` counts in steps of 2^-16.  Any shape; ``identity``
     has x's shape and its type, or is f32 beside a 16-bit x (the result is of identity's type).  ``seed`` fixes the mask (the same
     on every replay of a captured graph); without it each call draws its own."""
-    _need_cuda(x, identity)
-    _dt(x)
-    if identity is not None:
-        if identity.shape != x.shape:
-            raise ValueError(f'dropout: identity {tuple(identity.shape)} must have the shape of x {tuple(x.shape)}')
-        if identity.dtype != x.dtype and not (identity.dtype == torch.float32 and x.dtype in _DT):
-            raise TypeError(f'dropout: identity of {identity.dtype} beside x of {x.dtype}')
     p, seed, base = _drop_args(p, training, seed, 'dropout')
     if identity is None and p == 0.0:
+        _need_cuda(x)
+        _dt(x)
         return x
-    return _Dropout.apply(x, identity, p, seed, base)
+    return native().dropout(x, p, identity, seed, base)
 
 
 # ----------------------------------------------------------------------------------------------- layer norm
-class _LayerNorm(Function):
-    @staticmethod
-    def forward(ctx, x, gamma, beta, eps, need):
-        with _need_cuda(x, gamma, beta):
-            C = x.shape[-1]
-            xc = x.contiguous()
-            g = None if gamma is None else gamma.float().contiguous()
-            b = None if beta is None else beta.float().contiguous()
-            R = xc.numel() // C
-            y = torch.empty_like(xc)
-            stat = torch.empty(2, R, dtype=torch.float32, device=x.device) if need else None
-            check(lib().ubv_layer_norm_forward(_p(xc), _p(g), _p(b), _p(y), _p(stat[0]) if need else None,
-                                               _p(stat[1]) if need else None, R, C, float(eps), _dt(xc), _stream()),
-                  'layer_norm_forward')
-            if need:
-                ctx.save_for_backward(xc, g, stat)
-                ctx.dts = (None if gamma is None else gamma.dtype, None if beta is None else beta.dtype)
-            return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad_y):
-        xc, g, stat = ctx.saved_tensors
-        C = xc.shape[-1]
-        R = xc.numel() // C
-        nx, ng, nb = ctx.needs_input_grad[:3]
-        with _need_cuda(grad_y, xc):
-            gx = torch.empty_like(xc) if nx else None
-            dg = torch.empty(C, dtype=torch.float32, device=xc.device) if ng else None
-            db = torch.empty(C, dtype=torch.float32, device=xc.device) if nb else None
-            if R == 0:
-                dg, db = (None if t is None else t.zero_() for t in (dg, db))
-            else:
-                gy = grad_y.contiguous()
-                ws = torch.empty(int(lib().ubv_layer_norm_backward_workspace(R, C)), dtype=torch.uint8,
-                                 device=xc.device) if ng or nb else None
-                check(lib().ubv_layer_norm_backward(_p(gy), _p(xc), _p(g), _p(stat[0]), _p(stat[1]), _p(gx), _p(dg), _p(db), R, C,
-                                                    _dt(xc), _p(ws), 0 if ws is None else ws.numel(), _stream()),
-                      'layer_norm_backward')
-            return (gx, dg if dg is None else dg.to(ctx.dts[0]), db if db is None else db.to(ctx.dts[1]), None, None)
-
-
 def layer_norm(x, gamma=None, beta=None, eps=1e-5):
     """Layer norm over the last axis of any width (``ubv_layer_norm_*``): x (..., C) of f32 / f16 / bf16, ``gamma`` and ``beta``
     (C,) or None (taken in f32).  Statistics in f32; the weights' gradients are summed in fixed order."""
-    _need_cuda(x, gamma, beta)
-    _dt(x)
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise ValueError(f'layer_norm: x {tuple(x.shape)} has no last axis to normalise')
-    for name, w in (('gamma', gamma), ('beta', beta)):
-        if w is not None and w.shape != x.shape[-1:]:
-            raise ValueError(f'layer_norm: {name} {tuple(w.shape)} must be ({x.shape[-1]},)')
-        if w is not None:
-            _dt(w)
-    need = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, gamma, beta))
-    return _LayerNorm.apply(x, gamma, beta, eps, need)
+    return native().layer_norm(x, gamma, beta, eps)
 
 
 # ----------------------------------------------------------------------------------------------- differential attention
-def _attn_operand(t):
-    """``t`` as the attention kernels take it — last axis contiguous and whole 16-byte pieces, every row 16-byte aligned — as it is
-    where it already is so (views, expanded axes), else a copy (zero-padded last axis)."""
-    vec = 16 // t.element_size()
-    if t.shape[-1] % vec:
-        return torch.nn.functional.pad(t, (0, -t.shape[-1] % vec))
-    if t.stride(-1) != 1 or t.data_ptr() % 16 or any(s % vec for s, n in zip(t.stride()[:-1], t.shape) if n > 1) or \
-            (t.shape[1] > 1 and t.stride(1) * t.element_size() >= 1 << 24) or \
-            (t.dim() == 5 and t.stride(3) * t.element_size() >= 1 << 28):
-        return t.clone(memory_format=torch.contiguous_format)
-    return t
-
-
-def _attn_strides(q, k, v, go, mask):
-    out = []
-    for t, n in ((q, 4), (k, 4), (v, 3), (go, 3), (mask, 4)):
-        out += [0] * n if t is None else [s if m > 1 else 0 for s, m in zip(t.stride()[:n], t.shape)]
-    return (ctypes.c_int64 * len(out))(*out)
-
-
-def _attn_forward(q, k, v, lam, kpm, mask, sizes, scale, causal, drop, need):
-    B, H, Hk, Nq, Nk, Dh, Dv = sizes
-    if not B * H * Nq * Nk:                           # no row, or nothing to see
-        return q.new_zeros(B, Nq, H, Dv), None, None
-    out = torch.empty(B, Nq, H, Dv, dtype=q.dtype, device=q.device)
-    stat = torch.empty(B, H, Nq, 4, dtype=torch.float32, device=q.device) if need else None
-    maps = torch.empty(2, B, H, Nq, Dv, dtype=torch.float32, device=q.device) if need else None
-    p, seed, base = drop
-    nws = int(lib().ubv_diff_attention_forward_workspace(B, H, Hk, Nq, Nk, Dv))
-    ws = torch.empty(nws, dtype=torch.uint8, device=q.device) if nws else None
-    check(lib().ubv_diff_attention_forward(_p(q), _p(k), _p(v), _p(lam), _p(kpm), _p(mask), _mask_kind(mask), _p(out), _p(stat),
-                                           _p(maps), _attn_strides(q, k, v, None, mask), B, H, Hk, Nq, Nk, Dh, Dv, scale,
-                                           int(causal), p, seed, _p(base), _dt(q), _p(ws), nws, _stream()), 'diff_attention_forward')
-    return out, stat, maps
-
-
-def _mask_kind(mask):
-    return 0 if mask is None else 1 if mask.dtype == torch.bool else 2
-
-
-class _DiffAttention(Function):
-    @staticmethod
-    def forward(ctx, q, k, v, lam, kpm, mask, sizes, scale, causal, drop):
-        with _need_cuda(q, k, v, lam, kpm, mask):
-            qc, kc, vc = _attn_operand(q), _attn_operand(k), _attn_operand(v)
-            lc = lam.float().contiguous()
-            out, stat, maps = _attn_forward(qc, kc, vc, lc, kpm, mask, sizes, scale, causal, drop, True)
-            ctx.save_for_backward(qc, kc, vc, lc, kpm, mask, stat, maps)
-            ctx.args, ctx.lam_dtype = (sizes, scale, causal, drop), lam.dtype
-            return out
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad_out):
-        q, k, v, lam, kpm, mask, stat, maps = ctx.saved_tensors
-        (B, H, Hk, Nq, Nk, Dh, Dv), scale, causal, (p, seed, base) = ctx.args
-        nq, nk, nv, nl = ctx.needs_input_grad[:4]
-        with _need_cuda(grad_out, q):
-            dev, dt = q.device, q.dtype
-            if stat is None:                           # an empty call
-                return (q.new_zeros(B, Nq, H, 2, Dh), q.new_zeros(B, Nk, Hk, 2, Dh), q.new_zeros(B, Nk, Hk, Dv),
-                        torch.zeros(H, dtype=ctx.lam_dtype, device=dev), None, None, None, None, None, None)
-            gq = torch.empty(B, Nq, H, 2, Dh, dtype=dt, device=dev) if nq else None
-            gk = torch.empty(B, Nk, Hk, 2, Dh, dtype=dt, device=dev) if nk or nv else None
-            gv = torch.empty(B, Nk, Hk, Dv, dtype=dt, device=dev) if nk or nv else None
-            gl = torch.empty(H, dtype=torch.float32, device=dev) if nl else None
-            go = _attn_operand(grad_out)
-            ws = torch.empty(int(lib().ubv_diff_attention_backward_workspace(B, H, Nq)), dtype=torch.uint8, device=dev)
-            check(lib().ubv_diff_attention_backward(_p(go), _p(q), _p(k), _p(v), _p(lam), _p(kpm), _p(mask), _mask_kind(mask), _p(stat),
-                                                    _p(maps), _p(gq), _p(gk), _p(gv), _p(gl), _attn_strides(q, k, v, go, mask), B, H,
-                                                    Hk, Nq, Nk, Dh, Dv, scale, int(causal), p, seed, _p(base), _dt(q), _p(ws),
-                                                    ws.numel(), _stream()), 'diff_attention_backward')
-            return (gq, gk if nk else None, gv if nv else None, gl if gl is None else gl.to(ctx.lam_dtype),
-                    None, None, None, None, None, None)
-
-
 def diff_attention(q, k, v, lam, attn_mask=None, key_padding_mask=None, causal=False, scale=None, p=0.0, training=False, seed=None):
     """Differential attention ``(D o (softmax(scale q_1 k_1^T + mask) - lam softmax(scale q_2 k_2^T + mask))) v`` in one kernel forward
     (``ubv_diff_attention_*``); no score is ever stored.
@@ -952,51 +794,8 @@ def diff_attention(q, k, v, lam, attn_mask=None, key_padding_mask=None, causal=F
     j <= i + Nk - Nq.  scale: positive, default Dh ** -0.5.
 
     ``p``, ``training``, ``seed``: dropout D on the map, as in ``dropout`` (never stored)."""
-    _need_cuda(q, k, v, lam, attn_mask, key_padding_mask)
-    if q.dim() != 5 or k.dim() != 5 or v.dim() != 4 or q.shape[3] != 2 or k.shape[3] != 2:
-        raise ValueError(f'diff_attention: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} must be (B, Nq, H, 2, Dh), '
-                         '(B, Nk, Hk, 2, Dh), (B, Nk, Hk, Dv)')
-    B, Nq, H, _, Dh = q.shape
-    _, Nk, Hk, _, _ = k.shape
-    Dv = v.shape[3]
-    if k.shape != (B, Nk, Hk, 2, Dh) or v.shape != (B, Nk, Hk, Dv):
-        raise ValueError(f'diff_attention: q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not belong together')
-    if Hk < 1 or H % Hk:
-        raise ValueError(f'diff_attention: {H} query heads do not share {Hk} key heads evenly')
-    if not (1 <= Dh <= 128 and 1 <= Dv <= 256):
-        raise ValueError(f'diff_attention: head widths {Dh} and {Dv} (at most 128 and 256)')
-    _dt(q)
-    if not q.dtype == k.dtype == v.dtype:
-        raise TypeError(f'diff_attention: q, k and v of {q.dtype}, {k.dtype} and {v.dtype}')
-    if not lam.is_floating_point() or (lam.numel() != 1 and lam.shape != (H,)):
-        raise ValueError(f'diff_attention: lam {tuple(lam.shape)} of {lam.dtype} must be ({H},) or one value')
-    lam = lam.reshape(1).expand(H) if lam.numel() == 1 else lam
-    if attn_mask is not None:
-        if attn_mask.requires_grad:
-            raise ValueError('diff_attention: attn_mask gets no gradient; detach it')
-        if attn_mask.dtype != torch.bool and not attn_mask.is_floating_point():
-            raise TypeError(f'diff_attention: attn_mask of {attn_mask.dtype} (bool or float)')
-        m = attn_mask if attn_mask.dtype == torch.bool else attn_mask.float()
-        if m.dim() == 3 and m.shape == (B * H, Nq, Nk):
-            m = m.view(B, H, Nq, Nk) if m.is_contiguous() else m.reshape(B, H, Nq, Nk)
-        if m.dim() not in (2, 4) or any(s not in (1, t) for s, t in zip(m.shape[::-1], (Nk, Nq, H, B))):
-            raise ValueError(f'diff_attention: attn_mask {tuple(attn_mask.shape)} does not broadcast to {(B, H, Nq, Nk)}')
-        attn_mask = m.expand(B, H, Nq, Nk)
-    if key_padding_mask is not None:
-        if key_padding_mask.dtype != torch.bool or key_padding_mask.shape != (B, Nk):
-            raise ValueError(f'diff_attention: key_padding_mask {tuple(key_padding_mask.shape)} of {key_padding_mask.dtype} must be '
-                             f'bool {(B, Nk)}')
-        key_padding_mask = key_padding_mask.contiguous()
-    drop = _drop_args(p, training, seed, 'diff_attention')
-    scale = float(Dh ** -0.5 if scale is None else scale)
-    if not 0.0 < scale < 1e30:
-        raise ValueError(f'diff_attention: scale {scale} must be positive and finite')
-    sizes = (B, H, Hk, Nq, Nk, Dh, Dv)
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or lam.requires_grad):
-        return _DiffAttention.apply(q, k, v, lam, key_padding_mask, attn_mask, sizes, scale, causal, drop)
-    with _need_cuda(q, k, v, lam, attn_mask, key_padding_mask):
-        return _attn_forward(_attn_operand(q), _attn_operand(k), _attn_operand(v), lam.float().contiguous(), key_padding_mask, attn_mask,
-                             sizes, scale, causal, drop, False)[0]
+    p, seed, base = _drop_args(p, training, seed, 'diff_attention')
+    return native().diff_attention(q, k, v, lam, attn_mask, key_padding_mask, causal, scale, p, seed, base)
 
 
 # ----------------------------------------------------------------------------------------------- linear forward
