@@ -40,9 +40,25 @@ struct DiffAttnArgs {
   float2* rowl;                            // [B H Nq] {l_1, l_2}, with a float mask only
   float* dlrow;                            // [B H Nq] - sum_j A_2 G
   void *gq, *gk, *gv;                      // contiguous gradients
+  int work;                                // blocks with work (the grid is rounded up)
   int splits;                              // forward: blocks that share a row tile's keys, 1: none
-  float* part;                             // forward, splits > 1: [splits][tiles][(4 + DV) 64] maxima, sums, products
+  int halves;                              // forward: blocks that share a row tile's output columns
+  float* part;                             // forward, splits > 1: [tile][half][split][64 lanes][4 + columns] references, sums, products
 };
+
+// Splits of a row tile's keys in the forward pass: four blocks a CU where there are few row tiles, at least 512 keys each.
+constexpr int kAttnSplits = 1024;
+static inline int64_t attn_row_tiles(int B, int H, int Hk, int Nq, int Dv) {
+  return (int64_t)B * Hk * (((int64_t)(H / Hk) * Nq + 31) / 32) * (Dv > 128 ? 2 : 1);
+}
+static inline int64_t attn_splits(int B, int H, int Hk, int Nq, int Nk, int Dv) {
+  const int64_t tiles = attn_row_tiles(B, H, Hk, Nq, Dv), want = tiles > 128 ? 1 : (kAttnSplits + tiles - 1) / tiles, most = Nk / 512;
+  return want < most ? want : most > 1 ? most : 1;
+}
+static inline int64_t attn_part_bytes(int B, int H, int Hk, int Nq, int Dv, int64_t splits) {
+  const int width = Dv <= 32 ? 32 : Dv <= 64 ? 64 : 128;
+  return splits <= 1 ? 0 : attn_row_tiles(B, H, Hk, Nq, Dv) * splits * (4 + width) * 64 * 4;
+}
 
 // f16 holds nothing below 2^-24 and loses bits below 2^-14, which the probabilities of a long row reach: they enter the matrix
 // instructions 2^8 larger and their products leave 2^8 smaller (|lam| up to 255 stays in range)

@@ -45,11 +45,9 @@ static int attn_args(DiffAttnArgs& a, const void* q, const void* k, const void* 
 }  // namespace ubv
 
 extern "C" int64_t ubv_diff_attention_forward_workspace(int B, int H, int Hk, int Nq, int Nk, int Dv) {
-  // the partial sums of the most splits that attn_forward takes: 2 kAttnFill blocks of 32 rows' (4 + width) floats
-  if (B <= 0 || Hk <= 0 || H % Hk != 0 || Nq <= 0 || Nk < 256) return 0;
-  const int64_t blocks = (int64_t)B * Hk * (((int64_t)(H / Hk) * Nq + 31) / 32), splits = (1024 + blocks - 1) / blocks;
-  const int64_t most = (Nk + 31) / 32 / 4, width = Dv <= 32 ? 32 : Dv <= 64 ? 64 : Dv <= 128 ? 128 : 256;
-  return blocks >= 256 ? 0 : blocks * (splits < most ? splits : most) * (4 + width) * 64 * 4;
+  using namespace ubv;
+  if (B <= 0 || Hk <= 0 || H % Hk != 0 || Nq <= 0 || Nk <= 0) return 0;
+  return attn_part_bytes(B, H, Hk, Nq, Dv, attn_splits(B, H, Hk, Nq, Nk, Dv));
 }
 
 extern "C" int ubv_diff_attention_forward(const void* q, const void* k, const void* v, const float* lam, const uint8_t* key_padding_mask,

@@ -32,9 +32,14 @@ template <typename T, int DH, int DV, bool SHARED> struct AttnPlan {
   static constexpr int LDS = (SHARED ? 2 : WK) * S::bytes(N);
   static constexpr int merge(int floats) { return SHARED ? 0 : (WK / 2) * floats * 64 * 4; }     // joining `floats` per lane
   static constexpr int lds(int floats) { return LDS > merge(floats) ? LDS : merge(floats); }
-  // registers for two waves a SIMD where accumulators, operands and a tile in flight fit into half of them
-  static constexpr int MINW = (elem<T>::kBytes == 2 ? DH <= 64 && DV <= 128 : DH <= 32 && DV <= 64) ? 2 : 1;
+  // two waves a SIMD where accumulators, operands and a tile in flight fit half the registers (64 / 128, f16: forward 244 us with
+  // two waves that spill, 167 with one that does not)
+  static constexpr int MINW = DH <= 32 && DV <= 64 ? 2 : 1;
 };
+
+// What a call may hold beside hidden keys.  Each has kernels of its own: what a kernel can never meet costs it registers, and
+// with them a wave per SIMD (32 / 64 wide heads, bf16, 10 000 x 10 000: grad_k / grad_v 738 us with everything, 448 plain).
+constexpr int kAttnPlain = 0, kAttnDrop = 1, kAttnAny = 2;       // nothing | dropout | masks, causal, dropout or not
 
 // ---- staging ------------------------------------------------------------------------------------------------------------------
 template <typename T, int DH, int DV, int N, int LT> struct AttnStage {
@@ -147,7 +152,7 @@ __device__ __forceinline__ bool key_hidden(const DiffAttnArgs& a, int b, int j0,
 }
 
 // hides keys of a tile from the lane's row (query i of head h): `hid` bits of the 32 keys from j0, causal, the call's mask
-__device__ __forceinline__ void mask_tile(const DiffAttnArgs& a, af32x16_t (&x)[2], uint32_t hid, int b, int h, int i, int j0, float rscale,
+template <bool MASK> __device__ __forceinline__ void mask_tile(const DiffAttnArgs& a, af32x16_t (&x)[2], uint32_t hid, int b, int h, int i, int j0, float rscale,
                                           int lane) {
   const int half = 4 * (lane >> 5);
   if (hid != 0) {
@@ -156,6 +161,7 @@ __device__ __forceinline__ void mask_tile(const DiffAttnArgs& a, af32x16_t (&x)[
     for (int e = 0; e < 16; ++e)
       if (w & (1u << (8 * (e >> 2) + (e & 3)))) { x[0][e] = kNegInf; x[1][e] = kNegInf; }
   }
+  if constexpr (!MASK) return;
   if (a.causal) {
     const int lim = i + a.Nk - a.Nq - j0 - half;
     if (__any(lim < 31 - half)) {
@@ -203,6 +209,10 @@ __device__ __forceinline__ void mask_tile(const DiffAttnArgs& a, af32x16_t (&x)[
   }
 }
 
+// Blocks go round-robin over the 8 XCDs: XCD x takes the x-th eighth of the tiles, so that the tiles of a head, which read the
+// same keys (or rows), meet in one L2.  The grid is rounded up; a tile past the end has no work.
+__device__ __forceinline__ int xcd_tile(int blocks) { return xcd_remap(blockIdx.x, blocks >> 3); }
+
 // what forward and grad_q share: own = rows
 struct RowWave {
   int wave, lane, wq, wk, b, hk, rb, r, h, i;
@@ -210,7 +220,7 @@ struct RowWave {
   int64_t rowid;
   int kend;                            // keys that some row of the block sees: [0, kend)
 
-  template <int WQ, int WK> __device__ __forceinline__ void init(const DiffAttnArgs& a, int tile) {
+  template <int WQ, int WK, bool MASK> __device__ __forceinline__ void init(const DiffAttnArgs& a, int tile) {
     wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     lane = threadIdx.x & 63;
     wq = wave / WK; wk = wave % WK;
@@ -223,7 +233,7 @@ struct RowWave {
     h = hk * a.G + g; i = rc - g * a.Nq;
     rowid = ((int64_t)b * a.H + hk * a.G) * a.Nq + rc;
     kend = a.Nk;
-    if (a.causal) {
+    if (MASK && a.causal) {
       const int last = min(rb + 32 * WQ, a.R) - 1;
       const int imax = rb / a.Nq == last / a.Nq ? last % a.Nq : a.Nq - 1;
       kend = max(0, min(a.Nk, imax + a.Nk - a.Nq + 1));
@@ -233,7 +243,7 @@ struct RowWave {
 
 // the stream of staged key tiles: f(tile of T, it0, hid of its 32 keys, j0) for every 32 keys that are not all hidden
 template <typename T, int DH, int DV, bool SHARED, typename F>
-__device__ __forceinline__ void key_tiles(const DiffAttnArgs& a, const RowWave& w, int t0, int t1, char* smem, F&& f) {
+__device__ __forceinline__ void key_tiles(const DiffAttnArgs& a, const RowWave& w, int col, int t0, int t1, char* smem, F&& f) {
   using S = AttnTile<T, DH, DV>;
   using P = AttnPlan<T, DH, DV, SHARED>;
   constexpr int N = P::N, STEP = P::WK;
@@ -241,9 +251,9 @@ __device__ __forceinline__ void key_tiles(const DiffAttnArgs& a, const RowWave& 
   const int st = SHARED ? threadIdx.x : w.lane;
   AttnStage<T, DH, DV, N, P::LT> sg;
   const uint32_t xrow = (uint32_t)(a.ks[1] * elem<T>::kBytes), yrow = (uint32_t)(a.vs[1] * elem<T>::kBytes);
-  sg.init(st, xrow, (uint32_t)(a.ks[3] * elem<T>::kBytes), yrow, a.Dh, a.Dv);
+  sg.init(st, xrow, (uint32_t)(a.ks[3] * elem<T>::kBytes), yrow, a.Dh, a.Dv - col);
   const char* kb = (const char*)a.k + (w.b * a.ks[0] + w.hk * a.ks[2]) * elem<T>::kBytes;
-  const char* vb = (const char*)a.v + (w.b * a.vs[0] + w.hk * a.vs[2]) * elem<T>::kBytes;
+  const char* vb = (const char*)a.v + (w.b * a.vs[0] + w.hk * a.vs[2] + col) * elem<T>::kBytes;
   int t = t0 + w.wk;
   if (t >= t1) return;                                       // (private waves only: no barrier inside)
   auto load = [&](int tt, uint64_t hid) {
@@ -311,6 +321,18 @@ template <typename T, int DV> struct FwdState {
         for (int e = 0; e < 16; ++e) slot[(4 + (m * VO + d) * 16 + e) * 64] = acc[m][d][e];
     }
   }
+  // the same, a lane's FLOATS in one stretch (only the lanes of rows are written: few rows are few bytes)
+  __device__ __forceinline__ void put_row(float* at) const {
+    *reinterpret_cast<float4*>(at) = make_float4(top[0], l[0], top[1], l[1]);
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int d = 0; d < VO; ++d)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          *reinterpret_cast<float4*>(at + 4 + (m * VO + d) * 16 + 4 * q) =
+              make_float4(acc[m][d][4 * q], acc[m][d][4 * q + 1], acc[m][d][4 * q + 2], acc[m][d][4 * q + 3]);
+  }
   // joins what another wave put for the same rows
   __device__ __forceinline__ void join(const float* slot, float c) {
 #pragma unroll
@@ -330,7 +352,7 @@ template <typename T, int DV> struct FwdState {
 
 // the rows' outputs and what the backward pass wants, from the joined state
 template <typename T, int DV>
-__device__ __forceinline__ void fwd_finish(const DiffAttnArgs& a, const FwdState<T, DV>& s, const RowWave& w, float c) {
+__device__ __forceinline__ void fwd_finish(const DiffAttnArgs& a, const FwdState<T, DV>& s, const RowWave& w, int col, float c) {
   if (!w.ok) return;
   const bool fm = a.mask_kind == 2;
   const int64_t rows = (int64_t)a.B * a.H * a.Nq;
@@ -344,13 +366,13 @@ __device__ __forceinline__ void fwd_finish(const DiffAttnArgs& a, const FwdState
     st[2 * m] = dead ? 0.0f : fm ? s.top[m] : s.top[m] * c - kProbShift<T>;
     st[2 * m + 1] = dead ? -kNegInf : fm ? log2f(l) - kProbShift<T> : log2f(l);
   }
-  if (a.stat != nullptr && w.lane < 32) a.stat[w.rowid] = make_float4(st[0], st[1], st[2], st[3]);
+  if (a.stat != nullptr && w.lane < 32 && col == 0) a.stat[w.rowid] = make_float4(st[0], st[1], st[2], st[3]);
   T* orow = (T*)a.out + (((int64_t)w.b * a.Nq + w.i) * a.H + w.h) * a.Dv;
 #pragma unroll
   for (int d = 0; d < DV / 32; ++d)
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      const int dv = 32 * d + tile_item(4 * q, w.lane);
+      const int dv = col + 32 * d + tile_item(4 * q, w.lane);
       float o1[4], o2[4], o[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -366,34 +388,37 @@ __device__ __forceinline__ void fwd_finish(const DiffAttnArgs& a, const FwdState
     }
 }
 
-template <typename T, int DH, int DV, bool SHARED>
+template <typename T, int DH, int DV, bool SHARED, int MODE>
 __global__ __launch_bounds__((AttnPlan<T, DH, DV, SHARED>::NT), (AttnPlan<T, DH, DV, SHARED>::MINW)) void diff_attn_fwd_kernel(
     const DiffAttnArgs a) {
   using S = AttnTile<T, DH, DV>;
   using P = AttnPlan<T, DH, DV, SHARED>;
   using M = amma<T>;
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  const int tile = blockIdx.x / a.splits, split = blockIdx.x - tile * a.splits;
+  const int id = xcd_tile(gridDim.x);
+  if (id >= a.work) return;
+  const int part = id / a.splits, split = id - part * a.splits, tile = part / a.halves, col = (part - tile * a.halves) * DV;
   RowWave w;
-  w.init<P::WQ, P::WK>(a, tile);
+  w.init<P::WQ, P::WK, MODE == kAttnAny>(a, tile);
   typename M::frag qf[2][S::KB];
 #pragma unroll
   for (int m = 0; m < 2; ++m)
     own_frags<T, S::KB>(qf[m], (const T*)a.q + w.b * a.qs[0] + w.i * a.qs[1] + w.h * a.qs[2] + m * a.qs[3], w.ok, a.Dh, w.lane);
   const float c = a.scale * kLog2e, rscale = 1.0f / a.scale, grow = 6.0f / c;
-  const bool fm = a.mask_kind == 2, drop = a.t16 != 0;
+  constexpr bool MASK = MODE == kAttnAny;
+  const bool fm = MASK && a.mask_kind == 2, drop = MODE != kAttnPlain && a.t16 != 0;
   const uint32_t t32 = a.t16 << 16;
   const uint64_t zrow = attn_seed(a.seed, a.seed_dev) + (uint64_t)(w.rowid * a.n4) + (w.lane >> 5);
   FwdState<T, DV> s;
   s.init();
   float mu[2] = {0.0f, 0.0f};
   const int tn = (w.kend + P::N - 1) / P::N, per = (tn + a.splits - 1) / a.splits;
-  key_tiles<T, DH, DV, SHARED>(a, w, split * per, min(tn, (split + 1) * per), smem,
+  key_tiles<T, DH, DV, SHARED>(a, w, col, split * per, min(tn, (split + 1) * per), smem,
                                [&](const T* kt, int it0, uint32_t hid, int j0) {
     af32x16_t x[2];
 #pragma unroll
     for (int m = 0; m < 2; ++m) x[m] = tile_dot<T, S::KB, S::LDK>(kt + m * P::N * S::LDK, it0, qf[m], w.lane);
-    if (hid != 0 || a.causal || a.mask_kind != 0) mask_tile(a, x, hid, w.b, w.h, w.i, j0, rscale, w.lane);
+    if (hid != 0 || (MASK && (a.causal || a.mask_kind != 0))) mask_tile<MASK>(a, x, hid, w.b, w.h, w.i, j0, rscale, w.lane);
     float p[2][16];
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
@@ -458,32 +483,75 @@ __global__ __launch_bounds__((AttnPlan<T, DH, DV, SHARED>::NT), (AttnPlan<T, DH,
     if (w.wk != 0) return;
   }
   if (a.splits > 1) {
-    s.put(a.part + ((int64_t)blockIdx.x * P::WQ + w.wq) * (s.FLOATS * 64) + w.lane);
+    if (w.ok) s.put_row(a.part + ((int64_t)id * 64 + w.lane) * s.FLOATS);
     return;
   }
-  fwd_finish<T, DV>(a, s, w, c);
+  fwd_finish<T, DV>(a, s, w, col, c);
 }
 
-// joins the splits of a row tile in split order, one wave a tile of 32 rows
-template <typename T, int DV, int WQ>
-__global__ __launch_bounds__(64) void diff_attn_join_kernel(const DiffAttnArgs a) {
+// Joins the splits of a row: one block a row (and column half), a thread an element of one map's product.  Weights of the splits
+// first (one exponential each, in LDS), then the products' sum in split order.
+template <typename T, int DV>
+__global__ __launch_bounds__(256) void diff_attn_join_kernel(const DiffAttnArgs a) {
+  constexpr int FLOATS = FwdState<T, DV>::FLOATS, VO = DV / 32;
+  __shared__ float wt[2][kAttnSplits], red[4][4], o2s[128];
   const float c = a.scale * kLog2e;
-  RowWave w;
-  const int tile = blockIdx.x / WQ;
-  w.init<WQ, 1>(a, tile);
-  w.wq = blockIdx.x % WQ;
-  if (WQ > 1) {                                       // (the wave is that group's)
-    w.r = w.rb + 32 * w.wq + (w.lane & 31);
-    w.ok = w.r < a.R;
-    const int rc = w.ok ? w.r : a.R - 1, g = rc / a.Nq;
-    w.h = w.hk * a.G + g; w.i = rc - g * a.Nq;
-    w.rowid = ((int64_t)w.b * a.H + w.hk * a.G) * a.Nq + rc;
+  const int part = blockIdx.x, half = part % a.halves, row = part / a.halves, bh = row / a.R, r = row - bh * a.R;
+  const int tiles = (a.R + 31) / 32, tile = bh * tiles + r / 32, lane = r % 32, col = half * DV;
+  const int b = bh / a.Hk, hk = bh - b * a.Hk, h = hk * a.G + r / a.Nq, i = r % a.Nq;
+  const int64_t rows = (int64_t)a.B * a.H * a.Nq, rowid = ((int64_t)b * a.H + h) * a.Nq + i;
+  const float* p = a.part + ((int64_t)(tile * a.halves + half) * a.splits * 64 + lane) * FLOATS;      // split n, lane half: + (64 n + 32 s) FLOATS
+  const int t = threadIdx.x, wave = t >> 6;
+  auto block = [&](float x, float y, bool is_max, float& ox, float& oy) {
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1) {
+      const float u = __shfl_xor(x, m, 64), v = __shfl_xor(y, m, 64);
+      x = is_max ? fmaxf(x, u) : x + u;
+      y = is_max ? fmaxf(y, v) : y + v;
+    }
+    __syncthreads();
+    if ((t & 63) == 0) { red[wave][0] = x; red[wave][1] = y; }
+    __syncthreads();
+    ox = red[0][0]; oy = red[0][1];
+#pragma unroll
+    for (int w = 1; w < 4; ++w) {
+      ox = is_max ? fmaxf(ox, red[w][0]) : ox + red[w][0];
+      oy = is_max ? fmaxf(oy, red[w][1]) : oy + red[w][1];
+    }
+  };
+  float m1 = kNegInf, m2 = kNegInf, top[2], l[2], l1 = 0.0f, l2 = 0.0f;
+  for (int n = t; n < a.splits; n += 256) {
+    const float4 s = *reinterpret_cast<const float4*>(p + (int64_t)64 * n * FLOATS);
+    m1 = fmaxf(m1, s.x); m2 = fmaxf(m2, s.z);
   }
-  FwdState<T, DV> s;
-  s.init();
-  for (int n = 0; n < a.splits; ++n)
-    s.join(a.part + (((int64_t)tile * a.splits + n) * WQ + w.wq) * (s.FLOATS * 64) + w.lane, c);
-  fwd_finish<T, DV>(a, s, w, c);
+  block(m1, m2, true, top[0], top[1]);
+  for (int n = t; n < a.splits; n += 256) {
+    const float4 s = *reinterpret_cast<const float4*>(p + (int64_t)64 * n * FLOATS);
+    const float4 s2 = *reinterpret_cast<const float4*>(p + (int64_t)(64 * n + 32) * FLOATS);
+    wt[0][n] = s.x == kNegInf ? 0.0f : aexp2((s.x - top[0]) * c);
+    wt[1][n] = s.z == kNegInf ? 0.0f : aexp2((s.z - top[1]) * c);
+    l1 = fmaf(s.y + s2.y, wt[0][n], l1);
+    l2 = fmaf(s.w + s2.w, wt[1][n], l2);
+  }
+  block(l1, l2, false, l[0], l[1]);                  // (its barriers also order the weights)
+  const int m = t >> 7, d = t & 127;
+  float o = 0.0f;
+  if (d < DV) {
+    const float* e = p + (int64_t)(32 * ((d >> 2) & 1)) * FLOATS + 4 + (m * VO + (d >> 5)) * 16 + 4 * ((d >> 3) & 3) + (d & 3);
+#pragma unroll 8
+    for (int n = 0; n < a.splits; ++n) o = fmaf(e[(int64_t)64 * n * FLOATS], wt[m][n], o);
+  }
+  const bool fm = a.mask_kind == 2, dead = l[m] == 0.0f;
+  o *= dead ? 0.0f : a.up / l[m];
+  if (m == 1) o2s[d] = o;
+  __syncthreads();
+  const bool in = d < DV && col + d < a.Dv;
+  if (a.o != nullptr && in) a.o[(m * rows + rowid) * a.Dv + col + d] = o;
+  if (m == 0 && in)
+    ((T*)a.out)[(((int64_t)b * a.Nq + i) * a.H + h) * a.Dv + col + d] = elem<T>::from_float(fmaf(-a.lam[h], o2s[d], o));
+  if (a.stat != nullptr && col == 0 && d == 0)
+    reinterpret_cast<float2*>(a.stat + rowid)[m] =
+        make_float2(dead ? 0.0f : fm ? top[m] : top[m] * c - kProbShift<T>, dead ? -kNegInf : fm ? log2f(l[m]) - kProbShift<T> : log2f(l[m]));
 }
 
 // ---- backward: del_m = grad_out . o_m per row, 16 lanes a row; the statistics as row_probability takes them -------------------
@@ -539,16 +607,19 @@ __device__ __forceinline__ void join_waves(af32x16_t* const (&acc)[NB], float* s
 }
 
 // ---- backward: grad_q and the rows' parts of grad_lam; own = rows, staged = keys -----------------------------------------------
-template <typename T, int DH, int DV, bool SHARED>
+template <typename T, int DH, int DV, bool SHARED, int MODE>
 __global__ __launch_bounds__((AttnPlan<T, DH, DV, SHARED>::NT), (AttnPlan<T, DH, DV, SHARED>::MINW)) void diff_attn_bwd_q_kernel(
     const DiffAttnArgs a) {
   using S = AttnTile<T, DH, DV>;
   using P = AttnPlan<T, DH, DV, SHARED>;
   using M = amma<T>;
   extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int tile = xcd_tile(gridDim.x);
+  if (tile >= a.work) return;
   RowWave w;
-  w.init<P::WQ, P::WK>(a, blockIdx.x);
-  const bool fm = a.mask_kind == 2, drop = a.t16 != 0;
+  w.init<P::WQ, P::WK, MODE == kAttnAny>(a, tile);
+  constexpr bool MASK = MODE == kAttnAny;
+  const bool fm = MASK && a.mask_kind == 2, drop = MODE != kAttnPlain && a.t16 != 0;
   typename M::frag qf[2][S::KB], gf[S::VB];
 #pragma unroll
   for (int m = 0; m < 2; ++m)
@@ -565,12 +636,12 @@ __global__ __launch_bounds__((AttnPlan<T, DH, DV, SHARED>::NT), (AttnPlan<T, DH,
   for (int m = 0; m < 2; ++m)
 #pragma unroll
     for (int d = 0; d < S::KO; ++d) acc[m][d] = af32x16_t{0.0f};
-  key_tiles<T, DH, DV, SHARED>(a, w, 0, (w.kend + P::N - 1) / P::N, smem, [&](const T* kt, int it0, uint32_t hid, int j0) {
+  key_tiles<T, DH, DV, SHARED>(a, w, 0, 0, (w.kend + P::N - 1) / P::N, smem, [&](const T* kt, int it0, uint32_t hid, int j0) {
     af32x16_t x[2];
 #pragma unroll
     for (int m = 0; m < 2; ++m) x[m] = tile_dot<T, S::KB, S::LDK>(kt + m * P::N * S::LDK, it0, qf[m], w.lane);
     af32x16_t g = tile_dot<T, S::VB, S::LDV>(kt + 2 * P::N * S::LDK, it0, gf, w.lane);
-    if (hid != 0 || a.causal || a.mask_kind != 0) mask_tile(a, x, hid, w.b, w.h, w.i, j0, rscale, w.lane);
+    if (hid != 0 || (MASK && (a.causal || a.mask_kind != 0))) mask_tile<MASK>(a, x, hid, w.b, w.h, w.i, j0, rscale, w.lane);
     if (drop) {
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
@@ -650,7 +721,9 @@ __global__ __launch_bounds__(256) static void diff_attn_lam_kernel(const float* 
 
 // ---- backward: grad_k and grad_v; own = keys, staged = the rows of every head that shares them ----------------------------------
 // A tile of rows stays inside one head (its rows are one stretch of queries), heads one after the other.
-template <typename T, int DH, int DV, bool SHARED>
+// PART 0: both gradients in one pass; 1: grad_k, 2: grad_v by a pass of its own, where the accumulators of both (2 DH + DV
+// floats a lane's item pair) would not fit the register file (the scores are computed twice: less than spilling costs).
+template <typename T, int DH, int DV, bool SHARED, int MODE, int PART>
 __global__ __launch_bounds__((AttnPlan<T, DH, DV, SHARED>::NT), (AttnPlan<T, DH, DV, SHARED>::MINW)) void diff_attn_bwd_kv_kernel(
     const DiffAttnArgs a) {
   using S = AttnTile<T, DH, DV>;
@@ -659,19 +732,22 @@ __global__ __launch_bounds__((AttnPlan<T, DH, DV, SHARED>::NT), (AttnPlan<T, DH,
   constexpr int N = P::N;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, wq = wave / P::WK, wk = wave % P::WK;
-  const int tiles = (a.Nk + 32 * P::WQ - 1) / (32 * P::WQ), bh = blockIdx.x / tiles, jb = (blockIdx.x - bh * tiles) * 32 * P::WQ;
+  const int tile = xcd_tile(gridDim.x);
+  if (tile >= a.work) return;
+  const int tiles = (a.Nk + 32 * P::WQ - 1) / (32 * P::WQ), bh = tile / tiles, jb = (tile - bh * tiles) * 32 * P::WQ;
   const int b = bh / a.Hk, hk = bh - b * a.Hk;
   const int j = jb + 32 * wq + (lane & 31);
   // a hidden key's column is computed from zeros and its gradients are stored as zeros: no masking needed for it
   const bool in = j < a.Nk, ok = in && !(a.kpm != nullptr && a.kpm[(int64_t)b * a.Nk + (in ? j : 0)]);
   const int jc = in ? j : a.Nk - 1, off = a.Nk - a.Nq;
-  const bool fm = a.mask_kind == 2, drop = a.t16 != 0;
+  constexpr bool MASK = MODE == kAttnAny;
+  const bool fm = MASK && a.mask_kind == 2, drop = MODE != kAttnPlain && a.t16 != 0;
 
   typename M::frag kf[2][S::KB], vf[S::VB];
 #pragma unroll
   for (int m = 0; m < 2; ++m)
     own_frags<T, S::KB>(kf[m], (const T*)a.k + b * a.ks[0] + jc * a.ks[1] + hk * a.ks[2] + m * a.ks[3], ok, a.Dh, lane);
-  own_frags<T, S::VB>(vf, (const T*)a.v + b * a.vs[0] + jc * a.vs[1] + hk * a.vs[2], ok, a.Dv, lane);
+  if constexpr (PART != 2) own_frags<T, S::VB>(vf, (const T*)a.v + b * a.vs[0] + jc * a.vs[1] + hk * a.vs[2], ok, a.Dv, lane);
   af32x16_t ak[2][S::KO], av[S::VO];
 #pragma unroll
   for (int d = 0; d < S::KO; ++d) { ak[0][d] = af32x16_t{0.0f}; ak[1][d] = af32x16_t{0.0f}; }
@@ -682,7 +758,7 @@ __global__ __launch_bounds__((AttnPlan<T, DH, DV, SHARED>::NT), (AttnPlan<T, DH,
   const uint64_t zseed = attn_seed(a.seed, a.seed_dev) + (uint64_t)(j >> 2);
 
   // tiles of a head from the first whose rows may see a key of the block
-  const int first = a.causal ? max(0, jb - off) / N : 0, per = max(0, (a.Nq + N - 1) / N - first), total = per * a.G;
+  const int first = MASK && a.causal ? max(0, jb - off) / N : 0, per = max(0, (a.Nq + N - 1) / N - first), total = per * a.G;
   const int st = SHARED ? threadIdx.x : lane;
   AttnStage<T, DH, DV, N, P::LT> sg;
   const uint32_t xrow = (uint32_t)(a.qs[1] * elem<T>::kBytes), yrow = (uint32_t)(a.gs[1] * elem<T>::kBytes);
@@ -733,8 +809,9 @@ __global__ __launch_bounds__((AttnPlan<T, DH, DV, SHARED>::NT), (AttnPlan<T, DH,
       af32x16_t x[2];
 #pragma unroll
       for (int m = 0; m < 2; ++m) x[m] = tile_dot<T, S::KB, S::LDK>(qt + m * N * S::LDK, it0, kf[m], lane);
-      af32x16_t gm = tile_dot<T, S::VB, S::LDV>(gt, it0, vf, lane);
-      if (a.causal) {
+      af32x16_t gm = {0.0f};
+      if constexpr (PART != 2) gm = tile_dot<T, S::VB, S::LDV>(gt, it0, vf, lane);
+      if (MASK && a.causal) {
         const int lim = jc - off - i0 - 4 * (lane >> 5);                // rows before it do not see the key
         if (__any(lim > -4 * (lane >> 5))) {
 #pragma unroll
@@ -742,7 +819,7 @@ __global__ __launch_bounds__((AttnPlan<T, DH, DV, SHARED>::NT), (AttnPlan<T, DH,
             if (8 * (e >> 2) + (e & 3) < lim) { x[0][e] = kNegInf; x[1][e] = kNegInf; }
         }
       }
-      if (a.mask_kind != 0) {
+      if (MASK && a.mask_kind != 0) {
         const int64_t o = b * a.ms[0] + h * a.ms[1] + jc * a.ms[3];
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
@@ -780,11 +857,13 @@ __global__ __launch_bounds__((AttnPlan<T, DH, DV, SHARED>::NT), (AttnPlan<T, DH,
       }
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
-        const typename M::frag fp = M::pack(pc + 8 * s);
+        if constexpr (PART != 1) {
+          const typename M::frag fp = M::pack(pc + 8 * s);
 #pragma unroll
-        for (int d = 0; d < S::VO; ++d) av[d] = M::mul(M::template load_tr<S::LDV>(gt, it0 + 16 * s, 32 * d, lane), fp, av[d]);
+          for (int d = 0; d < S::VO; ++d) av[d] = M::mul(M::template load_tr<S::LDV>(gt, it0 + 16 * s, 32 * d, lane), fp, av[d]);
+        }
 #pragma unroll
-        for (int m = 0; m < 2; ++m) {
+        for (int m = 0; m < (PART != 2 ? 2 : 0); ++m) {
           float ds[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) ds[e] = x[m][8 * s + e];
@@ -803,18 +882,19 @@ __global__ __launch_bounds__((AttnPlan<T, DH, DV, SHARED>::NT), (AttnPlan<T, DH,
     }
   }
   if constexpr (!SHARED) {
-    af32x16_t* ptr[2 * S::KO + S::VO];
+    constexpr int NA = PART != 2 ? 2 * S::KO : 0, NB = NA + (PART != 1 ? S::VO : 0);
+    af32x16_t* ptr[NB];
 #pragma unroll
-    for (int d = 0; d < S::KO; ++d) { ptr[d] = &ak[0][d]; ptr[S::KO + d] = &ak[1][d]; }
+    for (int d = 0; d < NA / 2; ++d) { ptr[d] = &ak[0][d]; ptr[S::KO + d] = &ak[1][d]; }
 #pragma unroll
-    for (int d = 0; d < S::VO; ++d) ptr[2 * S::KO + d] = &av[d];
+    for (int d = 0; d < NB - NA; ++d) ptr[NA + d] = &av[d];
     join_waves<P::WK>(ptr, reinterpret_cast<float*>(smem), wk, lane);
     if (wk != 0) return;
   }
   if (!in) return;
   const float fk = ok && a.Nk > 1 ? a.scale : 0.0f, fv = a.up / kProbScale<T>;        // (Nk = 1: as for grad_q)
 #pragma unroll
-  for (int m = 0; m < 2; ++m) {
+  for (int m = 0; m < (PART != 2 ? 2 : 0); ++m) {
     T* row = (T*)a.gk + ((((int64_t)b * a.Nk + j) * a.Hk + hk) * 2 + m) * a.Dh;
 #pragma unroll
     for (int d = 0; d < S::KO; ++d)
@@ -826,6 +906,7 @@ __global__ __launch_bounds__((AttnPlan<T, DH, DV, SHARED>::NT), (AttnPlan<T, DH,
         store_quad<T>(row, 32 * d + tile_item(4 * q, lane), a.Dh, o);
       }
   }
+  if constexpr (PART == 1) return;
   T* row = (T*)a.gv + (((int64_t)b * a.Nk + j) * a.Hk + hk) * a.Dv;
 #pragma unroll
   for (int d = 0; d < S::VO; ++d)
@@ -840,7 +921,10 @@ __global__ __launch_bounds__((AttnPlan<T, DH, DV, SHARED>::NT), (AttnPlan<T, DH,
 
 // ---- launch -----------------------------------------------------------------------------------------------------------------------
 template <typename K>
-static int attn_launch(K kernel, int64_t blocks, int threads, int lds, const DiffAttnArgs& a, hipStream_t st, const char* who) {
+static int attn_launch(K kernel, int64_t blocks, int threads, int lds, const DiffAttnArgs& args, hipStream_t st, const char* who) {
+  DiffAttnArgs a = args;
+  a.work = (int)blocks;
+  blocks = (blocks + 7) / 8 * 8;                     // (xcd_tile)
   if (blocks >= (int64_t(1) << 31)) { set_error("%s: %ld blocks", who, (long)blocks); return UBV_ERR_UNSUPPORTED; }
   if (lds > 48 * 1024) (void)hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
   hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(threads), (size_t)lds, st, a);
@@ -848,40 +932,49 @@ static int attn_launch(K kernel, int64_t blocks, int threads, int lds, const Dif
   return UBV_OK;
 }
 
-#ifndef UBV_ATTN_FILL
-#define UBV_ATTN_FILL 512
-#endif
-constexpr int64_t kAttnFill = UBV_ATTN_FILL;      // blocks that keep the 256 CUs busy
+template <typename F> static int attn_mode(const DiffAttnArgs& a, F&& f) {
+  if (a.causal || a.mask_kind != 0) return f(std::integral_constant<int, kAttnAny>{});
+  if (a.t16 != 0) return f(std::integral_constant<int, kAttnDrop>{});
+  return f(std::integral_constant<int, kAttnPlain>{});
+}
 
-// blocks of 32 own items a head, by the arrangement
-static inline int64_t attn_blocks(int64_t heads, int64_t items, int wq) { return heads * ((items + 32 * wq - 1) / (32 * wq)); }
+// The arrangement of a call.  A shared block does four private blocks' work in `cost` times their time (it stages a tile once
+// for 128 own items), but there are a quarter as many: with 256 CUs the rounds of blocks decide.  Measured at one block per CU
+// (bf16, us, shared / private): 64 / 64 wide heads 80 / 121, 128 / 128 133 / 278; 32 / 64, 10 000 x 10 000 and 4 heads (316 or
+// 1252 blocks) 400 / 299.
+static bool attn_shared(int64_t heads, int64_t items, int DH) {
+  const int64_t wide = heads * ((items + 127) / 128), narrow = heads * ((items + 31) / 32);
+  const double cost = DH <= 32 ? 0.8 : 0.65;
+  return 4.0 * cost * (double)((wide + 255) / 256) < (double)((narrow + 255) / 256);
+}
 
 template <typename T, int DH, int DV>
 static int attn_forward(DiffAttnArgs a, void* ws, int64_t ws_bytes, hipStream_t st) {
-  const int64_t heads = (int64_t)a.B * a.Hk, wide = attn_blocks(heads, a.R, 4);
+  // heads of 256: two blocks with 128 columns each (both compute the scores; one block's accumulators would not fit)
+  constexpr int DC = DV > 128 ? 128 : DV;
+  const int64_t heads = (int64_t)a.B * a.Hk;
+  const char* who = "diff_attention_forward";
   a.splits = 1;
+  a.halves = (a.Dv + DC - 1) / DC;
   auto run = [&](auto shared) {
     constexpr bool SH = decltype(shared)::value;
-    using P = AttnPlan<T, DH, DV, SH>;
-    return attn_launch(diff_attn_fwd_kernel<T, DH, DV, SH>, attn_blocks(heads, a.R, P::WQ) * a.splits, P::NT,
-                       P::lds(FwdState<T, DV>::FLOATS), a, st, "diff_attention_forward");
+    using P = AttnPlan<T, DH, DC, SH>;
+    return attn_mode(a, [&](auto mode) {
+      return attn_launch(diff_attn_fwd_kernel<T, DH, DC, SH, decltype(mode)::value>, heads * ((a.R + 32 * P::WQ - 1) / (32 * P::WQ)) * a.halves * a.splits,
+                         P::NT, P::lds(FwdState<T, DC>::FLOATS), a, st, who);
+    });
   };
-  if (wide >= kAttnFill) return run(std::true_type{});
+  if (attn_shared(heads * a.halves, a.R, DH)) return run(std::true_type{});
   // few rows, many keys: blocks share the keys of a row tile and a second launch joins their sums
-  const int64_t blocks = attn_blocks(heads, a.R, 1), tiles = (a.Nk + 31) / 32;
-  if (blocks < kAttnFill / 2 && ws != nullptr) {
-    constexpr int PER = 2 * AttnPlan<T, DH, DV, false>::WK;                          // at least two tiles a wave
-    int64_t splits = (2 * kAttnFill + blocks - 1) / blocks;
-    splits = splits < tiles / PER ? splits : tiles / PER;
-    const int64_t most = ws_bytes / (blocks * FwdState<T, DV>::FLOATS * 64 * 4);
-    splits = splits < most ? splits : most;
-    if (splits > 1) {
-      a.splits = (int)splits;
-      a.part = (float*)ws;
-      const int rc = run(std::false_type{});
-      if (rc != UBV_OK) return rc;
-      return attn_launch(diff_attn_join_kernel<T, DV, 1>, blocks, 64, 0, a, st, "diff_attention_forward");
-    }
+  const int64_t splits = attn_splits(a.B, a.H, a.Hk, a.Nq, a.Nk, a.Dv);
+  if (splits > 1 && ws_bytes >= attn_part_bytes(a.B, a.H, a.Hk, a.Nq, a.Dv, splits)) {
+    a.splits = (int)splits;
+    a.part = (float*)ws;
+    const int rc = run(std::false_type{});
+    if (rc != UBV_OK) return rc;
+    hipLaunchKernelGGL((diff_attn_join_kernel<T, DC>), dim3((unsigned)(heads * a.R * a.halves)), dim3(256), 0, st, a);
+    UBV_CHECK_LAUNCH(who);
+    return UBV_OK;
   }
   return run(std::false_type{});
 }
@@ -890,30 +983,41 @@ template <typename T, int DH, int DV>
 static int attn_backward(const DiffAttnArgs& a, float* glam, hipStream_t st) {
   using S = AttnTile<T, DH, DV>;
   const int64_t heads = (int64_t)a.B * a.Hk, rows = (int64_t)a.B * a.H * a.Nq;
+  const char* who = "diff_attention_backward";
   hipLaunchKernelGGL(diff_attn_del_kernel<T>, dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, st, a);
-  UBV_CHECK_LAUNCH("diff_attention_backward");
-  auto run = [&](auto shared, auto which) {
+  UBV_CHECK_LAUNCH(who);
+  auto run = [&](auto shared, auto pass) {
     constexpr bool SH = decltype(shared)::value;
+    constexpr int PASS = decltype(pass)::value;                 // 0 .. 2: grad_k / grad_v of that part, 3: grad_q
     using P = AttnPlan<T, DH, DV, SH>;
-    if constexpr (decltype(which)::value)
-      return attn_launch(diff_attn_bwd_q_kernel<T, DH, DV, SH>, attn_blocks(heads, a.R, P::WQ), P::NT, P::lds((2 * S::KO + 1) * 16), a, st,
-                         "diff_attention_backward");
-    else
-      return attn_launch(diff_attn_bwd_kv_kernel<T, DH, DV, SH>, attn_blocks(heads, a.Nk, P::WQ), P::NT, P::lds((2 * S::KO + S::VO) * 16), a,
-                         st, "diff_attention_backward");
+    const int64_t blocks = heads * (((PASS == 3 ? a.R : a.Nk) + 32 * P::WQ - 1) / (32 * P::WQ));
+    return attn_mode(a, [&](auto mode) {
+      constexpr int MODE = decltype(mode)::value;
+      if constexpr (PASS == 3)
+        return attn_launch(diff_attn_bwd_q_kernel<T, DH, DV, SH, MODE>, blocks, P::NT, P::lds((2 * S::KO + 1) * 16), a, st, who);
+      else
+        return attn_launch(diff_attn_bwd_kv_kernel<T, DH, DV, SH, MODE, PASS>, blocks, P::NT, P::lds((2 * S::KO + S::VO) * 16), a, st, who);
+    });
+  };
+  auto pick = [&](int64_t items, auto pass) {
+    return attn_shared(heads, items, DH) ? run(std::true_type{}, pass) : run(std::false_type{}, pass);
   };
   int rc = UBV_OK;
   if (a.gq != nullptr || glam != nullptr) {
-    rc = attn_blocks(heads, a.R, 4) >= kAttnFill ? run(std::true_type{}, std::true_type{}) : run(std::false_type{}, std::true_type{});
+    rc = pick(a.R, std::integral_constant<int, 3>{});
     if (rc != UBV_OK) return rc;
     if (glam != nullptr) {
       hipLaunchKernelGGL(diff_attn_lam_kernel, dim3((unsigned)a.H), dim3(256), 0, st, a.dlrow, glam, a.B, a.H, a.Nq);
-      UBV_CHECK_LAUNCH("diff_attention_backward");
+      UBV_CHECK_LAUNCH(who);
     }
   }
-  if (a.gk != nullptr)
-    rc = attn_blocks(heads, a.Nk, 4) >= kAttnFill ? run(std::true_type{}, std::false_type{}) : run(std::false_type{}, std::false_type{});
-  return rc;
+  if (a.gk == nullptr) return rc;
+  if constexpr (2 * DH + DV > 2 * 128) {
+    rc = pick(a.Nk, std::integral_constant<int, 1>{});
+    return rc != UBV_OK ? rc : pick(a.Nk, std::integral_constant<int, 2>{});
+  } else {
+    return pick(a.Nk, std::integral_constant<int, 0>{});
+  }
 }
 
 // the smallest pair of widths that holds the call's
