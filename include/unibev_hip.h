@@ -710,16 +710,17 @@ int ubv_layer_norm_backward(const void* grad_y, const void* x, const float* gamm
  *   causal: query i sees keys j <= i + Nk - Nq.
  *   D as in ubv_dropout over the map: key j of row r = (b H + h) Nq + i is field j % 4 of group r ceil(Nk / 4) + j / 4.
  *   out [B, Nq, H, Dv] contiguous; stat f32 [B, H, Nq, 4] (the softmax sums) and maps f32 [2, B, H, Nq, Dv] (the two maps'
- *   products) are written for the backward pass, or both NULL.  workspace: ubv_diff_attention_forward_workspace bytes let few
- *   queries share many keys' blocks; with less (or NULL) fewer blocks do.
+ *   products) are written for the backward pass, or both NULL.  workspace: ubv_diff_attention_forward_workspace bytes let several
+ *   blocks share the keys of few queries; with less (or NULL) one does.
  * Backward: grad_q / grad_k / grad_v contiguous in the shapes of q, k, v, grad_lam f32 [H]; grad_q and grad_lam each or NULL,
- * grad_k and grad_v both or neither.  No atomics: the same bits on every run. */
+ * grad_k and grad_v both or neither.  workspace: ubv_diff_attention_backward_workspace bytes (at least 28 B H Nq, rounded up to
+ * 16, which all the call's blocks need; the rest as in the forward pass).  No atomics: the same bits on every run. */
 int ubv_diff_attention_forward(const void* q, const void* k, const void* v, const float* lam, const uint8_t* key_padding_mask,
                                const void* mask, int mask_kind, void* out, float* stat, float* maps, const int64_t* strides, int B,
                                int H, int Hk, int Nq, int Nk, int Dh, int Dv, float scale, int causal, float p, uint64_t seed,
                                const uint64_t* seed_dev, int dtype, void* workspace, int64_t workspace_bytes, void* stream);
-int64_t ubv_diff_attention_forward_workspace(int B, int H, int Hk, int Nq, int Nk, int Dv);
-int64_t ubv_diff_attention_backward_workspace(int B, int H, int Nq);
+int64_t ubv_diff_attention_forward_workspace(int B, int H, int Hk, int Nq, int Nk, int Dh, int Dv, int causal, int dtype);
+int64_t ubv_diff_attention_backward_workspace(int B, int H, int Hk, int Nq, int Nk, int Dh, int Dv, int causal, int dtype);
 int ubv_diff_attention_backward(const void* grad_out, const void* q, const void* k, const void* v, const float* lam,
                                 const uint8_t* key_padding_mask, const void* mask, int mask_kind, const float* stat,
                                 const float* maps, void* grad_q, void* grad_k, void* grad_v, float* grad_lam,

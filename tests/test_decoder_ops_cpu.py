@@ -61,13 +61,13 @@ def test_attention_forward_entry_refuses(kw, word):
 
 def test_attention_backward_entry_refuses():
     f = _lib.lib().ubv_diff_attention_backward
-    need = _lib.lib().ubv_diff_attention_backward_workspace(1, 4, 8)
+    need = _lib.lib().ubv_diff_attention_backward_workspace(1, 4, 2, 8, 8, 32, 64, 0, 0)
     s = (ctypes.c_int64 * 18)()
 
     def call(go=P, stat=P, gq=P, gk=P, gv=P, ws=P, n=need):
         return f(go, P, P, P, P, None, None, 0, stat, P, gq, gk, gv, P, s, 1, 4, 2, 8, 8, 32, 64, 0.1, 0, 0.0, 0, None, 0, ws, n, None)
 
-    assert need > 0 and _lib.lib().ubv_diff_attention_backward_workspace(0, 4, 8) == 0
+    assert need > 0 and _lib.lib().ubv_diff_attention_backward_workspace(0, 4, 2, 8, 8, 32, 64, 0, 0) == 0
     refused(call(go=None), 'grad_out')
     refused(call(stat=None), 'stat')
     refused(call(gv=None), 'come together')

@@ -495,12 +495,32 @@ def test_attention_many_heads_takes_the_wide_tiling(dt):
     attn_check(*attn_inputs(B, H, H, Nq, Nk, 16, 32, dt), dt, hidden=causal(Nq, Nk), causal=True, p=0.1)
 
 
+@pytest.mark.parametrize('Dh,Dv', [(16, 32), (32, 64), (64, 64), (64, 128), (128, 128), (128, 256)])
+@pytest.mark.parametrize('kind', ['plain', 'dropped', 'masked'])
+@pytest.mark.parametrize('dt', TYPES)
+def test_attention_both_arrangements_of_every_width(Dh, Dv, kind, dt):
+    """enough rows and keys for shared tiles (both passes), and few enough for private ones"""
+    for B, H, N in ((2, 128, 97), (1, 2, 70)):
+        kw, hidden = {}, None
+        if kind == 'masked':
+            m = torch.rand(N, N, generator=torch.Generator().manual_seed(1)) < 0.3
+            kw, hidden = dict(attn_mask=m.to(DEV), causal=True), m | causal(N, N)
+        attn_check(*attn_inputs(B, H, H, N, N, Dh, Dv, dt), dt, hidden=hidden, p=0.0 if kind == 'plain' else 0.1, **kw)
+
+
 @pytest.mark.parametrize('Nq,H,Hk', [(1, 4, 4), (1, 8, 2), (3, 4, 1), (7, 2, 2)])
 @pytest.mark.parametrize('dt', TYPES)
 def test_attention_few_queries_many_keys(Nq, H, Hk, dt):
     q, k, v, lam, go = attn_inputs(2, H, Hk, Nq, 5003, 32, 64, dt)
     pad = torch.arange(5003)[None] >= torch.tensor([[5003], [1234]])
     attn_check(q, k, v, lam, go, dt, hidden=pad[:, None, None], key_padding_mask=pad.to(DEV))
+
+
+@pytest.mark.parametrize('Nq,Nk,H,Hk,causal_', [(3001, 40, 2, 2, False), (2100, 33, 4, 1, False), (3, 4100, 2, 1, True), (1500, 1500, 1, 1, True)])
+@pytest.mark.parametrize('dt', [torch.float32, torch.bfloat16])
+def test_attention_long_axes_are_shared_by_blocks(Nq, Nk, H, Hk, causal_, dt):
+    kw = dict(hidden=causal(Nq, Nk), causal=True) if causal_ else {}
+    attn_check(*attn_inputs(1, H, Hk, Nq, Nk, 64, 128, dt), dt, p=0.1, **kw)
 
 
 def test_attention_large_scores():

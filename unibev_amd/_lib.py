@@ -63,10 +63,10 @@ SIGNATURES = {
     'ubv_layer_norm_forward': (c_int, [_P] * 6 + [c_int64, c_int, c_float, c_int, _P]),
     'ubv_layer_norm_backward_workspace': (c_int64, [c_int64, c_int]),
     'ubv_layer_norm_backward': (c_int, [_P] * 8 + [c_int64, c_int, c_int, _P, c_int64, _P]),
-    'ubv_diff_attention_forward_workspace': (c_int64, [c_int] * 6),
+    'ubv_diff_attention_forward_workspace': (c_int64, [c_int] * 9),
     'ubv_diff_attention_forward': (c_int, [_P] * 6 + [c_int] + [_P] * 4 + [c_int] * 7 + [c_float, c_int, c_float, c_uint64, _P, c_int,
                                            _P, c_int64, _P]),
-    'ubv_diff_attention_backward_workspace': (c_int64, [c_int] * 3),
+    'ubv_diff_attention_backward_workspace': (c_int64, [c_int] * 9),
     'ubv_diff_attention_backward': (c_int, [_P] * 7 + [c_int] + [_P] * 7 + [c_int] * 7 + [c_float, c_int, c_float, c_uint64, _P, c_int,
                                             _P, c_int64, _P]),
     'ubv_linear_workspace': (c_int64, []),

@@ -41,24 +41,12 @@ struct DiffAttnArgs {
   float* dlrow;                            // [B H Nq] - sum_j A_2 G
   void *gq, *gk, *gv;                      // contiguous gradients
   int work;                                // blocks with work (the grid is rounded up)
-  int splits;                              // forward: blocks that share a row tile's keys, 1: none
+  int splits;                              // blocks that share the staged items of an own tile, 1: none
   int halves;                              // forward: blocks that share a row tile's output columns
-  float* part;                             // forward, splits > 1: [tile][half][split][64 lanes][4 + columns] references, sums, products
+  float* part;                             // splits > 1: [tile][half][split][64 lanes][floats] the blocks' sums
 };
 
-// Splits of a row tile's keys in the forward pass: four blocks a CU where there are few row tiles, at least 512 keys each.
-constexpr int kAttnSplits = 1024;
-static inline int64_t attn_row_tiles(int B, int H, int Hk, int Nq, int Dv) {
-  return (int64_t)B * Hk * (((int64_t)(H / Hk) * Nq + 31) / 32) * (Dv > 128 ? 2 : 1);
-}
-static inline int64_t attn_splits(int B, int H, int Hk, int Nq, int Nk, int Dv) {
-  const int64_t tiles = attn_row_tiles(B, H, Hk, Nq, Dv), want = tiles > 128 ? 1 : (kAttnSplits + tiles - 1) / tiles, most = Nk / 512;
-  return want < most ? want : most > 1 ? most : 1;
-}
-static inline int64_t attn_part_bytes(int B, int H, int Hk, int Nq, int Dv, int64_t splits) {
-  const int width = Dv <= 32 ? 32 : Dv <= 64 ? 64 : 128;
-  return splits <= 1 ? 0 : attn_row_tiles(B, H, Hk, Nq, Dv) * splits * (4 + width) * 64 * 4;
-}
+constexpr int kAttnSplits = 256;         // most splits of an own tile's staged items
 
 // f16 holds nothing below 2^-24 and loses bits below 2^-14, which the probabilities of a long row reach: they enter the matrix
 // instructions 2^8 larger and their products leave 2^8 smaller (|lam| up to 255 stays in range)
@@ -75,7 +63,19 @@ typedef __attribute__((ext_vector_type(8))) __bf16 abf16x8_t;
 typedef __attribute__((ext_vector_type(8))) _Float16 af16x8_t;
 typedef __attribute__((ext_vector_type(4))) short ai16x4_t;
 
+// ---- staged rows in LDS ---------------------------------------------------------------------------------------------------------
+// A row of L 16-byte chunks (a power of two) lies unpadded; chunk c of row r is stored at place c ^ fold(r).  fold takes the row bits
+// that the bank (4 L r dwords mod 64) does not see, so that the 16 rows which one phase of a 16-byte read touches at one chunk, and
+// the 4 rows x 4 chunks which one phase of a transposing read touches, each cover all 64 banks once.  (Rows padded by 16 bytes
+// instead: a third of the LDS time was bank conflicts of the transposing reads.)  fold is linear over XOR, and so are addresses:
+// a lane's part ^ a constant.
+template <int L> __host__ __device__ constexpr int row_fold(int r) {
+  return L <= 4 ? (r >> 2) & 3 : L == 8 ? 4 * ((r >> 1) & 1) + ((r >> 2) & 3) : 4 * (r & 3) + ((r >> 2) & 3);
+}
+
 // ---- one 16-deep step of a 32 x 32 product: a lane holds items 8 (lane >> 5) + 0 .. 7 of the contraction -------------------
+// load<L>: row r0 + (lane & 31) (r0 a multiple of 32) of a tile, elements 16 s .. of the part that begins at chunk `c0`
+// load_tr<L>: column 32 d + (lane & 31) of that part, rows k0 + 8 (j >> 2) + 4 (lane >> 5) + (j & 3), j = 0 .. 7 (k0 a multiple of 16)
 template <typename T> struct amma {                       // 16-bit types: one MFMA
   struct frag { au32x4_t d; };
   static __device__ __forceinline__ af32x16_t mul(const frag& a, const frag& b, af32x16_t c) {
@@ -84,7 +84,7 @@ template <typename T> struct amma {                       // 16-bit types: one M
     else
       return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(abf16x8_t, a.d), __builtin_bit_cast(abf16x8_t, b.d), c, 0, 0, 0);
   }
-  static __device__ __forceinline__ frag load(const T* p) { return {*reinterpret_cast<const au32x4_t*>(p)}; }   // 16-byte aligned
+  static __device__ __forceinline__ frag own(const T* t) { return {*reinterpret_cast<const au32x4_t*>(t)}; }
   // rounding to the inputs' type: the matrix instruction takes no wider operand; half a step of each probability, random
   static __device__ __forceinline__ frag pack(const float* p) {
     frag f;
@@ -94,17 +94,26 @@ template <typename T> struct amma {                       // 16-bit types: one M
       for (int i = 0; i < 8; ++i) h[i] = (_Float16)p[i];
       f.d = __builtin_bit_cast(au32x4_t, h);
     } else {
+      // (the compiler's conversion, not cvt_pk_bf16: beside matrix instructions in flight its wait states are the compiler's to
+      //  place, which it does not do around inline assembly)
+      abf16x8_t h;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) f.d[i] = cvt_pk_bf16(p[2 * i], p[2 * i + 1]);
+      for (int i = 0; i < 8; ++i) h[i] = (__bf16)p[i];
+      f.d = __builtin_bit_cast(au32x4_t, h);
     }
     return f;
   }
-  // column n0 + (lane & 31) of staged rows k0 + 8 (j >> 2) + 4 (lane >> 5) + (j & 3), j = 0 .. 7
-  template <int LD> static __device__ __forceinline__ frag load_tr(const T* tile, int k0, int n0, int lane) {
+  template <int L> static __device__ __forceinline__ frag load(const char* tile, int r0, int c0, int s, int lane) {
+    const int r = lane & 31, base = r * 16 * L + (((lane >> 5) ^ row_fold<L>(r)) << 4);
+    return {*reinterpret_cast<const au32x4_t*>(tile + r0 * 16 * L + (base ^ ((c0 + 2 * s) << 4)))};
+  }
+  template <int L> static __device__ __forceinline__ frag load_tr(const char* tile, int k0, int c0, int d, int lane) {
     typedef __attribute__((address_space(3))) ai16x4_t lds_v4;
-    const T* p = tile + (k0 + 4 * (lane >> 5) + ((lane & 15) >> 2)) * LD + n0 + (lane & 16) + 4 * (lane & 3);
-    const ai16x4_t a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4*)p);
-    const ai16x4_t b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4*)(p + 8 * LD));
+    const int rr = (lane & 15) >> 2, r = 4 * (lane >> 5) + rr;
+    const int base = r * 16 * L + (((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ row_fold<L>(r)) << 4) + (lane & 1) * 8;
+    const char* t = tile + k0 * 16 * L;
+    const ai16x4_t a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4*)(t + (base ^ ((c0 + 4 * d) << 4))));
+    const ai16x4_t b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4*)(t + 8 * 16 * L + (base ^ (((c0 + 4 * d) ^ row_fold<L>(8)) << 4))));
     const au32x2_t ua = __builtin_bit_cast(au32x2_t, a), ub = __builtin_bit_cast(au32x2_t, b);
     return {au32x4_t{ua.x, ua.y, ub.x, ub.y}};
   }
@@ -116,23 +125,30 @@ template <> struct amma<float> {                          // f32: eight MFMAs of
     for (int j = 0; j < 8; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a.d[j], b.d[j], c, 0, 0, 0);
     return c;
   }
-  static __device__ __forceinline__ frag load(const float* p) {
-    frag f;
-    *reinterpret_cast<float4*>(f.d) = *reinterpret_cast<const float4*>(p);
-    *reinterpret_cast<float4*>(f.d + 4) = *reinterpret_cast<const float4*>(p + 4);
-    return f;
-  }
-  static __device__ __forceinline__ frag pack(const float* p) {
+  static __device__ __forceinline__ frag own(const float* t) {
     frag f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f.d[i] = p[i];
+    for (int i = 0; i < 8; ++i) f.d[i] = t[i];
     return f;
   }
-  template <int LD> static __device__ __forceinline__ frag load_tr(const float* tile, int k0, int n0, int lane) {
+  static __device__ __forceinline__ frag pack(const float* p) { return own(p); }
+  template <int L> static __device__ __forceinline__ frag load(const char* tile, int r0, int c0, int s, int lane) {
+    const int r = lane & 31, base = r * 16 * L + (((2 * (lane >> 5)) ^ row_fold<L>(r)) << 4);
+    const char* t = tile + r0 * 16 * L;
     frag f;
-    const float* p = tile + (k0 + 4 * (lane >> 5)) * LD + n0 + (lane & 31);
+    *reinterpret_cast<float4*>(f.d) = *reinterpret_cast<const float4*>(t + (base ^ ((c0 + 4 * s) << 4)));
+    *reinterpret_cast<float4*>(f.d + 4) = *reinterpret_cast<const float4*>(t + (base ^ ((c0 + 4 * s + 1) << 4)));
+    return f;
+  }
+  template <int L> static __device__ __forceinline__ frag load_tr(const char* tile, int k0, int c0, int d, int lane) {
+    const int r = 4 * (lane >> 5), base = r * 16 * L + ((((lane & 31) >> 2) ^ row_fold<L>(r)) << 4) + 4 * (lane & 3);
+    const char* t = tile + k0 * 16 * L;
+    frag f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) f.d[j] = p[(8 * (j >> 2) + (j & 3)) * LD];
+    for (int j = 0; j < 8; ++j) {
+      const int rj = 8 * (j >> 2) + (j & 3);
+      f.d[j] = *reinterpret_cast<const float*>(t + rj * 16 * L + (base ^ (((c0 + 8 * d) ^ row_fold<L>(rj)) << 4)));
+    }
     return f;
   }
 };

@@ -5,9 +5,21 @@ namespace ubv {
 int diff_attn_forward_f32(const DiffAttnArgs&, void*, int64_t, hipStream_t);
 int diff_attn_forward_f16(const DiffAttnArgs&, void*, int64_t, hipStream_t);
 int diff_attn_forward_bf16(const DiffAttnArgs&, void*, int64_t, hipStream_t);
-int diff_attn_backward_f32(const DiffAttnArgs&, float*, hipStream_t);
-int diff_attn_backward_f16(const DiffAttnArgs&, float*, hipStream_t);
-int diff_attn_backward_bf16(const DiffAttnArgs&, float*, hipStream_t);
+int diff_attn_backward_f32(const DiffAttnArgs&, float*, int64_t, hipStream_t);
+int diff_attn_backward_f16(const DiffAttnArgs&, float*, int64_t, hipStream_t);
+int diff_attn_backward_bf16(const DiffAttnArgs&, float*, int64_t, hipStream_t);
+int64_t diff_attn_bytes_f32(const DiffAttnArgs&, bool);
+int64_t diff_attn_bytes_f16(const DiffAttnArgs&, bool);
+int64_t diff_attn_bytes_bf16(const DiffAttnArgs&, bool);
+
+static int64_t attn_part_bytes(int B, int H, int Hk, int Nq, int Nk, int Dh, int Dv, int causal, int dtype, bool backward) {
+  if (B <= 0 || Hk <= 0 || H < Hk || H % Hk != 0 || Nq <= 0 || Nk <= 0 || Dh <= 0 || Dv <= 0 || Dh > 128 || Dv > 256) return 0;
+  DiffAttnArgs a{};
+  a.B = B; a.H = H; a.Hk = Hk; a.G = H / Hk; a.Nq = Nq; a.Nk = Nk; a.Dh = Dh; a.Dv = Dv; a.R = a.G * Nq; a.causal = causal != 0;
+  return dtype == UBV_F32 ? diff_attn_bytes_f32(a, backward) : dtype == UBV_F16 ? diff_attn_bytes_f16(a, backward) : diff_attn_bytes_bf16(a, backward);
+}
+// the backward pass's rows: statistics (float4 + float2) and grad_lam's part, then the splits' sums
+static int64_t attn_row_bytes(int64_t rows) { return (28 * rows + 15) / 16 * 16; }
 
 // what forward and backward share: shapes, strides (in elements: q 4, k 4, v 3, grad_out 3, mask 4), masks, dropout
 static int attn_args(DiffAttnArgs& a, const void* q, const void* k, const void* v, const float* lam, const uint8_t* kpm,
@@ -44,10 +56,8 @@ static int attn_args(DiffAttnArgs& a, const void* q, const void* k, const void* 
 }
 }  // namespace ubv
 
-extern "C" int64_t ubv_diff_attention_forward_workspace(int B, int H, int Hk, int Nq, int Nk, int Dv) {
-  using namespace ubv;
-  if (B <= 0 || Hk <= 0 || H % Hk != 0 || Nq <= 0 || Nk <= 0) return 0;
-  return attn_part_bytes(B, H, Hk, Nq, Dv, attn_splits(B, H, Hk, Nq, Nk, Dv));
+extern "C" int64_t ubv_diff_attention_forward_workspace(int B, int H, int Hk, int Nq, int Nk, int Dh, int Dv, int causal, int dtype) {
+  return ubv::attn_part_bytes(B, H, Hk, Nq, Nk, Dh, Dv, causal, dtype, false);
 }
 
 extern "C" int ubv_diff_attention_forward(const void* q, const void* k, const void* v, const float* lam, const uint8_t* key_padding_mask,
@@ -72,8 +82,9 @@ extern "C" int ubv_diff_attention_forward(const void* q, const void* k, const vo
   }
 }
 
-extern "C" int64_t ubv_diff_attention_backward_workspace(int B, int H, int Nq) {
-  return B <= 0 || H <= 0 || Nq <= 0 ? 0 : 28 * (int64_t)B * H * Nq;
+extern "C" int64_t ubv_diff_attention_backward_workspace(int B, int H, int Hk, int Nq, int Nk, int Dh, int Dv, int causal, int dtype) {
+  if (B <= 0 || H <= 0 || Nq <= 0) return 0;
+  return ubv::attn_row_bytes((int64_t)B * H * Nq) + ubv::attn_part_bytes(B, H, Hk, Nq, Nk, Dh, Dv, causal, dtype, true);
 }
 
 extern "C" int ubv_diff_attention_backward(const void* grad_out, const void* q, const void* k, const void* v, const float* lam,
@@ -90,16 +101,18 @@ extern "C" int ubv_diff_attention_backward(const void* grad_out, const void* q, 
   UBV_CHECK_ARG(grad_out && stat && maps && ((uintptr_t)grad_out | (uintptr_t)stat) % 16 == 0, "diff_attention_backward: grad_out, stat or maps");
   UBV_CHECK_ARG((grad_k == nullptr) == (grad_v == nullptr), "diff_attention_backward: grad_k and grad_v come together");
   UBV_CHECK_ARG(((uintptr_t)grad_q | (uintptr_t)grad_k | (uintptr_t)grad_v) % 16 == 0, "diff_attention_backward: gradients must be 16-byte aligned");
-  UBV_CHECK_ARG(workspace && (uintptr_t)workspace % 16 == 0 && workspace_bytes >= ubv_diff_attention_backward_workspace(B, H, Nq),
+  UBV_CHECK_ARG(workspace && (uintptr_t)workspace % 16 == 0 && workspace_bytes >= attn_row_bytes((int64_t)B * H * Nq),
                 "diff_attention_backward: the workspace is too small (%ld bytes)", (long)workspace_bytes);
   const int64_t rows = (int64_t)B * H * Nq;
   a.go = grad_out; a.stat = (float4*)const_cast<float*>(stat); a.o = const_cast<float*>(maps);
   a.gq = grad_q; a.gk = grad_k; a.gv = grad_v;
   a.row = (float4*)workspace; a.rowl = (float2*)(a.row + rows); a.dlrow = (float*)(a.rowl + rows);
+  const int64_t part = workspace_bytes - attn_row_bytes(rows);
+  a.part = (float*)((char*)workspace + attn_row_bytes(rows));
   hipStream_t st = as_stream(stream);
   switch (dtype) {
-    case UBV_F32: return diff_attn_backward_f32(a, grad_lam, st);
-    case UBV_F16: return diff_attn_backward_f16(a, grad_lam, st);
-    default: return diff_attn_backward_bf16(a, grad_lam, st);
+    case UBV_F32: return diff_attn_backward_f32(a, grad_lam, part, st);
+    case UBV_F16: return diff_attn_backward_f16(a, grad_lam, part, st);
+    default: return diff_attn_backward_bf16(a, grad_lam, part, st);
   }
 }

@@ -13,13 +13,19 @@ namespace ubv {
 
 template <typename T, int DH, int DV> struct AttnTile {
   static constexpr int VEC = 16 / elem<T>::kBytes;
-  static constexpr int LDK = DH + VEC, LDV = DV + VEC;      // 16 bytes of padding: fragment reads of 32 rows hit all banks alike
+  static constexpr int LX = 2 * DH / VEC, LY = DV / VEC;    // 16-byte chunks of a staged row: x of both maps, y
   static constexpr int KB = DH / 16, VB = DV / 16;          // 16-deep steps over a head's width
   static constexpr int KO = (DH + 31) / 32, VO = DV / 32;   // 32-wide output blocks
-  // a staged tile of n items: x of two maps, y, and the rows' statistics of the backward pass (float4 + float2 each)
-  static constexpr int elems(int n) { return n * (2 * LDK + LDV); }
-  static constexpr int bytes(int n) { return elems(n) * elem<T>::kBytes + 24 * n; }
-  static constexpr int WK = 4 * bytes(32) <= 150 * 1024 ? 4 : 2;                 // waves of a private block
+  // a staged tile of n items: x, y, and the rows' statistics of the backward pass (float4 + float2 each)
+  static constexpr int xbytes(int n) { return n * 16 * LX; }
+  static constexpr int xybytes(int n) { return n * 16 * (LX + LY); }
+  static constexpr int bytes(int n) { return xybytes(n) + 24 * n; }
+  static constexpr int QFLOATS = 32 * KO + 4, KFLOATS = 16 * (2 * KO + VO);      // a lane's sums in a split's workspace
+  // two waves a SIMD where accumulators, operands and a tile in flight fit half the registers (64 / 128, f16: forward 244 us with
+  // two waves that spill, 167 with one that does not)
+  static constexpr int MINW = DH <= 32 && DV <= 64 ? 2 : 1;
+  static constexpr int fit(int w) { return w > 2 && w * bytes(32) > 150 * 1024 ? fit(w / 2) : w; }
+  static constexpr int WK = fit(4 * MINW);                                       // waves of a private block: a CU's worth
   static constexpr int NS = 2 * bytes(64) <= 76 * 1024 ? 64 : 32;                // items of a shared tile
 };
 
@@ -32,9 +38,7 @@ template <typename T, int DH, int DV, bool SHARED> struct AttnPlan {
   static constexpr int LDS = (SHARED ? 2 : WK) * S::bytes(N);
   static constexpr int merge(int floats) { return SHARED ? 0 : (WK / 2) * floats * 64 * 4; }     // joining `floats` per lane
   static constexpr int lds(int floats) { return LDS > merge(floats) ? LDS : merge(floats); }
-  // two waves a SIMD where accumulators, operands and a tile in flight fit half the registers (64 / 128, f16: forward 244 us with
-  // two waves that spill, 167 with one that does not)
-  static constexpr int MINW = DH <= 32 && DV <= 64 ? 2 : 1;
+  static constexpr int MINW = S::MINW;
 };
 
 // What a call may hold beside hidden keys.  Each has kernels of its own: what a kernel can never meet costs it registers, and
@@ -44,7 +48,7 @@ constexpr int kAttnPlain = 0, kAttnDrop = 1, kAttnAny = 2;       // nothing | dr
 // ---- staging ------------------------------------------------------------------------------------------------------------------
 template <typename T, int DH, int DV, int N, int LT> struct AttnStage {
   using S = AttnTile<T, DH, DV>;
-  static constexpr int PX = 2 * DH / S::VEC, PY = DV / S::VEC, NX = N * PX / LT, NY = N * PY / LT;
+  static constexpr int PX = S::LX, PY = S::LY, NX = N * PX / LT, NY = N * PY / LT;
   static_assert(N * PX % LT == 0 && N * PY % LT == 0 && LT % PX == 0 && LT % PY == 0, "a thread keeps its column");
   au32x4_t x[NX], y[NY];
   uint32_t xoff, yoff;               // this thread's byte offset inside a tile, kOutside past the head's width
@@ -71,14 +75,17 @@ template <typename T, int DH, int DV, int N, int LT> struct AttnStage {
         y[c] = attn_piece(ry, (hid >> (t / PY + c * (LT / PY))) & 1 ? kOutside : yoff, c * (LT / PY) * yrow);
     }
   }
-  __device__ __forceinline__ void store(T* lds, int t) {
-    const int pc = t % PX, m = pc / (PX / 2);
-    T* lx = lds + (m * N + t / PX) * S::LDK + (pc % (PX / 2)) * S::VEC;
+  __device__ __forceinline__ void store(char* lds, int t) {
+    // (a thread's rows are its first one plus multiples of a power of two above it: their folds XOR)
+    const int ox = (t / PX) * 16 * PX + (((t % PX) ^ row_fold<PX>(t / PX)) << 4);
 #pragma unroll
-    for (int c = 0; c < NX; ++c) *reinterpret_cast<au32x4_t*>(lx + c * (LT / PX) * S::LDK) = x[c];
-    T* ly = lds + 2 * N * S::LDK + (t / PY) * S::LDV + (t % PY) * S::VEC;
+    for (int c = 0; c < NX; ++c)
+      *reinterpret_cast<au32x4_t*>(lds + c * (LT / PX) * 16 * PX + (ox ^ (row_fold<PX>(c * (LT / PX)) << 4))) = x[c];
+    const int oy = (t / PY) * 16 * PY + (((t % PY) ^ row_fold<PY>(t / PY)) << 4);
+    char* ly = lds + S::xbytes(N);
 #pragma unroll
-    for (int c = 0; c < NY; ++c) *reinterpret_cast<au32x4_t*>(ly + c * (LT / PY) * S::LDV) = y[c];
+    for (int c = 0; c < NY; ++c)
+      *reinterpret_cast<au32x4_t*>(ly + c * (LT / PY) * 16 * PY + (oy ^ (row_fold<PY>(c * (LT / PY)) << 4))) = y[c];
   }
 };
 
@@ -101,21 +108,20 @@ __device__ __forceinline__ void own_frags(typename amma<T>::frag (&f)[NB], const
     T t[8];
 #pragma unroll
     for (int w = 0; w < 8 / VEC; ++w) {
-      au32x4_t z = {0u, 0u, 0u, 0u};
-      if (ok && d + w * VEC < D) z = *reinterpret_cast<const au32x4_t*>(p + d + w * VEC);
-      *reinterpret_cast<au32x4_t*>(t + w * VEC) = z;
+      const bool in = ok && d + w * VEC < D;            // (p is a row of the tensor also where !ok: loaded, then dropped)
+      const au32x4_t v = *reinterpret_cast<const au32x4_t*>(p + (in ? d + w * VEC : 0)), z = {0u, 0u, 0u, 0u};
+      *reinterpret_cast<au32x4_t*>(t + w * VEC) = in ? v : z;
     }
-    f[s] = amma<T>::load(t);
+    f[s] = amma<T>::own(t);
   }
 }
 
-// 16 dot products of own item (lane & 31) with staged items it0 .. it0 + 31
-template <typename T, int NB, int LD>
-__device__ __forceinline__ af32x16_t tile_dot(const T* tile, int it0, const typename amma<T>::frag (&own)[NB], int lane) {
+// 16 dot products of own item (lane & 31) with staged items it0 .. it0 + 31, over the part of their rows from chunk c0
+template <typename T, int NB, int L>
+__device__ __forceinline__ af32x16_t tile_dot(const char* tile, int it0, int c0, const typename amma<T>::frag (&own)[NB], int lane) {
   af32x16_t c = {0.0f};
-  const T* p = tile + (it0 + (lane & 31)) * LD + 8 * (lane >> 5);
 #pragma unroll
-  for (int s = 0; s < NB; ++s) c = amma<T>::mul(amma<T>::load(p + 16 * s), own[s], c);
+  for (int s = 0; s < NB; ++s) c = amma<T>::mul(amma<T>::template load<L>(tile, it0, c0, s, lane), own[s], c);
   return c;
 }
 
@@ -147,8 +153,9 @@ __device__ __forceinline__ void quad_words(uint64_t mix, int lane, uint32_t (&w)
 // keys j0 .. j0 + n - 1 that no row may see: past the end or padded (this lane's part; the wave's ballot is the tile's)
 __device__ __forceinline__ bool key_hidden(const DiffAttnArgs& a, int b, int j0, int n, int lane) {
   const int j = j0 + lane;
-  if (lane >= n) return false;
-  return j >= a.Nk || (a.kpm != nullptr && a.kpm[(int64_t)b * a.Nk + j] != 0);
+  bool hide = j >= a.Nk;
+  if (a.kpm != nullptr) hide = hide || a.kpm[(int64_t)b * a.Nk + min(j, a.Nk - 1)] != 0;
+  return hide && lane < n;
 }
 
 // hides keys of a tile from the lane's row (query i of head h): `hid` bits of the 32 keys from j0, causal, the call's mask
@@ -173,6 +180,7 @@ template <bool MASK> __device__ __forceinline__ void mask_tile(const DiffAttnArg
   if (a.mask_kind == 0) return;
   const int64_t o = b * a.ms[0] + h * a.ms[1] + i * a.ms[2] + (j0 + half) * a.ms[3];
   const bool whole = j0 + 32 <= a.Nk;
+  const int last = a.Nk - 1 - j0 - half;               // (keys past the end, which `hid` hides, read the last one's)
   if (a.mask_kind == 1) {
     const uint8_t* m = (const uint8_t*)a.mask + o;
 #pragma unroll
@@ -181,8 +189,7 @@ template <bool MASK> __device__ __forceinline__ void mask_tile(const DiffAttnArg
       if (whole && a.ms[3] == 1) __builtin_memcpy(&w, m + 8 * q, 4);
       else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (j0 + half + 8 * q + e < a.Nk) w |= (uint32_t)m[(8 * q + e) * a.ms[3]] << (8 * e);
+        for (int e = 0; e < 4; ++e) w |= (uint32_t)(m[min(8 * q + e, last) * a.ms[3]] != 0 ? 1u : 0u) << (8 * e);
       }
 #pragma unroll
       for (int e = 0; e < 4; ++e)
@@ -196,8 +203,7 @@ template <bool MASK> __device__ __forceinline__ void mask_tile(const DiffAttnArg
       if (whole && a.ms[3] == 1) __builtin_memcpy(w, m + 8 * q, 16);
       else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (j0 + half + 8 * q + e < a.Nk) w[e] = m[(8 * q + e) * a.ms[3]];
+        for (int e = 0; e < 4; ++e) w[e] = m[min(8 * q + e, last) * a.ms[3]];
       }
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -210,8 +216,11 @@ template <bool MASK> __device__ __forceinline__ void mask_tile(const DiffAttnArg
 }
 
 // Blocks go round-robin over the 8 XCDs: XCD x takes the x-th eighth of the tiles, so that the tiles of a head, which read the
-// same keys (or rows), meet in one L2.  The grid is rounded up; a tile past the end has no work.
-__device__ __forceinline__ int xcd_tile(int blocks) { return xcd_remap(blockIdx.x, blocks >> 3); }
+// same keys (or rows), meet in one L2 (2 x 8 heads of 64 / 128, 4096 x 4096: forward 389 -> 376 us).  Not in a padded batch, whose
+// samples are unequal work, nor where splits of one tile share nothing.  The grid is rounded up; a tile past the end has no work.
+__device__ __forceinline__ int xcd_tile(const DiffAttnArgs& a) {
+  return a.kpm != nullptr || a.splits > 1 ? blockIdx.x : xcd_remap(blockIdx.x, gridDim.x >> 3);
+}
 
 // what forward and grad_q share: own = rows
 struct RowWave {
@@ -225,7 +234,9 @@ struct RowWave {
     lane = threadIdx.x & 63;
     wq = wave / WK; wk = wave % WK;
     const int tiles = (a.R + 32 * WQ - 1) / (32 * WQ), bh = tile / tiles;
-    rb = (tile - bh * tiles) * 32 * WQ;
+    int at = tile - bh * tiles;
+    if (MASK && a.causal) at = tiles - 1 - at;         // the rows that see most keys first: no long block at the end
+    rb = at * 32 * WQ;
     b = bh / a.Hk; hk = bh - b * a.Hk;
     r = rb + 32 * wq + (lane & 31);
     ok = r < a.R;
@@ -241,7 +252,7 @@ struct RowWave {
   }
 };
 
-// the stream of staged key tiles: f(tile of T, it0, hid of its 32 keys, j0) for every 32 keys that are not all hidden
+// the stream of staged key tiles: f(tile, it0, hid of its 32 keys, j0) for every 32 keys that are not all hidden
 template <typename T, int DH, int DV, bool SHARED, typename F>
 __device__ __forceinline__ void key_tiles(const DiffAttnArgs& a, const RowWave& w, int col, int t0, int t1, char* smem, F&& f) {
   using S = AttnTile<T, DH, DV>;
@@ -262,7 +273,7 @@ __device__ __forceinline__ void key_tiles(const DiffAttnArgs& a, const RowWave& 
   };
   uint64_t hid = __ballot(key_hidden(a, w.b, t * N, N, w.lane));
   load(t, hid);
-  T* buf = reinterpret_cast<T*>(smem + (SHARED ? 0 : w.wk * S::bytes(N)));
+  char* const buf = smem + (SHARED ? 0 : w.wk * S::bytes(N));
   sg.store(buf, st);
   tile_ready<SHARED>();
   bool nb = t + STEP < t1 && key_hidden(a, w.b, (t + STEP) * N, N, w.lane);
@@ -273,7 +284,7 @@ __device__ __forceinline__ void key_tiles(const DiffAttnArgs& a, const RowWave& 
     const uint64_t nhid = __ballot(nb);
     if (more) load(t + STEP, nhid);
     nb = t + 2 * STEP < t1 && key_hidden(a, w.b, (t + 2 * STEP) * N, N, w.lane);
-    const T* tile = SHARED ? reinterpret_cast<T*>(smem + cur * S::bytes(N)) : buf;
+    const char* tile = SHARED ? smem + cur * S::bytes(N) : buf;
 #pragma unroll 1
     for (int it0 = 0; it0 < N; it0 += 32) {
       const uint32_t h32 = (uint32_t)(hid >> it0);
@@ -282,7 +293,7 @@ __device__ __forceinline__ void key_tiles(const DiffAttnArgs& a, const RowWave& 
     if (more) {
       if constexpr (SHARED) cur ^= 1;
       else tile_ready<false>();
-      sg.store(SHARED ? reinterpret_cast<T*>(smem + cur * S::bytes(N)) : buf, st);
+      sg.store(SHARED ? smem + cur * S::bytes(N) : buf, st);
       tile_ready<SHARED>();
     }
     hid = nhid;
@@ -395,7 +406,7 @@ __global__ __launch_bounds__((AttnPlan<T, DH, DV, SHARED>::NT), (AttnPlan<T, DH,
   using P = AttnPlan<T, DH, DV, SHARED>;
   using M = amma<T>;
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  const int id = xcd_tile(gridDim.x);
+  const int id = xcd_tile(a);
   if (id >= a.work) return;
   const int part = id / a.splits, split = id - part * a.splits, tile = part / a.halves, col = (part - tile * a.halves) * DV;
   RowWave w;
@@ -414,10 +425,10 @@ __global__ __launch_bounds__((AttnPlan<T, DH, DV, SHARED>::NT), (AttnPlan<T, DH,
   float mu[2] = {0.0f, 0.0f};
   const int tn = (w.kend + P::N - 1) / P::N, per = (tn + a.splits - 1) / a.splits;
   key_tiles<T, DH, DV, SHARED>(a, w, col, split * per, min(tn, (split + 1) * per), smem,
-                               [&](const T* kt, int it0, uint32_t hid, int j0) {
+                               [&](const char* kt, int it0, uint32_t hid, int j0) {
     af32x16_t x[2];
 #pragma unroll
-    for (int m = 0; m < 2; ++m) x[m] = tile_dot<T, S::KB, S::LDK>(kt + m * P::N * S::LDK, it0, qf[m], w.lane);
+    for (int m = 0; m < 2; ++m) x[m] = tile_dot<T, S::KB, S::LX>(kt, it0, m * S::LX / 2, qf[m], w.lane);
     if (hid != 0 || (MASK && (a.causal || a.mask_kind != 0))) mask_tile<MASK>(a, x, hid, w.b, w.h, w.i, j0, rscale, w.lane);
     float p[2][16];
 #pragma unroll
@@ -458,13 +469,13 @@ __global__ __launch_bounds__((AttnPlan<T, DH, DV, SHARED>::NT), (AttnPlan<T, DH,
         }
       }
     }
-    const T* vt = kt + 2 * P::N * S::LDK;
+    const char* vt = kt + S::xbytes(P::N);
 #pragma unroll
     for (int st = 0; st < 2; ++st) {
       const typename M::frag f0 = M::pack(p[0] + 8 * st), f1 = M::pack(p[1] + 8 * st);
 #pragma unroll
       for (int d = 0; d < S::VO; ++d) {
-        const typename M::frag vf = M::template load_tr<S::LDV>(vt, it0 + 16 * st, 32 * d, w.lane);
+        const typename M::frag vf = M::template load_tr<S::LY>(vt, it0 + 16 * st, 0, d, w.lane);
         s.acc[0][d] = M::mul(vf, f0, s.acc[0][d]);
         s.acc[1][d] = M::mul(vf, f1, s.acc[1][d]);
       }
@@ -497,7 +508,7 @@ __global__ __launch_bounds__(256) void diff_attn_join_kernel(const DiffAttnArgs 
   __shared__ float wt[2][kAttnSplits], red[4][4], o2s[128];
   const float c = a.scale * kLog2e;
   const int part = blockIdx.x, half = part % a.halves, row = part / a.halves, bh = row / a.R, r = row - bh * a.R;
-  const int tiles = (a.R + 31) / 32, tile = bh * tiles + r / 32, lane = r % 32, col = half * DV;
+  const int tiles = (a.R + 31) / 32, tile = bh * tiles + (a.causal ? tiles - 1 - r / 32 : r / 32), lane = r % 32, col = half * DV;
   const int b = bh / a.Hk, hk = bh - b * a.Hk, h = hk * a.G + r / a.Nq, i = r % a.Nq;
   const int64_t rows = (int64_t)a.B * a.H * a.Nq, rowid = ((int64_t)b * a.H + h) * a.Nq + i;
   const float* p = a.part + ((int64_t)(tile * a.halves + half) * a.splits * 64 + lane) * FLOATS;      // split n, lane half: + (64 n + 32 s) FLOATS
@@ -606,6 +617,49 @@ __device__ __forceinline__ void join_waves(af32x16_t* const (&acc)[NB], float* s
   }
 }
 
+__device__ __forceinline__ void put_block(float* at, const af32x16_t& v) {
+#pragma unroll
+  for (int q = 0; q < 4; ++q) *reinterpret_cast<float4*>(at + 4 * q) = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+}
+// sum over the splits of a lane's 16 floats, in split order
+__device__ __forceinline__ af32x16_t sum_block(const float* at, int splits, int64_t step) {
+  af32x16_t v = {0.0f};
+#pragma unroll 2
+  for (int n = 0; n < splits; ++n)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const float4 f = *reinterpret_cast<const float4*>(at + n * step + 4 * q);
+      v[4 * q] += f.x; v[4 * q + 1] += f.y; v[4 * q + 2] += f.z; v[4 * q + 3] += f.w;
+    }
+  return v;
+}
+template <typename T> __device__ __forceinline__ void store_block(T* row, int d0, int D, const af32x16_t& v, float f, int lane) {
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    float o[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = f != 0.0f ? v[4 * q + e] * f : 0.0f;
+    store_quad<T>(row, d0 + tile_item(4 * q, lane), D, o);
+  }
+}
+// block n of a row's gradient: map n / KO, columns 32 (n % KO) ..
+template <typename T, int KO>
+__device__ __forceinline__ void store_gq(const DiffAttnArgs& a, const RowWave& w, int n, const af32x16_t& v) {
+  // a single key has probability 1 whatever its score: its gradient is zero, not the rounding of G - del
+  const float one = a.Nk > 1 ? a.scale : 0.0f;
+  store_block<T>((T*)a.gq + ((((int64_t)w.b * a.Nq + w.i) * a.H + w.h) * 2 + n / KO) * a.Dh, 32 * (n % KO), a.Dh, v,
+                 n < KO ? one : -a.lam[w.h] * one, w.lane);
+}
+// block n of a key's gradients: grad_k's 2 KO, then grad_v's; `ok`: a key that is seen
+template <typename T, int KO>
+__device__ __forceinline__ void store_gkv(const DiffAttnArgs& a, int b, int hk, int j, bool ok, int n, const af32x16_t& v, int lane) {
+  const int64_t row = ((int64_t)b * a.Nk + j) * a.Hk + hk;
+  if (n < 2 * KO)
+    store_block<T>((T*)a.gk + (row * 2 + n / KO) * a.Dh, 32 * (n % KO), a.Dh, v, ok && a.Nk > 1 ? a.scale : 0.0f, lane);
+  else
+    store_block<T>((T*)a.gv + row * a.Dv, 32 * (n - 2 * KO), a.Dv, v, ok ? a.up / kProbScale<T> : 0.0f, lane);
+}
+
 // ---- backward: grad_q and the rows' parts of grad_lam; own = rows, staged = keys -----------------------------------------------
 template <typename T, int DH, int DV, bool SHARED, int MODE>
 __global__ __launch_bounds__((AttnPlan<T, DH, DV, SHARED>::NT), (AttnPlan<T, DH, DV, SHARED>::MINW)) void diff_attn_bwd_q_kernel(
@@ -614,8 +668,9 @@ __global__ __launch_bounds__((AttnPlan<T, DH, DV, SHARED>::NT), (AttnPlan<T, DH,
   using P = AttnPlan<T, DH, DV, SHARED>;
   using M = amma<T>;
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  const int tile = xcd_tile(gridDim.x);
-  if (tile >= a.work) return;
+  const int id = xcd_tile(a);
+  if (id >= a.work) return;
+  const int tile = id / a.splits, split = id - tile * a.splits;
   RowWave w;
   w.init<P::WQ, P::WK, MODE == kAttnAny>(a, tile);
   constexpr bool MASK = MODE == kAttnAny;
@@ -636,11 +691,12 @@ __global__ __launch_bounds__((AttnPlan<T, DH, DV, SHARED>::NT), (AttnPlan<T, DH,
   for (int m = 0; m < 2; ++m)
 #pragma unroll
     for (int d = 0; d < S::KO; ++d) acc[m][d] = af32x16_t{0.0f};
-  key_tiles<T, DH, DV, SHARED>(a, w, 0, 0, (w.kend + P::N - 1) / P::N, smem, [&](const T* kt, int it0, uint32_t hid, int j0) {
+  const int tn = (w.kend + P::N - 1) / P::N, per = (tn + a.splits - 1) / a.splits;
+  key_tiles<T, DH, DV, SHARED>(a, w, 0, split * per, min(tn, (split + 1) * per), smem, [&](const char* kt, int it0, uint32_t hid, int j0) {
     af32x16_t x[2];
 #pragma unroll
-    for (int m = 0; m < 2; ++m) x[m] = tile_dot<T, S::KB, S::LDK>(kt + m * P::N * S::LDK, it0, qf[m], w.lane);
-    af32x16_t g = tile_dot<T, S::VB, S::LDV>(kt + 2 * P::N * S::LDK, it0, gf, w.lane);
+    for (int m = 0; m < 2; ++m) x[m] = tile_dot<T, S::KB, S::LX>(kt, it0, m * S::LX / 2, qf[m], w.lane);
+    af32x16_t g = tile_dot<T, S::VB, S::LY>(kt + S::xbytes(P::N), it0, 0, gf, w.lane);
     if (hid != 0 || (MASK && (a.causal || a.mask_kind != 0))) mask_tile<MASK>(a, x, hid, w.b, w.h, w.i, j0, rscale, w.lane);
     if (drop) {
 #pragma unroll
@@ -670,7 +726,7 @@ __global__ __launch_bounds__((AttnPlan<T, DH, DV, SHARED>::NT), (AttnPlan<T, DH,
         const typename M::frag f = M::pack(ds);
 #pragma unroll
         for (int d = 0; d < S::KO; ++d)
-          acc[m][d] = M::mul(M::template load_tr<S::LDK>(kt + m * P::N * S::LDK, it0 + 16 * st, 32 * d, w.lane), f, acc[m][d]);
+          acc[m][d] = M::mul(M::template load_tr<S::LX>(kt, it0 + 16 * st, m * S::LX / 2, d, w.lane), f, acc[m][d]);
       }
   });
   if constexpr (!SHARED) {
@@ -683,25 +739,19 @@ __global__ __launch_bounds__((AttnPlan<T, DH, DV, SHARED>::NT), (AttnPlan<T, DH,
     if (w.wk != 0) return;
     dl = dlv[0];
   }
-  dl = half_sum(dl);
   if (!w.ok) return;
+  if (a.splits > 1) {
+    float* at = a.part + ((int64_t)id * 64 + w.lane) * S::QFLOATS;
+#pragma unroll
+    for (int n = 0; n < 2 * S::KO; ++n) put_block(at + 16 * n, acc[n / S::KO][n % S::KO]);
+    at[32 * S::KO] = dl;
+    return;
+  }
+  dl = half_sum(dl);
   if (w.lane < 32) a.dlrow[w.rowid] = -dl;
   if (a.gq == nullptr) return;
-  // a single key has probability 1 whatever its score: its gradient is zero, not the rounding of G - del
-  const float one = a.Nk > 1 ? a.scale : 0.0f, f[2] = {one, -a.lam[w.h] * one};
 #pragma unroll
-  for (int m = 0; m < 2; ++m) {
-    T* row = (T*)a.gq + ((((int64_t)w.b * a.Nq + w.i) * a.H + w.h) * 2 + m) * a.Dh;
-#pragma unroll
-    for (int d = 0; d < S::KO; ++d)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        float o[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = acc[m][d][4 * q + e] * f[m];
-        store_quad<T>(row, 32 * d + tile_item(4 * q, w.lane), a.Dh, o);
-      }
-  }
+  for (int n = 0; n < 2 * S::KO; ++n) store_gq<T, S::KO>(a, w, n, acc[n / S::KO][n % S::KO]);
 }
 
 // grad_lam[h] = sum over the batch and the queries, one block a head, fixed order
@@ -732,8 +782,9 @@ __global__ __launch_bounds__((AttnPlan<T, DH, DV, SHARED>::NT), (AttnPlan<T, DH,
   constexpr int N = P::N;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, wq = wave / P::WK, wk = wave % P::WK;
-  const int tile = xcd_tile(gridDim.x);
-  if (tile >= a.work) return;
+  const int id = xcd_tile(a);
+  if (id >= a.work) return;
+  const int tile = id / a.splits, split = id - tile * a.splits;
   const int tiles = (a.Nk + 32 * P::WQ - 1) / (32 * P::WQ), bh = tile / tiles, jb = (tile - bh * tiles) * 32 * P::WQ;
   const int b = bh / a.Hk, hk = bh - b * a.Hk;
   const int j = jb + 32 * wq + (lane & 31);
@@ -758,11 +809,13 @@ __global__ __launch_bounds__((AttnPlan<T, DH, DV, SHARED>::NT), (AttnPlan<T, DH,
   const uint64_t zseed = attn_seed(a.seed, a.seed_dev) + (uint64_t)(j >> 2);
 
   // tiles of a head from the first whose rows may see a key of the block
-  const int first = MASK && a.causal ? max(0, jb - off) / N : 0, per = max(0, (a.Nq + N - 1) / N - first), total = per * a.G;
+  const int first = MASK && a.causal ? max(0, jb - off) / N : 0, per = max(0, (a.Nq + N - 1) / N - first);
+  const int all = per * a.G, share = (all + a.splits - 1) / a.splits, begin = split * share, total = min(all, begin + share);
   const int st = SHARED ? threadIdx.x : lane;
   AttnStage<T, DH, DV, N, P::LT> sg;
   const uint32_t xrow = (uint32_t)(a.qs[1] * elem<T>::kBytes), yrow = (uint32_t)(a.gs[1] * elem<T>::kBytes);
   sg.init(st, xrow, (uint32_t)(a.qs[3] * elem<T>::kBytes), yrow, a.Dh, a.Dv);
+  const int sr = st % N;
   float4 srow;
   float2 srowl = make_float2(0.0f, 0.0f);
   auto load = [&](int t) {
@@ -770,35 +823,34 @@ __global__ __launch_bounds__((AttnPlan<T, DH, DV, SHARED>::NT), (AttnPlan<T, DH,
     const char* xb = (const char*)a.q + (b * a.qs[0] + (int64_t)i0 * a.qs[1] + h * a.qs[2]) * elem<T>::kBytes;
     const char* yb = (const char*)a.go + (b * a.gs[0] + (int64_t)i0 * a.gs[1] + h * a.gs[2]) * elem<T>::kBytes;
     sg.load(xb, xrow, yb, yrow, left >= N ? 0ull : ~0ull << left, st);
-    if (st < N) {
-      const int64_t rid = ((int64_t)b * a.H + h) * a.Nq + i0 + min(st, left - 1);
-      srow = a.row[rid];
-      if (fm) srowl = a.rowl[rid];
-      if (st >= left) { srow = fm ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : make_float4(-kNegInf, -kNegInf, 0.0f, 0.0f); srowl = make_float2(-kNegInf, -kNegInf); }
-    }
+    // (threads past the tile's rows repeat a row's: no divergent branch in the loop)
+    const int64_t rid = ((int64_t)b * a.H + h) * a.Nq + i0 + min(sr, left - 1);
+    srow = a.row[rid];
+    if (fm) srowl = a.rowl[rid];
+    const bool gone = sr >= left;                      // as a row that sees no key (row_probability)
+    const float far = gone ? (fm ? 0.0f : -kNegInf) : 0.0f;
+    srow.x = gone ? far : srow.x; srow.y = gone ? far : srow.y; srow.z = gone ? 0.0f : srow.z; srow.w = gone ? 0.0f : srow.w;
+    srowl.x = gone ? -kNegInf : srowl.x; srowl.y = gone ? -kNegInf : srowl.y;
   };
   auto store = [&](char* at) {
-    sg.store(reinterpret_cast<T*>(at), st);
-    if (st < N) {
-      reinterpret_cast<float4*>(at + S::elems(N) * elem<T>::kBytes)[st] = srow;
-      if (fm) reinterpret_cast<float2*>(at + S::elems(N) * elem<T>::kBytes + 16 * N)[st] = srowl;
-    }
+    sg.store(at, st);
+    reinterpret_cast<float4*>(at + S::xybytes(N))[sr] = srow;
+    if (fm) reinterpret_cast<float2*>(at + S::xybytes(N) + 16 * N)[sr] = srowl;
   };
   char* const own = smem + (SHARED ? 0 : wk * S::bytes(N));
   int cur = 0;
-  if (wk < total) {
-    load(wk);
+  if (begin + wk < total) {
+    load(begin + wk);
     store(own);
     tile_ready<SHARED>();
   }
 #pragma unroll 1
-  for (int t = wk; t < total; t += P::WK) {
+  for (int t = begin + wk; t < total; t += P::WK) {
     const bool more = t + P::WK < total;
     if (more) load(t + P::WK);
-    const char* at = SHARED ? smem + cur * S::bytes(N) : own;
-    const T* qt = reinterpret_cast<const T*>(at);
-    const T* gt = qt + 2 * N * S::LDK;
-    const float4* rows = reinterpret_cast<const float4*>(at + S::elems(N) * elem<T>::kBytes);
+    const char* qt = SHARED ? smem + cur * S::bytes(N) : own;
+    const char* gt = qt + S::xbytes(N);
+    const float4* rows = reinterpret_cast<const float4*>(qt + S::xybytes(N));
     const float2* rowl = reinterpret_cast<const float2*>(rows + N);
     const int g = t / per, h = hk * a.G + g, i00 = (first + t - g * per) * N;
     const float lam = a.lam[h];
@@ -808,9 +860,9 @@ __global__ __launch_bounds__((AttnPlan<T, DH, DV, SHARED>::NT), (AttnPlan<T, DH,
       if (i0 >= a.Nq) break;
       af32x16_t x[2];
 #pragma unroll
-      for (int m = 0; m < 2; ++m) x[m] = tile_dot<T, S::KB, S::LDK>(qt + m * N * S::LDK, it0, kf[m], lane);
+      for (int m = 0; m < 2; ++m) x[m] = tile_dot<T, S::KB, S::LX>(qt, it0, m * S::LX / 2, kf[m], lane);
       af32x16_t gm = {0.0f};
-      if constexpr (PART != 2) gm = tile_dot<T, S::VB, S::LDV>(gt, it0, vf, lane);
+      if constexpr (PART != 2) gm = tile_dot<T, S::VB, S::LY>(gt, it0, 0, vf, lane);
       if (MASK && a.causal) {
         const int lim = jc - off - i0 - 4 * (lane >> 5);                // rows before it do not see the key
         if (__any(lim > -4 * (lane >> 5))) {
@@ -860,7 +912,7 @@ __global__ __launch_bounds__((AttnPlan<T, DH, DV, SHARED>::NT), (AttnPlan<T, DH,
         if constexpr (PART != 1) {
           const typename M::frag fp = M::pack(pc + 8 * s);
 #pragma unroll
-          for (int d = 0; d < S::VO; ++d) av[d] = M::mul(M::template load_tr<S::LDV>(gt, it0 + 16 * s, 32 * d, lane), fp, av[d]);
+          for (int d = 0; d < S::VO; ++d) av[d] = M::mul(M::template load_tr<S::LY>(gt, it0 + 16 * s, 0, d, lane), fp, av[d]);
         }
 #pragma unroll
         for (int m = 0; m < (PART != 2 ? 2 : 0); ++m) {
@@ -870,7 +922,7 @@ __global__ __launch_bounds__((AttnPlan<T, DH, DV, SHARED>::NT), (AttnPlan<T, DH,
           const typename M::frag f = M::pack(ds);
 #pragma unroll
           for (int d = 0; d < S::KO; ++d)
-            ak[m][d] = M::mul(M::template load_tr<S::LDK>(qt + m * N * S::LDK, it0 + 16 * s, 32 * d, lane), f, ak[m][d]);
+            ak[m][d] = M::mul(M::template load_tr<S::LX>(qt, it0 + 16 * s, m * S::LX / 2, d, lane), f, ak[m][d]);
         }
       }
     }
@@ -892,31 +944,47 @@ __global__ __launch_bounds__((AttnPlan<T, DH, DV, SHARED>::NT), (AttnPlan<T, DH,
     if (wk != 0) return;
   }
   if (!in) return;
-  const float fk = ok && a.Nk > 1 ? a.scale : 0.0f, fv = a.up / kProbScale<T>;        // (Nk = 1: as for grad_q)
+  // (a hidden key's columns may hold anything: stored as zeros)
+  constexpr int N0 = PART == 2 ? 2 * S::KO : 0, N1 = PART == 1 ? 2 * S::KO : 2 * S::KO + S::VO;
+  if (a.splits > 1) {
+    float* at = a.part + ((int64_t)id * 64 + lane) * S::KFLOATS;
 #pragma unroll
-  for (int m = 0; m < (PART != 2 ? 2 : 0); ++m) {
-    T* row = (T*)a.gk + ((((int64_t)b * a.Nk + j) * a.Hk + hk) * 2 + m) * a.Dh;
-#pragma unroll
-    for (int d = 0; d < S::KO; ++d)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        float o[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = fk != 0.0f ? ak[m][d][4 * q + e] * fk : 0.0f;
-        store_quad<T>(row, 32 * d + tile_item(4 * q, lane), a.Dh, o);
-      }
+    for (int n = N0; n < N1; ++n) put_block(at + 16 * n, n < 2 * S::KO ? ak[n / S::KO % 2][n % S::KO] : av[(n - 2 * S::KO) % S::VO]);
+    return;
   }
-  if constexpr (PART == 1) return;
-  T* row = (T*)a.gv + (((int64_t)b * a.Nk + j) * a.Hk + hk) * a.Dv;
 #pragma unroll
-  for (int d = 0; d < S::VO; ++d)
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      float o[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] = ok ? av[d][4 * q + e] * fv : 0.0f;
-      store_quad<T>(row, 32 * d + tile_item(4 * q, lane), a.Dv, o);
-    }
+  for (int n = N0; n < N1; ++n)
+    store_gkv<T, S::KO>(a, b, hk, j, ok, n, n < 2 * S::KO ? ak[n / S::KO % 2][n % S::KO] : av[(n - 2 * S::KO) % S::VO], lane);
+}
+
+// sums of the splits' gradients: one block an own tile of 32 rows (or keys) and block of 32 columns, one wave
+template <typename T, int DH, int DV>
+__global__ __launch_bounds__(64) void diff_attn_join_q_kernel(const DiffAttnArgs a) {
+  using S = AttnTile<T, DH, DV>;
+  RowWave w;
+  const int tile = blockIdx.x / (2 * S::KO), n = blockIdx.x - tile * 2 * S::KO;
+  w.init<1, 1, true>(a, tile);
+  if (!w.ok) return;
+  const int64_t step = 64 * S::QFLOATS;
+  const float* at = a.part + ((int64_t)tile * a.splits * 64 + w.lane) * S::QFLOATS;
+  if (n == 0) {
+    float dl = 0.0f;
+    for (int p = 0; p < a.splits; ++p) dl += at[p * step + 32 * S::KO];
+    dl = half_sum(dl);
+    if (w.lane < 32) a.dlrow[w.rowid] = -dl;
+  }
+  if (a.gq != nullptr) store_gq<T, S::KO>(a, w, n, sum_block(at + 16 * n, a.splits, step));
+}
+template <typename T, int DH, int DV>
+__global__ __launch_bounds__(64) void diff_attn_join_kv_kernel(const DiffAttnArgs a) {
+  using S = AttnTile<T, DH, DV>;
+  constexpr int NB = 2 * S::KO + S::VO;
+  const int tile = blockIdx.x / NB, n = blockIdx.x - tile * NB, lane = threadIdx.x;
+  const int tiles = (a.Nk + 31) / 32, bh = tile / tiles, j = (tile - bh * tiles) * 32 + (lane & 31), b = bh / a.Hk, hk = bh - b * a.Hk;
+  if (j >= a.Nk) return;
+  const bool ok = !(a.kpm != nullptr && a.kpm[(int64_t)b * a.Nk + j]);
+  const float* at = a.part + ((int64_t)tile * a.splits * 64 + lane) * S::KFLOATS;
+  store_gkv<T, S::KO>(a, b, hk, j, ok, n, sum_block(at + 16 * n, a.splits, 64 * S::KFLOATS), lane);
 }
 
 // ---- launch -----------------------------------------------------------------------------------------------------------------------
@@ -938,14 +1006,56 @@ template <typename F> static int attn_mode(const DiffAttnArgs& a, F&& f) {
   return f(std::integral_constant<int, kAttnPlain>{});
 }
 
-// The arrangement of a call.  A shared block does four private blocks' work in `cost` times their time (it stages a tile once
-// for 128 own items), but there are a quarter as many: with 256 CUs the rounds of blocks decide.  Measured at one block per CU
-// (bf16, us, shared / private): 64 / 64 wide heads 80 / 121, 128 / 128 133 / 278; 32 / 64, 10 000 x 10 000 and 4 heads (316 or
-// 1252 blocks) 400 / 299.
-static bool attn_shared(int64_t heads, int64_t items, int DH) {
-  const int64_t wide = heads * ((items + 127) / 128), narrow = heads * ((items + 31) / 32);
-  const double cost = DH <= 32 ? 0.8 : 0.65;
-  return 4.0 * cost * (double)((wide + 255) / 256) < (double)((narrow + 255) / 256);
+// How a pass over `own` items a head against `staged` ones is cut into blocks.
+//
+// shared: a shared block does four private blocks' work in `cost` times their time (it stages a tile once for 128 own items), but
+// there are a quarter as many: with 256 CUs the rounds of blocks decide; causal blocks are unequal, the longest twice the mean.
+// Measured at one block a CU (bf16, us, shared / private): 64 / 64 wide heads 80 / 121, 128 / 128 133 / 278; 32 / 64 at 10 000 x
+// 10 000 and 4 heads (316 or 1252 blocks) 400 / 299.
+// splits: private blocks that share the staged items of one own tile, where own tiles alone leave the chip empty: up to twice as
+// many waves as fill it (ragged batches and causal rows are unequal), at least four tiles for each wave.
+struct AttnCut { bool shared; int splits; };
+template <typename T, int DH, int DV> static AttnCut attn_cut(const DiffAttnArgs& a, int64_t heads, int64_t own, int64_t staged, bool may_share) {
+  using S = AttnTile<T, DH, DV>;
+  const int64_t wide = heads * ((own + 127) / 128), narrow = heads * ((own + 31) / 32);
+  const double cost = DH <= 32 ? 0.8 : 0.65, uneven = a.causal ? 2.0 : 1.0;
+  double ts = 4.0 * cost * (double)((wide + 255) / 256), tp = (double)((narrow + 255) / 256);
+  if (a.causal) {
+    ts = fmax(4.0 * cost, 4.0 * cost * wide / 512.0);
+    tp = fmax(1.0, narrow / 512.0);
+  }
+  if (may_share && ts < tp) return {true, 1};
+  const int64_t waves = narrow * S::WK, fill = 1024 * S::MINW * 2;
+  const int64_t each = (staged + 31) / 32 / S::WK / 4;
+  int64_t splits = waves * 2 > fill && uneven == 1.0 ? 1 : (fill + waves - 1) / waves;
+  splits = splits < each ? splits : each;
+  splits = splits < kAttnSplits ? splits : kAttnSplits;
+  return {false, (int)(splits > 1 ? splits : 1)};
+}
+template <typename T, int DH, int DV> static AttnCut attn_cut_fwd(const DiffAttnArgs& a) {
+  return attn_cut<T, DH, (DV > 128 ? 128 : DV)>(a, (int64_t)a.B * a.Hk * (a.Dv > 128 ? 2 : 1), a.R, a.Nk, true);
+}
+template <typename T, int DH, int DV> static AttnCut attn_cut_q(const DiffAttnArgs& a) {
+  return attn_cut<T, DH, DV>(a, (int64_t)a.B * a.Hk, a.R, a.Nk, true);
+}
+template <typename T, int DH, int DV> static AttnCut attn_cut_kv(const DiffAttnArgs& a) {
+  // (128 / 128 in one pass spills as a shared block: 357 us, private 277)
+  return attn_cut<T, DH, DV>(a, (int64_t)a.B * a.Hk, a.Nk, (int64_t)a.G * ((a.Nq + 31) / 32) * 32, !(DH == 128 && DV == 128));
+}
+
+// bytes of the splits' sums
+template <typename T, int DH, int DV> static int64_t attn_bytes_fwd(const DiffAttnArgs& a) {
+  constexpr int DC = DV > 128 ? 128 : DV;
+  const AttnCut c = attn_cut_fwd<T, DH, DV>(a);
+  return c.splits <= 1 ? 0 : (int64_t)a.B * a.Hk * ((a.R + 31) / 32) * ((a.Dv + DC - 1) / DC) * c.splits * 64 * FwdState<T, DC>::FLOATS * 4;
+}
+template <typename T, int DH, int DV> static int64_t attn_bytes_bwd(const DiffAttnArgs& a) {
+  using S = AttnTile<T, DH, DV>;
+  const AttnCut q = attn_cut_q<T, DH, DV>(a), kv = attn_cut_kv<T, DH, DV>(a);
+  const int64_t heads = (int64_t)a.B * a.Hk;
+  const int64_t bq = q.splits <= 1 ? 0 : heads * ((a.R + 31) / 32) * q.splits * 64 * S::QFLOATS * 4;
+  const int64_t bk = kv.splits <= 1 ? 0 : heads * ((a.Nk + 31) / 32) * kv.splits * 64 * S::KFLOATS * 4;
+  return bq > bk ? bq : bk;
 }
 
 template <typename T, int DH, int DV>
@@ -954,43 +1064,40 @@ static int attn_forward(DiffAttnArgs a, void* ws, int64_t ws_bytes, hipStream_t 
   constexpr int DC = DV > 128 ? 128 : DV;
   const int64_t heads = (int64_t)a.B * a.Hk;
   const char* who = "diff_attention_forward";
-  a.splits = 1;
+  AttnCut cut = attn_cut_fwd<T, DH, DV>(a);
+  if (ws_bytes < attn_bytes_fwd<T, DH, DV>(a)) cut.splits = 1;
+  a.splits = cut.splits;
+  a.part = (float*)ws;
   a.halves = (a.Dv + DC - 1) / DC;
   auto run = [&](auto shared) {
     constexpr bool SH = decltype(shared)::value;
     using P = AttnPlan<T, DH, DC, SH>;
     return attn_mode(a, [&](auto mode) {
-      return attn_launch(diff_attn_fwd_kernel<T, DH, DC, SH, decltype(mode)::value>, heads * ((a.R + 32 * P::WQ - 1) / (32 * P::WQ)) * a.halves * a.splits,
-                         P::NT, P::lds(FwdState<T, DC>::FLOATS), a, st, who);
+      return attn_launch(diff_attn_fwd_kernel<T, DH, DC, SH, decltype(mode)::value>,
+                         heads * ((a.R + 32 * P::WQ - 1) / (32 * P::WQ)) * a.halves * a.splits, P::NT, P::lds(FwdState<T, DC>::FLOATS), a, st, who);
     });
   };
-  if (attn_shared(heads * a.halves, a.R, DH)) return run(std::true_type{});
-  // few rows, many keys: blocks share the keys of a row tile and a second launch joins their sums
-  const int64_t splits = attn_splits(a.B, a.H, a.Hk, a.Nq, a.Nk, a.Dv);
-  if (splits > 1 && ws_bytes >= attn_part_bytes(a.B, a.H, a.Hk, a.Nq, a.Dv, splits)) {
-    a.splits = (int)splits;
-    a.part = (float*)ws;
-    const int rc = run(std::false_type{});
-    if (rc != UBV_OK) return rc;
-    hipLaunchKernelGGL((diff_attn_join_kernel<T, DC>), dim3((unsigned)(heads * a.R * a.halves)), dim3(256), 0, st, a);
-    UBV_CHECK_LAUNCH(who);
-    return UBV_OK;
-  }
-  return run(std::false_type{});
+  if (cut.shared) return run(std::true_type{});
+  const int rc = run(std::false_type{});
+  if (rc != UBV_OK || a.splits == 1) return rc;
+  hipLaunchKernelGGL((diff_attn_join_kernel<T, DC>), dim3((unsigned)(heads * a.R * a.halves)), dim3(256), 0, st, a);
+  UBV_CHECK_LAUNCH(who);
+  return UBV_OK;
 }
 
 template <typename T, int DH, int DV>
-static int attn_backward(const DiffAttnArgs& a, float* glam, hipStream_t st) {
+static int attn_backward(DiffAttnArgs a, float* glam, int64_t part_bytes, hipStream_t st) {
   using S = AttnTile<T, DH, DV>;
   const int64_t heads = (int64_t)a.B * a.Hk, rows = (int64_t)a.B * a.H * a.Nq;
   const char* who = "diff_attention_backward";
+  const bool room = part_bytes >= attn_bytes_bwd<T, DH, DV>(a);
   hipLaunchKernelGGL(diff_attn_del_kernel<T>, dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, st, a);
   UBV_CHECK_LAUNCH(who);
   auto run = [&](auto shared, auto pass) {
     constexpr bool SH = decltype(shared)::value;
     constexpr int PASS = decltype(pass)::value;                 // 0 .. 2: grad_k / grad_v of that part, 3: grad_q
     using P = AttnPlan<T, DH, DV, SH>;
-    const int64_t blocks = heads * (((PASS == 3 ? a.R : a.Nk) + 32 * P::WQ - 1) / (32 * P::WQ));
+    const int64_t blocks = heads * (((PASS == 3 ? a.R : a.Nk) + 32 * P::WQ - 1) / (32 * P::WQ)) * a.splits;
     return attn_mode(a, [&](auto mode) {
       constexpr int MODE = decltype(mode)::value;
       if constexpr (PASS == 3)
@@ -999,25 +1106,35 @@ static int attn_backward(const DiffAttnArgs& a, float* glam, hipStream_t st) {
         return attn_launch(diff_attn_bwd_kv_kernel<T, DH, DV, SH, MODE, PASS>, blocks, P::NT, P::lds((2 * S::KO + S::VO) * 16), a, st, who);
     });
   };
-  auto pick = [&](int64_t items, auto pass) {
-    return attn_shared(heads, items, DH) ? run(std::true_type{}, pass) : run(std::false_type{}, pass);
+  auto pass = [&](const AttnCut& cut, auto which) {
+    a.splits = room ? cut.splits : 1;
+    return cut.shared ? run(std::true_type{}, which) : run(std::false_type{}, which);
   };
   int rc = UBV_OK;
   if (a.gq != nullptr || glam != nullptr) {
-    rc = pick(a.R, std::integral_constant<int, 3>{});
+    rc = pass(attn_cut_q<T, DH, DV>(a), std::integral_constant<int, 3>{});
     if (rc != UBV_OK) return rc;
+    if (a.splits > 1) {
+      hipLaunchKernelGGL((diff_attn_join_q_kernel<T, DH, DV>), dim3((unsigned)(heads * ((a.R + 31) / 32) * 2 * S::KO)), dim3(64), 0, st, a);
+      UBV_CHECK_LAUNCH(who);
+    }
     if (glam != nullptr) {
       hipLaunchKernelGGL(diff_attn_lam_kernel, dim3((unsigned)a.H), dim3(256), 0, st, a.dlrow, glam, a.B, a.H, a.Nq);
       UBV_CHECK_LAUNCH(who);
     }
   }
   if (a.gk == nullptr) return rc;
-  if constexpr (2 * DH + DV > 2 * 128) {
-    rc = pick(a.Nk, std::integral_constant<int, 1>{});
-    return rc != UBV_OK ? rc : pick(a.Nk, std::integral_constant<int, 2>{});
+  const AttnCut cut = attn_cut_kv<T, DH, DV>(a);
+  if constexpr (2 * DH + DV > 384) {
+    rc = pass(cut, std::integral_constant<int, 1>{});
+    if (rc == UBV_OK) rc = pass(cut, std::integral_constant<int, 2>{});
   } else {
-    return pick(a.Nk, std::integral_constant<int, 0>{});
+    rc = pass(cut, std::integral_constant<int, 0>{});
   }
+  if (rc != UBV_OK || a.splits == 1) return rc;
+  hipLaunchKernelGGL((diff_attn_join_kv_kernel<T, DH, DV>), dim3((unsigned)(heads * ((a.Nk + 31) / 32) * (2 * S::KO + S::VO))), dim3(64), 0, st, a);
+  UBV_CHECK_LAUNCH(who);
+  return UBV_OK;
 }
 
 // the smallest pair of widths that holds the call's
@@ -1035,8 +1152,14 @@ int UBV_ATTN_NAME(forward)(const DiffAttnArgs& a, void* ws, int64_t ws_bytes, hi
 #undef UBV_DO
 }
 
-int UBV_ATTN_NAME(backward)(const DiffAttnArgs& a, float* glam, hipStream_t st) {
-#define UBV_DO(DH, DV) return attn_backward<UBV_ATTN_T, DH, DV>(a, glam, st);
+int UBV_ATTN_NAME(backward)(const DiffAttnArgs& a, float* glam, int64_t part_bytes, hipStream_t st) {
+#define UBV_DO(DH, DV) return attn_backward<UBV_ATTN_T, DH, DV>(a, glam, part_bytes, st);
+  UBV_ATTN_PAIRS(UBV_DO)
+#undef UBV_DO
+}
+
+int64_t UBV_ATTN_NAME(bytes)(const DiffAttnArgs& a, bool backward) {
+#define UBV_DO(DH, DV) return backward ? attn_bytes_bwd<UBV_ATTN_T, DH, DV>(a) : attn_bytes_fwd<UBV_ATTN_T, DH, DV>(a);
   UBV_ATTN_PAIRS(UBV_DO)
 #undef UBV_DO
 }

@@ -322,7 +322,7 @@ struct DiffAttentionBackward : Node {
       if (nl) gl = make({a.H}, o.dtype(at::kFloat));
       if (!a.empty() && (nq || nk || nv || nl)) {
         const Tensor go = operand(g[0]);
-        const int64_t nws = api.ubv_diff_attention_backward_workspace(a.B, a.H, a.Nq);
+        const int64_t nws = api.ubv_diff_attention_backward_workspace(a.B, a.H, a.Hk, a.Nq, a.Nk, a.Dh, a.Dv, (int)a.causal, type_code(q));
         const Tensor ws = bytes(nws, q);
         int64_t s[18];
         strides(s, q, k, v, go, a.mask);
@@ -403,7 +403,7 @@ Tensor diff_attention(const Tensor& q, const Tensor& k, const Tensor& v, const T
         stat = at::empty({B, H, Nq, 4}, q.options().dtype(at::kFloat));
         maps = at::empty({2, B, H, Nq, Dv}, q.options().dtype(at::kFloat));
       }
-      const int64_t nws = api.ubv_diff_attention_forward_workspace(a.B, a.H, a.Hk, a.Nq, a.Nk, a.Dv);
+      const int64_t nws = api.ubv_diff_attention_forward_workspace(a.B, a.H, a.Hk, a.Nq, a.Nk, a.Dh, a.Dv, (int)causal, dt);
       const Tensor ws = bytes(nws, q);
       int64_t s[18];
       strides(s, qc, kc, vc, Tensor(), a.mask);
