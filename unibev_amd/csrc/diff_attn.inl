@@ -24,8 +24,15 @@ template <typename T, int DH, int DV> struct AttnTile {
   // two waves a SIMD where accumulators, operands and a tile in flight fit half the registers (64 / 128, f16: forward 244 us with
   // two waves that spill, 167 with one that does not)
   static constexpr int MINW = DH <= 32 && DV <= 64 ? 2 : 1;
+  // own operands in registers: 2 KB + VB operands of 4 registers, f32 8: at 128 / 256 that is 256 beside the accumulators, and read
+  // again they cost less than spilled (8 heads, 1024 x 1024, us: grad_q 1360 spilled, 369; held where they fit: 64 / 128 1500 x 1500
+  // 188, read again 266)
+  static constexpr bool KEEP = elem<T>::kBytes == 2 || DH <= 64;
   static constexpr int fit(int w) { return w > 2 && w * bytes(32) > 150 * 1024 ? fit(w / 2) : w; }
-  static constexpr int WK = fit(4 * MINW);                                       // waves of a private block: a CU's worth
+  // waves of a private block.  16-bit heads up to 32 / 64: all of a CU's, which halves a block's time where blocks are few (2 x 4
+  // heads, 900 x 900 bf16, us: 56 with eight waves, 64 with four; 4 heads, 10 000 x 10 000: 1090, 1050); f32's tiles are longer
+  // (8 heads of 16 / 32, 2 x 900: 173, 148)
+  static constexpr int WK = fit(elem<T>::kBytes == 2 ? 4 * MINW : 4);
   static constexpr int NS = 2 * bytes(64) <= 76 * 1024 ? 64 : 32;                // items of a shared tile
 };
 
@@ -39,6 +46,9 @@ template <typename T, int DH, int DV, bool SHARED> struct AttnPlan {
   static constexpr int merge(int floats) { return SHARED ? 0 : (WK / 2) * floats * 64 * 4; }     // joining `floats` per lane
   static constexpr int lds(int floats) { return LDS > merge(floats) ? LDS : merge(floats); }
   static constexpr int MINW = S::MINW;
+  // 16-byte pieces of a tile that a thread holds: at most a quarter of its registers
+  static constexpr bool PREF = S::xybytes(N) / LT / 16 <= (MINW == 2 ? 8 : 16);
+  static_assert(PREF || !SHARED, "a shared tile passes through registers");
 };
 
 // What a call may hold beside hidden keys.  Each has kernels of its own: what a kernel can never meet costs it registers, and
@@ -46,11 +56,12 @@ template <typename T, int DH, int DV, bool SHARED> struct AttnPlan {
 constexpr int kAttnPlain = 0, kAttnDrop = 1, kAttnAny = 2;       // nothing | dropout | masks, causal, dropout or not
 
 // ---- staging ------------------------------------------------------------------------------------------------------------------
-template <typename T, int DH, int DV, int N, int LT> struct AttnStage {
+// PREF: a tile's pieces wait in registers until the present tile is done with; else they pass through in groups of 8
+template <typename T, int DH, int DV, int N, int LT, bool PREF> struct AttnStage {
   using S = AttnTile<T, DH, DV>;
   static constexpr int PX = S::LX, PY = S::LY, NX = N * PX / LT, NY = N * PY / LT;
   static_assert(N * PX % LT == 0 && N * PY % LT == 0 && LT % PX == 0 && LT % PY == 0, "a thread keeps its column");
-  au32x4_t x[NX], y[NY];
+  au32x4_t x[PREF ? NX : 1], y[PREF ? NY : 1];
   uint32_t xoff, yoff;               // this thread's byte offset inside a tile, kOutside past the head's width
 
   __device__ __forceinline__ void init(int t, uint32_t xrow, uint32_t xmap, uint32_t yrow, int Dh, int Dv) {
@@ -58,7 +69,8 @@ template <typename T, int DH, int DV, int N, int LT> struct AttnStage {
     xoff = dx < Dh ? (t / PX) * xrow + m * xmap + dx * elem<T>::kBytes : kOutside;
     yoff = dy < Dv ? (t / PY) * yrow + dy * elem<T>::kBytes : kOutside;
   }
-  // `hid`: bit i set: item i becomes zeros
+  // byte offset of piece c of x (y): kOutside where bit `item` of hid is set (the item becomes zeros)
+  __device__ __forceinline__ uint32_t at(uint32_t off, int item, uint64_t hid) const { return hid != 0 && ((hid >> item) & 1) ? kOutside : off; }
   __device__ __forceinline__ void load(const char* xb, uint32_t xrow, const char* yb, uint32_t yrow, uint64_t hid, int t) {
     const __amdgpu_buffer_rsrc_t rx = attn_rsrc(xb), ry = attn_rsrc(yb);
     if (hid == 0) {
@@ -68,24 +80,38 @@ template <typename T, int DH, int DV, int N, int LT> struct AttnStage {
       for (int c = 0; c < NY; ++c) y[c] = attn_piece(ry, yoff, c * (LT / PY) * yrow);
     } else {
 #pragma unroll
-      for (int c = 0; c < NX; ++c)
-        x[c] = attn_piece(rx, (hid >> (t / PX + c * (LT / PX))) & 1 ? kOutside : xoff, c * (LT / PX) * xrow);
+      for (int c = 0; c < NX; ++c) x[c] = attn_piece(rx, at(xoff, t / PX + c * (LT / PX), hid), c * (LT / PX) * xrow);
 #pragma unroll
-      for (int c = 0; c < NY; ++c)
-        y[c] = attn_piece(ry, (hid >> (t / PY + c * (LT / PY))) & 1 ? kOutside : yoff, c * (LT / PY) * yrow);
+      for (int c = 0; c < NY; ++c) y[c] = attn_piece(ry, at(yoff, t / PY + c * (LT / PY), hid), c * (LT / PY) * yrow);
     }
   }
+  // place of piece c (a thread's rows are its first one plus multiples of a power of two above it: their folds XOR)
+  template <int L> static __device__ __forceinline__ char* place(char* lds, int t, int c) {
+    const int o = (t / L) * 16 * L + (((t % L) ^ row_fold<L>(t / L)) << 4);
+    return lds + c * (LT / L) * 16 * L + (o ^ (row_fold<L>(c * (LT / L)) << 4));
+  }
   __device__ __forceinline__ void store(char* lds, int t) {
-    // (a thread's rows are its first one plus multiples of a power of two above it: their folds XOR)
-    const int ox = (t / PX) * 16 * PX + (((t % PX) ^ row_fold<PX>(t / PX)) << 4);
 #pragma unroll
-    for (int c = 0; c < NX; ++c)
-      *reinterpret_cast<au32x4_t*>(lds + c * (LT / PX) * 16 * PX + (ox ^ (row_fold<PX>(c * (LT / PX)) << 4))) = x[c];
-    const int oy = (t / PY) * 16 * PY + (((t % PY) ^ row_fold<PY>(t / PY)) << 4);
-    char* ly = lds + S::xbytes(N);
+    for (int c = 0; c < NX; ++c) *reinterpret_cast<au32x4_t*>(place<PX>(lds, t, c)) = x[c];
 #pragma unroll
-    for (int c = 0; c < NY; ++c)
-      *reinterpret_cast<au32x4_t*>(ly + c * (LT / PY) * 16 * PY + (oy ^ (row_fold<PY>(c * (LT / PY)) << 4))) = y[c];
+    for (int c = 0; c < NY; ++c) *reinterpret_cast<au32x4_t*>(place<PY>(lds + S::xbytes(N), t, c)) = y[c];
+  }
+  template <int L, int COUNT> __device__ __forceinline__ void pass(const char* base, uint32_t row, uint32_t off, uint64_t hid, char* lds, int t) const {
+    const __amdgpu_buffer_rsrc_t r = attn_rsrc(base);
+    constexpr int G = COUNT < 8 ? COUNT : 8;
+#pragma unroll
+    for (int c0 = 0; c0 < COUNT; c0 += G) {
+      au32x4_t v[G];
+#pragma unroll
+      for (int c = 0; c < G; ++c) v[c] = attn_piece(r, at(off, t / L + (c0 + c) * (LT / L), hid), (c0 + c) * (LT / L) * row);
+#pragma unroll
+      for (int c = 0; c < G; ++c) *reinterpret_cast<au32x4_t*>(place<L>(lds, t, c0 + c)) = v[c];
+      __builtin_amdgcn_sched_barrier(0);               // (or all groups' loads would be drawn together, and need the registers)
+    }
+  }
+  __device__ __forceinline__ void through(const char* xb, uint32_t xrow, const char* yb, uint32_t yrow, uint64_t hid, char* lds, int t) const {
+    pass<PX, NX>(xb, xrow, xoff, hid, lds, t);
+    pass<PY, NY>(yb, yrow, yoff, hid, lds + S::xbytes(N), t);
   }
 };
 
@@ -98,30 +124,51 @@ template <bool SHARED> __device__ __forceinline__ void tile_ready() {
   }
 }
 
-// a lane's own item as B operands: 8 elements at 16 s + 8 (lane >> 5) of step s
-template <typename T, int NB>
-__device__ __forceinline__ void own_frags(typename amma<T>::frag (&f)[NB], const T* p, bool ok, int D, int lane) {
-  constexpr int VEC = 16 / elem<T>::kBytes;
+// A lane's own item as B operands: 8 elements at 16 s + 8 (lane >> 5) of step s.  KEEP: held in registers; else read again (from L1:
+// a block's own rows are at most 64 KB) for every tile, where the accumulators leave no room for them.
+template <typename T, int NB, bool KEEP> struct OwnRow {
+  static constexpr int VEC = 16 / elem<T>::kBytes;
+  typename amma<T>::frag f[KEEP ? NB : 1];
+  const T* p;
+  bool ok;
+  int D, d0;
+
+  // p: a row of the tensor also where !ok (loaded, then dropped)
+  __device__ __forceinline__ void init(const T* row, bool ok_, int D_, int lane) {
+    p = row; ok = ok_; D = D_; d0 = 8 * (lane >> 5);
+    if constexpr (KEEP) {
 #pragma unroll
-  for (int s = 0; s < NB; ++s) {
-    const int d = 16 * s + 8 * (lane >> 5);
+      for (int s = 0; s < NB; ++s) f[s] = read(s);
+    }
+  }
+  __device__ __forceinline__ typename amma<T>::frag read(int s) const {
     T t[8];
 #pragma unroll
     for (int w = 0; w < 8 / VEC; ++w) {
-      const bool in = ok && d + w * VEC < D;            // (p is a row of the tensor also where !ok: loaded, then dropped)
-      const au32x4_t v = *reinterpret_cast<const au32x4_t*>(p + (in ? d + w * VEC : 0)), z = {0u, 0u, 0u, 0u};
+      const int d = 16 * s + d0 + w * VEC;
+      const bool in = ok && d < D;
+      const au32x4_t v = *reinterpret_cast<const au32x4_t*>(p + (in ? d : 0)), z = {0u, 0u, 0u, 0u};
       *reinterpret_cast<au32x4_t*>(t + w * VEC) = in ? v : z;
     }
-    f[s] = amma<T>::own(t);
+    return amma<T>::own(t);
   }
-}
+  __device__ __forceinline__ typename amma<T>::frag get(int s) const {
+    if constexpr (KEEP) return f[s];
+    else return read(s);
+  }
+  // a new tile: what was read for the last one is not to be kept
+  __device__ __forceinline__ void again() {
+    if constexpr (!KEEP) asm volatile("" : "+v"(p));
+  }
+};
 
 // 16 dot products of own item (lane & 31) with staged items it0 .. it0 + 31, over the part of their rows from chunk c0
-template <typename T, int NB, int L>
-__device__ __forceinline__ af32x16_t tile_dot(const char* tile, int it0, int c0, const typename amma<T>::frag (&own)[NB], int lane) {
+template <typename T, int NB, int L, bool KEEP>
+__device__ __forceinline__ af32x16_t tile_dot(const char* tile, int it0, int c0, OwnRow<T, NB, KEEP>& own, int lane) {
   af32x16_t c = {0.0f};
+  own.again();
 #pragma unroll
-  for (int s = 0; s < NB; ++s) c = amma<T>::mul(amma<T>::template load<L>(tile, it0, c0, s, lane), own[s], c);
+  for (int s = 0; s < NB; ++s) c = amma<T>::mul(amma<T>::template load<L>(tile, it0, c0, s, lane), own.get(s), c);
   return c;
 }
 
@@ -260,21 +307,23 @@ __device__ __forceinline__ void key_tiles(const DiffAttnArgs& a, const RowWave& 
   constexpr int N = P::N, STEP = P::WK;
   constexpr uint64_t ALL = N == 64 ? ~0ull : 0xffffffffull;
   const int st = SHARED ? threadIdx.x : w.lane;
-  AttnStage<T, DH, DV, N, P::LT> sg;
+  AttnStage<T, DH, DV, N, P::LT, P::PREF> sg;
   const uint32_t xrow = (uint32_t)(a.ks[1] * elem<T>::kBytes), yrow = (uint32_t)(a.vs[1] * elem<T>::kBytes);
   sg.init(st, xrow, (uint32_t)(a.ks[3] * elem<T>::kBytes), yrow, a.Dh, a.Dv - col);
   const char* kb = (const char*)a.k + (w.b * a.ks[0] + w.hk * a.ks[2]) * elem<T>::kBytes;
   const char* vb = (const char*)a.v + (w.b * a.vs[0] + w.hk * a.vs[2] + col) * elem<T>::kBytes;
   int t = t0 + w.wk;
   if (t >= t1) return;                                       // (private waves only: no barrier inside)
-  auto load = [&](int tt, uint64_t hid) {
+  auto load = [&](int tt, uint64_t hid, char* lds) {
     const int64_t j0 = (int64_t)tt * N;
-    if (hid != ALL) sg.load(kb + j0 * xrow, xrow, vb + j0 * yrow, yrow, hid, st);
+    if (hid == ALL) return;
+    if constexpr (P::PREF) sg.load(kb + j0 * xrow, xrow, vb + j0 * yrow, yrow, hid, st);
+    else sg.through(kb + j0 * xrow, xrow, vb + j0 * yrow, yrow, hid, lds, st);
   };
   uint64_t hid = __ballot(key_hidden(a, w.b, t * N, N, w.lane));
-  load(t, hid);
   char* const buf = smem + (SHARED ? 0 : w.wk * S::bytes(N));
-  sg.store(buf, st);
+  load(t, hid, buf);
+  if constexpr (P::PREF) sg.store(buf, st);
   tile_ready<SHARED>();
   bool nb = t + STEP < t1 && key_hidden(a, w.b, (t + STEP) * N, N, w.lane);
   int cur = 0;
@@ -282,7 +331,7 @@ __device__ __forceinline__ void key_tiles(const DiffAttnArgs& a, const RowWave& 
   for (; t < t1; t += STEP) {
     const bool more = t + STEP < t1;
     const uint64_t nhid = __ballot(nb);
-    if (more) load(t + STEP, nhid);
+    if (P::PREF && more) load(t + STEP, nhid, nullptr);
     nb = t + 2 * STEP < t1 && key_hidden(a, w.b, (t + 2 * STEP) * N, N, w.lane);
     const char* tile = SHARED ? smem + cur * S::bytes(N) : buf;
 #pragma unroll 1
@@ -293,7 +342,8 @@ __device__ __forceinline__ void key_tiles(const DiffAttnArgs& a, const RowWave& 
     if (more) {
       if constexpr (SHARED) cur ^= 1;
       else tile_ready<false>();
-      sg.store(SHARED ? smem + cur * S::bytes(N) : buf, st);
+      if constexpr (P::PREF) sg.store(SHARED ? smem + cur * S::bytes(N) : buf, st);
+      else load(t + STEP, nhid, buf);
       tile_ready<SHARED>();
     }
     hid = nhid;
@@ -411,10 +461,10 @@ __global__ __launch_bounds__((AttnPlan<T, DH, DV, SHARED>::NT), (AttnPlan<T, DH,
   const int part = id / a.splits, split = id - part * a.splits, tile = part / a.halves, col = (part - tile * a.halves) * DV;
   RowWave w;
   w.init<P::WQ, P::WK, MODE == kAttnAny>(a, tile);
-  typename M::frag qf[2][S::KB];
+  OwnRow<T, S::KB, S::KEEP> qf[2];
 #pragma unroll
   for (int m = 0; m < 2; ++m)
-    own_frags<T, S::KB>(qf[m], (const T*)a.q + w.b * a.qs[0] + w.i * a.qs[1] + w.h * a.qs[2] + m * a.qs[3], w.ok, a.Dh, w.lane);
+    qf[m].init((const T*)a.q + w.b * a.qs[0] + w.i * a.qs[1] + w.h * a.qs[2] + m * a.qs[3], w.ok, a.Dh, w.lane);
   const float c = a.scale * kLog2e, rscale = 1.0f / a.scale, grow = 6.0f / c;
   constexpr bool MASK = MODE == kAttnAny;
   const bool fm = MASK && a.mask_kind == 2, drop = MODE != kAttnPlain && a.t16 != 0;
@@ -428,7 +478,7 @@ __global__ __launch_bounds__((AttnPlan<T, DH, DV, SHARED>::NT), (AttnPlan<T, DH,
                                [&](const char* kt, int it0, uint32_t hid, int j0) {
     af32x16_t x[2];
 #pragma unroll
-    for (int m = 0; m < 2; ++m) x[m] = tile_dot<T, S::KB, S::LX>(kt, it0, m * S::LX / 2, qf[m], w.lane);
+    for (int m = 0; m < 2; ++m) x[m] = tile_dot<T, S::KB, S::LX, S::KEEP>(kt, it0, m * S::LX / 2, qf[m], w.lane);
     if (hid != 0 || (MASK && (a.causal || a.mask_kind != 0))) mask_tile<MASK>(a, x, hid, w.b, w.h, w.i, j0, rscale, w.lane);
     float p[2][16];
 #pragma unroll
@@ -675,11 +725,12 @@ __global__ __launch_bounds__((AttnPlan<T, DH, DV, SHARED>::NT), (AttnPlan<T, DH,
   w.init<P::WQ, P::WK, MODE == kAttnAny>(a, tile);
   constexpr bool MASK = MODE == kAttnAny;
   const bool fm = MASK && a.mask_kind == 2, drop = MODE != kAttnPlain && a.t16 != 0;
-  typename M::frag qf[2][S::KB], gf[S::VB];
+  OwnRow<T, S::KB, S::KEEP> qf[2];
+  OwnRow<T, S::VB, S::KEEP> gf;
 #pragma unroll
   for (int m = 0; m < 2; ++m)
-    own_frags<T, S::KB>(qf[m], (const T*)a.q + w.b * a.qs[0] + w.i * a.qs[1] + w.h * a.qs[2] + m * a.qs[3], w.ok, a.Dh, w.lane);
-  own_frags<T, S::VB>(gf, (const T*)a.go + w.b * a.gs[0] + w.i * a.gs[1] + w.h * a.gs[2], w.ok, a.Dv, w.lane);
+    qf[m].init((const T*)a.q + w.b * a.qs[0] + w.i * a.qs[1] + w.h * a.qs[2] + m * a.qs[3], w.ok, a.Dh, w.lane);
+  gf.init((const T*)a.go + w.b * a.gs[0] + w.i * a.gs[1] + w.h * a.gs[2], w.ok, a.Dv, w.lane);
   const float4 rw = a.row[w.rowid];
   const float2 rl = fm ? a.rowl[w.rowid] : make_float2(0.0f, 0.0f);
   const float c = a.scale * kLog2e, rscale = 1.0f / a.scale;
@@ -695,8 +746,8 @@ __global__ __launch_bounds__((AttnPlan<T, DH, DV, SHARED>::NT), (AttnPlan<T, DH,
   key_tiles<T, DH, DV, SHARED>(a, w, 0, split * per, min(tn, (split + 1) * per), smem, [&](const char* kt, int it0, uint32_t hid, int j0) {
     af32x16_t x[2];
 #pragma unroll
-    for (int m = 0; m < 2; ++m) x[m] = tile_dot<T, S::KB, S::LX>(kt, it0, m * S::LX / 2, qf[m], w.lane);
-    af32x16_t g = tile_dot<T, S::VB, S::LY>(kt + S::xbytes(P::N), it0, 0, gf, w.lane);
+    for (int m = 0; m < 2; ++m) x[m] = tile_dot<T, S::KB, S::LX, S::KEEP>(kt, it0, m * S::LX / 2, qf[m], w.lane);
+    af32x16_t g = tile_dot<T, S::VB, S::LY, S::KEEP>(kt + S::xbytes(P::N), it0, 0, gf, w.lane);
     if (hid != 0 || (MASK && (a.causal || a.mask_kind != 0))) mask_tile<MASK>(a, x, hid, w.b, w.h, w.i, j0, rscale, w.lane);
     if (drop) {
 #pragma unroll
@@ -794,11 +845,12 @@ __global__ __launch_bounds__((AttnPlan<T, DH, DV, SHARED>::NT), (AttnPlan<T, DH,
   constexpr bool MASK = MODE == kAttnAny;
   const bool fm = MASK && a.mask_kind == 2, drop = MODE != kAttnPlain && a.t16 != 0;
 
-  typename M::frag kf[2][S::KB], vf[S::VB];
+  OwnRow<T, S::KB, S::KEEP> kf[2];
+  OwnRow<T, S::VB, S::KEEP> vf;
 #pragma unroll
   for (int m = 0; m < 2; ++m)
-    own_frags<T, S::KB>(kf[m], (const T*)a.k + b * a.ks[0] + jc * a.ks[1] + hk * a.ks[2] + m * a.ks[3], ok, a.Dh, lane);
-  if constexpr (PART != 2) own_frags<T, S::VB>(vf, (const T*)a.v + b * a.vs[0] + jc * a.vs[1] + hk * a.vs[2], ok, a.Dv, lane);
+    kf[m].init((const T*)a.k + b * a.ks[0] + jc * a.ks[1] + hk * a.ks[2] + m * a.ks[3], ok, a.Dh, lane);
+  if constexpr (PART != 2) vf.init((const T*)a.v + b * a.vs[0] + jc * a.vs[1] + hk * a.vs[2], ok, a.Dv, lane);
   af32x16_t ak[2][S::KO], av[S::VO];
 #pragma unroll
   for (int d = 0; d < S::KO; ++d) { ak[0][d] = af32x16_t{0.0f}; ak[1][d] = af32x16_t{0.0f}; }
@@ -812,17 +864,19 @@ __global__ __launch_bounds__((AttnPlan<T, DH, DV, SHARED>::NT), (AttnPlan<T, DH,
   const int first = MASK && a.causal ? max(0, jb - off) / N : 0, per = max(0, (a.Nq + N - 1) / N - first);
   const int all = per * a.G, share = (all + a.splits - 1) / a.splits, begin = split * share, total = min(all, begin + share);
   const int st = SHARED ? threadIdx.x : lane;
-  AttnStage<T, DH, DV, N, P::LT> sg;
+  AttnStage<T, DH, DV, N, P::LT, P::PREF> sg;
   const uint32_t xrow = (uint32_t)(a.qs[1] * elem<T>::kBytes), yrow = (uint32_t)(a.gs[1] * elem<T>::kBytes);
   sg.init(st, xrow, (uint32_t)(a.qs[3] * elem<T>::kBytes), yrow, a.Dh, a.Dv);
   const int sr = st % N;
   float4 srow;
   float2 srowl = make_float2(0.0f, 0.0f);
-  auto load = [&](int t) {
+  auto load = [&](int t, char* lds) {
     const int g = t / per, i0 = (first + t - g * per) * N, h = hk * a.G + g, left = a.Nq - i0;
     const char* xb = (const char*)a.q + (b * a.qs[0] + (int64_t)i0 * a.qs[1] + h * a.qs[2]) * elem<T>::kBytes;
     const char* yb = (const char*)a.go + (b * a.gs[0] + (int64_t)i0 * a.gs[1] + h * a.gs[2]) * elem<T>::kBytes;
-    sg.load(xb, xrow, yb, yrow, left >= N ? 0ull : ~0ull << left, st);
+    const uint64_t hid = left >= N ? 0ull : ~0ull << left;
+    if constexpr (P::PREF) sg.load(xb, xrow, yb, yrow, hid, st);
+    else sg.through(xb, xrow, yb, yrow, hid, lds, st);
     // (threads past the tile's rows repeat a row's: no divergent branch in the loop)
     const int64_t rid = ((int64_t)b * a.H + h) * a.Nq + i0 + min(sr, left - 1);
     srow = a.row[rid];
@@ -833,21 +887,21 @@ __global__ __launch_bounds__((AttnPlan<T, DH, DV, SHARED>::NT), (AttnPlan<T, DH,
     srowl.x = gone ? -kNegInf : srowl.x; srowl.y = gone ? -kNegInf : srowl.y;
   };
   auto store = [&](char* at) {
-    sg.store(at, st);
+    if constexpr (P::PREF) sg.store(at, st);
     reinterpret_cast<float4*>(at + S::xybytes(N))[sr] = srow;
     if (fm) reinterpret_cast<float2*>(at + S::xybytes(N) + 16 * N)[sr] = srowl;
   };
   char* const own = smem + (SHARED ? 0 : wk * S::bytes(N));
   int cur = 0;
   if (begin + wk < total) {
-    load(begin + wk);
+    load(begin + wk, own);
     store(own);
     tile_ready<SHARED>();
   }
 #pragma unroll 1
   for (int t = begin + wk; t < total; t += P::WK) {
     const bool more = t + P::WK < total;
-    if (more) load(t + P::WK);
+    if (P::PREF && more) load(t + P::WK, nullptr);
     const char* qt = SHARED ? smem + cur * S::bytes(N) : own;
     const char* gt = qt + S::xbytes(N);
     const float4* rows = reinterpret_cast<const float4*>(qt + S::xybytes(N));
@@ -860,9 +914,9 @@ __global__ __launch_bounds__((AttnPlan<T, DH, DV, SHARED>::NT), (AttnPlan<T, DH,
       if (i0 >= a.Nq) break;
       af32x16_t x[2];
 #pragma unroll
-      for (int m = 0; m < 2; ++m) x[m] = tile_dot<T, S::KB, S::LX>(qt, it0, m * S::LX / 2, kf[m], lane);
+      for (int m = 0; m < 2; ++m) x[m] = tile_dot<T, S::KB, S::LX, S::KEEP>(qt, it0, m * S::LX / 2, kf[m], lane);
       af32x16_t gm = {0.0f};
-      if constexpr (PART != 2) gm = tile_dot<T, S::VB, S::LY>(gt, it0, 0, vf, lane);
+      if constexpr (PART != 2) gm = tile_dot<T, S::VB, S::LY, S::KEEP>(gt, it0, 0, vf, lane);
       if (MASK && a.causal) {
         const int lim = jc - off - i0 - 4 * (lane >> 5);                // rows before it do not see the key
         if (__any(lim > -4 * (lane >> 5))) {
@@ -929,6 +983,7 @@ __global__ __launch_bounds__((AttnPlan<T, DH, DV, SHARED>::NT), (AttnPlan<T, DH,
     if (more) {
       if constexpr (SHARED) cur ^= 1;
       else tile_ready<false>();
+      if constexpr (!P::PREF) load(t + P::WK, own);
       store(SHARED ? smem + cur * S::bytes(N) : own);
       tile_ready<SHARED>();
     }
@@ -1027,7 +1082,7 @@ template <typename T, int DH, int DV> static AttnCut attn_cut(const DiffAttnArgs
   if (may_share && ts < tp) return {true, 1};
   const int64_t waves = narrow * S::WK, fill = 1024 * S::MINW * 2;
   const int64_t each = (staged + 31) / 32 / S::WK / 4;
-  int64_t splits = waves * 2 > fill && uneven == 1.0 ? 1 : (fill + waves - 1) / waves;
+  int64_t splits = waves * 2 >= fill && uneven == 1.0 ? 1 : (fill + waves - 1) / waves;
   splits = splits < each ? splits : each;
   splits = splits < kAttnSplits ? splits : kAttnSplits;
   return {false, (int)(splits > 1 ? splits : 1)};
@@ -1038,9 +1093,10 @@ template <typename T, int DH, int DV> static AttnCut attn_cut_fwd(const DiffAttn
 template <typename T, int DH, int DV> static AttnCut attn_cut_q(const DiffAttnArgs& a) {
   return attn_cut<T, DH, DV>(a, (int64_t)a.B * a.Hk, a.R, a.Nk, true);
 }
+// (128 / 128 in one pass spills as a shared block: 357 us, private 277)
+template <int DH, int DV> constexpr bool kAttnKvPrivate = DH == 128 && DV == 128;
 template <typename T, int DH, int DV> static AttnCut attn_cut_kv(const DiffAttnArgs& a) {
-  // (128 / 128 in one pass spills as a shared block: 357 us, private 277)
-  return attn_cut<T, DH, DV>(a, (int64_t)a.B * a.Hk, a.Nk, (int64_t)a.G * ((a.Nq + 31) / 32) * 32, !(DH == 128 && DV == 128));
+  return attn_cut<T, DH, DV>(a, (int64_t)a.B * a.Hk, a.Nk, (int64_t)a.G * ((a.Nq + 31) / 32) * 32, !kAttnKvPrivate<DH, DV>);
 }
 
 // bytes of the splits' sums
@@ -1108,7 +1164,9 @@ static int attn_backward(DiffAttnArgs a, float* glam, int64_t part_bytes, hipStr
   };
   auto pass = [&](const AttnCut& cut, auto which) {
     a.splits = room ? cut.splits : 1;
-    return cut.shared ? run(std::true_type{}, which) : run(std::false_type{}, which);
+    if constexpr (decltype(which)::value == 3 || !kAttnKvPrivate<DH, DV>)
+      if (cut.shared) return run(std::true_type{}, which);
+    return run(std::false_type{}, which);
   };
   int rc = UBV_OK;
   if (a.gq != nullptr || glam != nullptr) {
