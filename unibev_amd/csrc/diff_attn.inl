@@ -615,16 +615,12 @@ __global__ __launch_bounds__(256) void diff_attn_join_kernel(const DiffAttnArgs 
         make_float2(dead ? 0.0f : fm ? top[m] : top[m] * c - kProbShift<T>, dead ? -kNegInf : fm ? log2f(l[m]) - kProbShift<T> : log2f(l[m]));
 }
 
-// ---- backward: del_m = grad_out . o_m per row, 16 lanes a row; the statistics as row_probability takes them -------------------
+// ---- backward: del_m = grad_out . o_m of a row by 16 lanes (t: this lane's number); all of them get the sums --------------------
 template <typename T>
-__global__ __launch_bounds__(256) void diff_attn_del_kernel(const DiffAttnArgs a) {
-  const int64_t rows = (int64_t)a.B * a.H * a.Nq, rowid = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
-  const int t = threadIdx.x & 15;
-  const int64_t rr = rowid < rows ? rowid : rows - 1;
-  const int i = (int)(rr % a.Nq), h = (int)(rr / a.Nq % a.H);
-  const int64_t b = rr / a.Nq / a.H;
+__device__ __forceinline__ float2 row_del(const DiffAttnArgs& a, int64_t rowid, int64_t b, int h, int i, int t) {
+  const int64_t rows = (int64_t)a.B * a.H * a.Nq;
   const T* g = (const T*)a.go + b * a.gs[0] + i * a.gs[1] + h * a.gs[2];
-  const float *o1 = a.o + rr * a.Dv, *o2 = a.o + (rows + rr) * a.Dv;
+  const float *o1 = a.o + rowid * a.Dv, *o2 = a.o + (rows + rowid) * a.Dv;
   float s1 = 0.0f, s2 = 0.0f;
   for (int d = t; d < a.Dv; d += 16) {
     const float gv = elem<T>::to_float(g[d]);
@@ -633,14 +629,26 @@ __global__ __launch_bounds__(256) void diff_attn_del_kernel(const DiffAttnArgs a
   }
 #pragma unroll
   for (int m = 8; m >= 1; m >>= 1) { s1 += __shfl_xor(s1, m, 64); s2 += __shfl_xor(s2, m, 64); }
-  if (t == 0 && rowid < rows) {
-    const float4 st = a.stat[rr];
-    if (a.mask_kind == 2) {
-      a.row[rr] = make_float4(st.x, st.z, s1, s2);
-      a.rowl[rr] = make_float2(st.y, st.w);
-    } else {
-      a.row[rr] = make_float4(st.x + st.y, st.z + st.w, s1, s2);
-    }
+  return make_float2(s1, s2);
+}
+// the row's numbers as row_probability takes them
+__device__ __forceinline__ void row_stats(const DiffAttnArgs& a, bool fm, int64_t rowid, float2 del, float4& rw, float2& rl) {
+  const float4 st = a.stat[rowid];
+  rw = fm ? make_float4(st.x, st.z, del.x, del.y) : make_float4(st.x + st.y, st.z + st.w, del.x, del.y);
+  rl = fm ? make_float2(st.y, st.w) : make_float2(0.0f, 0.0f);
+}
+// what grad_q's pass leaves for grad_k's, by itself where that pass does not run
+template <typename T>
+__global__ __launch_bounds__(256) void diff_attn_del_kernel(const DiffAttnArgs a) {
+  const int64_t rows = (int64_t)a.B * a.H * a.Nq, rowid = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
+  const int64_t rr = rowid < rows ? rowid : rows - 1;
+  const float2 del = row_del<T>(a, rr, rr / a.Nq / a.H, (int)(rr / a.Nq % a.H), (int)(rr % a.Nq), threadIdx.x & 15);
+  if ((threadIdx.x & 15) == 0 && rowid < rows) {
+    float4 rw;
+    float2 rl;
+    row_stats(a, a.mask_kind == 2, rr, del, rw, rl);
+    a.row[rr] = rw;
+    if (a.mask_kind == 2) a.rowl[rr] = rl;
   }
 }
 
@@ -731,8 +739,21 @@ __global__ __launch_bounds__((AttnPlan<T, DH, DV, SHARED>::NT), (AttnPlan<T, DH,
   for (int m = 0; m < 2; ++m)
     qf[m].init((const T*)a.q + w.b * a.qs[0] + w.i * a.qs[1] + w.h * a.qs[2] + m * a.qs[3], w.ok, a.Dh, w.lane);
   gf.init((const T*)a.go + w.b * a.gs[0] + w.i * a.gs[1] + w.h * a.gs[2], w.ok, a.Dv, w.lane);
-  const float4 rw = a.row[w.rowid];
-  const float2 rl = fm ? a.rowl[w.rowid] : make_float2(0.0f, 0.0f);
+  // del of the own rows, 16 lanes a row, the waves of the same rows taking turns; kept for the pass of grad_k
+  __shared__ float2 dels[P::WQ][32];
+  for (int n = 4 * w.wk + (w.lane >> 4); n < 32; n += 4 * P::WK) {
+    const int r = min(w.rb + 32 * w.wq + n, a.R - 1), g = r / a.Nq;
+    const float2 del = row_del<T>(a, ((int64_t)w.b * a.H + w.hk * a.G) * a.Nq + r, w.b, w.hk * a.G + g, r - g * a.Nq, w.lane & 15);
+    if ((w.lane & 15) == 0) dels[w.wq][n] = del;
+  }
+  __syncthreads();
+  float4 rw;
+  float2 rl;
+  row_stats(a, fm, w.rowid, dels[w.wq][w.lane & 31], rw, rl);
+  if (w.ok && w.wk == 0 && split == 0 && w.lane < 32) {
+    a.row[w.rowid] = rw;
+    if (fm) a.rowl[w.rowid] = rl;
+  }
   const float c = a.scale * kLog2e, rscale = 1.0f / a.scale;
   const uint32_t t32 = a.t16 << 16;
   const uint64_t zrow = attn_seed(a.seed, a.seed_dev) + (uint64_t)(w.rowid * a.n4) + (w.lane >> 5);
@@ -1147,8 +1168,6 @@ static int attn_backward(DiffAttnArgs a, float* glam, int64_t part_bytes, hipStr
   const int64_t heads = (int64_t)a.B * a.Hk, rows = (int64_t)a.B * a.H * a.Nq;
   const char* who = "diff_attention_backward";
   const bool room = part_bytes >= attn_bytes_bwd<T, DH, DV>(a);
-  hipLaunchKernelGGL(diff_attn_del_kernel<T>, dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, st, a);
-  UBV_CHECK_LAUNCH(who);
   auto run = [&](auto shared, auto pass) {
     constexpr bool SH = decltype(shared)::value;
     constexpr int PASS = decltype(pass)::value;                 // 0 .. 2: grad_k / grad_v of that part, 3: grad_q
@@ -1180,6 +1199,9 @@ static int attn_backward(DiffAttnArgs a, float* glam, int64_t part_bytes, hipStr
       hipLaunchKernelGGL(diff_attn_lam_kernel, dim3((unsigned)a.H), dim3(256), 0, st, a.dlrow, glam, a.B, a.H, a.Nq);
       UBV_CHECK_LAUNCH(who);
     }
+  } else {
+    hipLaunchKernelGGL(diff_attn_del_kernel<T>, dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, st, a);
+    UBV_CHECK_LAUNCH(who);
   }
   if (a.gk == nullptr) return rc;
   const AttnCut cut = attn_cut_kv<T, DH, DV>(a);
