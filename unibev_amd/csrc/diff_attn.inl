@@ -959,42 +959,40 @@ __global__ __launch_bounds__((AttnPlan<T, DH, DV, SHARED>::NT), (AttnPlan<T, DH,
         }
       }
       const uint64_t zt = zseed + (uint64_t)((((int64_t)b * a.H + h) * a.Nq + i0 + 4 * (lane >> 5) + (lane & 3)) * a.n4);
-      float pc[16];
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int r0 = it0 + tile_item(4 * q, lane);
-        uint32_t word[4];
-        if (drop) quad_words(attn_mix(zt + (uint64_t)(8 * q * (int64_t)a.n4)), lane, word);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int n = 4 * q + e;
-          const float4 rw = rows[r0 + e];
-          const float2 rl = fm ? rowl[r0 + e] : make_float2(0.0f, 0.0f);
-          const float p1 = row_probability(fm, x[0][n], c, rw.x, rl.x), p2 = lam * row_probability(fm, x[1][n], c, rw.y, rl.y);
-          float gn = gm[n], pn = p1 - p2;
-          if (drop) {
-            const bool keep = attn_keep(word[e], lane & 1, t32);
-            gn = keep ? gn * a.up : 0.0f;
-            pn = keep ? pn : 0.0f;
-          }
-          pc[n] = kProbScale<T> == 1.0f ? pn : pn * kProbScale<T>;
-          x[0][n] = p1 * (gn - rw.z);
-          x[1][n] = p2 * (rw.w - gn);
-        }
-      }
+      // 16 rows at a time: the matrix instructions of one half run beside the arithmetic of the other
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
+        float pc[8], ds[2][8];
+#pragma unroll
+        for (int q = 2 * s; q < 2 * s + 2; ++q) {
+          const int r0 = it0 + tile_item(4 * q, lane);
+          uint32_t word[4];
+          if (drop) quad_words(attn_mix(zt + (uint64_t)(8 * q * (int64_t)a.n4)), lane, word);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int n = 4 * q + e, k = n - 8 * s;
+            const float4 rw = rows[r0 + e];
+            const float2 rl = fm ? rowl[r0 + e] : make_float2(0.0f, 0.0f);
+            const float p1 = row_probability(fm, x[0][n], c, rw.x, rl.x), p2 = lam * row_probability(fm, x[1][n], c, rw.y, rl.y);
+            float gn = gm[n], pn = p1 - p2;
+            if (drop) {
+              const bool keep = attn_keep(word[e], lane & 1, t32);
+              gn = keep ? gn * a.up : 0.0f;
+              pn = keep ? pn : 0.0f;
+            }
+            pc[k] = kProbScale<T> == 1.0f ? pn : pn * kProbScale<T>;
+            ds[0][k] = p1 * (gn - rw.z);
+            ds[1][k] = p2 * (rw.w - gn);
+          }
+        }
         if constexpr (PART != 1) {
-          const typename M::frag fp = M::pack(pc + 8 * s);
+          const typename M::frag fp = M::pack(pc);
 #pragma unroll
           for (int d = 0; d < S::VO; ++d) av[d] = M::mul(M::template load_tr<S::LY>(gt, it0 + 16 * s, 0, d, lane), fp, av[d]);
         }
 #pragma unroll
         for (int m = 0; m < (PART != 2 ? 2 : 0); ++m) {
-          float ds[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) ds[e] = x[m][8 * s + e];
-          const typename M::frag f = M::pack(ds);
+          const typename M::frag f = M::pack(ds[m]);
 #pragma unroll
           for (int d = 0; d < S::KO; ++d)
             ak[m][d] = M::mul(M::template load_tr<S::LX>(qt, it0 + 16 * s, m * S::LX / 2, d, lane), f, ak[m][d]);
