@@ -630,9 +630,9 @@ def test_attention_refusals():
     for err, kw in ((ValueError, dict(q=q[0])), (ValueError, dict(k=k[:1])), (ValueError, dict(v=v[:, :5])), (ValueError, dict(q=q[:, :, :3])),
                     (TypeError, dict(q=q.half())), (TypeError, dict(q=q.double(), k=k.double(), v=v.double())),
                     (ValueError, dict(lam=lam[:3])), (ValueError, dict(lam=lam.long())), (ValueError, dict(attn_mask=ok[:5])),
-                    (ValueError, dict(attn_mask=ok[0])), (TypeError, dict(attn_mask=ok.long())),
+                    (ValueError, dict(attn_mask=ok[0])), (TypeError, dict(attn_mask=ok.long())), (TypeError, dict(attn_mask=ok.double())),
                     (ValueError, dict(attn_mask=ok.float().requires_grad_())), (ValueError, dict(key_padding_mask=ok[:3])),
-                    (ValueError, dict(key_padding_mask=torch.zeros(2, 11, device=DEV))), (ValueError, dict(p=2.0)),
+                    (ValueError, dict(key_padding_mask=torch.zeros(2, 11, device=DEV))), (ValueError, dict(p=2.0)), (ValueError, dict(scale=0.0)), (ValueError, dict(scale=-1.0)), (ValueError, dict(scale=math.nan)),
                     (ValueError, dict(p=0.1, training=True, seed=1 << 63)), (RuntimeError, dict(q=q.cpu())),
                     (RuntimeError, dict(key_padding_mask=torch.zeros(2, 11, dtype=torch.bool)))):
         args = dict(dict(q=q, k=k, v=v, lam=lam), **kw)
@@ -668,6 +668,48 @@ def test_operators_on_another_stream():
         gn = F.dropout(F.layer_norm(got), 0.3, True, identity=got, seed=4)
     side.synchronize()
     assert torch.equal(got, want) and torch.equal(gn, wn)
+
+
+def test_second_derivatives_are_refused_and_first_ones_are_not():
+    F = UF()
+    x = torch.randn(2, 5, 2, 2, 16, device=DEV, requires_grad=True)
+    lam = torch.ones(2, device=DEV, requires_grad=True)
+    for f in (lambda: F.dropout(x, 0.3, True, seed=1), lambda: F.layer_norm(x), lambda: F.diff_attention(x, x, x.detach().flatten(3), lam)):
+        want, = torch.autograd.grad(f().sum(), x)
+        got, = torch.autograd.grad(f().sum(), x, create_graph=True)
+        assert torch.equal(got, want)
+        with pytest.raises(RuntimeError, match='once_differentiable'):
+            got.sum().backward()
+
+
+def test_a_graph_is_walked_once_and_a_changed_operand_is_noticed():
+    F = UF()
+    x = torch.randn(6, 32, device=DEV, requires_grad=True)
+    y = F.layer_norm(x)
+    y.sum().backward()
+    with pytest.raises(RuntimeError, match='second time'):
+        y.sum().backward()
+    w = torch.ones(32, device=DEV, requires_grad=True)
+    y = F.layer_norm(x, w)
+    with torch.no_grad():
+        w.mul_(2)
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        y.sum().backward()
+
+
+def test_the_call_hook_sees_every_launch():
+    from unibev_amd import _lib
+    F, seen = UF(), []
+    x = torch.randn(2, 9, 2, 2, 16, device=DEV, requires_grad=True)
+    w = torch.ones(16, device=DEV, requires_grad=True)
+    prev = _lib.set_call_hook(seen.append)
+    try:
+        o = F.diff_attention(x, x, x.detach().flatten(3), torch.ones(2, device=DEV))
+        F.dropout(F.layer_norm(o[..., :16], w), 0.5, True).sum().backward()
+    finally:
+        _lib.set_call_hook(prev)
+    assert seen == ['ubv_diff_attention_forward', 'ubv_layer_norm_forward', 'ubv_dropout', 'ubv_dropout', 'ubv_layer_norm_backward',
+                    'ubv_diff_attention_backward']
 
 
 def block(x, w, lam, seed=None):

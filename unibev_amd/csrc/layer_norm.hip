@@ -83,6 +83,20 @@ __device__ __forceinline__ void ln_sum2(float& a, float& b, float (*red)[2]) {
   }
 }
 
+// the same for one sum
+template <int TPR> __device__ __forceinline__ void ln_sum(float& a, float (*red)[2]) {
+#pragma unroll
+  for (int m = (TPR < 64 ? TPR : 64) >> 1; m >= 1; m >>= 1) a += __shfl_xor(a, m, 64);
+  if constexpr (TPR > 64) {
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6][0] = a;
+    __syncthreads();
+    a = 0.0f;
+#pragma unroll
+    for (int w = 0; w < TPR / 64; ++w) a += red[w][0];
+  }
+}
+
 constexpr int ln_block(int tpr) { return tpr < 256 ? 256 : tpr; }
 
 template <typename T, bool ALN, int TPR, int K>
@@ -98,14 +112,14 @@ __global__ __launch_bounds__(ln_block(TPR)) void layer_norm_fwd_kernel(const T* 
     const long r = r0 + sub;
     const bool ok = r < R;
     const T* xr = x + (ok ? r : R - 1) * C;
-    float v[K][VEC], sum = 0.0f, dummy = 0.0f;
+    float v[K][VEC], sum = 0.0f;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       ln_load<T, ALN>(xr, tc + k * TPR * VEC, C, v[k]);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) sum += v[k][i];
     }
-    ln_sum2<TPR>(sum, dummy, red);
+    ln_sum<TPR>(sum, red);
     const float mu = sum * inv;
     float var = 0.0f;
 #pragma unroll
@@ -117,7 +131,7 @@ __global__ __launch_bounds__(ln_block(TPR)) void layer_norm_fwd_kernel(const T* 
         v[k][i] = d;
         var = fmaf(d, d, var);
       }
-    ln_sum2<TPR>(var, dummy, red);
+    ln_sum<TPR>(var, red);
     const float rs = 1.0f / sqrtf(var * inv + eps);
     if (ok) {
 #pragma unroll
@@ -240,20 +254,20 @@ __global__ __launch_bounds__(1024) void layer_norm_wide_fwd_kernel(const T* __re
   __shared__ float red[16][2];
   const T* xr = x + (long)blockIdx.x * C;
   T* yr = y + (long)blockIdx.x * C;
-  float sum = 0.0f, var = 0.0f, dummy = 0.0f, v[VEC];
+  float sum = 0.0f, var = 0.0f, v[VEC];
   for (int c = threadIdx.x * VEC; c < C; c += 1024 * VEC) {
     ln_load<T, false>(xr, c, C, v);
 #pragma unroll
     for (int i = 0; i < VEC; ++i) sum += v[i];
   }
-  ln_sum2<1024>(sum, dummy, red);
+  ln_sum<1024>(sum, red);
   const float mu = sum / (float)C;
   for (int c = threadIdx.x * VEC; c < C; c += 1024 * VEC) {
     ln_load<T, false>(xr, c, C, v);
 #pragma unroll
     for (int i = 0; i < VEC; ++i) { const float d = c + i < C ? v[i] - mu : 0.0f; var = fmaf(d, d, var); }
   }
-  ln_sum2<1024>(var, dummy, red);
+  ln_sum<1024>(var, red);
   const float rs = 1.0f / sqrtf(var / (float)C + eps);
   for (int c = threadIdx.x * VEC; c < C; c += 1024 * VEC) {
     float g[VEC], b[VEC];

@@ -377,8 +377,7 @@ Tensor diff_attention(const Tensor& q, const Tensor& k, const Tensor& v, const T
     at::AutoDispatchBelowADInplaceOrView below;
     if (mask_in.defined()) {
       if (mask_in.requires_grad()) throw py::value_error(who + "attn_mask gets no gradient; detach it");
-      if (mask_in.scalar_type() != at::kBool && !mask_in.is_floating_point())
-        throw py::type_error(who + "attn_mask of " + c10::toString(mask_in.scalar_type()) + " (bool or float)");
+      if (mask_in.scalar_type() != at::kBool) type_code(mask_in);      // (f64's lowest value would become f32's -inf)
       Tensor m = mask_in.scalar_type() == at::kBool ? mask_in : mask_in.to(at::kFloat);
       if (m.dim() == 3 && m.size(0) == B * H && m.size(1) == Nq && m.size(2) == Nk) m = m.reshape({B, H, Nq, Nk});
       const int64_t full[4] = {B, H, Nq, Nk};

@@ -763,7 +763,8 @@ def dropout(x, p=0.0, training=False, identity=None, seed=None):
     """``identity + dropout(x, p)`` (without ``identity``: ``dropout(x, p)``) in one pass each way (``ubv_dropout``).  The mask is a
     function of the seed and the element's index and is never stored; ``p`` counts in steps of 2^-16.  Any shape; ``identity``
     has x's shape and its type, or is f32 beside a 16-bit x (the result is of identity's type).  ``seed`` fixes the mask (the same
-    on every replay of a captured graph); without it each call draws its own."""
+    on every replay of a captured graph); without it each call draws its own.  Nothing to do (p = 0 or not training, no identity)
+    returns x itself.  Differentiable once."""
     p, seed, base = _drop_args(p, training, seed, 'dropout')
     if identity is None and p == 0.0:
         _need_cuda(x)
@@ -775,7 +776,7 @@ def dropout(x, p=0.0, training=False, identity=None, seed=None):
 # ----------------------------------------------------------------------------------------------- layer norm
 def layer_norm(x, gamma=None, beta=None, eps=1e-5):
     """Layer norm over the last axis of any width (``ubv_layer_norm_*``): x (..., C) of f32 / f16 / bf16, ``gamma`` and ``beta``
-    (C,) or None (taken in f32).  Statistics in f32; the weights' gradients are summed in fixed order."""
+    (C,) or None (taken in f32).  Statistics in f32; the weights' gradients are summed in fixed order.  Differentiable once."""
     return native().layer_norm(x, gamma, beta, eps)
 
 
@@ -788,12 +789,15 @@ def diff_attention(q, k, v, lam, attn_mask=None, key_padding_mask=None, causal=F
     query head h reads key / value head h // (H // Hk).  lam (H,), or one value for all heads.  Dh <= 128, Dv <= 256.  Returns
     (B, Nq, H, Dv); a query that sees no key gets zeros (and zero gradients).
 
-    attn_mask: bool (True hides, as in ``torch.nn.MultiheadAttention``) or float (added; -inf hides), (Nq, Nk), (B H, Nq, Nk) or
-    broadcastable to (B, H, Nq, Nk); it gets no gradient.  key_padding_mask: bool (B, Nk), True hides the key from every query;
-    what k and v hold there is never used.  A key that only attn_mask or causal hides must be finite.  causal: query i sees keys
+    attn_mask: bool (True hides, as in ``torch.nn.MultiheadAttention``) or f32 / f16 / bf16 (added; -inf hides, +inf counts as the
+    largest value), (Nq, Nk), (B H, Nq, Nk) or broadcastable to (B, H, Nq, Nk); it gets no gradient.  key_padding_mask: bool
+    (B, Nk), True hides the key from every query; what k and v hold there is never used.  A key that only attn_mask or causal hides must be finite.  causal: query i sees keys
     j <= i + Nk - Nq.  scale: positive, default Dh ** -0.5.
 
-    ``p``, ``training``, ``seed``: dropout D on the map, as in ``dropout`` (never stored)."""
+    ``p``, ``training``, ``seed``: dropout D on the map, as in ``dropout`` (never stored).
+
+    Sums are f32; probabilities and their gradients enter the matrix instructions in q's type.  f16: |lam| below 255, and
+    gradients scaled into f16's range, as in any f16 backward pass.  Differentiable once."""
     p, seed, base = _drop_args(p, training, seed, 'diff_attention')
     return native().diff_attention(q, k, v, lam, attn_mask, key_padding_mask, causal, scale, p, seed, base)
 
