@@ -702,7 +702,7 @@ int ubv_layer_norm_backward(const void* grad_y, const void* x, const float* gamm
  * key gives a zero row (and zero gradients).
  *   q [B, Nq, H, 2, Dh], k [B, Nk, Hk, 2, Dh], v [B, Nk, Hk, Dv] of dtype, lam [H] f32.  Query head h reads key / value head
  *   h / (H / Hk).  Dh <= 128, Dv <= 256, the last axis contiguous and readable up to the next multiple of 16 bytes (zeros there);
- *   16-byte aligned, other strides multiples of 16 bytes, token strides below 16 MiB, map strides below 256 MiB.  scale > 0.
+ *   16-byte aligned, other strides multiples of 16 bytes, token strides below 16 MiB, map strides below 256 MiB.  scale in [1e-30, 1e30).
  *   strides (HOST, elements): q batch, token, head, map | k the same | v batch, token, head | grad_out batch, token, head
  *   (forward: 0) | mask batch, head, query, key.
  *   key_padding_mask [B, Nk] bytes or NULL: nonzero hides the key from every query; what k and v hold there is never used.

@@ -211,6 +211,21 @@ def test_layer_norm(R, C, dt):
     norm_check(x, gamma, beta, g, y, xd.grad, wd.grad, bd.grad, dt)
 
 
+def test_layer_norm_more_wide_rows_than_blocks():
+    """a block that walks several rows gives each what a call of that row alone gives"""
+    x, g = (torch.randn(4099, 8200, device=DEV, generator=torch.Generator(DEV).manual_seed(s)).half() for s in (1, 2))
+    w, b = (torch.randn(8200, device=DEV) for _ in range(2))
+
+    def run(rows):
+        xd = x[rows].clone().requires_grad_()
+        y = UF().layer_norm(xd, w, b)
+        return y, torch.autograd.grad(y, xd, g[rows])[0]
+    whole = run(slice(None))
+    for rows in (slice(0, 3), slice(4095, 4099)):
+        for got, want in zip(whole, run(rows)):
+            assert torch.equal(got[rows], want)
+
+
 def test_layer_norm_many_rows_is_deterministic():
     x, gamma, beta, g = norm_case(20011, 96, torch.bfloat16)
     outs = []
@@ -273,6 +288,11 @@ def test_layer_norm_empty_and_refusals():
         F.layer_norm(z[:, :0])
     with pytest.raises(TypeError):
         F.layer_norm(z.double())
+    with pytest.raises(ValueError, match='at most'):
+        F.layer_norm(z[0, :1].expand((1 << 32) + 4))
+    for eps in (-1e-5, math.nan):
+        with pytest.raises(ValueError, match='eps'):
+            F.layer_norm(z, eps=eps)
     with pytest.raises(RuntimeError, match='GPU only'):
         F.layer_norm(z, torch.ones(32))
 
@@ -632,7 +652,8 @@ def test_attention_refusals():
                     (ValueError, dict(lam=lam[:3])), (ValueError, dict(lam=lam.long())), (ValueError, dict(attn_mask=ok[:5])),
                     (ValueError, dict(attn_mask=ok[0])), (TypeError, dict(attn_mask=ok.long())), (TypeError, dict(attn_mask=ok.double())),
                     (ValueError, dict(attn_mask=ok.float().requires_grad_())), (ValueError, dict(key_padding_mask=ok[:3])),
-                    (ValueError, dict(key_padding_mask=torch.zeros(2, 11, device=DEV))), (ValueError, dict(p=2.0)), (ValueError, dict(scale=0.0)), (ValueError, dict(scale=-1.0)), (ValueError, dict(scale=math.nan)),
+                    (ValueError, dict(key_padding_mask=torch.zeros(2, 11, device=DEV))), (ValueError, dict(p=2.0)), (ValueError, dict(scale=0.0)),
+                    (ValueError, dict(scale=-1.0)), (ValueError, dict(scale=math.nan)), (ValueError, dict(scale=1e-38)),
                     (ValueError, dict(p=0.1, training=True, seed=1 << 63)), (RuntimeError, dict(q=q.cpu())),
                     (RuntimeError, dict(key_padding_mask=torch.zeros(2, 11, dtype=torch.bool)))):
         args = dict(dict(q=q, k=k, v=v, lam=lam), **kw)
@@ -695,6 +716,26 @@ def test_a_graph_is_walked_once_and_a_changed_operand_is_noticed():
         w.mul_(2)
     with pytest.raises(RuntimeError, match='modified by an inplace operation'):
         y.sum().backward()
+
+
+@pytest.mark.parametrize('name,shape', [('attn_mask', (9, 9)), ('key_padding_mask', (2, 9))])
+def test_a_changed_mask_is_noticed(name, shape):
+    x = torch.randn(2, 9, 2, 2, 16, device=DEV, requires_grad=True)
+    mask = torch.zeros(shape, dtype=torch.bool, device=DEV)
+    o = UF().diff_attention(x, x, x.detach().flatten(3), torch.ones(2, device=DEV), **{name: mask})
+    mask[0, 1] = True
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        o.sum().backward()
+
+
+def test_attention_at_the_smallest_scale():
+    """every seen key counts alike"""
+    q, k = (torch.randn(1, n, 1, 2, 16, device=DEV, generator=torch.Generator(DEV).manual_seed(3)).requires_grad_() for n in (5, 7))
+    v = torch.arange(7 * 32, device=DEV, dtype=torch.float32).view(1, 7, 1, 32)
+    o = UF().diff_attention(q, k, v, torch.tensor([0.5], device=DEV), scale=1e-30)
+    want = 0.5 * v[0, :, 0].mean(0).expand(5, 32)                           # seven equal weights, each product and sum rounded
+    assert torch.allclose(o[0, :, 0], want, rtol=32 * 2.0 ** -24, atol=0)
+    assert all(float(g.abs().max()) < 1e-25 for g in torch.autograd.grad(o.sum(), (q, k)))
 
 
 def test_the_call_hook_sees_every_launch():

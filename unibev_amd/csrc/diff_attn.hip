@@ -32,8 +32,9 @@ static int attn_args(DiffAttnArgs& a, const void* q, const void* k, const void* 
   UBV_CHECK_ARG(Dh > 0 && Dh <= 128 && Dv > 0 && Dv <= 256, "%s: head widths %d (at most 128) and %d (at most 256)", who, Dh, Dv);
   UBV_CHECK_ARG((int64_t)(H / Hk) * Nq < (int64_t(1) << 31) - 256 && Nk < (1 << 31) - 256 && (int64_t)B * H < (int64_t(1) << 31),
                 "%s: Nq=%d x %d heads or Nk=%d out of range", who, Nq, H / Hk, Nk);
+  UBV_CHECK_ARG(!causal || (int64_t)Nq + Nk < (int64_t(1) << 31), "%s: Nq=%d + Nk=%d out of range", who, Nq, Nk);
   UBV_CHECK_ARG(p >= 0.0f && p <= 1.0f, "%s: p = %g must be in [0, 1]", who, (double)p);
-  UBV_CHECK_ARG(scale > 0.0f && scale < 1.0e30f, "%s: scale %g must be positive and finite", who, (double)scale);
+  UBV_CHECK_ARG(scale >= 0.99e-30f && scale < 1.01e30f, "%s: scale %g must be in [1e-30, 1e30)", who, (double)scale);
   UBV_CHECK_ARG(mask_kind >= 0 && mask_kind <= 2 && (mask_kind == 0) == (mask == nullptr), "%s: mask kind %d", who, mask_kind);
   const int vec = dtype == UBV_F32 ? 4 : 8;
   for (int n = 0; n < 14; ++n)

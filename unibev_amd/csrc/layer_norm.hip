@@ -244,72 +244,76 @@ __global__ __launch_bounds__(ln_block(TPR)) void layer_norm_bwd_kernel(const T* 
   }
 }
 
-// ---- rows too wide for a block's registers: one block per row, the row read again for each pass (from L2) ----------------
+// ---- rows too wide for a block's registers: a block walks a row, which it reads again for each pass (from L2) --------------
 template <typename T>
 __global__ __launch_bounds__(1024) void layer_norm_wide_fwd_kernel(const T* __restrict__ x, const float* __restrict__ gamma,
                                                                   const float* __restrict__ beta, T* __restrict__ y,
-                                                                  float* __restrict__ mean, float* __restrict__ rstd, int C,
+                                                                  float* __restrict__ mean, float* __restrict__ rstd, long R, int C,
                                                                   float eps) {
   constexpr int VEC = 16 / elem<T>::kBytes;
   __shared__ float red[16][2];
-  const T* xr = x + (long)blockIdx.x * C;
-  T* yr = y + (long)blockIdx.x * C;
-  float sum = 0.0f, var = 0.0f, v[VEC];
-  for (int c = threadIdx.x * VEC; c < C; c += 1024 * VEC) {
-    ln_load<T, false>(xr, c, C, v);
+  for (long r = blockIdx.x; r < R; r += gridDim.x) {
+    const T* xr = x + r * C;
+    T* yr = y + r * C;
+    float sum = 0.0f, var = 0.0f, v[VEC];
+    for (int c = threadIdx.x * VEC; c < C; c += 1024 * VEC) {
+      ln_load<T, false>(xr, c, C, v);
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) sum += v[i];
-  }
-  ln_sum<1024>(sum, red);
-  const float mu = sum / (float)C;
-  for (int c = threadIdx.x * VEC; c < C; c += 1024 * VEC) {
-    ln_load<T, false>(xr, c, C, v);
+      for (int i = 0; i < VEC; ++i) sum += v[i];
+    }
+    ln_sum<1024>(sum, red);
+    const float mu = sum / (float)C;
+    for (int c = threadIdx.x * VEC; c < C; c += 1024 * VEC) {
+      ln_load<T, false>(xr, c, C, v);
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) { const float d = c + i < C ? v[i] - mu : 0.0f; var = fmaf(d, d, var); }
-  }
-  ln_sum<1024>(var, red);
-  const float rs = 1.0f / sqrtf(var / (float)C + eps);
-  for (int c = threadIdx.x * VEC; c < C; c += 1024 * VEC) {
-    float g[VEC], b[VEC];
-    ln_load<T, false>(xr, c, C, v);
-    ln_weight<VEC>(gamma, c, C, 1.0f, g);
-    ln_weight<VEC>(beta, c, C, 0.0f, b);
+      for (int i = 0; i < VEC; ++i) { const float d = c + i < C ? v[i] - mu : 0.0f; var = fmaf(d, d, var); }
+    }
+    ln_sum<1024>(var, red);
+    const float rs = 1.0f / sqrtf(var / (float)C + eps);
+    for (int c = threadIdx.x * VEC; c < C; c += 1024 * VEC) {
+      float g[VEC], b[VEC];
+      ln_load<T, false>(xr, c, C, v);
+      ln_weight<VEC>(gamma, c, C, 1.0f, g);
+      ln_weight<VEC>(beta, c, C, 0.0f, b);
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) v[i] = fmaf((v[i] - mu) * rs, g[i], b[i]);
-    ln_store<T, false>(yr, c, C, v);
+      for (int i = 0; i < VEC; ++i) v[i] = fmaf((v[i] - mu) * rs, g[i], b[i]);
+      ln_store<T, false>(yr, c, C, v);
+    }
+    if (threadIdx.x == 0 && mean != nullptr) { mean[r] = mu; rstd[r] = rs; }
   }
-  if (threadIdx.x == 0 && mean != nullptr) { mean[blockIdx.x] = mu; rstd[blockIdx.x] = rs; }
 }
 
 template <typename T>
 __global__ __launch_bounds__(1024) void layer_norm_wide_bwd_kernel(const T* __restrict__ gy, const T* __restrict__ x,
                                                                   const float* __restrict__ gamma, const float* __restrict__ mean,
-                                                                  const float* __restrict__ rstd, T* __restrict__ gx, int C) {
+                                                                  const float* __restrict__ rstd, T* __restrict__ gx, long R, int C) {
   constexpr int VEC = 16 / elem<T>::kBytes;
   __shared__ float red[16][2];
-  const long base = (long)blockIdx.x * C;
-  const float mu = mean[blockIdx.x], rs = rstd[blockIdx.x];
-  float s1 = 0.0f, s2 = 0.0f, v[VEC], go[VEC], g[VEC];
-  for (int c = threadIdx.x * VEC; c < C; c += 1024 * VEC) {
-    ln_load<T, false>(x + base, c, C, v);
-    ln_load<T, false>(gy + base, c, C, go);
-    ln_weight<VEC>(gamma, c, C, 1.0f, g);
+  for (long r = blockIdx.x; r < R; r += gridDim.x) {
+    const long base = r * C;
+    const float mu = mean[r], rs = rstd[r];
+    float s1 = 0.0f, s2 = 0.0f, v[VEC], go[VEC], g[VEC];
+    for (int c = threadIdx.x * VEC; c < C; c += 1024 * VEC) {
+      ln_load<T, false>(x + base, c, C, v);
+      ln_load<T, false>(gy + base, c, C, go);
+      ln_weight<VEC>(gamma, c, C, 1.0f, g);
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      const float u = c + i < C ? go[i] * g[i] : 0.0f;
-      s1 += u;
-      s2 = fmaf(u, (v[i] - mu) * rs, s2);
+      for (int i = 0; i < VEC; ++i) {
+        const float u = c + i < C ? go[i] * g[i] : 0.0f;
+        s1 += u;
+        s2 = fmaf(u, (v[i] - mu) * rs, s2);
+      }
     }
-  }
-  ln_sum2<1024>(s1, s2, red);
-  s1 /= (float)C; s2 /= (float)C;
-  for (int c = threadIdx.x * VEC; c < C; c += 1024 * VEC) {
-    ln_load<T, false>(x + base, c, C, v);
-    ln_load<T, false>(gy + base, c, C, go);
-    ln_weight<VEC>(gamma, c, C, 1.0f, g);
+    ln_sum2<1024>(s1, s2, red);
+    s1 /= (float)C; s2 /= (float)C;
+    for (int c = threadIdx.x * VEC; c < C; c += 1024 * VEC) {
+      ln_load<T, false>(x + base, c, C, v);
+      ln_load<T, false>(gy + base, c, C, go);
+      ln_weight<VEC>(gamma, c, C, 1.0f, g);
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) v[i] = rs * (go[i] * g[i] - s1 - (v[i] - mu) * rs * s2);
-    ln_store<T, false>(gx + base, c, C, v);
+      for (int i = 0; i < VEC; ++i) v[i] = rs * (go[i] * g[i] - s1 - (v[i] - mu) * rs * s2);
+      ln_store<T, false>(gx + base, c, C, v);
+    }
   }
 }
 
@@ -397,7 +401,7 @@ static void ln_fwd(const void* xv, const float* gamma, const float* beta, void* 
     else hipLaunchKernelGGL((layer_norm_fwd_kernel<T, false, TPR, K>), grid, blk, 0, st, x, gamma, beta, y, mean, rstd, R, C, eps);
   });
   if (!held)
-    hipLaunchKernelGGL(layer_norm_wide_fwd_kernel<T>, dim3((unsigned)R), dim3(1024), 0, st, x, gamma, beta, y, mean, rstd, C, eps);
+    hipLaunchKernelGGL(layer_norm_wide_fwd_kernel<T>, dim3((unsigned)min(R, 4096L)), dim3(1024), 0, st, x, gamma, beta, y, mean, rstd, R, C, eps);
 }
 
 template <typename T>
@@ -417,7 +421,7 @@ static void ln_bwd(const void* gyv, const void* xv, const float* gamma, const fl
   });
   if (!held) {
     if (gx != nullptr)
-      hipLaunchKernelGGL(layer_norm_wide_bwd_kernel<T>, dim3((unsigned)R), dim3(1024), 0, st, gy, x, gamma, mean, rstd, gx, C);
+      hipLaunchKernelGGL(layer_norm_wide_bwd_kernel<T>, dim3((unsigned)min(R, 4096L)), dim3(1024), 0, st, gy, x, gamma, mean, rstd, gx, R, C);
     nrows = (int)min(R, (long)kLnWideSlabs);
     if (part != nullptr)
       hipLaunchKernelGGL(layer_norm_wide_cols_kernel<T>, dim3((C + 255) / 256, nrows), dim3(256), 0, st, gy, x, mean, rstd, part, R, C);

@@ -227,6 +227,8 @@ Tensor layer_norm(const Tensor& x, const OptTensor& gamma_, const OptTensor& bet
   const int dt = type_code(x);
   if (x.dim() < 1 || x.size(-1) < 1) throw py::value_error("layer_norm: x " + shape(x) + " has no last axis to normalise");
   const int64_t C = x.size(-1), R = x.numel() / C;
+  if (C > (1 << 29)) throw py::value_error("layer_norm: rows of " + std::to_string(C) + " (at most 2^29)");
+  if (!(eps >= 0.0)) throw py::value_error("layer_norm: eps " + std::to_string(eps) + " must not be negative");
   for (const Tensor* w : {&gamma, &beta}) {
     if (!w->defined()) continue;
     if (w->dim() != 1 || w->size(0) != C)
@@ -292,19 +294,22 @@ void strides(int64_t (&s)[18], const Tensor& q, const Tensor& k, const Tensor& v
 }
 
 struct DiffAttentionBackward : Node {
-  SavedVariable q_, k_, v_, lam_;
+  SavedVariable q_, k_, v_, lam_, mask_, padding_;      // the caller's masks: to notice that one was changed
   Attn a;
   Tensor stat, maps;
   at::ScalarType lam_type = at::kFloat;
   std::string name() const override { return "UbvDiffAttentionBackward"; }
   void release_variables() override {
-    q_.reset_data(); k_.reset_data(); v_.reset_data(); lam_.reset_data();
+    for (SavedVariable* s : {&q_, &k_, &v_, &lam_, &mask_, &padding_}) s->reset_data();
     stat.reset(); maps.reset();
+    a.mask.reset(); a.padding.reset();
   }
   variable_list apply(variable_list&& g) override {
     variable_list out(4);
     if (!g[0].defined()) return out;
     const Tensor q = q_.unpack(), k = k_.unpack(), v = v_.unpack(), lam = lam_.unpack();
+    if (a.mask.defined()) mask_.unpack();
+    if (a.padding.defined()) padding_.unpack();
     const bool nq = task_should_compute_output(0), nk = task_should_compute_output(1), nv = task_should_compute_output(2),
                nl = task_should_compute_output(3);
     const c10::Device dev = q.device();
@@ -367,7 +372,8 @@ Tensor diff_attention(const Tensor& q, const Tensor& k, const Tensor& v, const T
                           ",) or one value");
   const Tensor lam = lam_in.numel() == 1 && H != 1 ? lam_in.reshape({1}).expand({H}) : lam_in.dim() == 1 ? lam_in : lam_in.reshape({1});
   const double sc = scale.has_value() ? *scale : 1.0 / std::sqrt((double)Dh);
-  if (!(sc > 0.0 && sc < 1e30)) throw py::value_error(who + "scale " + std::to_string(sc) + " must be positive and finite");
+  if (!(sc >= 1e-30 && sc < 1e30)) throw py::value_error(who + "scale " + std::to_string(sc) + " must be in [1e-30, 1e30)");
+  if (causal && Nq + Nk > most) throw py::value_error(who + three + " out of range");
 
   Attn a{(int)B, (int)H, (int)Hk, (int)Nq, (int)Nk, (int)Dh, (int)Dv, (float)sc, causal, Drop{p, seed, given(base)}, Tensor(), Tensor()};
   const bool need = wants_grad({&q, &k, &v, &lam});
@@ -418,6 +424,8 @@ Tensor diff_attention(const Tensor& q, const Tensor& k, const Tensor& v, const T
     n->k_ = SavedVariable(kc, false);
     n->v_ = SavedVariable(vc, false);
     n->lam_ = SavedVariable(lc, false);
+    if (mask_in.defined()) n->mask_ = SavedVariable(mask_in, false);
+    if (padding.defined()) n->padding_ = SavedVariable(padding, false);
     n->lam_type = lam.scalar_type();
     n->a = std::move(a);
     n->stat = stat;
