@@ -826,19 +826,27 @@ __global__ __launch_bounds__((AttnPlan<T, DH, DV, SHARED>::NT), (AttnPlan<T, DH,
   for (int n = 0; n < 2 * S::KO; ++n) store_gq<T, S::KO>(a, w, n, acc[n / S::KO][n % S::KO]);
 }
 
-// grad_lam[h] = sum over the batch and the queries, one block a head, fixed order
-__global__ __launch_bounds__(256) static void diff_attn_lam_kernel(const float* __restrict__ dlrow, float* __restrict__ glam, int B, int H,
-                                                                   int Nq) {
-  __shared__ float red[4];
+// grad_lam[h] = sum over the batch and the queries, one block a head, fixed order (256 threads: 11 us for 10 000 rows)
+__global__ __launch_bounds__(1024) static void diff_attn_lam_kernel(const float* __restrict__ dlrow, float* __restrict__ glam, int B, int H,
+                                                                    int Nq) {
+  __shared__ float red[16];
   const int h = blockIdx.x;
   float s = 0.0f;
-  for (int b = 0; b < B; ++b)
-    for (int i = threadIdx.x; i < Nq; i += 256) s += dlrow[((int64_t)b * H + h) * Nq + i];
+  for (int b = 0; b < B; ++b) {
+    const float* row = dlrow + ((int64_t)b * H + h) * Nq;
+#pragma unroll 8
+    for (int i = threadIdx.x; i < Nq; i += 1024) s += row[i];
+  }
 #pragma unroll
   for (int m = 32; m >= 1; m >>= 1) s += __shfl_xor(s, m, 64);
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
   __syncthreads();
-  if (threadIdx.x == 0) glam[h] = (red[0] + red[1]) + (red[2] + red[3]);
+  if (threadIdx.x < 16) {
+    s = red[threadIdx.x];
+#pragma unroll
+    for (int m = 8; m >= 1; m >>= 1) s += __shfl_xor(s, m, 64);
+    if (threadIdx.x == 0) glam[h] = s;
+  }
 }
 
 // ---- backward: grad_k and grad_v; own = keys, staged = the rows of every head that shares them ----------------------------------
@@ -1194,7 +1202,7 @@ static int attn_backward(DiffAttnArgs a, float* glam, int64_t part_bytes, hipStr
       UBV_CHECK_LAUNCH(who);
     }
     if (glam != nullptr) {
-      hipLaunchKernelGGL(diff_attn_lam_kernel, dim3((unsigned)a.H), dim3(256), 0, st, a.dlrow, glam, a.B, a.H, a.Nq);
+      hipLaunchKernelGGL(diff_attn_lam_kernel, dim3((unsigned)a.H), dim3(1024), 0, st, a.dlrow, glam, a.B, a.H, a.Nq);
       UBV_CHECK_LAUNCH(who);
     }
   } else {

@@ -7,7 +7,7 @@
 // (K 16-byte pieces each) between its one load and its one store, with the variance taken around the mean in a second pass
 // over those registers; a row of a few pieces shares its wave with others (TPR < 64), a row of more than 256 pieces takes a
 // block.  Rows whose width is no multiple of a 16-byte piece start at any element border: the same kernels with
-// element-aligned accesses (one instruction too) and a scalar tail.  Rows wider than 2048 pieces (16-bit: 1024) are streamed.
+// element-aligned accesses (one instruction too) and a last piece that overlaps the one before.  Rows wider than 2048 pieces (16-bit: 1024) are streamed.
 //
 // The weight's gradient: a thread owns the same columns of every row that its block visits and keeps their sums in f32
 // registers; the block's threads are added through LDS, the blocks' sums [block][2][C] go to a workspace and are added in
@@ -20,50 +20,54 @@ namespace ubv {
 
 typedef __attribute__((ext_vector_type(4))) uint32_t lu32x4_t;
 
-// VEC = 16 bytes of T at p[c ..], elements from C on as 0
-template <typename T, bool ALN>
-__device__ __forceinline__ void ln_load(const T* p, int c, int C, float (&v)[16 / elem<T>::kBytes]) {
+// rows that start at 16-byte borders and are whole pieces | of at least one piece | narrower than a piece
+constexpr int kLnAligned = 0, kLnAny = 1, kLnNarrow = 2;
+
+// Where the piece of VEC elements that begins at column c is taken from: the last one of a row that is no whole number of pieces
+// is moved back to end with the row, and one past the row's end is that piece again; ln_in: the elements that are the piece's own.
+// Both holders of an element compute and store the same value.  (A scalar tail instead, whose loads wait for one another: 5001 x 1021
+// f16 forward 9.2 us, backward 19.8.)
+template <int VEC> __device__ __forceinline__ int ln_place(int c, int C) { return max(0, min(c, C - VEC)); }
+template <int AL> __device__ __forceinline__ bool ln_in(int c, int at, int i, int C) { return AL == kLnAligned ? c < C : at + i >= c && at + i < C; }
+
+// the piece at `at` (ln_place); a row narrower than a piece repeats its last element
+template <typename T, int AL>
+__device__ __forceinline__ void ln_load(const T* p, int at, int C, float (&v)[16 / elem<T>::kBytes]) {
   constexpr int VEC = 16 / elem<T>::kBytes;
-  if (c + VEC <= C) {
-    T t[VEC];
-    if constexpr (ALN) *reinterpret_cast<lu32x4_t*>(t) = *reinterpret_cast<const lu32x4_t*>(p + c);
-    else __builtin_memcpy(t, p + c, 16);
+  T t[VEC];
+  if constexpr (AL == kLnAligned) *reinterpret_cast<lu32x4_t*>(t) = *reinterpret_cast<const lu32x4_t*>(p + at);
+  else if constexpr (AL == kLnAny) __builtin_memcpy(t, p + at, 16);
+  else {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) v[i] = elem<T>::to_float(t[i]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      v[i] = 0.0f;
-      if (!ALN && c + i < C) v[i] = elem<T>::to_float(p[c + i]);
-    }
+    for (int i = 0; i < VEC; ++i) t[i] = p[min(i, C - 1)];
   }
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) v[i] = elem<T>::to_float(t[i]);
 }
-template <typename T, bool ALN>
-__device__ __forceinline__ void ln_store(T* p, int c, int C, const float (&v)[16 / elem<T>::kBytes]) {
+template <typename T, int AL>
+__device__ __forceinline__ void ln_store(T* p, int at, int C, const float (&v)[16 / elem<T>::kBytes]) {
   constexpr int VEC = 16 / elem<T>::kBytes;
-  if (c + VEC <= C) {
-    T t[VEC];
+  T t[VEC];
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) t[i] = elem<T>::from_float(v[i]);
-    if constexpr (ALN) *reinterpret_cast<lu32x4_t*>(p + c) = *reinterpret_cast<const lu32x4_t*>(t);
-    else __builtin_memcpy(p + c, t, 16);
-  } else if (!ALN) {
-#pragma unroll
-    for (int i = 0; i < VEC; ++i)
-      if (c + i < C) p[c + i] = elem<T>::from_float(v[i]);
-  }
-}
-// VEC f32 weights (gamma or beta; any alignment), `fill` where there are none
-template <int VEC>
-__device__ __forceinline__ void ln_weight(const float* w, int c, int C, float fill, float (&v)[VEC]) {
-#pragma unroll
-  for (int i = 0; i < VEC; ++i) v[i] = fill;
-  if (w == nullptr) return;
-  if (c + VEC <= C) __builtin_memcpy(v, w + c, 4 * VEC);
+  for (int i = 0; i < VEC; ++i) t[i] = elem<T>::from_float(v[i]);
+  if constexpr (AL == kLnAligned) *reinterpret_cast<lu32x4_t*>(p + at) = *reinterpret_cast<const lu32x4_t*>(t);
+  else if constexpr (AL == kLnAny) __builtin_memcpy(p + at, t, 16);
   else {
 #pragma unroll
     for (int i = 0; i < VEC; ++i)
-      if (c + i < C) v[i] = w[c + i];
+      if (i < C) p[i] = t[i];
+  }
+}
+// VEC f32 weights (gamma or beta; any alignment), `fill` where there are none
+template <int AL, int VEC>
+__device__ __forceinline__ void ln_weight(const float* w, int at, int C, float fill, float (&v)[VEC]) {
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) v[i] = fill;
+  if (w == nullptr) return;
+  if constexpr (AL != kLnNarrow) __builtin_memcpy(v, w + at, 4 * VEC);
+  else {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) v[i] = w[min(i, C - 1)];
   }
 }
 
@@ -99,7 +103,7 @@ template <int TPR> __device__ __forceinline__ void ln_sum(float& a, float (*red)
 
 constexpr int ln_block(int tpr) { return tpr < 256 ? 256 : tpr; }
 
-template <typename T, bool ALN, int TPR, int K>
+template <typename T, int AL, int TPR, int K>
 __global__ __launch_bounds__(ln_block(TPR)) void layer_norm_fwd_kernel(const T* __restrict__ x, const float* __restrict__ gamma,
                                                                      const float* __restrict__ beta, T* __restrict__ y,
                                                                      float* __restrict__ mean, float* __restrict__ rstd, long R,
@@ -108,6 +112,16 @@ __global__ __launch_bounds__(ln_block(TPR)) void layer_norm_fwd_kernel(const T* 
   __shared__ float red[TPR > 64 ? TPR / 64 : 1][2];
   const int sub = threadIdx.x / TPR, tc = (threadIdx.x % TPR) * VEC;
   const float inv = 1.0f / (float)C;
+  constexpr bool HOLD = K * VEC <= 16;                         // weights held for all the block's rows, else read for each
+  float gh[HOLD ? K : 1][VEC], bh[HOLD ? K : 1][VEC];
+  if constexpr (HOLD) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int at = ln_place<VEC>(tc + k * TPR * VEC, C);
+      ln_weight<AL, VEC>(gamma, at, C, 1.0f, gh[k]);
+      ln_weight<AL, VEC>(beta, at, C, 0.0f, bh[k]);
+    }
+  }
   for (long r0 = (long)blockIdx.x * ROWS; r0 < R; r0 += (long)gridDim.x * ROWS) {
     const long r = r0 + sub;
     const bool ok = r < R;
@@ -115,35 +129,40 @@ __global__ __launch_bounds__(ln_block(TPR)) void layer_norm_fwd_kernel(const T* 
     float v[K][VEC], sum = 0.0f;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      ln_load<T, ALN>(xr, tc + k * TPR * VEC, C, v[k]);
+      const int c = tc + k * TPR * VEC, at = ln_place<VEC>(c, C);
+      ln_load<T, AL>(xr, at, C, v[k]);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) sum += v[k][i];
+      for (int i = 0; i < VEC; ++i) sum += ln_in<AL>(c, at, i, C) ? v[k][i] : 0.0f;
     }
     ln_sum<TPR>(sum, red);
     const float mu = sum * inv;
     float var = 0.0f;
 #pragma unroll
-    for (int k = 0; k < K; ++k)
+    for (int k = 0; k < K; ++k) {
+      const int c = tc + k * TPR * VEC, at = ln_place<VEC>(c, C);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
-        const bool in = ALN ? tc + k * TPR * VEC < C : tc + k * TPR * VEC + i < C;
-        const float d = in ? v[k][i] - mu : 0.0f;
-        v[k][i] = d;
+        v[k][i] -= mu;
+        const float d = ln_in<AL>(c, at, i, C) ? v[k][i] : 0.0f;
         var = fmaf(d, d, var);
       }
+    }
     ln_sum<TPR>(var, red);
     const float rs = 1.0f / sqrtf(var * inv + eps);
     if (ok) {
 #pragma unroll
       for (int k = 0; k < K; ++k) {
-        const int c = tc + k * TPR * VEC;
+        const int c = tc + k * TPR * VEC, at = ln_place<VEC>(c, C);
         if (c < C) {
-          float g[VEC], b[VEC], o[VEC];
-          ln_weight<VEC>(gamma, c, C, 1.0f, g);
-          ln_weight<VEC>(beta, c, C, 0.0f, b);
+          float o[VEC];
+          float (&g)[VEC] = gh[HOLD ? k : 0], (&b)[VEC] = bh[HOLD ? k : 0];
+          if constexpr (!HOLD) {
+            ln_weight<AL, VEC>(gamma, at, C, 1.0f, g);
+            ln_weight<AL, VEC>(beta, at, C, 0.0f, b);
+          }
 #pragma unroll
           for (int i = 0; i < VEC; ++i) o[i] = fmaf(v[k][i] * rs, g[i], b[i]);
-          ln_store<T, ALN>(y + r * C, c, C, o);
+          ln_store<T, AL>(y + r * C, at, C, o);
         }
       }
       if (threadIdx.x % TPR == 0 && mean != nullptr) { mean[r] = mu; rstd[r] = rs; }
@@ -151,7 +170,7 @@ __global__ __launch_bounds__(ln_block(TPR)) void layer_norm_fwd_kernel(const T* 
   }
 }
 
-template <typename T, bool ALN, int TPR, int K>
+template <typename T, int AL, int TPR, int K>
 __global__ __launch_bounds__(ln_block(TPR)) void layer_norm_bwd_kernel(const T* __restrict__ gy, const T* __restrict__ x,
                                                                      const float* __restrict__ gamma,
                                                                      const float* __restrict__ mean,
@@ -163,7 +182,12 @@ __global__ __launch_bounds__(ln_block(TPR)) void layer_norm_bwd_kernel(const T* 
   __shared__ float cols[TPR > 64 ? 1 : 3][TPR > 64 ? 1 : GW * VEC * K];
   const int sub = threadIdx.x / TPR, tc = (threadIdx.x % TPR) * VEC;
   const float inv = 1.0f / (float)C;
-  float ag[K][VEC], ab[K][VEC];
+  constexpr bool HOLD = K * VEC <= 16;
+  float ag[K][VEC], ab[K][VEC], gh[HOLD ? K : 1][VEC];
+  if constexpr (HOLD) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) ln_weight<AL, VEC>(gamma, ln_place<VEC>(tc + k * TPR * VEC, C), C, 1.0f, gh[k]);
+  }
 #pragma unroll
   for (int k = 0; k < K; ++k)
 #pragma unroll
@@ -176,21 +200,22 @@ __global__ __launch_bounds__(ln_block(TPR)) void layer_norm_bwd_kernel(const T* 
     float h[K][VEC], u[K][VEC], s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const int c = tc + k * TPR * VEC;
-      float g[VEC];
-      ln_load<T, ALN>(x + rr * C, c, C, h[k]);
-      ln_load<T, ALN>(gy + rr * C, c, C, u[k]);
-      ln_weight<VEC>(gamma, c, C, 1.0f, g);
+      const int c = tc + k * TPR * VEC, at = ln_place<VEC>(c, C);
+      float (&g)[VEC] = gh[HOLD ? k : 0];
+      ln_load<T, AL>(x + rr * C, at, C, h[k]);
+      ln_load<T, AL>(gy + rr * C, at, C, u[k]);
+      if constexpr (!HOLD) ln_weight<AL, VEC>(gamma, at, C, 1.0f, g);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
-        const bool in = ok && (ALN ? c < C : c + i < C);
-        h[k][i] = in ? (h[k][i] - mu) * rs : 0.0f;
-        const float go = in ? u[k][i] : 0.0f;
-        ag[k][i] = fmaf(go, h[k][i], ag[k][i]);
+        const bool in = ok && ln_in<AL>(c, at, i, C);
+        h[k][i] = (h[k][i] - mu) * rs;
+        const float hi = in ? h[k][i] : 0.0f, go = in ? u[k][i] : 0.0f;
+        u[k][i] *= g[i];
+        ag[k][i] = fmaf(go, hi, ag[k][i]);
         ab[k][i] += go;
-        u[k][i] = go * g[i];
-        s1 += u[k][i];
-        s2 = fmaf(u[k][i], h[k][i], s2);
+        const float ui = in ? u[k][i] : 0.0f;
+        s1 += ui;
+        s2 = fmaf(ui, hi, s2);
       }
     }
     ln_sum2<TPR>(s1, s2, red);
@@ -202,7 +227,7 @@ __global__ __launch_bounds__(ln_block(TPR)) void layer_norm_bwd_kernel(const T* 
         float o[VEC];
 #pragma unroll
         for (int i = 0; i < VEC; ++i) o[i] = rs * (u[k][i] - s1 - h[k][i] * s2);
-        if (c < C) ln_store<T, ALN>(gx + r * C, c, C, o);
+        if (c < C) ln_store<T, AL>(gx + r * C, ln_place<VEC>(c, C), C, o);
       }
     }
   }
@@ -210,12 +235,12 @@ __global__ __launch_bounds__(ln_block(TPR)) void layer_norm_bwd_kernel(const T* 
   float* out = part + (long)blockIdx.x * 2 * C;
   if constexpr (TPR > 64) {
 #pragma unroll
-    for (int k = 0; k < K; ++k)
+    for (int k = 0; k < K; ++k) {
+      const int c = tc + k * TPR * VEC, at = ln_place<VEC>(c, C);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        const int c = tc + k * TPR * VEC + i;
-        if (c < C) { out[c] = ag[k][i]; out[C + c] = ab[k][i]; }
-      }
+      for (int i = 0; i < VEC; ++i)
+        if (ln_in<AL>(c, at, i, C)) { out[at + i] = ag[k][i]; out[C + at + i] = ab[k][i]; }
+    }
   } else {
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
 #pragma unroll
@@ -232,12 +257,14 @@ __global__ __launch_bounds__(ln_block(TPR)) void layer_norm_bwd_kernel(const T* 
       __syncthreads();
       if (wv == 0 && lane < GW) {
 #pragma unroll
-        for (int k = 0; k < K; ++k)
+        for (int k = 0; k < K; ++k) {
+          const int c = tc + k * TPR * VEC, at = ln_place<VEC>(c, C);
 #pragma unroll
           for (int i = 0; i < VEC; ++i) {
-            const int c = tc + k * TPR * VEC + i, o = (k * GW + lane) * VEC + i;
-            if (c < C) out[half * C + c] = ((a[k][i] + cols[0][o]) + cols[1][o]) + cols[2][o];
+            const int o = (k * GW + lane) * VEC + i;
+            if (ln_in<AL>(c, at, i, C)) out[half * C + at + i] = ((a[k][i] + cols[0][o]) + cols[1][o]) + cols[2][o];
           }
+        }
       }
       __syncthreads();
     }
@@ -257,27 +284,30 @@ __global__ __launch_bounds__(1024) void layer_norm_wide_fwd_kernel(const T* __re
     T* yr = y + r * C;
     float sum = 0.0f, var = 0.0f, v[VEC];
     for (int c = threadIdx.x * VEC; c < C; c += 1024 * VEC) {
-      ln_load<T, false>(xr, c, C, v);
+      const int at = ln_place<VEC>(c, C);
+      ln_load<T, kLnAny>(xr, at, C, v);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) sum += v[i];
+      for (int i = 0; i < VEC; ++i) sum += at + i >= c ? v[i] : 0.0f;
     }
     ln_sum<1024>(sum, red);
     const float mu = sum / (float)C;
     for (int c = threadIdx.x * VEC; c < C; c += 1024 * VEC) {
-      ln_load<T, false>(xr, c, C, v);
+      const int at = ln_place<VEC>(c, C);
+      ln_load<T, kLnAny>(xr, at, C, v);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) { const float d = c + i < C ? v[i] - mu : 0.0f; var = fmaf(d, d, var); }
+      for (int i = 0; i < VEC; ++i) { const float d = at + i >= c ? v[i] - mu : 0.0f; var = fmaf(d, d, var); }
     }
     ln_sum<1024>(var, red);
     const float rs = 1.0f / sqrtf(var / (float)C + eps);
     for (int c = threadIdx.x * VEC; c < C; c += 1024 * VEC) {
+      const int at = ln_place<VEC>(c, C);
       float g[VEC], b[VEC];
-      ln_load<T, false>(xr, c, C, v);
-      ln_weight<VEC>(gamma, c, C, 1.0f, g);
-      ln_weight<VEC>(beta, c, C, 0.0f, b);
+      ln_load<T, kLnAny>(xr, at, C, v);
+      ln_weight<kLnAny, VEC>(gamma, at, C, 1.0f, g);
+      ln_weight<kLnAny, VEC>(beta, at, C, 0.0f, b);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) v[i] = fmaf((v[i] - mu) * rs, g[i], b[i]);
-      ln_store<T, false>(yr, c, C, v);
+      ln_store<T, kLnAny>(yr, at, C, v);
     }
     if (threadIdx.x == 0 && mean != nullptr) { mean[r] = mu; rstd[r] = rs; }
   }
@@ -294,12 +324,13 @@ __global__ __launch_bounds__(1024) void layer_norm_wide_bwd_kernel(const T* __re
     const float mu = mean[r], rs = rstd[r];
     float s1 = 0.0f, s2 = 0.0f, v[VEC], go[VEC], g[VEC];
     for (int c = threadIdx.x * VEC; c < C; c += 1024 * VEC) {
-      ln_load<T, false>(x + base, c, C, v);
-      ln_load<T, false>(gy + base, c, C, go);
-      ln_weight<VEC>(gamma, c, C, 1.0f, g);
+      const int at = ln_place<VEC>(c, C);
+      ln_load<T, kLnAny>(x + base, at, C, v);
+      ln_load<T, kLnAny>(gy + base, at, C, go);
+      ln_weight<kLnAny, VEC>(gamma, at, C, 1.0f, g);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
-        const float u = c + i < C ? go[i] * g[i] : 0.0f;
+        const float u = at + i >= c ? go[i] * g[i] : 0.0f;
         s1 += u;
         s2 = fmaf(u, (v[i] - mu) * rs, s2);
       }
@@ -307,12 +338,13 @@ __global__ __launch_bounds__(1024) void layer_norm_wide_bwd_kernel(const T* __re
     ln_sum2<1024>(s1, s2, red);
     s1 /= (float)C; s2 /= (float)C;
     for (int c = threadIdx.x * VEC; c < C; c += 1024 * VEC) {
-      ln_load<T, false>(x + base, c, C, v);
-      ln_load<T, false>(gy + base, c, C, go);
-      ln_weight<VEC>(gamma, c, C, 1.0f, g);
+      const int at = ln_place<VEC>(c, C);
+      ln_load<T, kLnAny>(x + base, at, C, v);
+      ln_load<T, kLnAny>(gy + base, at, C, go);
+      ln_weight<kLnAny, VEC>(gamma, at, C, 1.0f, g);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) v[i] = rs * (go[i] * g[i] - s1 - (v[i] - mu) * rs * s2);
-      ln_store<T, false>(gx + base, c, C, v);
+      ln_store<T, kLnAny>(gx + base, at, C, v);
     }
   }
 }
@@ -334,30 +366,27 @@ __global__ __launch_bounds__(256) void layer_norm_wide_cols_kernel(const T* __re
   part[((long)blockIdx.y * 2 + 1) * C + c] = ab;
 }
 
-// out[t] = sum over the blocks' rows IN BLOCK ORDER, t < 2 C: 16 columns x 16 groups of rows per block
-__global__ __launch_bounds__(256) void layer_norm_cols_final_kernel(const float* __restrict__ part, int nrows, int C,
-                                                                   float* __restrict__ dgamma, float* __restrict__ dbeta) {
-  __shared__ float red[16][17];
+// out[t] = sum over the blocks' rows in fixed order, t < 2 C: 16 columns x 64 groups of rows per block (16 groups: 7.5 us for
+// 1024 x 2042)
+__global__ __launch_bounds__(1024) void layer_norm_cols_final_kernel(const float* __restrict__ part, int nrows, int C,
+                                                                    float* __restrict__ dgamma, float* __restrict__ dbeta) {
+  __shared__ float red[64][17];
   const int cl = threadIdx.x & 15, rg = threadIdx.x >> 4;
   const int t = blockIdx.x * 16 + cl;
-  const int per = (nrows + 15) / 16;
+  const int per = (nrows + 63) / 64;
   float sum = 0.0f;
   if (t < 2 * C) {
     const int r1 = min(nrows, (rg + 1) * per);
-    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    int r = rg * per;
-    for (; r + 3 < r1; r += 4)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) s[j] += part[(long)(r + j) * 2 * C + t];
-    for (; r < r1; ++r) s[0] += part[(long)r * 2 * C + t];
-    sum = (s[0] + s[1]) + (s[2] + s[3]);
+#pragma unroll 8
+    for (int r = rg * per; r < r1; ++r) sum += part[(long)r * 2 * C + t];
   }
   red[rg][cl] = sum;
   __syncthreads();
   if (rg == 0 && t < 2 * C) {
-    float tot = 0.0f;
+    float q[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int g = 0; g < 16; ++g) tot += red[g][cl];
+    for (int g = 0; g < 64; ++g) q[g >> 4] += red[g][cl];
+    const float tot = (q[0] + q[1]) + (q[2] + q[3]);
     if (t < C) { if (dgamma != nullptr) dgamma[t] = tot; }
     else if (dbeta != nullptr) dbeta[t - C] = tot;
   }
@@ -397,8 +426,11 @@ static void ln_fwd(const void* xv, const float* gamma, const float* beta, void* 
   const bool held = ln_plan<VEC>(C, [&](auto tpr, auto k) {
     constexpr int TPR = decltype(tpr)::value, K = decltype(k)::value, ROWS = ln_block(TPR) / TPR;
     const dim3 grid((unsigned)min((R + ROWS - 1) / ROWS, 4096L)), blk(ln_block(TPR));
-    if (aln) hipLaunchKernelGGL((layer_norm_fwd_kernel<T, true, TPR, K>), grid, blk, 0, st, x, gamma, beta, y, mean, rstd, R, C, eps);
-    else hipLaunchKernelGGL((layer_norm_fwd_kernel<T, false, TPR, K>), grid, blk, 0, st, x, gamma, beta, y, mean, rstd, R, C, eps);
+    auto run = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, blk, 0, st, x, gamma, beta, y, mean, rstd, R, C, eps); };
+    if (aln) return run(layer_norm_fwd_kernel<T, kLnAligned, TPR, K>);
+    if constexpr (TPR == 4)
+      if (C < VEC) return run(layer_norm_fwd_kernel<T, kLnNarrow, TPR, K>);
+    run(layer_norm_fwd_kernel<T, kLnAny, TPR, K>);
   });
   if (!held)
     hipLaunchKernelGGL(layer_norm_wide_fwd_kernel<T>, dim3((unsigned)min(R, 4096L)), dim3(1024), 0, st, x, gamma, beta, y, mean, rstd, R, C, eps);
@@ -414,10 +446,14 @@ static void ln_bwd(const void* gyv, const void* xv, const float* gamma, const fl
   int nrows = 0;
   const bool held = ln_plan<VEC>(C, [&](auto tpr, auto k) {
     constexpr int TPR = decltype(tpr)::value, K = decltype(k)::value, ROWS = ln_block(TPR) / TPR;
-    nrows = (int)min((R + ROWS - 1) / ROWS, (long)kLnBwdBlocks);
+    const long steps = (R + ROWS - 1) / ROWS, each = (steps + kLnBwdBlocks - 1) / kLnBwdBlocks;
+    nrows = (int)((steps + each - 1) / each);          // as few blocks as take the same number of steps
     const dim3 grid((unsigned)nrows), blk(ln_block(TPR));
-    if (aln) hipLaunchKernelGGL((layer_norm_bwd_kernel<T, true, TPR, K>), grid, blk, 0, st, gy, x, gamma, mean, rstd, gx, part, R, C);
-    else hipLaunchKernelGGL((layer_norm_bwd_kernel<T, false, TPR, K>), grid, blk, 0, st, gy, x, gamma, mean, rstd, gx, part, R, C);
+    auto run = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, blk, 0, st, gy, x, gamma, mean, rstd, gx, part, R, C); };
+    if (aln) return run(layer_norm_bwd_kernel<T, kLnAligned, TPR, K>);
+    if constexpr (TPR == 4)
+      if (C < VEC) return run(layer_norm_bwd_kernel<T, kLnNarrow, TPR, K>);
+    run(layer_norm_bwd_kernel<T, kLnAny, TPR, K>);
   });
   if (!held) {
     if (gx != nullptr)
@@ -427,7 +463,7 @@ static void ln_bwd(const void* gyv, const void* xv, const float* gamma, const fl
       hipLaunchKernelGGL(layer_norm_wide_cols_kernel<T>, dim3((C + 255) / 256, nrows), dim3(256), 0, st, gy, x, mean, rstd, part, R, C);
   }
   if (part != nullptr)
-    hipLaunchKernelGGL(layer_norm_cols_final_kernel, dim3((2 * C + 15) / 16), dim3(256), 0, st, part, nrows, C, dgamma, dbeta);
+    hipLaunchKernelGGL(layer_norm_cols_final_kernel, dim3((2 * C + 15) / 16), dim3(1024), 0, st, part, nrows, C, dgamma, dbeta);
 }
 
 static int ln_check(int64_t R, int C, int dtype, const char* who) {
