@@ -543,6 +543,18 @@ def test_attention_long_axes_are_shared_by_blocks(Nq, Nk, H, Hk, causal_, dt):
     attn_check(*attn_inputs(1, H, Hk, Nq, Nk, 64, 128, dt), dt, p=0.1, **kw)
 
 
+@pytest.mark.parametrize('Nq,Nk,H,Hk,causal_', [(1100, 1100, 4, 2, True), (600, 2100, 2, 2, False), (1040, 129, 4, 1, False),
+                                                 (1300, 1030, 2, 1, True), (700, 1633, 2, 2, True)])
+@pytest.mark.parametrize('Dh,Dv', [(64, 64), (64, 128), (128, 128), (128, 256)])
+@pytest.mark.parametrize('dt', [torch.float16, torch.float32])
+def test_attention_wide_heads_share_long_axes(Nq, Nk, H, Hk, causal_, Dh, Dv, dt):
+    """blocks of 128 own items that share the staged ones, in unequal parts where causal"""
+    hidden = kw = None
+    if causal_:
+        hidden, kw = causal(Nq, Nk), dict(causal=True)
+    attn_check(*attn_inputs(1, H, Hk, Nq, Nk, Dh, Dv, dt), dt, hidden=hidden, **(kw or {}))
+
+
 def test_attention_large_scores():
     """scores far beyond f32's exponent range: the row's largest is subtracted first"""
     q, k, v, lam, go = attn_inputs(1, 2, 2, 20, 50, 32, 64, torch.float32)

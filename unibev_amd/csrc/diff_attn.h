@@ -12,6 +12,7 @@
 // operands of one), and the A operand is read transposed from the same staged rows (ds_read_b64_tr_b16).  So no score ever
 // goes through memory or LDS, and the softmax of a row is arithmetic of its own lane and the one 32 lanes away.
 #pragma once
+#include <algorithm>
 #include <type_traits>
 
 #include "ubv_common.h"
@@ -41,9 +42,11 @@ struct DiffAttnArgs {
   float* dlrow;                            // [B H Nq] - sum_j A_2 G
   void *gq, *gk, *gv;                      // contiguous gradients
   int work;                                // blocks with work (the grid is rounded up)
-  int splits;                              // blocks that share the staged items of an own tile, 1: none
+  int splits;                              // most blocks that share the staged items of an own tile, 1: none
+  int chunk;                               // staged tiles of each of them (fewer in the last)
+  int own, n;                              // own items of a block, items of a staged tile
   int halves;                              // forward: blocks that share a row tile's output columns
-  float* part;                             // splits > 1: [tile][half][split][64 lanes][floats] the blocks' sums
+  float* part;                             // splits > 1: [32 own items][half][split][64 lanes][floats] the blocks' sums
 };
 
 constexpr int kAttnSplits = 256;         // most splits of an own tile's staged items

@@ -53,7 +53,7 @@ template <typename T, int DH, int DV, bool SHARED> struct AttnPlan {
 
 // What a call may hold beside hidden keys.  Each has kernels of its own: what a kernel can never meet costs it registers, and
 // with them a wave per SIMD (32 / 64 wide heads, bf16, 10 000 x 10 000: grad_k / grad_v 738 us with everything, 448 plain).
-constexpr int kAttnPlain = 0, kAttnDrop = 1, kAttnAny = 2;       // nothing | dropout | masks, causal, dropout or not
+constexpr int kAttnPlain = 0, kAttnDrop = 1, kAttnCausal = 2, kAttnAny = 3;       // nothing | dropout | causal | masks, any of it together
 
 // ---- staging ------------------------------------------------------------------------------------------------------------------
 // PREF: a tile's pieces wait in registers until the present tile is done with; else they pass through in groups of 8
@@ -206,7 +206,7 @@ __device__ __forceinline__ bool key_hidden(const DiffAttnArgs& a, int b, int j0,
 }
 
 // hides keys of a tile from the lane's row (query i of head h): `hid` bits of the 32 keys from j0, causal, the call's mask
-template <bool MASK> __device__ __forceinline__ void mask_tile(const DiffAttnArgs& a, af32x16_t (&x)[2], uint32_t hid, int b, int h, int i, int j0, float rscale,
+template <int MODE> __device__ __forceinline__ void mask_tile(const DiffAttnArgs& a, af32x16_t (&x)[2], uint32_t hid, int b, int h, int i, int j0, float rscale,
                                           int lane) {
   const int half = 4 * (lane >> 5);
   if (hid != 0) {
@@ -215,8 +215,8 @@ template <bool MASK> __device__ __forceinline__ void mask_tile(const DiffAttnArg
     for (int e = 0; e < 16; ++e)
       if (w & (1u << (8 * (e >> 2) + (e & 3)))) { x[0][e] = kNegInf; x[1][e] = kNegInf; }
   }
-  if constexpr (!MASK) return;
-  if (a.causal) {
+  if constexpr (MODE < kAttnCausal) return;
+  if (MODE == kAttnCausal || a.causal) {
     const int lim = i + a.Nk - a.Nq - j0 - half;
     if (__any(lim < 31 - half)) {
 #pragma unroll
@@ -224,7 +224,7 @@ template <bool MASK> __device__ __forceinline__ void mask_tile(const DiffAttnArg
         if (8 * (e >> 2) + (e & 3) > lim) { x[0][e] = kNegInf; x[1][e] = kNegInf; }
     }
   }
-  if (a.mask_kind == 0) return;
+  if (MODE != kAttnAny || a.mask_kind == 0) return;
   const int64_t o = b * a.ms[0] + h * a.ms[1] + i * a.ms[2] + (j0 + half) * a.ms[3];
   const bool whole = j0 + 32 <= a.Nk;
   const int last = a.Nk - 1 - j0 - half;               // (keys past the end, which `hid` hides, read the last one's)
@@ -263,10 +263,32 @@ template <bool MASK> __device__ __forceinline__ void mask_tile(const DiffAttnArg
 }
 
 // Blocks go round-robin over the 8 XCDs: XCD x takes the x-th eighth of the tiles, so that the tiles of a head, which read the
-// same keys (or rows), meet in one L2 (2 x 8 heads of 64 / 128, 4096 x 4096: forward 389 -> 376 us).  Not in a padded batch, whose
-// samples are unequal work, nor where splits of one tile share nothing.  The grid is rounded up; a tile past the end has no work.
+// same keys (or rows), meet in one L2 (2 x 8 heads of 64 / 128, 4096 x 4096: forward 389 -> 376 us; causal, f16, 2 x 2 shared heads,
+// 2047 x 2047: 153 -> 128).  Not in a padded batch, whose samples are unequal work, nor where splits of one tile share nothing.
+// The grid is rounded up; a tile past the end has no work.
 __device__ __forceinline__ int xcd_tile(const DiffAttnArgs& a) {
-  return a.kpm != nullptr || a.splits > 1 ? blockIdx.x : xcd_remap(blockIdx.x, gridDim.x >> 3);
+  return a.kpm != nullptr || (a.splits > 1 && !a.causal) ? blockIdx.x : xcd_remap(blockIdx.x, gridDim.x >> 3);
+}
+// block `id`'s own tile and which of its splits.  Causal tiles of a head are unequal: where an eighth is a part of a head (m parts),
+// the parts take its tiles in turns, there and back, longest first; the last splits, short or empty, come last
+__device__ __forceinline__ int2 tile_split(const DiffAttnArgs& a, int id) {
+  if (!a.causal) return make_int2(id / a.splits, id % a.splits);
+  const int heads = a.B * a.Hk, units = a.work / heads, tiles = units / a.splits, bh = id / units, u = id - bh * units;
+  const int m = heads & 1 ? 8 : heads & 2 ? 4 : heads & 4 ? 2 : 1, q = units / m, r = units - q * m;
+  const int longer = r * (q + 1);                      // (r parts have a unit more)
+  const int part = u < longer ? u / (q + 1) : r + (u - longer) / max(q, 1);
+  const int at = u < longer ? u - part * (q + 1) : u - longer - (part - r) * q;
+  const int o = at * m + ((at & 1) && at < q ? m - 1 - part : part);
+  return make_int2(bh * tiles + o % tiles, o / tiles);
+}
+
+// keys that some row of rb .. rb + n - 1 sees: [0, rows_end)
+__device__ __forceinline__ int rows_end(const DiffAttnArgs& a, int rb, int n) {
+  if (!a.causal) return a.Nk;
+  const int last = (rb + n < a.R ? rb + n : a.R) - 1;
+  const int imax = rb / a.Nq == last / a.Nq ? last % a.Nq : a.Nq - 1;
+  const int end = imax + a.Nk - a.Nq + 1;
+  return end < 0 ? 0 : end < a.Nk ? end : a.Nk;
 }
 
 // what forward and grad_q share: own = rows
@@ -290,12 +312,11 @@ struct RowWave {
     const int rc = ok ? r : a.R - 1, g = rc / a.Nq;
     h = hk * a.G + g; i = rc - g * a.Nq;
     rowid = ((int64_t)b * a.H + hk * a.G) * a.Nq + rc;
-    kend = a.Nk;
-    if (MASK && a.causal) {
-      const int last = min(rb + 32 * WQ, a.R) - 1;
-      const int imax = rb / a.Nq == last / a.Nq ? last % a.Nq : a.Nq - 1;
-      kend = max(0, min(a.Nk, imax + a.Nk - a.Nq + 1));
-    }
+    kend = MASK ? rows_end(a, rb, 32 * WQ) : a.Nk;
+  }
+  // this wave's 32 rows among those of all heads
+  __device__ __forceinline__ int64_t tile32(const DiffAttnArgs& a) const {
+    return ((int64_t)b * a.Hk + hk) * ((a.R + 31) / 32) + rb / 32 + wq;
   }
 };
 
@@ -350,6 +371,13 @@ __device__ __forceinline__ void key_tiles(const DiffAttnArgs& a, const RowWave& 
   }
 }
 
+// 16 floats of a lane as 4 pieces, `step` floats apart
+__device__ __forceinline__ void put_block(float* at, const af32x16_t& v, int step) {
+#pragma unroll
+  for (int q = 0; q < 4; ++q)
+    *reinterpret_cast<float4*>(at + q * step) = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+}
+
 // ---- forward ------------------------------------------------------------------------------------------------------------------
 template <typename T, int DV> struct FwdState {
   static constexpr int VO = DV / 32;
@@ -382,17 +410,16 @@ template <typename T, int DV> struct FwdState {
         for (int e = 0; e < 16; ++e) slot[(4 + (m * VO + d) * 16 + e) * 64] = acc[m][d][e];
     }
   }
-  // the same, a lane's FLOATS in one stretch (only the lanes of rows are written: few rows are few bytes)
-  __device__ __forceinline__ void put_row(float* at) const {
+  // the same for the splits' workspace, pieces of 4 floats.  Rows by the wave: piece by piece, 1 KB each; few rows: a lane's in one
+  // stretch (only the lanes of rows are written: few bytes)
+  static __device__ __forceinline__ int64_t lane_at(bool few, int lane) { return few ? lane * FLOATS : lane * 4; }
+  static __device__ __forceinline__ int piece(bool few) { return few ? 4 : 256; }
+  __device__ __forceinline__ void put_row(float* at, int step) const {
     *reinterpret_cast<float4*>(at) = make_float4(top[0], l[0], top[1], l[1]);
 #pragma unroll
     for (int m = 0; m < 2; ++m)
 #pragma unroll
-      for (int d = 0; d < VO; ++d)
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-          *reinterpret_cast<float4*>(at + 4 + (m * VO + d) * 16 + 4 * q) =
-              make_float4(acc[m][d][4 * q], acc[m][d][4 * q + 1], acc[m][d][4 * q + 2], acc[m][d][4 * q + 3]);
+      for (int d = 0; d < VO; ++d) put_block(at + (1 + (m * VO + d) * 4) * step, acc[m][d], step);
   }
   // joins what another wave put for the same rows
   __device__ __forceinline__ void join(const float* slot, float c) {
@@ -458,28 +485,30 @@ __global__ __launch_bounds__((AttnPlan<T, DH, DV, SHARED>::NT), (AttnPlan<T, DH,
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int id = xcd_tile(a);
   if (id >= a.work) return;
-  const int part = id / a.splits, split = id - part * a.splits, tile = part / a.halves, col = (part - tile * a.halves) * DV;
+  const int2 cut = tile_split(a, id);
+  const int split = cut.y, tile = cut.x / a.halves, col = (cut.x - tile * a.halves) * DV;
   RowWave w;
-  w.init<P::WQ, P::WK, MODE == kAttnAny>(a, tile);
+  w.init<P::WQ, P::WK, (MODE >= kAttnCausal)>(a, tile);
+  const int tn = (w.kend + P::N - 1) / P::N, t0 = split * a.chunk;
+  if (split > 0 && t0 >= tn) return;                   // (an own tile that sees less has fewer splits)
   OwnRow<T, S::KB, S::KEEP> qf[2];
 #pragma unroll
   for (int m = 0; m < 2; ++m)
     qf[m].init((const T*)a.q + w.b * a.qs[0] + w.i * a.qs[1] + w.h * a.qs[2] + m * a.qs[3], w.ok, a.Dh, w.lane);
   const float c = a.scale * kLog2e, rscale = 1.0f / a.scale, grow = 6.0f / c;
-  constexpr bool MASK = MODE == kAttnAny;
-  const bool fm = MASK && a.mask_kind == 2, drop = MODE != kAttnPlain && a.t16 != 0;
+  constexpr bool MASK = MODE >= kAttnCausal;
+  const bool fm = MODE == kAttnAny && a.mask_kind == 2, drop = (MODE == kAttnDrop || MODE == kAttnAny) && a.t16 != 0;
   const uint32_t t32 = a.t16 << 16;
   const uint64_t zrow = attn_seed(a.seed, a.seed_dev) + (uint64_t)(w.rowid * a.n4) + (w.lane >> 5);
   FwdState<T, DV> s;
   s.init();
   float mu[2] = {0.0f, 0.0f};
-  const int tn = (w.kend + P::N - 1) / P::N, per = (tn + a.splits - 1) / a.splits;
-  key_tiles<T, DH, DV, SHARED>(a, w, col, split * per, min(tn, (split + 1) * per), smem,
+  key_tiles<T, DH, DV, SHARED>(a, w, col, t0, min(tn, t0 + a.chunk), smem,
                                [&](const char* kt, int it0, uint32_t hid, int j0) {
     af32x16_t x[2];
 #pragma unroll
     for (int m = 0; m < 2; ++m) x[m] = tile_dot<T, S::KB, S::LX, S::KEEP>(kt, it0, m * S::LX / 2, qf[m], w.lane);
-    if (hid != 0 || (MASK && (a.causal || a.mask_kind != 0))) mask_tile<MASK>(a, x, hid, w.b, w.h, w.i, j0, rscale, w.lane);
+    if (hid != 0 || MASK) mask_tile<MODE>(a, x, hid, w.b, w.h, w.i, j0, rscale, w.lane);
     float p[2][16];
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
@@ -543,14 +572,53 @@ __global__ __launch_bounds__((AttnPlan<T, DH, DV, SHARED>::NT), (AttnPlan<T, DH,
     }
     if (w.wk != 0) return;
   }
-  if (a.splits > 1) {
-    if (w.ok) s.put_row(a.part + ((int64_t)id * 64 + w.lane) * s.FLOATS);
+  if (tn > a.chunk) {
+    const bool few = a.R < 32;
+    if (w.ok) s.put_row(a.part + ((w.tile32(a) * a.halves + col / DV) * a.splits + split) * 64 * s.FLOATS + s.lane_at(few, w.lane), s.piece(few));
     return;
   }
   fwd_finish<T, DV>(a, s, w, col, c);
 }
 
-// Joins the splits of a row: one block a row (and column half), a thread an element of one map's product.  Weights of the splits
+// Joins the splits of 32 rows: one wave a tile and 32 columns of a half
+template <typename T, int DV>
+__global__ __launch_bounds__(64) void diff_attn_join_rows_kernel(const DiffAttnArgs a) {
+  constexpr int VO = DV / 32, FLOATS = FwdState<T, DV>::FLOATS;
+  const int part = blockIdx.x / VO, d = blockIdx.x - part * VO, tile = part / a.halves, half = part - tile * a.halves;
+  RowWave w;
+  w.init<1, 1, true>(a, tile);
+  const int parts = ((rows_end(a, w.rb / a.own * a.own, a.own) + a.n - 1) / a.n + a.chunk - 1) / a.chunk;
+  if (!w.ok || parts <= 1) return;                     // (written by its one block)
+  const float c = a.scale * kLog2e;
+  const float* at = a.part + (w.tile32(a) * a.halves + half) * a.splits * 64 * FLOATS + w.lane * 4;
+  FwdState<T, 32> s;
+  s.init();
+#pragma unroll 2
+  for (int p = 0; p < parts; ++p) {
+    const float* f = at + (int64_t)p * 64 * FLOATS;
+    const float4 r = *reinterpret_cast<const float4*>(f);
+    const float to[2] = {r.x, r.z}, lo[2] = {r.y, r.w};
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      const float t = fmaxf(s.top[m], to[m]);
+      const float f0 = s.top[m] == kNegInf ? 0.0f : aexp2((s.top[m] - t) * c), f1 = to[m] == kNegInf ? 0.0f : aexp2((to[m] - t) * c);
+      s.scale(m, f0);
+      s.l[m] = fmaf(lo[m], f1, s.l[m]);
+      s.top[m] = t;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const float4 v = *reinterpret_cast<const float4*>(f + (1 + (m * VO + d) * 4 + q) * 256);
+        s.acc[m][0][4 * q] = fmaf(v.x, f1, s.acc[m][0][4 * q]);
+        s.acc[m][0][4 * q + 1] = fmaf(v.y, f1, s.acc[m][0][4 * q + 1]);
+        s.acc[m][0][4 * q + 2] = fmaf(v.z, f1, s.acc[m][0][4 * q + 2]);
+        s.acc[m][0][4 * q + 3] = fmaf(v.w, f1, s.acc[m][0][4 * q + 3]);
+      }
+    }
+  }
+  fwd_finish<T, 32>(a, s, w, half * DV + 32 * d, c);
+}
+
+// Joins the splits of few rows (under 32 a group): one block a row (and column half), a thread an element of one map's product.  Weights of the splits
 // first (one exponential each, in LDS), then the products' sum in split order.
 template <typename T, int DV>
 __global__ __launch_bounds__(256) void diff_attn_join_kernel(const DiffAttnArgs a) {
@@ -558,10 +626,13 @@ __global__ __launch_bounds__(256) void diff_attn_join_kernel(const DiffAttnArgs 
   __shared__ float wt[2][kAttnSplits], red[4][4], o2s[128];
   const float c = a.scale * kLog2e;
   const int part = blockIdx.x, half = part % a.halves, row = part / a.halves, bh = row / a.R, r = row - bh * a.R;
-  const int tiles = (a.R + 31) / 32, tile = bh * tiles + (a.causal ? tiles - 1 - r / 32 : r / 32), lane = r % 32, col = half * DV;
+  const int parts = ((rows_end(a, r / a.own * a.own, a.own) + a.n - 1) / a.n + a.chunk - 1) / a.chunk;
+  if (parts <= 1) return;                              // (written by its one block)
+  const int lane = r % 32, col = half * DV;
+  const int64_t tile = (int64_t)bh * ((a.R + 31) / 32) + r / 32;
   const int b = bh / a.Hk, hk = bh - b * a.Hk, h = hk * a.G + r / a.Nq, i = r % a.Nq;
   const int64_t rows = (int64_t)a.B * a.H * a.Nq, rowid = ((int64_t)b * a.H + h) * a.Nq + i;
-  const float* p = a.part + ((int64_t)(tile * a.halves + half) * a.splits * 64 + lane) * FLOATS;      // split n, lane half: + (64 n + 32 s) FLOATS
+  const float* p = a.part + ((tile * a.halves + half) * a.splits * 64 + lane) * FLOATS;      // split n, lane half: + (64 n + 32 s) FLOATS
   const int t = threadIdx.x, wave = t >> 6;
   auto block = [&](float x, float y, bool is_max, float& ox, float& oy) {
 #pragma unroll
@@ -581,12 +652,12 @@ __global__ __launch_bounds__(256) void diff_attn_join_kernel(const DiffAttnArgs 
     }
   };
   float m1 = kNegInf, m2 = kNegInf, top[2], l[2], l1 = 0.0f, l2 = 0.0f;
-  for (int n = t; n < a.splits; n += 256) {
+  for (int n = t; n < parts; n += 256) {
     const float4 s = *reinterpret_cast<const float4*>(p + (int64_t)64 * n * FLOATS);
     m1 = fmaxf(m1, s.x); m2 = fmaxf(m2, s.z);
   }
   block(m1, m2, true, top[0], top[1]);
-  for (int n = t; n < a.splits; n += 256) {
+  for (int n = t; n < parts; n += 256) {
     const float4 s = *reinterpret_cast<const float4*>(p + (int64_t)64 * n * FLOATS);
     const float4 s2 = *reinterpret_cast<const float4*>(p + (int64_t)(64 * n + 32) * FLOATS);
     wt[0][n] = s.x == kNegInf ? 0.0f : aexp2((s.x - top[0]) * c);
@@ -600,7 +671,7 @@ __global__ __launch_bounds__(256) void diff_attn_join_kernel(const DiffAttnArgs 
   if (d < DV) {
     const float* e = p + (int64_t)(32 * ((d >> 2) & 1)) * FLOATS + 4 + (m * VO + (d >> 5)) * 16 + 4 * ((d >> 3) & 3) + (d & 3);
 #pragma unroll 8
-    for (int n = 0; n < a.splits; ++n) o = fmaf(e[(int64_t)64 * n * FLOATS], wt[m][n], o);
+    for (int n = 0; n < parts; ++n) o = fmaf(e[(int64_t)64 * n * FLOATS], wt[m][n], o);
   }
   const bool fm = a.mask_kind == 2, dead = l[m] == 0.0f;
   o *= dead ? 0.0f : a.up / l[m];
@@ -675,10 +746,6 @@ __device__ __forceinline__ void join_waves(af32x16_t* const (&acc)[NB], float* s
   }
 }
 
-__device__ __forceinline__ void put_block(float* at, const af32x16_t& v) {
-#pragma unroll
-  for (int q = 0; q < 4; ++q) *reinterpret_cast<float4*>(at + 4 * q) = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
-}
 // sum over the splits of a lane's 16 floats, in split order
 __device__ __forceinline__ af32x16_t sum_block(const float* at, int splits, int64_t step) {
   af32x16_t v = {0.0f};
@@ -686,7 +753,7 @@ __device__ __forceinline__ af32x16_t sum_block(const float* at, int splits, int6
   for (int n = 0; n < splits; ++n)
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      const float4 f = *reinterpret_cast<const float4*>(at + n * step + 4 * q);
+      const float4 f = *reinterpret_cast<const float4*>(at + n * step + 256 * q);
       v[4 * q] += f.x; v[4 * q + 1] += f.y; v[4 * q + 2] += f.z; v[4 * q + 3] += f.w;
     }
   return v;
@@ -728,11 +795,14 @@ __global__ __launch_bounds__((AttnPlan<T, DH, DV, SHARED>::NT), (AttnPlan<T, DH,
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int id = xcd_tile(a);
   if (id >= a.work) return;
-  const int tile = id / a.splits, split = id - tile * a.splits;
+  const int2 cut = tile_split(a, id);
+  const int tile = cut.x, split = cut.y;
   RowWave w;
-  w.init<P::WQ, P::WK, MODE == kAttnAny>(a, tile);
-  constexpr bool MASK = MODE == kAttnAny;
-  const bool fm = MASK && a.mask_kind == 2, drop = MODE != kAttnPlain && a.t16 != 0;
+  w.init<P::WQ, P::WK, (MODE >= kAttnCausal)>(a, tile);
+  const int tn = (w.kend + P::N - 1) / P::N, t0 = split * a.chunk;
+  if (split > 0 && t0 >= tn) return;
+  constexpr bool MASK = MODE >= kAttnCausal;
+  const bool fm = MODE == kAttnAny && a.mask_kind == 2, drop = (MODE == kAttnDrop || MODE == kAttnAny) && a.t16 != 0;
   OwnRow<T, S::KB, S::KEEP> qf[2];
   OwnRow<T, S::VB, S::KEEP> gf;
 #pragma unroll
@@ -763,13 +833,12 @@ __global__ __launch_bounds__((AttnPlan<T, DH, DV, SHARED>::NT), (AttnPlan<T, DH,
   for (int m = 0; m < 2; ++m)
 #pragma unroll
     for (int d = 0; d < S::KO; ++d) acc[m][d] = af32x16_t{0.0f};
-  const int tn = (w.kend + P::N - 1) / P::N, per = (tn + a.splits - 1) / a.splits;
-  key_tiles<T, DH, DV, SHARED>(a, w, 0, split * per, min(tn, (split + 1) * per), smem, [&](const char* kt, int it0, uint32_t hid, int j0) {
+  key_tiles<T, DH, DV, SHARED>(a, w, 0, t0, min(tn, t0 + a.chunk), smem, [&](const char* kt, int it0, uint32_t hid, int j0) {
     af32x16_t x[2];
 #pragma unroll
     for (int m = 0; m < 2; ++m) x[m] = tile_dot<T, S::KB, S::LX, S::KEEP>(kt, it0, m * S::LX / 2, qf[m], w.lane);
     af32x16_t g = tile_dot<T, S::VB, S::LY, S::KEEP>(kt + S::xbytes(P::N), it0, 0, gf, w.lane);
-    if (hid != 0 || (MASK && (a.causal || a.mask_kind != 0))) mask_tile<MASK>(a, x, hid, w.b, w.h, w.i, j0, rscale, w.lane);
+    if (hid != 0 || MASK) mask_tile<MODE>(a, x, hid, w.b, w.h, w.i, j0, rscale, w.lane);
     if (drop) {
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
@@ -812,11 +881,11 @@ __global__ __launch_bounds__((AttnPlan<T, DH, DV, SHARED>::NT), (AttnPlan<T, DH,
     dl = dlv[0];
   }
   if (!w.ok) return;
-  if (a.splits > 1) {
-    float* at = a.part + ((int64_t)id * 64 + w.lane) * S::QFLOATS;
+  if (tn > a.chunk) {
+    float* at = a.part + (w.tile32(a) * a.splits + split) * 64 * S::QFLOATS + w.lane * 4;
 #pragma unroll
-    for (int n = 0; n < 2 * S::KO; ++n) put_block(at + 16 * n, acc[n / S::KO][n % S::KO]);
-    at[32 * S::KO] = dl;
+    for (int n = 0; n < 2 * S::KO; ++n) put_block(at + 1024 * n, acc[n / S::KO][n % S::KO], 256);
+    at[2048 * S::KO] = dl;
     return;
   }
   dl = half_sum(dl);
@@ -864,15 +933,16 @@ __global__ __launch_bounds__((AttnPlan<T, DH, DV, SHARED>::NT), (AttnPlan<T, DH,
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, wq = wave / P::WK, wk = wave % P::WK;
   const int id = xcd_tile(a);
   if (id >= a.work) return;
-  const int tile = id / a.splits, split = id - tile * a.splits;
+  const int2 cut = tile_split(a, id);
+  const int tile = cut.x, split = cut.y;
   const int tiles = (a.Nk + 32 * P::WQ - 1) / (32 * P::WQ), bh = tile / tiles, jb = (tile - bh * tiles) * 32 * P::WQ;
   const int b = bh / a.Hk, hk = bh - b * a.Hk;
   const int j = jb + 32 * wq + (lane & 31);
   // a hidden key's column is computed from zeros and its gradients are stored as zeros: no masking needed for it
   const bool in = j < a.Nk, ok = in && !(a.kpm != nullptr && a.kpm[(int64_t)b * a.Nk + (in ? j : 0)]);
   const int jc = in ? j : a.Nk - 1, off = a.Nk - a.Nq;
-  constexpr bool MASK = MODE == kAttnAny;
-  const bool fm = MASK && a.mask_kind == 2, drop = MODE != kAttnPlain && a.t16 != 0;
+  constexpr bool MASK = MODE >= kAttnCausal;
+  const bool fm = MODE == kAttnAny && a.mask_kind == 2, drop = (MODE == kAttnDrop || MODE == kAttnAny) && a.t16 != 0;
 
   OwnRow<T, S::KB, S::KEEP> kf[2];
   OwnRow<T, S::VB, S::KEEP> vf;
@@ -891,7 +961,8 @@ __global__ __launch_bounds__((AttnPlan<T, DH, DV, SHARED>::NT), (AttnPlan<T, DH,
 
   // tiles of a head from the first whose rows may see a key of the block
   const int first = MASK && a.causal ? max(0, jb - off) / N : 0, per = max(0, (a.Nq + N - 1) / N - first);
-  const int all = per * a.G, share = (all + a.splits - 1) / a.splits, begin = split * share, total = min(all, begin + share);
+  const int all = per * a.G, begin = split * a.chunk, total = min(all, begin + a.chunk);
+  if (split > 0 && begin >= all) return;
   const int st = SHARED ? threadIdx.x : lane;
   AttnStage<T, DH, DV, N, P::LT, P::PREF> sg;
   const uint32_t xrow = (uint32_t)(a.qs[1] * elem<T>::kBytes), yrow = (uint32_t)(a.gs[1] * elem<T>::kBytes);
@@ -954,7 +1025,7 @@ __global__ __launch_bounds__((AttnPlan<T, DH, DV, SHARED>::NT), (AttnPlan<T, DH,
             if (8 * (e >> 2) + (e & 3) < lim) { x[0][e] = kNegInf; x[1][e] = kNegInf; }
         }
       }
-      if (MASK && a.mask_kind != 0) {
+      if (MODE == kAttnAny && a.mask_kind != 0) {
         const int64_t o = b * a.ms[0] + h * a.ms[1] + jc * a.ms[3];
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
@@ -1028,10 +1099,10 @@ __global__ __launch_bounds__((AttnPlan<T, DH, DV, SHARED>::NT), (AttnPlan<T, DH,
   if (!in) return;
   // (a hidden key's columns may hold anything: stored as zeros)
   constexpr int N0 = PART == 2 ? 2 * S::KO : 0, N1 = PART == 1 ? 2 * S::KO : 2 * S::KO + S::VO;
-  if (a.splits > 1) {
-    float* at = a.part + ((int64_t)id * 64 + lane) * S::KFLOATS;
+  if (all > a.chunk) {
+    float* at = a.part + ((((int64_t)bh * ((a.Nk + 31) / 32) + jb / 32 + wq) * a.splits + split) * 64) * S::KFLOATS + lane * 4;
 #pragma unroll
-    for (int n = N0; n < N1; ++n) put_block(at + 16 * n, n < 2 * S::KO ? ak[n / S::KO % 2][n % S::KO] : av[(n - 2 * S::KO) % S::VO]);
+    for (int n = N0; n < N1; ++n) put_block(at + 1024 * n, n < 2 * S::KO ? ak[n / S::KO % 2][n % S::KO] : av[(n - 2 * S::KO) % S::VO], 256);
     return;
   }
 #pragma unroll
@@ -1046,16 +1117,17 @@ __global__ __launch_bounds__(64) void diff_attn_join_q_kernel(const DiffAttnArgs
   RowWave w;
   const int tile = blockIdx.x / (2 * S::KO), n = blockIdx.x - tile * 2 * S::KO;
   w.init<1, 1, true>(a, tile);
-  if (!w.ok) return;
+  const int parts = ((rows_end(a, w.rb / a.own * a.own, a.own) + a.n - 1) / a.n + a.chunk - 1) / a.chunk;
+  if (!w.ok || parts <= 1) return;
   const int64_t step = 64 * S::QFLOATS;
-  const float* at = a.part + ((int64_t)tile * a.splits * 64 + w.lane) * S::QFLOATS;
+  const float* at = a.part + w.tile32(a) * a.splits * 64 * S::QFLOATS + w.lane * 4;
   if (n == 0) {
     float dl = 0.0f;
-    for (int p = 0; p < a.splits; ++p) dl += at[p * step + 32 * S::KO];
+    for (int p = 0; p < parts; ++p) dl += at[p * step + 2048 * S::KO];
     dl = half_sum(dl);
     if (w.lane < 32) a.dlrow[w.rowid] = -dl;
   }
-  if (a.gq != nullptr) store_gq<T, S::KO>(a, w, n, sum_block(at + 16 * n, a.splits, step));
+  if (a.gq != nullptr) store_gq<T, S::KO>(a, w, n, sum_block(at + 1024 * n, parts, step));
 }
 template <typename T, int DH, int DV>
 __global__ __launch_bounds__(64) void diff_attn_join_kv_kernel(const DiffAttnArgs a) {
@@ -1063,10 +1135,12 @@ __global__ __launch_bounds__(64) void diff_attn_join_kv_kernel(const DiffAttnArg
   constexpr int NB = 2 * S::KO + S::VO;
   const int tile = blockIdx.x / NB, n = blockIdx.x - tile * NB, lane = threadIdx.x;
   const int tiles = (a.Nk + 31) / 32, bh = tile / tiles, j = (tile - bh * tiles) * 32 + (lane & 31), b = bh / a.Hk, hk = bh - b * a.Hk;
-  if (j >= a.Nk) return;
+  const int jb = (tile - bh * tiles) * 32 / a.own * a.own, first = a.causal ? max(0, jb - (a.Nk - a.Nq)) / a.n : 0;
+  const int parts = (max(0, (a.Nq + a.n - 1) / a.n - first) * a.G + a.chunk - 1) / a.chunk;
+  if (j >= a.Nk || parts <= 1) return;
   const bool ok = !(a.kpm != nullptr && a.kpm[(int64_t)b * a.Nk + j]);
-  const float* at = a.part + ((int64_t)tile * a.splits * 64 + lane) * S::KFLOATS;
-  store_gkv<T, S::KO>(a, b, hk, j, ok, n, sum_block(at + 16 * n, a.splits, 64 * S::KFLOATS), lane);
+  const float* at = a.part + (int64_t)tile * a.splits * 64 * S::KFLOATS + lane * 4;
+  store_gkv<T, S::KO>(a, b, hk, j, ok, n, sum_block(at + 1024 * n, parts, 64 * S::KFLOATS), lane);
 }
 
 // ---- launch -----------------------------------------------------------------------------------------------------------------------
@@ -1083,47 +1157,52 @@ static int attn_launch(K kernel, int64_t blocks, int threads, int lds, const Dif
 }
 
 template <typename F> static int attn_mode(const DiffAttnArgs& a, F&& f) {
-  if (a.causal || a.mask_kind != 0) return f(std::integral_constant<int, kAttnAny>{});
+  if (a.mask_kind != 0 || (a.causal && a.t16 != 0)) return f(std::integral_constant<int, kAttnAny>{});
+  if (a.causal) return f(std::integral_constant<int, kAttnCausal>{});
   if (a.t16 != 0) return f(std::integral_constant<int, kAttnDrop>{});
   return f(std::integral_constant<int, kAttnPlain>{});
 }
 
 // How a pass over `own` items a head against `staged` ones is cut into blocks.
 //
-// shared: a shared block does four private blocks' work in `cost` times their time (it stages a tile once for 128 own items), but
-// there are a quarter as many: with 256 CUs the rounds of blocks decide; causal blocks are unequal, the longest twice the mean.
-// Measured at one block a CU (bf16, us, shared / private): 64 / 64 wide heads 80 / 121, 128 / 128 133 / 278; 32 / 64 at 10 000 x
-// 10 000 and 4 heads (316 or 1252 blocks) 400 / 299.
-// splits: private blocks that share the staged items of one own tile, where own tiles alone leave the chip empty: up to twice as
-// many waves as fill it (ragged batches and causal rows are unequal), at least four tiles for each wave.
-struct AttnCut { bool shared; int splits; };
-template <typename T, int DH, int DV> static AttnCut attn_cut(const DiffAttnArgs& a, int64_t heads, int64_t own, int64_t staged, bool may_share) {
+// shared: a shared block does four private blocks' work in 4 `cost` times their time (it stages a tile once for 128 own items), but
+// there are a quarter as many: with 256 CUs the rounds of blocks decide.  Measured at one block a CU (bf16, us, shared / private):
+// 64 / 64 wide heads 80 / 121, 128 / 128 133 / 278; 32 / 64 at 10 000 x 10 000 and 4 heads (316 or 1252 blocks) 400 / 299.
+// splits: private blocks that share the staged items of one own tile, `chunk` staged tiles each, where own tiles alone leave the chip
+// empty: up to twice as many waves as fill it (ragged batches and causal rows are unequal), at least four tiles for each wave.
+// (Shared blocks that split a causal own tile into equal chunks fill the chip too, but lose to it what joining them costs: 64 / 128
+// wide f16 heads, 2 x 2 shared by four each, 2047 causal, us: forward 109 + 14, private 125; grad_q 135 + 8, 126; grad_k / grad_v
+// 182 + 8, 148 + 5.)
+struct AttnCut {
+  bool shared;
+  int splits, chunk;
+  AttnCut whole() const { return {shared, 1, 1 << 29}; }
+};
+// staged: items that an own tile meets at most, in `heads` heads with ends of their own
+template <typename T, int DH, int DV>
+static AttnCut attn_cut(const DiffAttnArgs& a, int64_t groups, int64_t own, int64_t staged, int heads, bool may_share) {
   using S = AttnTile<T, DH, DV>;
-  const int64_t wide = heads * ((own + 127) / 128), narrow = heads * ((own + 31) / 32);
-  const double cost = DH <= 32 ? 0.8 : 0.65, uneven = a.causal ? 2.0 : 1.0;
-  double ts = 4.0 * cost * (double)((wide + 255) / 256), tp = (double)((narrow + 255) / 256);
-  if (a.causal) {
-    ts = fmax(4.0 * cost, 4.0 * cost * wide / 512.0);
-    tp = fmax(1.0, narrow / 512.0);
-  }
-  if (may_share && ts < tp) return {true, 1};
-  const int64_t waves = narrow * S::WK, fill = 1024 * S::MINW * 2;
-  const int64_t each = (staged + 31) / 32 / S::WK / 4;
-  int64_t splits = waves * 2 >= fill && uneven == 1.0 ? 1 : (fill + waves - 1) / waves;
-  splits = splits < each ? splits : each;
-  splits = splits < kAttnSplits ? splits : kAttnSplits;
-  return {false, (int)(splits > 1 ? splits : 1)};
+  const int64_t wide = groups * ((own + 127) / 128), narrow = groups * ((own + 31) / 32);
+  const double cost = 4.0 * (DH <= 32 ? 0.8 : 0.65);
+  const double ts = a.causal ? std::max(cost, cost * wide / 512.0) : cost * ((wide + 255) / 256);
+  const double tp = a.causal ? std::max(1.0, narrow / 512.0) : (double)((narrow + 255) / 256);
+  if (may_share && ts < tp) return AttnCut{true}.whole();
+  const int64_t tiles = (staged + 31) / 32 * heads, waves = narrow * S::WK, fill = 1024 * S::MINW * 2;
+  int64_t splits = waves * 2 >= fill && !a.causal ? 1 : (fill + waves - 1) / waves;
+  splits = std::min<int64_t>({splits, tiles / S::WK / 4, kAttnSplits});
+  if (splits <= 1) return AttnCut{false}.whole();
+  return {false, (int)splits, (int)((tiles + splits - 1) / splits)};
 }
 template <typename T, int DH, int DV> static AttnCut attn_cut_fwd(const DiffAttnArgs& a) {
-  return attn_cut<T, DH, (DV > 128 ? 128 : DV)>(a, (int64_t)a.B * a.Hk * (a.Dv > 128 ? 2 : 1), a.R, a.Nk, true);
+  return attn_cut<T, DH, (DV > 128 ? 128 : DV)>(a, (int64_t)a.B * a.Hk * (a.Dv > 128 ? 2 : 1), a.R, a.Nk, 1, true);
 }
 template <typename T, int DH, int DV> static AttnCut attn_cut_q(const DiffAttnArgs& a) {
-  return attn_cut<T, DH, DV>(a, (int64_t)a.B * a.Hk, a.R, a.Nk, true);
+  return attn_cut<T, DH, DV>(a, (int64_t)a.B * a.Hk, a.R, a.Nk, 1, true);
 }
 // (128 / 128 in one pass spills as a shared block: 357 us, private 277)
 template <int DH, int DV> constexpr bool kAttnKvPrivate = DH == 128 && DV == 128;
 template <typename T, int DH, int DV> static AttnCut attn_cut_kv(const DiffAttnArgs& a) {
-  return attn_cut<T, DH, DV>(a, (int64_t)a.B * a.Hk, a.Nk, (int64_t)a.G * ((a.Nq + 31) / 32) * 32, !kAttnKvPrivate<DH, DV>);
+  return attn_cut<T, DH, DV>(a, (int64_t)a.B * a.Hk, a.Nk, a.Nq, a.G, !kAttnKvPrivate<DH, DV>);
 }
 
 // bytes of the splits' sums
@@ -1148,22 +1227,24 @@ static int attn_forward(DiffAttnArgs a, void* ws, int64_t ws_bytes, hipStream_t 
   const int64_t heads = (int64_t)a.B * a.Hk;
   const char* who = "diff_attention_forward";
   AttnCut cut = attn_cut_fwd<T, DH, DV>(a);
-  if (ws_bytes < attn_bytes_fwd<T, DH, DV>(a)) cut.splits = 1;
-  a.splits = cut.splits;
+  if (ws_bytes < attn_bytes_fwd<T, DH, DV>(a)) cut = cut.whole();
+  a.splits = cut.splits; a.chunk = cut.chunk;
   a.part = (float*)ws;
   a.halves = (a.Dv + DC - 1) / DC;
   auto run = [&](auto shared) {
     constexpr bool SH = decltype(shared)::value;
     using P = AttnPlan<T, DH, DC, SH>;
+    a.own = 32 * P::WQ; a.n = P::N;
     return attn_mode(a, [&](auto mode) {
       return attn_launch(diff_attn_fwd_kernel<T, DH, DC, SH, decltype(mode)::value>,
                          heads * ((a.R + 32 * P::WQ - 1) / (32 * P::WQ)) * a.halves * a.splits, P::NT, P::lds(FwdState<T, DC>::FLOATS), a, st, who);
     });
   };
-  if (cut.shared) return run(std::true_type{});
-  const int rc = run(std::false_type{});
+  const int rc = cut.shared ? run(std::true_type{}) : run(std::false_type{});
   if (rc != UBV_OK || a.splits == 1) return rc;
-  hipLaunchKernelGGL((diff_attn_join_kernel<T, DC>), dim3((unsigned)(heads * a.R * a.halves)), dim3(256), 0, st, a);
+  if (a.R < 32) hipLaunchKernelGGL((diff_attn_join_kernel<T, DC>), dim3((unsigned)(heads * a.R * a.halves)), dim3(256), 0, st, a);
+  else
+    hipLaunchKernelGGL((diff_attn_join_rows_kernel<T, DC>), dim3((unsigned)(heads * ((a.R + 31) / 32) * a.halves * (DC / 32))), dim3(64), 0, st, a);
   UBV_CHECK_LAUNCH(who);
   return UBV_OK;
 }
@@ -1178,6 +1259,7 @@ static int attn_backward(DiffAttnArgs a, float* glam, int64_t part_bytes, hipStr
     constexpr bool SH = decltype(shared)::value;
     constexpr int PASS = decltype(pass)::value;                 // 0 .. 2: grad_k / grad_v of that part, 3: grad_q
     using P = AttnPlan<T, DH, DV, SH>;
+    a.own = 32 * P::WQ; a.n = P::N;
     const int64_t blocks = heads * (((PASS == 3 ? a.R : a.Nk) + 32 * P::WQ - 1) / (32 * P::WQ)) * a.splits;
     return attn_mode(a, [&](auto mode) {
       constexpr int MODE = decltype(mode)::value;
@@ -1187,8 +1269,9 @@ static int attn_backward(DiffAttnArgs a, float* glam, int64_t part_bytes, hipStr
         return attn_launch(diff_attn_bwd_kv_kernel<T, DH, DV, SH, MODE, PASS>, blocks, P::NT, P::lds((2 * S::KO + S::VO) * 16), a, st, who);
     });
   };
-  auto pass = [&](const AttnCut& cut, auto which) {
-    a.splits = room ? cut.splits : 1;
+  auto pass = [&](AttnCut cut, auto which) {
+    if (!room) cut = cut.whole();
+    a.splits = cut.splits; a.chunk = cut.chunk;
     if constexpr (decltype(which)::value == 3 || !kAttnKvPrivate<DH, DV>)
       if (cut.shared) return run(std::true_type{}, which);
     return run(std::false_type{}, which);
