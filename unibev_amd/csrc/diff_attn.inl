@@ -479,7 +479,7 @@ __device__ __forceinline__ void fwd_finish(const DiffAttnArgs& a, const FwdState
 // One pass over the keys with a running reference and sum for each map.  Per pair and map: Dh + Dv multiply-adds on the matrix cores
 // against one exponential (a quarter of the VALU's rate), a fma, a maximum, an addition and a rounding: at 32 / 64 wide heads
 // the VALU is what bounds it (its issue and the matrix cores' add up to ~80 % of the time).  4 heads of 32 / 64, 10 000 x 10 000
-// bf16: 305 us (503 TFLOP/s); 2 x 8 heads of 64 / 128, 4096 x 4096: 400 us (515 TFLOP/s); one query, 8 x 4 heads of 32 / 64,
+// bf16: 310 us (495 TFLOP/s); 2 x 8 heads of 64 / 128, 4096 x 4096: 400 us (515 TFLOP/s); one query, 8 x 4 heads of 32 / 64,
 // 40 000 keys ragged: 54 us (4.7 TB/s, bound by memory).
 template <typename T, int DH, int DV, bool SHARED, int MODE>
 __global__ __launch_bounds__((AttnPlan<T, DH, DV, SHARED>::NT), (AttnPlan<T, DH, DV, SHARED>::MINW)) void diff_attn_fwd_kernel(
@@ -792,7 +792,7 @@ __device__ __forceinline__ void store_gkv(const DiffAttnArgs& a, int b, int hk, 
 
 // ---- backward: grad_q and the rows' parts of grad_lam; own = rows, staged = keys -----------------------------------------------
 // dq_m = scale sum_j dS_m k_m,  dS_1 = A_1 o (G - del_1),  dS_2 = -lam A_2 o (G - del_2),  G = D o (grad_out v^T);  A from the row's
-// statistics.  Bound as the forward pass: 10 000 x 10 000, 4 heads of 32 / 64 bf16 325 us (473 TFLOP/s, the scores computed again).
+// statistics.  Bound as the forward pass: 10 000 x 10 000, 4 heads of 32 / 64 bf16 329 us (467 TFLOP/s, the scores computed again).
 template <typename T, int DH, int DV, bool SHARED, int MODE>
 __global__ __launch_bounds__((AttnPlan<T, DH, DV, SHARED>::NT), (AttnPlan<T, DH, DV, SHARED>::MINW)) void diff_attn_bwd_q_kernel(
     const DiffAttnArgs a) {
@@ -927,8 +927,8 @@ __global__ __launch_bounds__(1024) static void diff_attn_lam_kernel(const float*
 
 // ---- backward: grad_k and grad_v; own = keys, staged = the rows of every head that shares them ----------------------------------
 // A tile of rows stays inside one head (its rows are one stretch of queries), heads one after the other.
-// dk_m = scale sum_i dS_m q_m,  dv = sum_i (D o (A_1 - lam A_2)) grad_out.  10 000 x 10 000, 4 heads of 32 / 64 bf16: 465 us (440
-// TFLOP/s); VALU and LDS reads (the rows' statistics, 4 floats each) bound it.
+// dk_m = scale sum_i dS_m q_m,  dv = sum_i (D o (A_1 - lam A_2)) grad_out.  10 000 x 10 000, 4 heads of 32 / 64 bf16: 510 us (400
+// TFLOP/s; the same loop with 242 registers instead of 250 took 470); VALU and LDS reads (the rows' statistics, 4 floats each) bound it.
 // PART 0: both gradients in one pass; 1: grad_k, 2: grad_v by a pass of its own, where the accumulators of both (2 DH + DV
 // floats a lane's item pair) would not fit the register file (the scores are computed twice: less than spilling costs).
 template <typename T, int DH, int DV, bool SHARED, int MODE, int PART>
