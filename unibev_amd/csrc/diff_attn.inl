@@ -927,8 +927,8 @@ __global__ __launch_bounds__(1024) static void diff_attn_lam_kernel(const float*
 
 // ---- backward: grad_k and grad_v; own = keys, staged = the rows of every head that shares them ----------------------------------
 // A tile of rows stays inside one head (its rows are one stretch of queries), heads one after the other.
-// dk_m = scale sum_i dS_m q_m,  dv = sum_i (D o (A_1 - lam A_2)) grad_out.  10 000 x 10 000, 4 heads of 32 / 64 bf16: 510 us (400
-// TFLOP/s; the same loop with 242 registers instead of 250 took 470); VALU and LDS reads (the rows' statistics, 4 floats each) bound it.
+// dk_m = scale sum_i dS_m q_m,  dv = sum_i (D o (A_1 - lam A_2)) grad_out.  10 000 x 10 000, 4 heads of 32 / 64 bf16: 470 to 515 us
+// by card (400 TFLOP/s and more); VALU and LDS reads (the rows' statistics, 4 floats each) bound it.
 // PART 0: both gradients in one pass; 1: grad_k, 2: grad_v by a pass of its own, where the accumulators of both (2 DH + DV
 // floats a lane's item pair) would not fit the register file (the scores are computed twice: less than spilling costs).
 template <typename T, int DH, int DV, bool SHARED, int MODE, int PART>
