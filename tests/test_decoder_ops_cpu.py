@@ -99,3 +99,54 @@ def test_module_builds_from_the_registry():
     for bad in (dict(num_heads=3), dict(num_heads=64), dict(num_heads=4, num_kv_heads=3)):
         with pytest.raises(ValueError):
             build_attention(dict(type='DifferentialAttention', embed_dims=64, **bad))
+
+
+def decoder_calls():
+    """name -> call with one operand replaced"""
+    from unibev_amd import functional as UF
+    x, w = torch.randn(2, 3, 2, 16), torch.ones(16)
+    q, v, lam, mask = torch.randn(1, 3, 2, 2, 8), torch.randn(1, 3, 2, 16), torch.ones(2), torch.zeros(3, 3)
+    return {'dropout x': (x, lambda t: UF.dropout(t, 0.1, True)), 'dropout identity': (x, lambda t: UF.dropout(x, 0.1, True, identity=t)),
+            'norm x': (x, lambda t: UF.layer_norm(t, w, w)), 'norm gamma': (w, lambda t: UF.layer_norm(x, t, w)),
+            'norm beta': (w, lambda t: UF.layer_norm(x, w, t)), 'attention q': (q, lambda t: UF.diff_attention(t, q, v, lam)),
+            'attention k': (q, lambda t: UF.diff_attention(q, t, v, lam)), 'attention v': (v, lambda t: UF.diff_attention(q, q, t, lam)),
+            'attention lam': (lam, lambda t: UF.diff_attention(q, q, v, t)),
+            'attention mask': (mask, lambda t: UF.diff_attention(q, q, v, lam, attn_mask=t))}
+
+
+@pytest.mark.parametrize('name', list(decoder_calls()))
+def test_forward_mode_derivatives_are_refused(name):
+    import torch.autograd.forward_ad as forward_ad
+    t, call = decoder_calls()[name]
+    with forward_ad.dual_level():
+        with pytest.raises(RuntimeError, match='forward-mode'):
+            call(forward_ad.make_dual(t, torch.ones_like(t)))
+    with pytest.raises(RuntimeError, match='forward-mode|ordinary tensors'):
+        torch.autograd.functional.jacobian(call, t, strategy='forward-mode', vectorize=True)
+
+
+@pytest.mark.parametrize('name', list(decoder_calls()))
+def test_tracing_is_refused(name):
+    t, call = decoder_calls()[name]
+    with pytest.raises(RuntimeError, match='trace'):
+        torch.jit.trace(call, (t,))
+    from torch._subclasses import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+    for mode in ('real', 'fake'):
+        with pytest.raises(RuntimeError, match='trace'):
+            make_fx(call, tracing_mode=mode)(t)
+    with FakeTensorMode() as fake, pytest.raises(RuntimeError, match='trace'):
+        call(fake.from_tensor(t))
+
+
+@pytest.mark.parametrize('name', list(decoder_calls()))
+def test_transformed_tensors_are_refused(name):
+    t, call = decoder_calls()[name]
+    with pytest.raises(RuntimeError, match='ordinary tensors'):
+        torch.vmap(call)(torch.stack([t, t]))
+    with pytest.raises(RuntimeError, match='ordinary tensors'):
+        torch.func.grad(lambda t: call(t).sum())(t)
+    with pytest.raises(RuntimeError, match='ordinary tensors'):
+        torch.func.jvp(call, (t,), (torch.ones_like(t),))
+    with pytest.raises(RuntimeError, match='ordinary tensors'):
+        call(t.to_sparse())

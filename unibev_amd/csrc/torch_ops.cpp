@@ -5,9 +5,11 @@
 // libunibev_hip.so (bind), so that this module follows whichever build of the library the process has loaded.
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 
 #include "unibev_hip.h"
 
@@ -62,6 +64,23 @@ template <typename F, typename... A> void launch(const char* name, F f, A... a) 
   }
   const int rc = f(a...);
   if (rc != 0) throw HipError(std::string(name + 4) + " failed (status " + std::to_string(rc) + "): " + api.ubv_last_error());
+}
+
+// The bodies run below autograd on the tensors' memory and hang their node on the result by hand: what else would follow an
+// operation from its inputs to its result is refused (a forward-mode tangent or a trace would lose it without a word).
+void plain(const char* who, std::initializer_list<const Tensor*> ts) {
+  using Modes = c10::impl::TorchDispatchModeTLS;
+  if (torch::jit::tracer::isTracing() || Modes::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value() ||
+      Modes::get_mode(c10::impl::TorchDispatchModeKey::FAKE).has_value())
+    throw std::runtime_error(std::string(who) + ": a trace cannot record this operator");
+  const c10::DispatchKeySet wrapped = c10::python_ks | c10::DispatchKeySet({c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::FuncTorchGradWrapper,
+                                                                            c10::DispatchKey::Batched, c10::DispatchKey::Functionalize});
+  for (const Tensor* t : ts) {
+    if (!t->defined()) continue;
+    if (t->layout() != at::kStrided || !t->has_storage() || t->key_set().has_any(wrapped))
+      throw std::runtime_error(std::string(who) + ": takes ordinary tensors with memory (no sparse, batched or otherwise wrapped ones)");
+    if (t->_fw_grad(/*level=*/0).defined()) throw std::runtime_error(std::string(who) + ": has no forward-mode derivative");
+  }
 }
 
 // every given tensor on ONE GPU
@@ -151,6 +170,7 @@ struct DropoutBackward : Node {
   variable_list apply(variable_list&& g) override {
     variable_list out(2);
     if (!g[0].defined()) return out;
+    plain("dropout's gradient", {&g[0]});
     if (task_should_compute_output(0)) out[0] = dropout_raw(g[0], Tensor(), x_type, drop);
     if (task_should_compute_output(1)) out[1] = g[0];
     return once("dropout", std::move(out));
@@ -159,6 +179,7 @@ struct DropoutBackward : Node {
 
 Tensor dropout(const Tensor& x, double p, const OptTensor& identity_, uint64_t seed, const OptTensor& base) {
   const Tensor identity = given(identity_);
+  plain("dropout", {&x, &identity});
   one_gpu({&x, &identity});
   type_code(x);
   if (identity.defined()) {
@@ -194,6 +215,7 @@ struct LayerNormBackward : Node {
   variable_list apply(variable_list&& g) override {
     variable_list out(3);
     if (!g[0].defined()) return out;
+    plain("layer_norm's gradient", {&g[0]});
     const Tensor x = x_.unpack(), gamma = has_gamma ? gamma_.unpack() : Tensor();
     const bool nx = task_should_compute_output(0), ng = task_should_compute_output(1), nb = task_should_compute_output(2);
     const int64_t C = x.size(-1), R = x.numel() / C;
@@ -223,6 +245,7 @@ struct LayerNormBackward : Node {
 
 Tensor layer_norm(const Tensor& x, const OptTensor& gamma_, const OptTensor& beta_, double eps) {
   const Tensor gamma = given(gamma_), beta = given(beta_);
+  plain("layer_norm", {&x, &gamma, &beta});
   const c10::Device dev = one_gpu({&x, &gamma, &beta});
   const int dt = type_code(x);
   if (x.dim() < 1 || x.size(-1) < 1) throw py::value_error("layer_norm: x " + shape(x) + " has no last axis to normalise");
@@ -307,6 +330,7 @@ struct DiffAttentionBackward : Node {
   variable_list apply(variable_list&& g) override {
     variable_list out(4);
     if (!g[0].defined()) return out;
+    plain("diff_attention's gradient", {&g[0]});
     const Tensor q = q_.unpack(), k = k_.unpack(), v = v_.unpack(), lam = lam_.unpack();
     if (a.mask.defined()) mask_.unpack();
     if (a.padding.defined()) padding_.unpack();
@@ -349,6 +373,7 @@ Tensor diff_attention(const Tensor& q, const Tensor& k, const Tensor& v, const T
                       const OptTensor& key_padding_mask, bool causal, std::optional<double> scale, double p, uint64_t seed,
                       const OptTensor& base) {
   const Tensor mask_in = given(attn_mask), padding = given(key_padding_mask);
+  plain("diff_attention", {&q, &k, &v, &lam_in, &mask_in, &padding});
   const c10::Device dev = one_gpu({&q, &k, &v, &lam_in, &mask_in, &padding});
   const std::string who = "diff_attention: ";
   const std::string three = "q " + shape(q) + ", k " + shape(k) + ", v " + shape(v);
