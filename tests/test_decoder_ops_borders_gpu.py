@@ -54,3 +54,23 @@ def test_tracing_and_batched_gradients_are_refused(op):
     y = operators(x, lam)[op]()
     with pytest.raises(RuntimeError, match='ordinary tensors'):
         torch.autograd.grad(y, x, torch.ones(3, *y.shape, device=DEV), is_grads_batched=True)
+
+
+# ----------------------------------------------------------------------------------------------------- layouts that are copied
+@pytest.mark.parametrize('Dh,Dv', [(20, 20), (7, 13), (6, 42), (16, 20), (20, 32)])
+@pytest.mark.parametrize('dt', TYPES)
+def test_attention_channels_first_views_of_any_width(Dh, Dv, dt):
+    """operands and grad_out whose tokens are the fastest axis, at widths that are no whole 16-byte pieces"""
+    B, H, Hk, Nq, Nk = 2, 4, 2, 9, 33
+    q, k, v, lam, go = (t.to(DEV) for t in attn_inputs(B, H, Hk, Nq, Nk, Dh, Dv, dt))
+
+    def run(f):
+        leaves = [f(t).requires_grad_() for t in (q, k, v)] + [lam.clone().requires_grad_()]
+        y = UF().diff_attention(*leaves)
+        return [y.detach(), *torch.autograd.grad(y, leaves, f(go))]
+
+    def tokens_last(t):
+        return t.movedim(1, -1).contiguous().movedim(-1, 1)
+    assert tokens_last(v).stride(1) == 1
+    for got, want in zip(run(tokens_last), run(torch.clone)):
+        assert torch.equal(got, want)

@@ -302,7 +302,13 @@ struct Attn {
 // where it already is so (views, expanded axes), else a copy (zero-padded last axis)
 Tensor operand(const Tensor& t) {
   const int64_t size = t.element_size(), vec = 16 / size, D = t.size(-1);
-  if (D % vec) return at::constant_pad_nd(t, {0, vec - D % vec});
+  if (D % vec) {                                       // (constant_pad_nd would keep a channels-last order of t)
+    auto sizes = t.sizes().vec();
+    sizes.back() += vec - D % vec;
+    Tensor p = at::zeros(sizes, t.options());
+    p.narrow(-1, 0, D).copy_(t);
+    return p;
+  }
   bool fits = (t.stride(-1) == 1 || D == 1) && reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0;
   for (int64_t i = 0; i + 1 < t.dim(); ++i) fits = fits && (t.size(i) <= 1 || t.stride(i) % vec == 0);
   fits = fits && (t.size(1) <= 1 || t.stride(1) * size < (1 << 24)) && (t.dim() < 5 || t.stride(3) * size < (1 << 28));
