@@ -74,3 +74,45 @@ def test_attention_channels_first_views_of_any_width(Dh, Dv, dt):
     assert tokens_last(v).stride(1) == 1
     for got, want in zip(run(tokens_last), run(torch.clone)):
         assert torch.equal(got, want)
+
+
+# ------------------------------------------------------------------------------------------------------ lambdas of any size
+@pytest.mark.parametrize('Dh,Dv,size', [(16, 32, 0.01), (32, 64, 0.01), (16, 256, 2.0)])
+def test_attention_f16_lam_beyond_the_types_range(Dh, Dv, size):
+    """|lam| past 255: (A_1 - lam A_2) 2^8 and dS_2 would leave f16's range, the gradients do not.  Both enter the products at a
+    power of two s <= 1 of their usual size, (1 + largest |lam| of the group) 2^8 s < 2^15: beside the usual bounds they may be off
+    by half of f16's smallest step, 2^-25 over s (2^8 s), times what they are multiplied with."""
+    B, H, Hk, Nq, Nk, dt = 1, 4, 2, 6, 5, torch.float16
+    q, k, v, _, go = attn_inputs(B, H, Hk, Nq, Nk, Dh, Dv, dt)
+    go = (go.float() * size).to(dt)
+    lam = torch.tensor([0.5, -300.0, 20000.0, 3.0])
+    scale = 2.0 ** -6
+    leaves = [t.to(DEV).requires_grad_() for t in (q, k, v, lam)]
+    y = UF().diff_attention(*leaves, scale=scale)
+    y.backward(go.to(DEV))
+    r = Ref(q, k, v, lam, go, dt, scale=scale)
+    assert max(t.abs().max() for t in (r.out, r.q, r.k, r.v)) < 65504
+    s = torch.tensor([2.0 ** -2, 2.0 ** -8]).double()                          # 14 - floor(log2(1 + |lam|)) - 8 of 300 and 20000
+    rows = Nq * H // Hk
+    ek = r.ek + scale * 2.0 ** -25 / s.view(1, 1, Hk, 1, 1) * rows * q.double().abs().max()
+    ev = r.ev + 2.0 ** -33 / s.view(1, 1, Hk, 1) * rows * go.double().abs().max()
+    within(y, r.out, r.e_out, 'out')
+    for t, ref, e, what in ((leaves[0], r.q, r.eq, 'grad_q'), (leaves[1], r.k, ek, 'grad_k'), (leaves[2], r.v, ev, 'grad_v'),
+                            (leaves[3], r.lam, r.e_lam, 'grad_lam')):
+        within(t.grad, ref, e, what)
+
+
+def test_attention_f16_lam_of_the_last_of_many_shared_heads():
+    """the largest |lam| of a group counts, whichever of its heads has it, where a few keys' rows are split over blocks too"""
+    B, H, Hk, Nq, Nk, Dh, Dv, dt = 1, 8, 1, 400, 5, 32, 64, torch.float16
+    q, k, v, _, go = attn_inputs(B, H, Hk, Nq, Nk, Dh, Dv, dt)
+    go = (go.float() * 0.01).to(dt)
+    lam = torch.tensor([0.5] * 7 + [-5000.0])                                  # s = 2^(14 - 12 - 8)
+    leaves = [t.to(DEV).requires_grad_() for t in (q, k, v, lam)]
+    y = UF().diff_attention(*leaves)
+    y.backward(go.to(DEV))
+    r = Ref(q, k, v, lam, go, dt)
+    rows, s = Nq * H, 2.0 ** -6
+    within(y, r.out, r.e_out, 'out')
+    within(leaves[1].grad, r.k, r.ek + Dh ** -0.5 * 2.0 ** -25 / s * rows * q.double().abs().max(), 'grad_k')
+    within(leaves[2].grad, r.v, r.ev + 2.0 ** -33 / s * rows * go.double().abs().max(), 'grad_v')

@@ -52,9 +52,31 @@ struct DiffAttnArgs {
 constexpr int kAttnSplits = 256;         // most splits of an own tile's staged items
 
 // f16 holds nothing below 2^-24 and loses bits below 2^-14, which the probabilities of a long row reach: they enter the matrix
-// instructions 2^8 larger and their products leave 2^8 smaller (|lam| up to 255 stays in range)
+// instructions 2^8 larger and their products leave 2^8 smaller.  dS enters as it is: a common factor would take from its upper
+// range, which a scaled loss uses, what it gives below.
 template <typename T> constexpr float kProbShift = std::is_same<T, f16_t>::value ? 8.0f : 0.0f;
 template <typename T> constexpr float kProbScale = std::is_same<T, f16_t>::value ? 256.0f : 1.0f;
+
+// a value that is the wave's in every lane: kept in a scalar register
+__device__ __forceinline__ float uniform(float v) { return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(v))); }
+
+// What grad_k / grad_v's pass takes lam by on top of that: f16's A_1 - lam A_2 and dS_2 would leave its range beside a |lam| past 255
+// though the gradients may not.  A power of two s with (1 + |lam|) 2^8 s below 2^15 for every query head that shares key head hk
+// (they are added in one sum); 1 up to 255 and in the other types.
+// In two steps, a load that need not be waited for at once (lam_top) and what follows from it.
+template <typename T> __device__ __forceinline__ float lam_top(const float* lam, int hk, int G, int lane) {
+  float m = 0.0f;
+  if constexpr (std::is_same<T, f16_t>::value)
+    for (int g = lane; g < G; g += 64) m = fmaxf(m, fabsf(lam[hk * G + g]));
+  return m;
+}
+template <typename T> __device__ __forceinline__ float lam_scale(float m) {
+  if constexpr (!std::is_same<T, f16_t>::value) return 1.0f;
+  if (!__any(m > 255.0f)) return 1.0f;
+#pragma unroll
+  for (int w = 32; w >= 1; w >>= 1) m = fmaxf(m, __shfl_xor(m, w, 64));
+  return uniform(ldexpf(1.0f, 6 - ilogbf(1.0f + fminf(m, 3.0e38f))));
+}
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNegInf = -__builtin_inff();

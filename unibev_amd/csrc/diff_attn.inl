@@ -780,14 +780,14 @@ __device__ __forceinline__ void store_gq(const DiffAttnArgs& a, const RowWave& w
   store_block<T>((T*)a.gq + ((((int64_t)w.b * a.Nq + w.i) * a.H + w.h) * 2 + n / KO) * a.Dh, 32 * (n % KO), a.Dh, v,
                  n < KO ? one : -a.lam[w.h] * one, w.lane);
 }
-// block n of a key's gradients: grad_k's 2 KO, then grad_v's; `ok`: a key that is seen
+// block n of a key's gradients: grad_k's 2 KO, then grad_v's; `ok`: a key that is seen; ls: lam_scale of its head
 template <typename T, int KO>
-__device__ __forceinline__ void store_gkv(const DiffAttnArgs& a, int b, int hk, int j, bool ok, int n, const af32x16_t& v, int lane) {
+__device__ __forceinline__ void store_gkv(const DiffAttnArgs& a, int b, int hk, int j, bool ok, int n, const af32x16_t& v, float ls, int lane) {
   const int64_t row = ((int64_t)b * a.Nk + j) * a.Hk + hk;
   if (n < 2 * KO)
-    store_block<T>((T*)a.gk + (row * 2 + n / KO) * a.Dh, 32 * (n % KO), a.Dh, v, ok && a.Nk > 1 ? a.scale : 0.0f, lane);
+    store_block<T>((T*)a.gk + (row * 2 + n / KO) * a.Dh, 32 * (n % KO), a.Dh, v, !ok || a.Nk <= 1 ? 0.0f : n < KO ? a.scale : a.scale / ls, lane);
   else
-    store_block<T>((T*)a.gv + row * a.Dv, 32 * (n - 2 * KO), a.Dv, v, ok ? a.up / kProbScale<T> : 0.0f, lane);
+    store_block<T>((T*)a.gv + row * a.Dv, 32 * (n - 2 * KO), a.Dv, v, ok ? a.up / (kProbScale<T> * ls) : 0.0f, lane);
 }
 
 // ---- backward: grad_q and the rows' parts of grad_lam; own = rows, staged = keys -----------------------------------------------
@@ -964,7 +964,7 @@ __global__ __launch_bounds__((AttnPlan<T, DH, DV, SHARED>::NT), (AttnPlan<T, DH,
   for (int d = 0; d < S::KO; ++d) { ak[0][d] = af32x16_t{0.0f}; ak[1][d] = af32x16_t{0.0f}; }
 #pragma unroll
   for (int d = 0; d < S::VO; ++d) av[d] = af32x16_t{0.0f};
-  const float c = a.scale * kLog2e, rscale = 1.0f / a.scale;
+  const float c = a.scale * kLog2e, rscale = 1.0f / a.scale, lt = lam_top<T>(a.lam, hk, a.G, lane);
   const uint32_t t32 = a.t16 << 16;
   const uint64_t zseed = attn_seed(a.seed, a.seed_dev) + (uint64_t)(j >> 2);
 
@@ -1007,6 +1007,7 @@ __global__ __launch_bounds__((AttnPlan<T, DH, DV, SHARED>::NT), (AttnPlan<T, DH,
     store(own);
     tile_ready<SHARED>();
   }
+  const float ls = lam_scale<T>(lt), ps = uniform(kProbScale<T> * ls);
 #pragma unroll 1
   for (int t = begin + wk; t < total; t += P::WK) {
     const bool more = t + P::WK < total;
@@ -1016,7 +1017,7 @@ __global__ __launch_bounds__((AttnPlan<T, DH, DV, SHARED>::NT), (AttnPlan<T, DH,
     const float4* rows = reinterpret_cast<const float4*>(qt + S::xybytes(N));
     const float2* rowl = reinterpret_cast<const float2*>(rows + N);
     const int g = t / per, h = hk * a.G + g, i00 = (first + t - g * per) * N;
-    const float lam = a.lam[h];
+    const float lam = a.lam[h], lams = std::is_same<T, f16_t>::value ? uniform(lam * ls) : lam;
 #pragma unroll 1
     for (int it0 = 0; it0 < N; it0 += 32) {
       const int i0 = i00 + it0;
@@ -1061,14 +1062,15 @@ __global__ __launch_bounds__((AttnPlan<T, DH, DV, SHARED>::NT), (AttnPlan<T, DH,
             const int n = 4 * q + e, k = n - 8 * s;
             const float4 rw = rows[r0 + e];
             const float2 rl = fm ? rowl[r0 + e] : make_float2(0.0f, 0.0f);
-            const float p1 = row_probability(fm, x[0][n], c, rw.x, rl.x), p2 = lam * row_probability(fm, x[1][n], c, rw.y, rl.y);
-            float gn = gm[n], pn = p1 - p2;
+            const float p1 = row_probability(fm, x[0][n], c, rw.x, rl.x), a2 = row_probability(fm, x[1][n], c, rw.y, rl.y);
+            const float p2 = lams * a2;
+            float gn = gm[n], pn = fmaf(-lam, a2, p1);
             if (drop) {
               const bool keep = attn_keep(word[e], lane & 1, t32);
               gn = keep ? gn * a.up : 0.0f;
               pn = keep ? pn : 0.0f;
             }
-            pc[k] = kProbScale<T> == 1.0f ? pn : pn * kProbScale<T>;
+            pc[k] = kProbScale<T> == 1.0f ? pn : pn * ps;
             ds[0][k] = p1 * (gn - rw.z);
             ds[1][k] = p2 * (rw.w - gn);
           }
@@ -1116,7 +1118,7 @@ __global__ __launch_bounds__((AttnPlan<T, DH, DV, SHARED>::NT), (AttnPlan<T, DH,
   }
 #pragma unroll
   for (int n = N0; n < N1; ++n)
-    store_gkv<T, S::KO>(a, b, hk, j, ok, n, n < 2 * S::KO ? ak[n / S::KO % 2][n % S::KO] : av[(n - 2 * S::KO) % S::VO], lane);
+    store_gkv<T, S::KO>(a, b, hk, j, ok, n, n < 2 * S::KO ? ak[n / S::KO % 2][n % S::KO] : av[(n - 2 * S::KO) % S::VO], ls, lane);
 }
 
 // sums of the splits' gradients: one block an own tile of 32 rows (or keys) and block of 32 columns, one wave
@@ -1146,10 +1148,11 @@ __global__ __launch_bounds__(64) void diff_attn_join_kv_kernel(const DiffAttnArg
   const int tiles = (a.Nk + 31) / 32, bh = tile / tiles, j = (tile - bh * tiles) * 32 + (lane & 31), b = bh / a.Hk, hk = bh - b * a.Hk;
   const int jb = (tile - bh * tiles) * 32 / a.own * a.own, first = a.causal ? max(0, jb - (a.Nk - a.Nq)) / a.n : 0;
   const int parts = (max(0, (a.Nq + a.n - 1) / a.n - first) * a.G + a.chunk - 1) / a.chunk;
+  const float ls = lam_scale<T>(lam_top<T>(a.lam, hk, a.G, lane));        // (by all lanes, before some leave)
   if (j >= a.Nk || parts <= 1) return;
   const bool ok = !(a.kpm != nullptr && a.kpm[(int64_t)b * a.Nk + j]);
   const float* at = a.part + (int64_t)tile * a.splits * 64 * S::KFLOATS + lane * 4;
-  store_gkv<T, S::KO>(a, b, hk, j, ok, n, sum_block(at + 1024 * n, parts, 64 * S::KFLOATS), lane);
+  store_gkv<T, S::KO>(a, b, hk, j, ok, n, sum_block(at + 1024 * n, parts, 64 * S::KFLOATS), ls, lane);
 }
 
 // ---- launch -----------------------------------------------------------------------------------------------------------------------

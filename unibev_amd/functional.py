@@ -796,7 +796,7 @@ def diff_attention(q, k, v, lam, attn_mask=None, key_padding_mask=None, causal=F
 
     ``p``, ``training``, ``seed``: dropout D on the map, as in ``dropout`` (never stored).
 
-    Sums are f32, scaled scores lie within +-2^24; probabilities and their gradients enter the matrix instructions in q's type.  f16: |lam| below 255, and
+    Sums are f32, scaled scores lie within +-2^24; probabilities and their gradients enter the matrix instructions in q's type.  f16:
     gradients scaled into f16's range, as in any f16 backward pass.  Differentiable once."""
     p, seed, base = _drop_args(p, training, seed, 'diff_attention')
     return native().diff_attention(q, k, v, lam, attn_mask, key_padding_mask, causal, scale, p, seed, base)
