@@ -116,3 +116,26 @@ def test_attention_f16_lam_of_the_last_of_many_shared_heads():
     within(y, r.out, r.e_out, 'out')
     within(leaves[1].grad, r.k, r.ek + Dh ** -0.5 * 2.0 ** -25 / s * rows * q.double().abs().max(), 'grad_k')
     within(leaves[2].grad, r.v, r.ev + 2.0 ** -33 / s * rows * go.double().abs().max(), 'grad_v')
+
+
+# ------------------------------------------------------------------------------------------------------ the device seed base
+@pytest.mark.parametrize('op', ['dropout', 'diff_attention'])
+def test_a_changed_seed_base_is_noticed(op):
+    """the backward pass draws the forward pass's mask again: not from another base"""
+    F = UF()
+    base = torch.zeros(1, dtype=torch.int64, device=DEV)
+    x = torch.randn(2, 9, 2, 2, 16, device=DEV, requires_grad=True)
+    lam = torch.ones(2, device=DEV)
+    F.set_seed_base(base)
+    try:
+        y = operators(x, lam)[op]()
+        base.add_(1)
+        with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+            y.sum().backward()
+        y = operators(x, lam, seed=3)[op]()                                    # a given seed does not look at it
+        base.add_(1)
+        y.sum().backward()
+        y = operators(x, lam)[op]()
+        torch.autograd.grad(y.sum(), x)
+    finally:
+        F.set_seed_base(None)

@@ -165,12 +165,14 @@ Tensor dropout_raw(const Tensor& x, const Tensor& identity, at::ScalarType out_t
 
 struct DropoutBackward : Node {
   Drop drop;
+  SavedVariable base_;              // (to notice that the base was changed: the mask is drawn again from it)
   at::ScalarType x_type;
   std::string name() const override { return "UbvDropoutBackward"; }
   variable_list apply(variable_list&& g) override {
     variable_list out(2);
     if (!g[0].defined()) return out;
     plain("dropout's gradient", {&g[0]});
+    if (drop.base.defined()) base_.unpack();
     if (task_should_compute_output(0)) out[0] = dropout_raw(g[0], Tensor(), x_type, drop);
     if (task_should_compute_output(1)) out[1] = g[0];
     return once("dropout", std::move(out));
@@ -179,8 +181,9 @@ struct DropoutBackward : Node {
 
 Tensor dropout(const Tensor& x, double p, const OptTensor& identity_, uint64_t seed, const OptTensor& base) {
   const Tensor identity = given(identity_);
+  Drop d{p, seed, given(base)};
   plain("dropout", {&x, &identity});
-  one_gpu({&x, &identity});
+  one_gpu({&x, &identity, &d.base});
   type_code(x);
   if (identity.defined()) {
     if (!identity.sizes().equals(x.sizes()))
@@ -189,10 +192,10 @@ Tensor dropout(const Tensor& x, double p, const OptTensor& identity_, uint64_t s
       throw py::type_error(std::string("dropout: identity of ") + c10::toString(identity.scalar_type()) + " beside x of " +
                            c10::toString(x.scalar_type()));
   }
-  Drop d{p, seed, given(base)};
   Tensor y = dropout_raw(x, identity, identity.defined() ? identity.scalar_type() : x.scalar_type(), d);
   if (wants_grad({&x, &identity})) {
     auto n = make_node<DropoutBackward>({x, identity});
+    if (d.base.defined()) n->base_ = SavedVariable(d.base, false);
     n->drop = std::move(d);
     n->x_type = x.scalar_type();
     torch::autograd::set_history(y, n);
@@ -323,7 +326,7 @@ void strides(int64_t (&s)[18], const Tensor& q, const Tensor& k, const Tensor& v
 }
 
 struct DiffAttentionBackward : Node {
-  SavedVariable q_, k_, v_, lam_, mask_, padding_;      // the caller's masks: to notice that one was changed
+  SavedVariable q_, k_, v_, lam_, mask_, padding_, base_;      // the caller's masks and seed base: to notice that one was changed
   Attn a;
   Tensor stat, maps;
   at::ScalarType lam_type = at::kFloat;
@@ -340,6 +343,7 @@ struct DiffAttentionBackward : Node {
     const Tensor q = q_.unpack(), k = k_.unpack(), v = v_.unpack(), lam = lam_.unpack();
     if (a.mask.defined()) mask_.unpack();
     if (a.padding.defined()) padding_.unpack();
+    if (a.drop.base.defined()) base_.unpack();
     const bool nq = task_should_compute_output(0), nk = task_should_compute_output(1), nv = task_should_compute_output(2),
                nl = task_should_compute_output(3);
     const c10::Device dev = q.device();
@@ -378,9 +382,9 @@ struct DiffAttentionBackward : Node {
 Tensor diff_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& lam_in, const OptTensor& attn_mask,
                       const OptTensor& key_padding_mask, bool causal, std::optional<double> scale, double p, uint64_t seed,
                       const OptTensor& base) {
-  const Tensor mask_in = given(attn_mask), padding = given(key_padding_mask);
+  const Tensor mask_in = given(attn_mask), padding = given(key_padding_mask), seed_base = given(base);
   plain("diff_attention", {&q, &k, &v, &lam_in, &mask_in, &padding});
-  const c10::Device dev = one_gpu({&q, &k, &v, &lam_in, &mask_in, &padding});
+  const c10::Device dev = one_gpu({&q, &k, &v, &lam_in, &mask_in, &padding, &seed_base});
   const std::string who = "diff_attention: ";
   const std::string three = "q " + shape(q) + ", k " + shape(k) + ", v " + shape(v);
   if (q.dim() != 5 || k.dim() != 5 || v.dim() != 4 || q.size(3) != 2 || k.size(3) != 2)
@@ -406,7 +410,7 @@ Tensor diff_attention(const Tensor& q, const Tensor& k, const Tensor& v, const T
   if (!(sc >= 1e-30 && sc < 1e30)) throw py::value_error(who + "scale " + std::to_string(sc) + " must be in [1e-30, 1e30)");
   if (causal && Nq + Nk > most) throw py::value_error(who + three + " out of range");
 
-  Attn a{(int)B, (int)H, (int)Hk, (int)Nq, (int)Nk, (int)Dh, (int)Dv, (float)sc, causal, Drop{p, seed, given(base)}, Tensor(), Tensor()};
+  Attn a{(int)B, (int)H, (int)Hk, (int)Nq, (int)Nk, (int)Dh, (int)Dv, (float)sc, causal, Drop{p, seed, seed_base}, Tensor(), Tensor()};
   const bool need = wants_grad({&q, &k, &v, &lam});
   c10::DeviceGuard guard(dev);
   Tensor out, qc, kc, vc, lc, stat, maps;
@@ -457,6 +461,7 @@ Tensor diff_attention(const Tensor& q, const Tensor& k, const Tensor& v, const T
     n->lam_ = SavedVariable(lc, false);
     if (mask_in.defined()) n->mask_ = SavedVariable(mask_in, false);
     if (padding.defined()) n->padding_ = SavedVariable(padding, false);
+    if (a.drop.base.defined()) n->base_ = SavedVariable(a.drop.base, false);
     n->lam_type = lam.scalar_type();
     n->a = std::move(a);
     n->stat = stat;
