@@ -139,3 +139,63 @@ def test_a_changed_seed_base_is_noticed(op):
         torch.autograd.grad(y.sum(), x)
     finally:
         F.set_seed_base(None)
+
+
+# ------------------------------------------------------------------------------------------------- tiles that four waves share
+def check_heads(B, H, Hk, Nq, Nk, Dh, Dv, dt, hidden=None, bias=None, p=0.0, **kw):
+    """a call of many heads, of which the first, a middle and the last key head (and their query heads) are compared"""
+    gen = torch.Generator(DEV).manual_seed(Dh + Dv)
+
+    def randn(*shape, std=1.0):
+        return (torch.randn(*shape, generator=gen, device=DEV) * std).to(dt)
+    q, k, v, go = randn(B, Nq, H, 2, Dh, std=1.5), randn(B, Nk, Hk, 2, Dh), randn(B, Nk, Hk, Dv), randn(B, Nq, H, Dv)
+    lam = torch.randn(H, generator=gen, device=DEV) * 0.2 + 0.5
+    leaves = [t.requires_grad_() for t in (q, k, v, lam)]
+    y = UF().diff_attention(*leaves, p=p, training=True, seed=77, **kw)
+    y.backward(go)
+    kv, G = [0, Hk // 2 - 1, Hk - 1], H // Hk
+    hq = [h * G + g for h in kv for g in range(G)]
+    D = attn_drop(77, B, H, Nq, Nk, p)
+    r = Ref(*(t.detach().cpu() for t in (q[:, :, hq], k[:, :, kv], v[:, :, kv], lam[hq], go[:, :, hq])), dt, hidden,
+            None if bias is None else bias[:, hq].cpu(), None if D is None else D[:, hq])
+    within(y[:, :, hq], r.out, r.e_out, 'out')
+    for t, ref, e, what in ((q.grad[:, :, hq], r.q, r.eq, 'grad_q'), (k.grad[:, :, kv], r.k, r.ek, 'grad_k'),
+                            (v.grad[:, :, kv], r.v, r.ev, 'grad_v'), (lam.grad[hq], r.lam, r.e_lam, 'grad_lam')):
+        within(t, ref, e, what)
+    assert all(torch.isfinite(t.grad).all() for t in leaves) and torch.isfinite(y).all()
+
+
+@pytest.mark.parametrize('Dh,Dv', [(16, 32), (32, 64), (64, 64), (64, 128), (128, 128), (128, 256)])
+@pytest.mark.parametrize('kind', ['plain', 'dropped', 'causal', 'padded causal', 'masked', 'float dropped causal'])
+@pytest.mark.parametrize('dt', TYPES)
+def test_attention_shared_tiles_of_every_kind_of_call(Dh, Dv, kind, dt):
+    """So many heads that tiles of 128 own items fill the chip (causal: over 1638 tiles of 32 items; else several rounds of the
+    chip's 256 blocks), in every pass but grad_k / grad_v at 128 / 128, which has none.  Several such tiles a head, the last of
+    them part empty, and with two query heads to a key head rows that run on from one to the other inside a tile."""
+    if kind in ('plain', 'dropped'):
+        return check_heads(2, 56, 56, 250, 250, Dh, Dv, dt, p=0.1 if kind == 'dropped' else 0.0)
+    if kind == 'masked':
+        Nq = Nk = 250
+        m = torch.rand(Nq, Nk, generator=torch.Generator().manual_seed(1)) < 0.3
+        m[::9] = True
+        return check_heads(2, 56, 56, Nq, Nk, Dh, Dv, dt, hidden=m, attn_mask=m.to(DEV))
+    B, H, Hk, Nq, Nk = 2, 192, 96, 230, 300
+    hidden, kw = causal(Nq, Nk), dict(causal=True)
+    if kind == 'padded causal':
+        pad = torch.arange(Nk)[None] >= torch.tensor([[Nk], [171]])
+        hidden, kw['key_padding_mask'] = hidden | pad[:, None, None], pad.to(DEV)
+    elif kind == 'float dropped causal':
+        gen = torch.Generator(DEV).manual_seed(2)
+        bias = -torch.rand(1, H, Nq, Nk, generator=gen, device=DEV) * 20
+        kw.update(attn_mask=bias, bias=bias, p=0.1)
+    check_heads(B, H, Hk, Nq, Nk, Dh, Dv, dt, hidden=hidden, **kw)
+
+
+@pytest.mark.parametrize('Nq,Nk', [(45, 77), (77, 45), (300, 300)])
+@pytest.mark.parametrize('dt', TYPES)
+def test_attention_padded_causal_without_dropout(Nq, Nk, dt):
+    """the causal kernels beside hidden keys, a sample with none left"""
+    pad = torch.arange(Nk)[None] >= torch.tensor([[Nk], [20], [0]])
+    pad[1, 3:7] = True
+    attn_check(*attn_inputs(3, 4, 2, Nq, Nk, 32, 64, dt), dt, hidden=pad[:, None, None] | causal(Nq, Nk), causal=True,
+               key_padding_mask=pad.to(DEV))
