@@ -199,3 +199,106 @@ def test_attention_padded_causal_without_dropout(Nq, Nk, dt):
     pad[1, 3:7] = True
     attn_check(*attn_inputs(3, 4, 2, Nq, Nk, 32, 64, dt), dt, hidden=pad[:, None, None] | causal(Nq, Nk), causal=True,
                key_padding_mask=pad.to(DEV))
+
+
+# ------------------------------------------------------------------------------------------------------ gradients of the module
+class NoisyLinear(torch.autograd.Function):
+    """a Linear in 64 bits whose products (y, grad_x, grad_w) and sum (grad_b) are off by up to eps of the sum of their terms' sizes"""
+
+    @staticmethod
+    def forward(ctx, x, w, b, eps, gen):
+        ctx.save_for_backward(x, w)
+        ctx.eps, ctx.gen = eps, gen
+        return NoisyLinear.off(x @ w.t(), x.abs() @ w.abs().t(), eps, gen) + b
+
+    @staticmethod
+    def off(y, size, eps, gen):
+        return y + eps * size * (torch.randint(0, 2, y.shape, generator=gen) * 2 - 1) if eps else y
+
+    @staticmethod
+    def backward(ctx, g):
+        x, w = ctx.saved_tensors
+        gf, xf = g.flatten(0, -2), x.flatten(0, -2)
+        return (NoisyLinear.off(g @ w, g.abs() @ w.abs(), ctx.eps, ctx.gen),
+                NoisyLinear.off(gf.t() @ xf, gf.abs().t() @ xf.abs(), ctx.eps, ctx.gen),
+                NoisyLinear.off(gf.sum(0), gf.abs().sum(0), ctx.eps, ctx.gen), None, None)
+
+
+def module_pass(m, ins, go, hidden, eps, seed=0):
+    """output and gradients (parameters by name, then inputs) of the module's definition in 64 bits on the CPU"""
+    gen = torch.Generator().manual_seed(seed)
+    P = {n: t.detach().double().cpu().requires_grad_() for n, t in m.named_parameters()}
+    query, key, value, identity, qpos, kpos = (None if t is None else t.double().requires_grad_() for t in ins)
+    leaves = [t for t in (query, key, value, identity, qpos, kpos) if t is not None]
+    flip = (lambda t: t) if m.batch_first else (lambda t: t.transpose(0, 1))
+
+    def lin(x, name):
+        return NoisyLinear.apply(x, P[name + '.weight'], P[name + '.bias'], eps, gen)
+    k_in = query if key is None else key
+    v_in = k_in if value is None else value
+    kp = qpos if kpos is None and qpos is not None and qpos.shape == k_in.shape else kpos
+    q = flip(lin(query if qpos is None else query + qpos, 'q_proj'))
+    k = flip(lin(k_in if kp is None else k_in + kp, 'k_proj'))
+    v = flip(lin(v_in, 'v_proj'))
+    H, dv = m.num_heads, m.head_dims
+    q, k, v = q.unflatten(-1, (H, 2, dv // 2)), k.unflatten(-1, (-1, 2, dv // 2)), v.unflatten(-1, (-1, dv))
+    G = H // k.shape[2]
+    k, v = k.repeat_interleave(G, 2), v.repeat_interleave(G, 2)
+    e = (P['lambda_a'] * P['lambda_b']).sum(-1).exp()
+    lam = e[0] - e[1] + m.lambda_init
+    A = []
+    for i in (0, 1):
+        s = torch.einsum('bqhd,bkhd->bhqk', q[:, :, :, i], k[:, :, :, i]) / math.sqrt(dv // 2)
+        A.append((s if hidden is None else s.masked_fill(hidden, -math.inf)).softmax(-1))
+    o = torch.einsum('bhqk,bkhd->bqhd', A[0] - lam * A[1], v)
+    o = torch.nn.functional.layer_norm(o, (dv,), P['head_norm.weight'], P['head_norm.bias'], m.head_norm.eps) * (1 - m.lambda_init)
+    y = lin(flip(o.flatten(2)), 'out_proj') + (query if identity is None else identity)
+    named = {**P, **dict(zip(('query', 'key', 'value', 'identity', 'query_pos', 'key_pos'), (query, key, value, identity, qpos, kpos)))}
+    named = {n: t for n, t in named.items() if t is not None}
+    return y.detach(), dict(zip(named, torch.autograd.grad(y, list(named.values()), go.double())))
+
+
+@pytest.mark.parametrize('case', ['self', 'self batch_first shared', 'cross', 'cross padded batch_first'])
+def test_module_gradients(case):
+    """Training mode without dropout, f32.  Each of the module's Linears is a split-bf16 product (2^-16 of its terms' sizes, forward
+    and both gradients), its bias gradient an f32 sum over at most 166 tokens (166 x 2^-24 < 2^-16 of its terms' sizes: what remains of
+    k_proj.bias, whose gradient is zero because a softmax does not see it), everything else f32 operators within a few 2^-24.  So the bound of a gradient is what such errors do to
+    it in the definition: the largest of three draws of errors of FULL size and random sign, by norm, times 4."""
+    from unibev_amd import build_attention
+    torch.manual_seed(11)
+    batch_first, kv = 'batch_first' in case, 2 if 'shared' in case else None
+    m = build_attention(dict(type='DifferentialAttention', embed_dims=128, num_heads=4, num_kv_heads=kv, batch_first=batch_first)).to(DEV).train()
+    with torch.no_grad():
+        m.head_norm.weight.uniform_(0.5, 1.5)
+        m.head_norm.bias.uniform_(-0.5, 0.5)
+        for lin in (m.q_proj, m.k_proj, m.v_proj, m.out_proj):
+            lin.bias.uniform_(-0.5, 0.5)
+    B, Nq, Nk = 2, 60, 83 if 'cross' in case else 60
+
+    def tokens(n):
+        return torch.randn(B, n, 128) if batch_first else torch.randn(n, B, 128)
+    cross = 'cross' in case
+    ins = [tokens(Nq), tokens(Nk) if cross else None, tokens(Nk) if cross else None, tokens(Nq) if cross else None, tokens(Nq),
+           tokens(Nk) if cross else None]
+    go = tokens(Nq)
+    hidden, kw = None, {}
+    if 'padded' in case:
+        pad = torch.arange(Nk)[None] >= torch.tensor([[Nk], [50]])
+        hidden, kw = pad[:, None, None], dict(key_padding_mask=pad.to(DEV))
+    elif not cross:
+        mask = torch.rand(Nq, Nq) < 0.3
+        hidden, kw = mask, dict(attn_mask=mask.to(DEV))
+    y0, ref = module_pass(m, ins, go, hidden, 0.0)
+    noisy = [module_pass(m, ins, go, hidden, 2.0 ** -16, seed) for seed in (1, 2, 3)]
+    dev = [None if t is None else t.to(DEV).requires_grad_() for t in ins]
+    y = m(dev[0], key=dev[1], value=dev[2], identity=dev[3], query_pos=dev[4], key_pos=dev[5], **kw)
+    y.backward(go.to(DEV))
+    got = {**{n: p.grad for n, p in m.named_parameters()},
+           **{n: t.grad for n, t in zip(('query', 'key', 'value', 'identity', 'query_pos', 'key_pos'), dev) if t is not None}}
+    assert set(got) == set(ref)
+    off = (y.detach().double().cpu() - y0).norm()
+    assert off <= 4 * max((n[0] - y0).norm() for n in noisy), f'out: {off:.3e}'
+    for name in ref:
+        off = (got[name].double().cpu() - ref[name]).norm().item()
+        bound = 4 * max((n[1][name] - ref[name]).norm().item() for n in noisy) + 2.0 ** -20 * ref[name].norm().item()
+        assert off <= bound, f'{name}: off by {off:.3e}, bound {bound:.3e} (norm {ref[name].norm().item():.3e})'
