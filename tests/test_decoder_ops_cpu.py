@@ -101,6 +101,14 @@ def test_module_builds_from_the_registry():
             build_attention(dict(type='DifferentialAttention', embed_dims=64, **bad))
 
 
+def test_layer_norm_workspace_counts_the_rows_that_are_written():
+    """rows of at most 8192 elements: one row of 2 C sums a block, 1024 blocks at most; wider ones are summed in 64 slabs"""
+    need = _lib.lib().ubv_layer_norm_backward_workspace
+    assert need(1000, 256) == 1000 * 2 * 256 * 4 and need(5000, 8192) == 1024 * 2 * 8192 * 4
+    assert need(5000, 8193) == 64 * 2 * 8193 * 4 and need(3, 20000) == 3 * 2 * 20000 * 4
+    assert need(0, 20000) == 0
+
+
 def decoder_calls():
     """name -> call with one operand replaced"""
     from unibev_amd import functional as UF

@@ -394,11 +394,13 @@ __global__ __launch_bounds__(1024) void layer_norm_cols_final_kernel(const float
 }
 
 constexpr int kLnBwdBlocks = 1024;      // most blocks of a backward launch = rows of the workspace
-constexpr int kLnWideSlabs = 64;
+constexpr int kLnWideSlabs = 64;        // the same where rows are streamed
+constexpr int kLnHeld = 8192;           // widest row that ln_plan holds in registers, of every type
 
 // f(TPR, K) for a row of C elements of 16 / VEC bytes; false: stream the row
 template <int VEC, typename F>
 static bool ln_plan(int C, F&& f) {
+  if (C > kLnHeld) return false;
   const long n = ((long)C + VEC - 1) / VEC;
 #define UBV_LN(TPR, K) (f(std::integral_constant<int, TPR>{}, std::integral_constant<int, K>{}), true)
   if (n <= 4) return UBV_LN(4, 1);
@@ -493,7 +495,7 @@ extern "C" int ubv_layer_norm_forward(const void* x, const float* gamma, const f
 }
 
 extern "C" int64_t ubv_layer_norm_backward_workspace(int64_t R, int C) {
-  const int64_t rows = R < ubv::kLnBwdBlocks ? R : ubv::kLnBwdBlocks;
+  const int64_t most = C > ubv::kLnHeld ? ubv::kLnWideSlabs : ubv::kLnBwdBlocks, rows = R < most ? R : most;
   return R <= 0 || C <= 0 ? 0 : rows * 2 * (int64_t)C * 4;
 }
 
