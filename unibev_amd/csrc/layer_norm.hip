@@ -7,8 +7,8 @@
 // (K 16-byte pieces each) between its one load and its one store, with the variance taken around the mean in a second pass
 // over those registers; a row of a few pieces shares its wave with others (TPR < 64), a row of more than 256 pieces takes a
 // block.  Rows whose width is no multiple of a 16-byte piece start at any element border: the same kernels with
-// element-aligned accesses (one instruction too) and a last piece that overlaps the one before.  Rows wider than 2048 pieces
-// (16-bit: 1024) are streamed.  80 000 x 256 f32: forward 27 us (6.0 TB/s), backward 42 (5.9 TB/s) + 4; 5001 x 1021 f16: 7.3, 13.1 + 4.8.
+// element-aligned accesses (one instruction too) and a last piece that overlaps the one before.  Rows wider than 8192 elements
+// are streamed (ln_plan).  80 000 x 256 f32: forward 27 us (6.0 TB/s), backward 42 (5.9 TB/s) + 4; 5001 x 1021 f16: 7.3, 13.1 + 4.8.
 //
 // The weight's gradient: a thread owns the same columns of every row that its block visits and keeps their sums in f32
 // registers; the block's threads are added through LDS, the blocks' sums [block][2][C] go to a workspace and are added in
@@ -412,7 +412,10 @@ static bool ln_plan(int C, F&& f) {
   if (n <= 256) return UBV_LN(64, 4);
   if (n <= 512) return UBV_LN(256, 2);
   if (n <= 1024) return UBV_LN(256, 4);
-  if constexpr (VEC == 4) {            // (16-bit rows of this many pieces would hold 2 x 64 sums per thread: streamed)
+  // f32 up to kLnHeld.  16-bit rows of as many pieces are wider than that and streamed: 1024 threads have 128 registers each, which
+  // the backward kernel's x, grad_y and sums of 2 x 8 elements pass by 16 to 37.  2000 x 10 000 f16, us, streamed / held: forward
+  // 25 / 30, backward 57 / 159 (300 x 9001 bf16: 7.7 / 8.9, 31 / 50; only very many rows gain, 20 000 x 16 384: 395 / 298, 842 / 774).
+  if constexpr (VEC == 4) {
     if (n <= 2048) return UBV_LN(1024, 2);
   }
 #undef UBV_LN
