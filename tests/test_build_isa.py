@@ -131,3 +131,15 @@ def test_weight_stationary_gemm_stage_issues_exactly_the_counted_memory_instruct
             assert (ppt, 4, e) in kinds and (ppt, 0, 0) in kinds, (m.group(2), kinds)
             seen += 1
     assert seen >= 12, f'only {seen} gemm_ws_kernel instantiations found in the library'
+
+
+def test_there_is_one_build_and_it_names_the_packed_f32_switch():
+    """Every kernel source is compiled with the packed-f32 target feature off (core.hip's synthetic co-runners name the instruction),
+    and no variable of the Makefile gives a second library."""
+    csrc = os.path.join(ROOT, 'unibev_amd', 'csrc')
+    out = [subprocess.run(['make', '-n', '-B', '-C', csrc, *v], check=True, capture_output=True, text=True).stdout for v in ((), ('SLP=1',))]
+    assert out[0] == out[1]
+    lines = [line for line in out[0].splitlines() if re.search(r' -c \S+\.hip ', line)]
+    assert len(lines) > 20
+    for line in lines:
+        assert '-fno-slp-vectorize' in line and ('-packed-fp32-ops' in line) == (' core.hip ' not in line), line
