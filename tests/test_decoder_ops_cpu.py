@@ -1,12 +1,14 @@
 """Dropout, layer norm and differential attention where no GPU is needed: the C entries refuse bad arguments before any launch,
 the Python entries refuse CPU tensors, the module builds from the registry."""
 import ctypes
+import os
 
 import pytest
 import torch
 
 from unibev_amd import _lib
 
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 P = ctypes.c_void_p(1 << 20)          # a 16-byte aligned address that no refused call may touch
 
 
@@ -74,6 +76,20 @@ def test_attention_backward_entry_refuses():
     refused(call(gq=ctypes.c_void_p((1 << 20) + 4)), 'aligned')
     refused(call(n=need - 1), 'workspace')
     refused(call(ws=None), 'workspace')
+
+
+@pytest.mark.parametrize('Nq,Nk,causal', [(1 << 30, 8, 0), (1 << 29, 8, 0), (8, (1 << 31) - 1, 0), (8, (1 << 31) - 256, 0), (1 << 28, (1 << 31) - 300, 1)])
+def test_attention_workspace_of_a_call_out_of_range(Nq, Nk, causal):
+    """sizes that 32-bit counts do not hold: the workspace entries answer (another process: they used to divide by zero), the call refuses"""
+    import subprocess
+    import sys
+    code = (f'from unibev_amd import _lib; l = _lib.lib(); a = (1, 8, 2, {Nq}, {Nk}, 32, 64, {causal}, 0); '
+            'print(l.ubv_diff_attention_forward_workspace(*a), l.ubv_diff_attention_backward_workspace(*a) >= 28 * 8 * a[3])')
+    r = subprocess.run([sys.executable, '-c', code], capture_output=True, text=True, cwd=ROOT)
+    assert r.returncode == 0 and r.stdout.split() == ['0', 'True'], (r.returncode, r.stdout, r.stderr[-500:])
+    s = (ctypes.c_int64 * 18)()
+    refused(_lib.lib().ubv_diff_attention_forward(P, P, P, P, None, None, 0, P, None, None, s, 1, 8, 2, Nq, Nk, 32, 64, 0.1, causal, 0.0, 0, None,
+                                                  0, None, 0, None), 'out of range')
 
 
 def test_cpu_tensors_are_refused():

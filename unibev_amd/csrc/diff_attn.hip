@@ -12,8 +12,14 @@ int64_t diff_attn_bytes_f32(const DiffAttnArgs&, bool);
 int64_t diff_attn_bytes_f16(const DiffAttnArgs&, bool);
 int64_t diff_attn_bytes_bf16(const DiffAttnArgs&, bool);
 
+// rows of a group, keys and heads count in 32 bits, the next tile's included
+static bool attn_in_reach(int B, int H, int Hk, int Nq, int Nk, int causal) {
+  constexpr int64_t most = (int64_t(1) << 31) - 256;
+  return (int64_t)(H / Hk) * Nq < most && Nk < most && (int64_t)B * H < (int64_t(1) << 31) && (!causal || (int64_t)Nq + Nk < (int64_t(1) << 31));
+}
 static int64_t attn_part_bytes(int B, int H, int Hk, int Nq, int Nk, int Dh, int Dv, int causal, int dtype, bool backward) {
   if (B <= 0 || Hk <= 0 || H < Hk || H % Hk != 0 || Nq <= 0 || Nk <= 0 || Dh <= 0 || Dv <= 0 || Dh > 128 || Dv > 256) return 0;
+  if (!attn_in_reach(B, H, Hk, Nq, Nk, causal)) return 0;      // (such a call is refused)
   DiffAttnArgs a{};
   a.B = B; a.H = H; a.Hk = Hk; a.G = H / Hk; a.Nq = Nq; a.Nk = Nk; a.Dh = Dh; a.Dv = Dv; a.R = a.G * Nq; a.causal = causal != 0;
   return dtype == UBV_F32 ? diff_attn_bytes_f32(a, backward) : dtype == UBV_F16 ? diff_attn_bytes_f16(a, backward) : diff_attn_bytes_bf16(a, backward);
@@ -30,9 +36,7 @@ static int attn_args(DiffAttnArgs& a, const void* q, const void* k, const void* 
   UBV_CHECK_ARG(B > 0 && H > 0 && Hk > 0 && Nq > 0 && Nk > 0, "%s: empty shape B=%d H=%d Hk=%d Nq=%d Nk=%d", who, B, H, Hk, Nq, Nk);
   UBV_CHECK_ARG(H % Hk == 0, "%s: %d query heads do not share %d key heads evenly", who, H, Hk);
   UBV_CHECK_ARG(Dh > 0 && Dh <= 128 && Dv > 0 && Dv <= 256, "%s: head widths %d (at most 128) and %d (at most 256)", who, Dh, Dv);
-  UBV_CHECK_ARG((int64_t)(H / Hk) * Nq < (int64_t(1) << 31) - 256 && Nk < (1 << 31) - 256 && (int64_t)B * H < (int64_t(1) << 31),
-                "%s: Nq=%d x %d heads or Nk=%d out of range", who, Nq, H / Hk, Nk);
-  UBV_CHECK_ARG(!causal || (int64_t)Nq + Nk < (int64_t(1) << 31), "%s: Nq=%d + Nk=%d out of range", who, Nq, Nk);
+  UBV_CHECK_ARG(attn_in_reach(B, H, Hk, Nq, Nk, causal), "%s: Nq=%d x %d heads, Nk=%d or B=%d x H=%d out of range", who, Nq, H / Hk, Nk, B, H);
   UBV_CHECK_ARG(p >= 0.0f && p <= 1.0f, "%s: p = %g must be in [0, 1]", who, (double)p);
   UBV_CHECK_ARG(scale >= 0.99e-30f && scale < 1.01e30f, "%s: scale %g must be in [1e-30, 1e30)", who, (double)scale);
   UBV_CHECK_ARG(mask_kind >= 0 && mask_kind <= 2 && (mask_kind == 0) == (mask == nullptr), "%s: mask kind %d", who, mask_kind);
