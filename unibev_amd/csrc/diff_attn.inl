@@ -21,12 +21,14 @@ template <typename T, int DH, int DV> struct AttnTile {
   static constexpr int xybytes(int n) { return n * 16 * (LX + LY); }
   static constexpr int bytes(int n) { return xybytes(n) + 24 * n; }
   static constexpr int QFLOATS = 32 * KO + 4, KFLOATS = 16 * (2 * KO + VO);      // a lane's sums in a split's workspace
-  // two waves a SIMD where accumulators, operands and a tile in flight fit half the registers (64 / 128, f16: forward 244 us with
-  // two waves that spill, 167 with one that does not)
+  // two waves a SIMD (256 registers each) up to 32 / 64, where a 16-bit type's accumulators, operands and tile in flight fit (only
+  // grad_k / grad_v with masks spills, 12); wider heads take one (64 / 128, f16: forward 244 us with two waves that spill, 167 with
+  // one that does not).  f32's operands are twice as long: its grad_k / grad_v spills at 32 / 64, 2 to 33 registers as private blocks
+  // and 45 to 137 as shared ones.
   static constexpr int MINW = DH <= 32 && DV <= 64 ? 2 : 1;
   // own operands in registers: 2 KB + VB operands of 4 registers, f32 8: at 128 / 256 that is 256 beside the accumulators, and read
   // again they cost less than spilled (8 heads, 1024 x 1024, us: grad_q 1360 spilled, 369; held where they fit: 64 / 128 1500 x 1500
-  // 188, read again 266)
+  // 188, read again 266).  16-bit 128 / 256 keeps 128 of them and spills 4 to 84 others, most in shared blocks of grad_k.
   static constexpr bool KEEP = elem<T>::kBytes == 2 || DH <= 64;
   static constexpr int fit(int w) { return w > 2 && w * bytes(32) > 150 * 1024 ? fit(w / 2) : w; }
   // waves of a private block.  16-bit heads up to 32 / 64: all of a CU's, which halves a block's time where blocks are few (2 x 4
@@ -124,8 +126,10 @@ template <bool SHARED> __device__ __forceinline__ void tile_ready() {
   }
 }
 
-// A lane's own item as B operands: 8 elements at 16 s + 8 (lane >> 5) of step s.  KEEP: held in registers; else read again (from L1:
-// a block's own rows are at most 64 KB) for every tile, where the accumulators leave no room for them.
+// A lane's own item as B operands: 8 elements at 16 s + 8 (lane >> 5) of step s.  KEEP: held in registers; else (f32 heads past 64)
+// read again for every tile, where the accumulators leave no room for them: 48 to 64 KB a tile in a private block, 192 to 256 KB in a
+// shared one, more than the L1, so from L2.  Four rows of waves to a tile make up for it: 2 x 16 heads of 128 / 128, 1024 x 1024, us,
+// shared / private: forward 445 / 862, grad_q 610 / 1293.
 template <typename T, int NB, bool KEEP> struct OwnRow {
   static constexpr int VEC = 16 / elem<T>::kBytes;
   typename amma<T>::frag f[KEEP ? NB : 1];
@@ -477,10 +481,11 @@ __device__ __forceinline__ void fwd_finish(const DiffAttnArgs& a, const FwdState
 }
 
 // One pass over the keys with a running reference and sum for each map.  Per pair and map: Dh + Dv multiply-adds on the matrix cores
-// against one exponential (a quarter of the VALU's rate), a fma, a maximum, an addition and a rounding: at 32 / 64 wide heads
-// the VALU is what bounds it (its issue and the matrix cores' add up to ~80 % of the time).  4 heads of 32 / 64, 10 000 x 10 000
-// bf16: 310 us (495 TFLOP/s); 2 x 8 heads of 64 / 128, 4096 x 4096: 400 us (515 TFLOP/s); one query, 8 x 4 heads of 32 / 64,
-// 40 000 keys ragged: 54 us (4.7 TB/s, bound by memory).
+// against one exponential (a quarter of the VALU's rate), a fma, a maximum, an addition and a rounding.  A wave's products and its
+// softmax follow one another, and one or two waves a SIMD do not fill the gaps: at 32 / 64, 10 000 x 10 000, the VALU issues 52 % of
+// the time and the matrix cores are busy 23 %; at 64 / 128, 4096 x 4096, 46 and 22 %.  4 heads of 32 / 64, 10 000 x 10 000 bf16: 271 us
+// (567 TFLOP/s); 2 x 8 heads of 64 / 128, 4096 x 4096: 386 us (534 TFLOP/s); one query, 8 x 4 heads of 32 / 64, 40 000 keys ragged:
+// 54 to 61 us (4.2 to 4.7 TB/s, bound by memory).
 template <typename T, int DH, int DV, bool SHARED, int MODE>
 __global__ __launch_bounds__((AttnPlan<T, DH, DV, SHARED>::NT), (AttnPlan<T, DH, DV, SHARED>::MINW)) void diff_attn_fwd_kernel(
     const DiffAttnArgs a) {
@@ -792,7 +797,8 @@ __device__ __forceinline__ void store_gkv(const DiffAttnArgs& a, int b, int hk, 
 
 // ---- backward: grad_q and the rows' parts of grad_lam; own = rows, staged = keys -----------------------------------------------
 // dq_m = scale sum_j dS_m k_m,  dS_1 = A_1 o (G - del_1),  dS_2 = -lam A_2 o (G - del_2),  G = D o (grad_out v^T);  A from the row's
-// statistics.  Bound as the forward pass: 10 000 x 10 000, 4 heads of 32 / 64 bf16 329 us (467 TFLOP/s, the scores computed again).
+// statistics.  Bound as the forward pass: 10 000 x 10 000, 4 heads of 32 / 64 bf16 288 us (533 TFLOP/s, the scores computed again;
+// VALU 51 %, matrix cores 22 %).
 template <typename T, int DH, int DV, bool SHARED, int MODE>
 __global__ __launch_bounds__((AttnPlan<T, DH, DV, SHARED>::NT), (AttnPlan<T, DH, DV, SHARED>::MINW)) void diff_attn_bwd_q_kernel(
     const DiffAttnArgs a) {
@@ -927,8 +933,9 @@ __global__ __launch_bounds__(1024) static void diff_attn_lam_kernel(const float*
 
 // ---- backward: grad_k and grad_v; own = keys, staged = the rows of every head that shares them ----------------------------------
 // A tile of rows stays inside one head (its rows are one stretch of queries), heads one after the other.
-// dk_m = scale sum_i dS_m q_m,  dv = sum_i (D o (A_1 - lam A_2)) grad_out.  10 000 x 10 000, 4 heads of 32 / 64 bf16: 470 to 515 us
-// by card (400 TFLOP/s and more); VALU and LDS reads (the rows' statistics, 4 floats each) bound it.
+// dk_m = scale sum_i dS_m q_m,  dv = sum_i (D o (A_1 - lam A_2)) grad_out.  10 000 x 10 000, 4 heads of 32 / 64 bf16: 437 to 515 us
+// by card and clock (400 to 470 TFLOP/s); bound as the others (VALU 47 %, matrix cores 18 %) with LDS reads on top (the rows'
+// statistics, 4 floats each).
 // PART 0: both gradients in one pass; 1: grad_k, 2: grad_v by a pass of its own, where the accumulators of both (2 DH + DV
 // floats a lane's item pair) would not fit the register file (the scores are computed twice: less than spilling costs).
 template <typename T, int DH, int DV, bool SHARED, int MODE, int PART>
@@ -1180,6 +1187,10 @@ template <typename F> static int attn_mode(const DiffAttnArgs& a, F&& f) {
 // shared: a shared block does four private blocks' work in 4 `cost` times their time (it stages a tile once for 128 own items), but
 // there are a quarter as many: with 256 CUs the rounds of blocks decide.  Measured at one block a CU (bf16, us, shared / private):
 // 64 / 64 wide heads 80 / 121, 128 / 128 133 / 278; 32 / 64 at 10 000 x 10 000 and 4 heads (316 or 1252 blocks) 400 / 299.
+// f32 at 8 x 8 heads, 900 x 900, grad_q: 64 / 64 386 / 476, 128 / 128 1119 / 2338, 128 / 256 1440 / 2593.  What the rule does not see
+// yet: causal f32 heads up to 64 / 128 are slower shared (2 x 16 heads, 2048 causal, forward / grad_q / grad_k and grad_v: 32 / 64
+// 405, 432, 674, private 283, 293, 385; 64 / 128 771, 851, 1474, private 634, 620, 862), and f32 128 / 128 at half a chip of wide
+// tiles (4 heads, 4096 x 4096) slower private: forward 1706, shared 1527, grad_q 2554, 2050.
 // splits: private blocks that share the staged items of one own tile, `chunk` staged tiles each, where own tiles alone leave the chip
 // empty: up to twice as many waves as fill it (ragged batches and causal rows are unequal), at least four tiles for each wave.
 // (Shared blocks that split a causal own tile into equal chunks fill the chip too, but lose to it what joining them costs: 64 / 128

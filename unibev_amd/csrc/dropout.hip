@@ -7,8 +7,8 @@
 //
 // Bound by memory: 6 bytes per 16-bit element with the residual against ~11 VALU slots of hash.  A thread takes 8 elements a
 // step, 16-byte accesses; buffers that start off a 16-byte border take the same kernel with element-aligned accesses.
-// 41 M bf16 elements with the residual 47 us (5.2 TB/s), without it 27 us (6.0 TB/s, part of it cached); below ~1 M elements the
-// launch is what it takes (2.8 us).
+// 41 M bf16 elements with the residual 45 to 47 us (5.2 to 5.5 TB/s), without it 27 to 28 us (5.9 to 6.0 TB/s, part of it cached);
+// below ~1 M elements the launch is what it takes (2.6 to 2.8 us).
 #include "ubv_common.h"
 
 namespace ubv {

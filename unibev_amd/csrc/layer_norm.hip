@@ -8,7 +8,8 @@
 // over those registers; a row of a few pieces shares its wave with others (TPR < 64), a row of more than 256 pieces takes a
 // block.  Rows whose width is no multiple of a 16-byte piece start at any element border: the same kernels with
 // element-aligned accesses (one instruction too) and a last piece that overlaps the one before.  Rows wider than 8192 elements
-// are streamed (ln_plan).  80 000 x 256 f32: forward 27 us (6.0 TB/s), backward 42 (5.9 TB/s) + 4; 5001 x 1021 f16: 7.3, 13.1 + 4.8.
+// are streamed (ln_plan).  80 000 x 256 f32: forward 27 to 31 us (5.3 to 6.0 TB/s),
+// backward 42 (5.9 TB/s) + 4, bf16: 15 (5.3), 22 (5.6) + 4; 5001 x 1021 f16: 7.1, 12.4 + 4.9, bf16: 7.0, 12.6 + 4.9.
 //
 // The weight's gradient: a thread owns the same columns of every row that its block visits and keeps their sums in f32
 // registers; the block's threads are added through LDS, the blocks' sums [block][2][C] go to a workspace and are added in
