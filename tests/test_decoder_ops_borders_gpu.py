@@ -141,6 +141,32 @@ def test_a_changed_seed_base_is_noticed(op):
         F.set_seed_base(None)
 
 
+# ------------------------------------------------------------------------------------------------- what the 16-bit types keep
+@pytest.mark.parametrize('Dh,Dv', [(16, 32), (32, 64), (64, 64), (64, 128), (128, 128), (128, 256)])
+@pytest.mark.parametrize('kind', ['plain', 'causal dropped shared heads'])
+@pytest.mark.parametrize('dt', [torch.float16, torch.bfloat16])
+def test_attention_16_bit_results_are_off_by_little_more_than_their_own_rounding(Dh, Dv, kind, dt):
+    """By norm, in units of what rounding the exact result to the type does.  out and grad_v add one rounding of each probability:
+    the errors of N terms against one of the sum, sqrt(1 + 1) at most where the terms are independent.  dS enters with the rest of
+    its rounding, so grad_q and grad_k add what del = grad_out . o takes over from out, P del k in size: over rows whose squared
+    probabilities sum to S, sqrt(S) of a rounding; S is under 0.2 here (300 keys, scores of deviation 1.5 and under), so
+    sqrt(1 + 0.2) = 1.1.  Both with a tenth on top."""
+    B, H, Hk, Nq, Nk = 1, 4, 4, 300, 300
+    hidden, p, kw = None, 0.0, {}
+    if kind != 'plain':
+        Hk, Nq, hidden, p, kw = 2, 60, causal(60, 300), 0.1, dict(causal=True)
+    q, k, v, lam, go = attn_inputs(B, H, Hk, Nq, Nk, Dh, Dv, dt)
+    leaves = [t.to(DEV).requires_grad_() for t in (q, k, v, lam)]
+    y = UF().diff_attention(*leaves, p=p, training=True, seed=77, **kw)
+    y.backward(go.to(DEV))
+    r = Ref(q, k, v, lam, go, dt, hidden, None, attn_drop(77, B, H, Nq, Nk, p))
+    for what, t, ref, most in (('out', y, r.out, 1.56), ('grad_q', leaves[0].grad, r.q, 1.21), ('grad_k', leaves[1].grad, r.k, 1.21),
+                               ('grad_v', leaves[2].grad, r.v, 1.56)):
+        one = (ref.to(dt).double() - ref).norm()
+        off = (t.detach().double().cpu() - ref).norm()
+        assert off <= most * one, f'{what}: {(off / one).item():.2f} roundings'
+
+
 # ------------------------------------------------------------------------------------------------- tiles that four waves share
 def check_heads(B, H, Hk, Nq, Nk, Dh, Dv, dt, hidden=None, bias=None, p=0.0, **kw):
     """a call of many heads, of which the first, a middle and the last key head (and their query heads) are compared"""

@@ -52,7 +52,7 @@ struct DiffAttnArgs {
 constexpr int kAttnSplits = 256;         // most splits of an own tile's staged items
 
 // f16 holds nothing below 2^-24 and loses bits below 2^-14, which the probabilities of a long row reach: they enter the matrix
-// instructions 2^8 larger and their products leave 2^8 smaller.  dS enters as it is: a common factor would take from its upper
+// instructions 2^8 larger and their products leave 2^8 smaller.  dS enters at its size: a common factor would take from its upper
 // range, which a scaled loss uses, what it gives below.
 template <typename T> constexpr float kProbShift = std::is_same<T, f16_t>::value ? 8.0f : 0.0f;
 template <typename T> constexpr float kProbScale = std::is_same<T, f16_t>::value ? 256.0f : 1.0f;
@@ -102,6 +102,7 @@ template <int L> __host__ __device__ constexpr int row_fold(int r) {
 // load<L>: row r0 + (lane & 31) (r0 a multiple of 32) of a tile, elements 16 s .. of the part that begins at chunk `c0`
 // load_tr<L>: column 32 d + (lane & 31) of that part, rows k0 + 8 (j >> 2) + 4 (lane >> 5) + (j & 3), j = 0 .. 7 (k0 a multiple of 16)
 template <typename T> struct amma {                       // 16-bit types: one MFMA
+  static constexpr bool SPLIT = true;                     // what split gives is in two operands
   struct frag { au32x4_t d; };
   static __device__ __forceinline__ af32x16_t mul(const frag& a, const frag& b, af32x16_t c) {
     if constexpr (std::is_same<T, f16_t>::value)
@@ -110,7 +111,8 @@ template <typename T> struct amma {                       // 16-bit types: one M
       return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(abf16x8_t, a.d), __builtin_bit_cast(abf16x8_t, b.d), c, 0, 0, 0);
   }
   static __device__ __forceinline__ frag own(const T* t) { return {*reinterpret_cast<const au32x4_t*>(t)}; }
-  // rounding to the inputs' type: the matrix instruction takes no wider operand; half a step of each probability, random
+  // probabilities, rounded to the inputs' type: the matrix instruction takes no wider operand.  Half a step of each, random: out and
+  // grad_v, which are rounded to the type themselves, are off by 1.1 to 1.4 times that one rounding, by norm.
   static __device__ __forceinline__ frag pack(const float* p) {
     frag f;
     if constexpr (std::is_same<T, f16_t>::value) {
@@ -128,6 +130,26 @@ template <typename T> struct amma {                       // 16-bit types: one M
     }
     return f;
   }
+  // dS, as the sum of two operands.  Its rows sum to zero, so that errors of one rounding weigh more in grad_q and grad_k than in out
+  // (1.45 to 1.55 times the roundings of the results themselves, 1.0 to 1.1 with the rest of each).  bf16 is cut off, not rounded: the
+  // upper part is there in f32 without a conversion back.  The second product costs where the VALU is short: 4 heads of 32 / 64,
+  // 10 000 x 10 000 bf16, grad_q 290 -> 345 us, grad_k / grad_v 500 -> 575; 2 x 8 heads of 64 / 128, 4096: 373 -> 421, 604 -> 617.
+  static __device__ __forceinline__ void split(const float* p, frag& hi, frag& lo) {
+    float r[8];
+    if constexpr (std::is_same<T, f16_t>::value) {
+      hi = pack(p);
+      const af16x8_t h = __builtin_bit_cast(af16x8_t, hi.d);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) r[i] = __builtin_fmaf((float)h[i], -1.0f, p[i]);
+    } else {
+      uint32_t u[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) { u[i] = __float_as_uint(p[i]); r[i] = p[i] - __uint_as_float(u[i] & 0xffff0000u); }
+      hi.d = au32x4_t{__builtin_amdgcn_perm(u[1], u[0], 0x07060302u), __builtin_amdgcn_perm(u[3], u[2], 0x07060302u),
+                      __builtin_amdgcn_perm(u[5], u[4], 0x07060302u), __builtin_amdgcn_perm(u[7], u[6], 0x07060302u)};
+    }
+    lo = pack(r);
+  }
   template <int L> static __device__ __forceinline__ frag load(const char* tile, int r0, int c0, int s, int lane) {
     const int r = lane & 31, base = r * 16 * L + (((lane >> 5) ^ row_fold<L>(r)) << 4);
     return {*reinterpret_cast<const au32x4_t*>(tile + r0 * 16 * L + (base ^ ((c0 + 2 * s) << 4)))};
@@ -144,6 +166,7 @@ template <typename T> struct amma {                       // 16-bit types: one M
   }
 };
 template <> struct amma<float> {                          // f32: eight MFMAs of depth 2 (lane halves), IEEE products
+  static constexpr bool SPLIT = false;
   struct frag { float d[8]; };
   static __device__ __forceinline__ af32x16_t mul(const frag& a, const frag& b, af32x16_t c) {
 #pragma unroll
@@ -157,6 +180,7 @@ template <> struct amma<float> {                          // f32: eight MFMAs of
     return f;
   }
   static __device__ __forceinline__ frag pack(const float* p) { return own(p); }
+  static __device__ __forceinline__ void split(const float* p, frag& hi, frag&) { hi = own(p); }
   template <int L> static __device__ __forceinline__ frag load(const char* tile, int r0, int c0, int s, int lane) {
     const int r = lane & 31, base = r * 16 * L + (((2 * (lane >> 5)) ^ row_fold<L>(r)) << 4);
     const char* t = tile + r0 * 16 * L;

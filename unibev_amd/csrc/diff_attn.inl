@@ -877,10 +877,14 @@ __global__ __launch_bounds__((AttnPlan<T, DH, DV, SHARED>::NT), (AttnPlan<T, DH,
         float ds[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) ds[e] = x[m][8 * st + e];
-        const typename M::frag f = M::pack(ds);
+        typename M::frag f, rest;
+        M::split(ds, f, rest);
 #pragma unroll
-        for (int d = 0; d < S::KO; ++d)
-          acc[m][d] = M::mul(M::template load_tr<S::LX>(kt, it0 + 16 * st, m * S::LX / 2, d, w.lane), f, acc[m][d]);
+        for (int d = 0; d < S::KO; ++d) {
+          const typename M::frag kf = M::template load_tr<S::LX>(kt, it0 + 16 * st, m * S::LX / 2, d, w.lane);
+          acc[m][d] = M::mul(kf, f, acc[m][d]);
+          if constexpr (M::SPLIT) acc[m][d] = M::mul(kf, rest, acc[m][d]);
+        }
       }
   });
   if constexpr (!SHARED) {
@@ -1089,10 +1093,14 @@ __global__ __launch_bounds__((AttnPlan<T, DH, DV, SHARED>::NT), (AttnPlan<T, DH,
         }
 #pragma unroll
         for (int m = 0; m < (PART != 2 ? 2 : 0); ++m) {
-          const typename M::frag f = M::pack(ds[m]);
+          typename M::frag f, rest;
+          M::split(ds[m], f, rest);
 #pragma unroll
-          for (int d = 0; d < S::KO; ++d)
-            ak[m][d] = M::mul(M::template load_tr<S::LX>(qt, it0 + 16 * s, m * S::LX / 2, d, lane), f, ak[m][d]);
+          for (int d = 0; d < S::KO; ++d) {
+            const typename M::frag qf = M::template load_tr<S::LX>(qt, it0 + 16 * s, m * S::LX / 2, d, lane);
+            ak[m][d] = M::mul(qf, f, ak[m][d]);
+            if constexpr (M::SPLIT) ak[m][d] = M::mul(qf, rest, ak[m][d]);
+          }
         }
       }
     }
