@@ -21,14 +21,14 @@ template <typename T, int DH, int DV> struct AttnTile {
   static constexpr int xybytes(int n) { return n * 16 * (LX + LY); }
   static constexpr int bytes(int n) { return xybytes(n) + 24 * n; }
   static constexpr int QFLOATS = 32 * KO + 4, KFLOATS = 16 * (2 * KO + VO);      // a lane's sums in a split's workspace
-  // two waves a SIMD (256 registers each) up to 32 / 64, where a 16-bit type's accumulators, operands and tile in flight fit (only
-  // grad_k / grad_v with masks spills, 12); wider heads take one (64 / 128, f16: forward 244 us with two waves that spill, 167 with
-  // one that does not).  f32's operands are twice as long: its grad_k / grad_v spills at 32 / 64, 2 to 33 registers as private blocks
-  // and 45 to 137 as shared ones.
+  // two waves a SIMD (256 registers each) up to 32 / 64, where a 16-bit type's accumulators, operands and tile in flight about fit
+  // (grad_k / grad_v at 32 / 64 spills 2 to 11, with masks 27); wider heads take one (64 / 128, f16: forward 244 us with two waves that
+  // spill, 167 with one that does not).  f32's operands are twice as long: its grad_k / grad_v spills at 32 / 64, 2 to 33 registers as
+  // private blocks and 45 to 137 as shared ones.
   static constexpr int MINW = DH <= 32 && DV <= 64 ? 2 : 1;
   // own operands in registers: 2 KB + VB operands of 4 registers, f32 8: at 128 / 256 that is 256 beside the accumulators, and read
   // again they cost less than spilled (8 heads, 1024 x 1024, us: grad_q 1360 spilled, 369; held where they fit: 64 / 128 1500 x 1500
-  // 188, read again 266).  16-bit 128 / 256 keeps 128 of them and spills 4 to 84 others, most in shared blocks of grad_k.
+  // 188, read again 266).  16-bit heads past 64 keep them and spill up to 84 others, most in shared blocks of grad_k at 128 / 256.
   static constexpr bool KEEP = elem<T>::kBytes == 2 || DH <= 64;
   static constexpr int fit(int w) { return w > 2 && w * bytes(32) > 150 * 1024 ? fit(w / 2) : w; }
   // waves of a private block.  16-bit heads up to 32 / 64: all of a CU's, which halves a block's time where blocks are few (2 x 4
@@ -54,7 +54,8 @@ template <typename T, int DH, int DV, bool SHARED> struct AttnPlan {
 };
 
 // What a call may hold beside hidden keys.  Each has kernels of its own: what a kernel can never meet costs it registers, and
-// with them a wave per SIMD (32 / 64 wide heads, bf16, 10 000 x 10 000: grad_k / grad_v 738 us with everything, 448 plain).
+// with them a wave per SIMD (32 / 64 wide heads, bf16, 10 000 x 10 000: grad_k / grad_v 738 us with everything, 448 plain,
+// dS in one operand).
 constexpr int kAttnPlain = 0, kAttnDrop = 1, kAttnCausal = 2, kAttnAny = 3;       // nothing | dropout | causal | masks, any of it together
 
 // ---- staging ------------------------------------------------------------------------------------------------------------------
@@ -483,8 +484,8 @@ __device__ __forceinline__ void fwd_finish(const DiffAttnArgs& a, const FwdState
 // One pass over the keys with a running reference and sum for each map.  Per pair and map: Dh + Dv multiply-adds on the matrix cores
 // against one exponential (a quarter of the VALU's rate), a fma, a maximum, an addition and a rounding.  A wave's products and its
 // softmax follow one another, and one or two waves a SIMD do not fill the gaps: at 32 / 64, 10 000 x 10 000, the VALU issues 52 % of
-// the time and the matrix cores are busy 23 %; at 64 / 128, 4096 x 4096, 46 and 22 %.  4 heads of 32 / 64, 10 000 x 10 000 bf16: 271 us
-// (567 TFLOP/s); 2 x 8 heads of 64 / 128, 4096 x 4096: 386 us (534 TFLOP/s); one query, 8 x 4 heads of 32 / 64, 40 000 keys ragged:
+// the time and the matrix cores are busy 23 %; at 64 / 128, 4096 x 4096, 46 and 22 %.  4 heads of 32 / 64, 10 000 x 10 000 bf16: 267 us
+// (575 TFLOP/s); 2 x 8 heads of 64 / 128, 4096 x 4096: 380 us (542 TFLOP/s); one query, 8 x 4 heads of 32 / 64, 40 000 keys ragged:
 // 54 to 61 us (4.2 to 4.7 TB/s, bound by memory).
 template <typename T, int DH, int DV, bool SHARED, int MODE>
 __global__ __launch_bounds__((AttnPlan<T, DH, DV, SHARED>::NT), (AttnPlan<T, DH, DV, SHARED>::MINW)) void diff_attn_fwd_kernel(
@@ -797,8 +798,8 @@ __device__ __forceinline__ void store_gkv(const DiffAttnArgs& a, int b, int hk, 
 
 // ---- backward: grad_q and the rows' parts of grad_lam; own = rows, staged = keys -----------------------------------------------
 // dq_m = scale sum_j dS_m k_m,  dS_1 = A_1 o (G - del_1),  dS_2 = -lam A_2 o (G - del_2),  G = D o (grad_out v^T);  A from the row's
-// statistics.  Bound as the forward pass: 10 000 x 10 000, 4 heads of 32 / 64 bf16 288 us (533 TFLOP/s, the scores computed again;
-// VALU 51 %, matrix cores 22 %).
+// statistics.  Bound as the forward pass: 10 000 x 10 000, 4 heads of 32 / 64 bf16 340 us (VALU 60 %, matrix
+// cores 25 %; the scores computed again, dS in two operands).
 template <typename T, int DH, int DV, bool SHARED, int MODE>
 __global__ __launch_bounds__((AttnPlan<T, DH, DV, SHARED>::NT), (AttnPlan<T, DH, DV, SHARED>::MINW)) void diff_attn_bwd_q_kernel(
     const DiffAttnArgs a) {
@@ -937,9 +938,8 @@ __global__ __launch_bounds__(1024) static void diff_attn_lam_kernel(const float*
 
 // ---- backward: grad_k and grad_v; own = keys, staged = the rows of every head that shares them ----------------------------------
 // A tile of rows stays inside one head (its rows are one stretch of queries), heads one after the other.
-// dk_m = scale sum_i dS_m q_m,  dv = sum_i (D o (A_1 - lam A_2)) grad_out.  10 000 x 10 000, 4 heads of 32 / 64 bf16: 437 to 515 us
-// by card and clock (400 to 470 TFLOP/s); bound as the others (VALU 47 %, matrix cores 18 %) with LDS reads on top (the rows'
-// statistics, 4 floats each).
+// dk_m = scale sum_i dS_m q_m,  dv = sum_i (D o (A_1 - lam A_2)) grad_out.  10 000 x 10 000, 4 heads of 32 / 64 bf16: 513 to 590 us
+// by card and clock; bound as the others (VALU 49 %, matrix cores 19 %) with LDS reads on top (the rows' statistics, 4 floats each).
 // PART 0: both gradients in one pass; 1: grad_k, 2: grad_v by a pass of its own, where the accumulators of both (2 DH + DV
 // floats a lane's item pair) would not fit the register file (the scores are computed twice: less than spilling costs).
 template <typename T, int DH, int DV, bool SHARED, int MODE, int PART>
