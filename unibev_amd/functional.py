@@ -790,14 +790,14 @@ def diff_attention(q, k, v, lam, attn_mask=None, key_padding_mask=None, causal=F
     (B, Nq, H, Dv); a query that sees no key gets zeros (and zero gradients).
 
     attn_mask: bool (True hides, as in ``torch.nn.MultiheadAttention``) or f32 / f16 / bf16 (added; -inf hides, +inf counts as the
-    largest value), (Nq, Nk), (B H, Nq, Nk) or broadcastable to (B, H, Nq, Nk); it gets no gradient.  key_padding_mask: bool
+    largest value), (Nq, Nk), (B H, Nq, Nk) or 4-D, in 2-D and 4-D an axis may be 1; it gets no gradient.  key_padding_mask: bool
     (B, Nk), True hides the key from every query; what k and v hold there is never used.  A key that only attn_mask or causal
     hides must be finite.  causal: query i sees keys j <= i + Nk - Nq.  scale: in [1e-30, 1e30), default Dh ** -0.5.
 
     ``p``, ``training``, ``seed``: dropout D on the map, as in ``dropout`` (never stored).
 
-    Sums are f32, scaled scores lie within +-2^24; probabilities and their gradients enter the matrix instructions in q's type.  f16:
-    gradients scaled into f16's range, as in any f16 backward pass.  Differentiable once."""
+    Sums are f32, scaled scores lie within +-2^24; probabilities enter the matrix instructions in q's type, their
+    gradients (16-bit types) as the sum of two values of it.  f16: gradients scaled into f16's range, as in any f16 backward pass.  Differentiable once."""
     p, seed, base = _drop_args(p, training, seed, 'diff_attention')
     return native().diff_attention(q, k, v, lam, attn_mask, key_padding_mask, causal, scale, p, seed, base)
 
